@@ -1,0 +1,298 @@
+// Causal attention that also adds up, for every cached row and kv head, the softmax weight that the step's tokens give it: what
+// an eviction by accumulated attention weight goes by.
+//
+//   mass[r, g] = (r < past ? mass[r, g] : 0) + sum_i sum_{h of g} w_ihr        (w as in attn_rows.cu, r <= past + i)
+//
+// The attention itself is that of attn_rows.cu and leaves log2 of every row's sum, lse_ih. With it a weight needs no second
+// softmax: w_ihr = 2^(scale log2(e) q_ih . k_gr - lse_ih), so the sums take one more look at the keys alone, with the keys as
+// the resident operand and the step's packed rows going by: a key's sum stays with its thread, no two CTAs add to the same
+// word, and the order of the sum does not depend on timing. Sums are fp32.
+//
+// Long steps are cut over their rows too (units of `rt` row tiles, as in row_units.cuh): the cut pieces' sums are left in
+// scratch and added in order by a second launch.
+#include "attn_rows.cuh"
+
+#include <math.h>
+
+int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs a, int max_q_len, const void* k_cache, const void* v_cache,
+                  const int* cu_q, const int* kv_len, PageTable pt, const long long* masks, float* scratch, long long scratch_floats,
+                  float* lse, int* status, cudaStream_t stream);
+
+namespace {
+
+// Units of the sums: a unit is `keys` cached rows of one sequence and `rt` of its row tiles of `rows` packed rows.
+struct MassArgs {
+    RowsArgs r;
+    int keys, rows;
+    int target;                       // units to aim at over all kv heads; 0: rows are never cut
+};
+
+struct MassUnit {
+    int b, kt, piece, pieces, rt, unit0;
+    SeqShape s;
+};
+
+__device__ __forceinline__ int mass_ktiles(const SeqShape& s, const MassArgs& a) { return s.n_q > 0 ? (s.kvl + a.keys - 1) / a.keys : 0; }
+__device__ __forceinline__ int mass_rtiles(const SeqShape& s, const MassArgs& a) { return (s.n_q * a.r.G + a.rows - 1) / a.rows; }
+
+__device__ __forceinline__ int mass_rt(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const MassArgs& a, int* status) {
+    if (a.target == 0) return 1 << 28;
+    const int lane = threadIdx.x & 31;
+    long long work = 0;
+    for (int b0 = 0; b0 < a.r.B; b0 += 32) {
+        if (b0 + lane < a.r.B) {
+            const SeqShape s = seq_shape(cu_q, kv_len, b0 + lane, a.r, status);
+            work += (long long)mass_ktiles(s, a) * mass_rtiles(s, a);
+        }
+    }
+    work = warp_sum_ll(work);
+    return (int)max(1ll, (work * a.r.KV + a.target - 1) / a.target);
+}
+
+// Finds unit `flat`, like find_row_unit: a sequence's units lie together, key tiles ascending (the first keys have the most
+// rows above them), a key tile's pieces one after the other.
+__device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const MassArgs& a, int flat,
+                                               MassUnit& u, int* status) {
+    __shared__ int found_s[3];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        const int rt = mass_rt(cu_q, kv_len, a, status);
+        int fb = -1, base = 0, first = 0;
+        for (int b0 = 0; b0 < a.r.B && fb < 0; b0 += 32) {
+            int n = 0;
+            if (b0 + lane < a.r.B) {
+                const SeqShape s = seq_shape(cu_q, kv_len, b0 + lane, a.r, status);
+                n = mass_ktiles(s, a) * ((mass_rtiles(s, a) + rt - 1) / rt);
+            }
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const int excl = incl - n;
+            const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && flat >= base + excl && flat < base + incl);
+            if (hit != 0u) {
+                const int src = __ffs(hit) - 1;
+                fb = b0 + src;
+                first = base + __shfl_sync(0xffffffffu, excl, src);
+            }
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) {
+            found_s[0] = fb;
+            found_s[1] = first;
+            found_s[2] = rt;
+        }
+    }
+    __syncthreads();
+    u.b = found_s[0];
+    if (u.b < 0) return false;
+    u.unit0 = found_s[1];
+    u.rt = found_s[2];
+    u.s = seq_shape(cu_q, kv_len, u.b, a.r, status);
+    u.pieces = (mass_rtiles(u.s, a) + u.rt - 1) / u.rt;
+    const int at = flat - u.unit0;
+    u.kt = at / u.pieces;
+    u.piece = at % u.pieces;
+    return true;
+}
+
+// The first row tile with a token that sees the key tile's first key.
+__device__ __forceinline__ int mass_first_tile(const MassUnit& u, const MassArgs& a) {
+    const int tok = max(0, u.kt * a.keys - (u.s.kvl - u.s.n_q));
+    return tok * a.r.G / a.rows;
+}
+
+// Where a key's sum lies, or -1.
+__device__ __forceinline__ long long mass_at(const PageTable& pt, int b, int key, int KV, int g) {
+    const int page = page_of(pt, b, key);
+    return page < 0 ? -1 : ((long long)page * KV + g) * PAGE_TOKENS + key % PAGE_TOKENS;
+}
+
+__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four_of(const bf16* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+}
+
+constexpr int GK = 64, GR = 32;      // keys (a page) and packed rows a tile of the general kernel
+
+// 16 x 16 threads; thread (ty, tx) has the keys ty + 16 i (i < 4) of the page and the rows tx + 16 j of a tile.
+template <typename T>
+__global__ void __launch_bounds__(256)
+attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const float* __restrict__ lse, float* __restrict__ mass,
+                 float* __restrict__ part, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, MassArgs a,
+                 int* __restrict__ status) {
+    extern __shared__ __align__(16) unsigned char smem_mass[];
+    const int HD = a.r.HD, p = HD + 4;
+    float* k_s = reinterpret_cast<float*>(smem_mass);              // [GK][p]
+    float* q_s = k_s + GK * p;                                     // [GR][p]
+    __shared__ float lse_s[GR];
+    MassUnit u;
+    if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
+    const int g = blockIdx.y, G = a.r.G, past = u.s.kvl - u.s.n_q, key0 = u.kt * GK, n_rows = u.s.n_q * G;
+    const int tiles = mass_rtiles(u.s, a);
+    const int r0 = max(u.piece * u.rt, mass_first_tile(u, a)), r1 = (int)min((long long)tiles, (long long)(u.piece + 1) * u.rt);
+    if (r0 >= r1) return;                                          // no token of this piece sees the page
+    const int page = page_of(pt, u.b, key0);
+    if (page < 0) {
+        if (threadIdx.x == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
+        return;
+    }
+    const T* k = k_cache + ((size_t)page * a.r.KV + g) * PAGE_TOKENS * HD;
+    for (int i = threadIdx.x * 4; i < GK * HD; i += 256 * 4) *reinterpret_cast<float4*>(k_s + i / HD * p + i % HD) = four_of(k + i);
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int rt = r0; rt < r1; rt++) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < GR * HD; i += 256) {
+            const int r = i / HD, d = i % HD, pr = rt * GR + r;
+            q_s[r * p + d] = pr < n_rows ? to_f32(q[(size_t)(u.s.q_begin + pr / G) * a.r.ldq + (size_t)(g * G + pr % G) * HD + d]) : 0.f;
+        }
+        if (threadIdx.x < GR) {
+            const int pr = rt * GR + threadIdx.x;
+            lse_s[threadIdx.x] = pr < n_rows ? lse[(size_t)(u.s.q_begin + pr / G) * a.r.H + g * G + pr % G] : 0.f;
+        }
+        __syncthreads();
+        float s[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i][0] = s[i][1] = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < HD; d += 4) {
+            const float4 q0 = four_of(q_s + tx * p + d), q1 = four_of(q_s + (tx + 16) * p + d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 kv = four_of(k_s + (ty + 16 * i) * p + d);
+                s[i][0] = fmaf(q0.x, kv.x, s[i][0]);
+                s[i][0] = fmaf(q0.y, kv.y, s[i][0]);
+                s[i][0] = fmaf(q0.z, kv.z, s[i][0]);
+                s[i][0] = fmaf(q0.w, kv.w, s[i][0]);
+                s[i][1] = fmaf(q1.x, kv.x, s[i][1]);
+                s[i][1] = fmaf(q1.y, kv.y, s[i][1]);
+                s[i][1] = fmaf(q1.z, kv.z, s[i][1]);
+                s[i][1] = fmaf(q1.w, kv.w, s[i][1]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int r = tx + 16 * j, pr = rt * GR + r;
+            if (pr >= n_rows) continue;
+            const int last = past + pr / G;                        // the last key that the row sees
+            const float z = lse_s[r];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (key0 + ty + 16 * i <= last) sum[i] += exp2f(fmaf(s[i][j], a.r.scale_log2, -z));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+        const int key = key0 + ty + 16 * i;
+        if (tx != 0 || key >= u.s.kvl) continue;
+        if (u.pieces > 1) {
+            part[((long long)blockIdx.x * a.r.KV + g) * GK + ty + 16 * i] = sum[i];
+        } else {
+            float* m = mass + ((size_t)page * a.r.KV + g) * PAGE_TOKENS + ty + 16 * i;
+            *m = key < past ? *m + sum[i] : sum[i];
+        }
+    }
+}
+
+// Adds the pieces of every key's sum in order. A thread a key of a key tile; key tiles are numbered sequence by sequence.
+__global__ void attn_mass_add_kernel(float* __restrict__ mass, const float* __restrict__ part, const int* __restrict__ cu_q,
+                                     const int* __restrict__ kv_len, PageTable pt, MassArgs a, int* __restrict__ status) {
+    MassUnit u;
+    // the units of key tile n of the step: unit numbers are found as the first launch's were, from the tile's first piece on
+    if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
+    if (u.piece != 0 || u.pieces <= 1) return;                     // one CTA a key tile; uncut tiles are done
+    const int g = blockIdx.y, past = u.s.kvl - u.s.n_q, key = u.kt * a.keys + threadIdx.x;
+    if (threadIdx.x >= a.keys || key >= u.s.kvl) return;
+    const long long at = mass_at(pt, u.b, key, a.r.KV, g);
+    if (at < 0) return;                                            // reported by the first launch
+    float sum = key < past ? mass[at] : 0.f;
+    const int first = mass_first_tile(u, a);
+    for (int c = first / u.rt; c < u.pieces; c++) sum += part[((long long)(blockIdx.x + c) * a.r.KV + g) * a.keys + threadIdx.x];
+    mass[at] = sum;
+}
+
+// Most units (of one kv head) for `n_ids` pages of all sequences.
+long long mass_units_max(const MassArgs& a, int n_ids) {
+    const long long kt = ceil_div_ll((long long)n_ids * PAGE_TOKENS, a.keys) + a.r.B;
+    return kt + (a.target > 0 ? ceil_div(a.target, a.r.KV) : 0);
+}
+
+void mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
+    a.keys = GK;
+    a.rows = GR;
+    a.target = 4 * mynah_sm_count();
+    if ((long long)max_q_len * a.r.G <= a.rows) a.target = 0;      // one row tile a sequence: nothing to cut
+    (void)dtype, (void)aligned;
+}
+
+long long mass_scratch(const MassArgs& a, int n_ids) {
+    return (long long)a.r.T * a.r.H + 4 + (a.target > 0 ? mass_units_max(a, n_ids) * a.r.KV * a.keys : 0);
+}
+
+}  // namespace
+
+MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype);
+
+// Floats of scratch for mynah_attn_mass, whichever kernels take the call.
+MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int n_ids) {
+    if (T <= 0 || B <= 0 || KV <= 0 || H % KV != 0 || H <= 0 || HD <= 0) return 0;
+    long long need = 0;
+    for (int aligned = 0; aligned < 2; aligned++) {
+        MassArgs a{};
+        a.r.T = T, a.r.B = B, a.r.H = H, a.r.KV = KV, a.r.HD = HD, a.r.G = H / KV;
+        mass_plan(a, dtype, aligned != 0, max_q_len);
+        const long long n = mass_scratch(a, n_ids);
+        if (n > need) need = n;
+    }
+    return ((mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dtype) + 3) & ~3ll) + need;
+}
+
+// As mynah_attn_tree with causal rows, and mass [n_pages, KV, 64] fp32. n_ids: entries of page_ids (no fewer than the
+// sequences' pages together).
+MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, int T, int B, int max_q_len, int H, int KV, int HD, int ldq,
+                              int ldo, const void* k_cache, const void* v_cache, const int* cu_q, const int* kv_len,
+                              const int* page_indptr, const int* page_ids, const int* page_base, int n_pages, int n_ids, float scale,
+                              float* scratch, long long scratch_floats, int* status, cudaStream_t stream) {
+    if (T <= 0 || B <= 0) return 0;
+    MYNAH_REQUIRE(mass != nullptr && n_ids >= 0, "attn_mass: sums and the number of page entries are required");
+    MYNAH_REQUIRE(scale >= 0.f, "attn_mass: the score scale %g is negative", scale);
+    MYNAH_REQUIRE(KV > 0 && H > 0 && H % KV == 0, "attn_mass: %d heads over %d kv heads", H, KV);
+    MYNAH_REQUIRE(scratch != nullptr && ((uintptr_t)scratch & 15) == 0, "attn_mass: 16-byte aligned scratch is required");
+    RowsArgs r{};
+    r.T = T, r.B = B, r.H = H, r.KV = KV, r.HD = HD, r.G = H / KV, r.ldq = ldq, r.ldo = ldo, r.causal = 1;
+    r.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
+    const int es = dtype == MYNAH_F32 ? 4 : 2;
+    const bool aligned = ((uintptr_t)q & 15) == 0 && (long long)ldq * es % 16 == 0;
+    MassArgs a{};
+    a.r = r;
+    mass_plan(a, dtype, aligned, max_q_len);
+    const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids);
+    MYNAH_REQUIRE(scratch_floats >= need, "attn_mass: scratch holds %lld floats, %lld are needed", scratch_floats, need);
+    const long long attn = (mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dtype) + 3) & ~3ll;
+    float* lse = scratch + attn;
+    float* part = lse + (((long long)T * H + 3) & ~3ll);
+    const PageTable pt{page_indptr, page_ids, page_base, n_pages};
+    const int rc = attn_rows_run("attn_mass", q, out, dtype, r, max_q_len, k_cache, v_cache, cu_q, kv_len, pt, nullptr, scratch, attn, lse, status, stream);
+    if (rc != 0) return rc;
+    const long long units = mass_units_max(a, n_ids);
+    MYNAH_REQUIRE(units < (1ll << 31), "attn_mass: launch too large");
+    const dim3 grid((unsigned)units, KV);
+    const size_t smem = (size_t)(GK + GR) * (HD + 4) * sizeof(float);
+    auto kf = attn_mass_kernel<float>;
+    auto kb = attn_mass_kernel<bf16>;
+    const cudaError_t e = dtype == MYNAH_F32 ? cudaFuncSetAttribute(kf, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
+                                             : cudaFuncSetAttribute(kb, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
+    if (dtype == MYNAH_F32) kf<<<grid, 256, smem, stream>>>((const float*)q, (const float*)k_cache, lse, mass, part, cu_q, kv_len, pt, a, status);
+    else kb<<<grid, 256, smem, stream>>>((const bf16*)q, (const bf16*)k_cache, lse, mass, part, cu_q, kv_len, pt, a, status);
+    if (mynah_check_launch("attn_mass")) return -1;
+    if (a.target == 0) return 0;
+    attn_mass_add_kernel<<<grid, a.keys, 0, stream>>>(mass, part, cu_q, kv_len, pt, a, status);
+    return mynah_check_launch("attn_mass_add");
+}

@@ -1,0 +1,434 @@
+// Attention of a few rows a sequence over the paged cache, with any mask among the step's own rows: the tokens of a drafted
+// tree (every token sees what was held before the step and its ancestors), or causal rows.
+//
+//   visible(i, r) = r < past, or bit (r - past) of token i's mask words (causal: r <= past + i), and r < kv_len
+//   s_ihr = scale * q_ih . k_gr,   w = softmax over the visible r,   out_ih = sum_r w_ihr v_gr      (g = h / (H / KV))
+//
+// with past = kv_len - n_q. A token that sees nothing gives zeros. The query heads of a kv head are rows of one problem, so a
+// page is read once for all of them; the keys of a tile are cut into chunks that run side by side, each with its own running
+// maximum and sum, and joined by a second launch where a tile has more than one (row_units.cuh has the rule).
+//
+// This file holds the general kernel (fp32, and bfloat16 heads that the tensor-core kernel does not take), the joining of
+// chunks, and the entry points.
+#include "attn_rows.cuh"
+
+#include <math.h>
+
+namespace {
+
+constexpr int KT = 32;               // keys a tile of the general kernel
+constexpr int MAX_HEAD = 256;
+
+__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four_of(const bf16* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+}
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Row pitch of a staged K or V tile: 16 bytes of padding, so that eight lanes' 16-byte reads of eight rows meet no bank twice.
+template <typename T> __host__ __device__ constexpr int pitch_of(int HD) { return HD + 16 / (int)sizeof(T); }
+
+// TY x TX threads; thread (ty, tx) has the packed rows ty + TY * i (i < 4) of the tile, for the scores the keys tx + TX * j of
+// KT, for the output the columns 4 * tx + 4 * TX * c. fp32 throughout, products and sums as written (FFMA). The row's maximum
+// and sum are kept by every thread of the row. A weight of an unseen key is stored as -1, and such keys are left out of the
+// output by a select: what lies in an unseen row of V (a stale NaN, an infinity) cannot reach a result, while a seen one does
+// what arithmetic does. K and V come KT keys at a time by asynchronous copies, two tiles in flight.
+// 16-row tiles (TY = 4, TX = 32) are for the few rows of decode steps and small trees, 64-row tiles (TY = TX = 16) for the rest.
+template <typename T, int TY, int TX, int NC>
+__global__ void __launch_bounds__(TY * TX)
+attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
+                 const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, const long long* __restrict__ masks,
+                 RowsArgs a, RowsScratch sc, int* __restrict__ status) {
+    constexpr int R = 4 * TY, KJ = KT / TX, THREADS = TY * TX;
+    extern __shared__ __align__(16) unsigned char smem_rows[];
+    const int HD = a.HD, kp = pitch_of<T>(HD), qp = HD + 4;
+    float* q_s = reinterpret_cast<float*>(smem_rows);              // [R][qp]
+    float* p_s = q_s + R * qp;                                     // [R][KT + 4]
+    T* k_s = reinterpret_cast<T*>(p_s + R * (KT + 4));             // [2][KT][kp]
+    T* v_s = k_s + 2 * KT * kp;                                    // [2][KT][kp]
+    __shared__ int bad_s;
+
+    RowUnit u;
+    if (threadIdx.x == 0) bad_s = 0;
+    if (!find_row_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
+    const int g = blockIdx.y, n_rows = u.rows(a), past = u.past(), row0 = u.tile * a.tile_rows;
+    const int pages = u.tile_pages(a), pg0 = u.chunk * u.cp, pg1 = min(pages, pg0 + u.cp);
+    const int n_chunks = (pages + u.cp - 1) / u.cp;
+    if (threadIdx.x == 0 && g == 0 && u.tile == u.s.tiles - 1 && u.chunk == 0) sc.info[u.b] = RowInfo{u.unit0, u.cp};
+    if (u.chunk >= n_chunks) return;                               // a causal tile that ends before this chunk
+    // every page of the chunk must be there: a chunk that lacks one counts as keys that nobody sees
+    for (int p = pg0 + (int)threadIdx.x; p < pg1; p += THREADS)
+        if (page_of(pt, u.b, p * PAGE_TOKENS) < 0) bad_s = 1;
+
+    const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
+    for (int i = threadIdx.x; i < R * HD; i += THREADS) {
+        const int r = i / HD, d = i % HD;
+        float x = 0.f;
+        if (r < n_rows) {
+            const int pr = row0 + r;
+            x = to_f32(q[(size_t)(u.s.q_begin + pr / a.G) * a.ldq + (size_t)(g * a.G + pr % a.G) * HD + d]);
+        }
+        q_s[r * qp + d] = x;
+    }
+    __syncthreads();
+    const bool bad = bad_s != 0;
+    if (bad && threadIdx.x == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
+
+    const int first_tok = row0 / a.G;
+    const int t0 = bad ? 0 : pg0 * (PAGE_TOKENS / KT), t1 = bad ? 0 : min(pg1 * (PAGE_TOKENS / KT), (u.s.kvl + KT - 1) / KT);
+    auto bring = [&](int t, int st) {
+        const int page = page_of(pt, u.b, t * KT);
+        const size_t base = (((size_t)page * a.KV + g) * PAGE_TOKENS + (t * KT) % PAGE_TOKENS) * HD;
+        const int per_row = HD * (int)sizeof(T) / 16;
+        for (int i = threadIdx.x; i < KT * per_row; i += THREADS) {
+            const int r = i / per_row, c = i % per_row;
+            copy16_async(reinterpret_cast<unsigned char*>(k_s + (st * KT + r) * kp) + c * 16, reinterpret_cast<const unsigned char*>(k_cache + base + (size_t)r * HD) + c * 16);
+            copy16_async(reinterpret_cast<unsigned char*>(v_s + (st * KT + r) * kp) + c * 16, reinterpret_cast<const unsigned char*>(v_cache + base + (size_t)r * HD) + c * 16);
+        }
+        copies_commit();
+    };
+
+    float m[4], l[4], acc[4][NC][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[i][c][e] = 0.f;
+    }
+    if (t0 < t1) bring(t0, 0);
+    for (int t = t0; t < t1; t++) {
+        const int st = (t - t0) & 1;
+        if (t + 1 < t1) {
+            bring(t + 1, st ^ 1);
+            copies_wait<1>();
+        } else {
+            copies_wait<0>();
+        }
+        __syncthreads();
+        const T* ks = k_s + st * KT * kp;
+        const T* vs = v_s + st * KT * kp;
+        float s[4][KJ];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < KJ; j++) s[i][j] = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < HD; d += 4) {
+            float4 qv[4], kv[KJ];
+#pragma unroll
+            for (int i = 0; i < 4; i++) qv[i] = four_of(q_s + (ty + TY * i) * qp + d);
+#pragma unroll
+            for (int j = 0; j < KJ; j++) kv[j] = four_of(ks + (tx + TX * j) * kp + d);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < KJ; j++) {
+                    s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
+                    s[i][j] = fmaf(qv[i].y, kv[j].y, s[i][j]);
+                    s[i][j] = fmaf(qv[i].z, kv[j].z, s[i][j]);
+                    s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
+                }
+        }
+        const int key0 = t * KT;
+        // is there a key in the tile that some row of the tile must not see?
+        const bool need_mask = key0 + KT > u.s.kvl || (a.causal ? key0 + KT - 1 > past + first_tok : key0 + KT > past);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = ty + TY * i, pr = row0 + r, tok = pr / a.G;
+            uint32_t seen = 0xffffffffu;
+            if (need_mask) {
+                const unsigned long long vis = r < n_rows ? visible64(key0 & ~63, u.s.kvl, past, tok, a.causal, masks + (size_t)(u.s.q_begin + tok) * a.words, a.words) : 0ull;
+                seen = (uint32_t)(vis >> (key0 & 63));
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < KJ; j++) {
+                s[i][j] = (seen >> (tx + TX * j)) & 1u ? s[i][j] * a.scale_log2 : -INFINITY;
+                mx = fmaxf(mx, s[i][j]);
+            }
+#pragma unroll
+            for (int o = TX / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float m_new = fmaxf(m[i], mx);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = exp2f(m[i] - m_use);               // 0 before the first seen key
+            m[i] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < KJ; j++) {
+                const bool in = (seen >> (tx + TX * j)) & 1u;
+                const float p = exp2f(s[i][j] - m_use);
+                if (in) sum += p;
+                p_s[r * (KT + 4) + tx + TX * j] = in ? p : -1.f;
+            }
+#pragma unroll
+            for (int o = TX / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[i] = l[i] * alpha + sum;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][c][e] *= alpha;
+        }
+        __syncwarp();                                              // a row's weights are written and read within one warp
+#pragma unroll 2
+        for (int kk = 0; kk < KT; kk += 4) {
+            float p[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) *reinterpret_cast<float4*>(p[i]) = *reinterpret_cast<const float4*>(p_s + (ty + TY * i) * (KT + 4) + kk);
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const int col = 4 * tx + 4 * TX * c;
+                    if (col >= HD) continue;
+                    const float4 x = four_of(vs + (kk + e4) * kp + col);
+                    if (need_mask) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float w = p[i][e4];
+                            acc[i][c][0] = w < 0.f ? acc[i][c][0] : fmaf(w, x.x, acc[i][c][0]);
+                            acc[i][c][1] = w < 0.f ? acc[i][c][1] : fmaf(w, x.y, acc[i][c][1]);
+                            acc[i][c][2] = w < 0.f ? acc[i][c][2] : fmaf(w, x.z, acc[i][c][2]);
+                            acc[i][c][3] = w < 0.f ? acc[i][c][3] : fmaf(w, x.w, acc[i][c][3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            acc[i][c][0] = fmaf(p[i][e4], x.x, acc[i][c][0]);
+                            acc[i][c][1] = fmaf(p[i][e4], x.y, acc[i][c][1]);
+                            acc[i][c][2] = fmaf(p[i][e4], x.z, acc[i][c][2]);
+                            acc[i][c][3] = fmaf(p[i][e4], x.w, acc[i][c][3]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();                                           // the stage and the weights are free again
+    }
+
+    const long long slot = (long long)blockIdx.x * a.KV + g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = ty + TY * i;
+        if (r >= n_rows) continue;
+        const int pr = row0 + r, tok = pr / a.G, h = g * a.G + pr % a.G;
+        if (n_chunks == 1) {
+            const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);    // a NaN stays one
+            T* o = out + (size_t)(u.s.q_begin + tok) * a.ldo + (size_t)h * HD;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int col = 4 * tx + 4 * TX * c + e;
+                    if (col < HD) o[col] = from_f32<T>(acc[i][c][e] * inv);
+                }
+            if (tx == 0 && sc.lse != nullptr) sc.lse[(size_t)(u.s.q_begin + tok) * a.H + h] = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
+        } else {
+            float* o = sc.o + (slot * a.tile_rows + r) * HD;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const int col = 4 * tx + 4 * TX * c;
+                if (col < HD) *reinterpret_cast<float4*>(o + col) = make_float4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
+            }
+            if (tx == 0) sc.ml[slot * a.tile_rows + r] = make_float2(m[i], l[i]);
+        }
+    }
+}
+
+// Joins the chunks of a cut tile: with M = max m_c, out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c. A warp a row; rows
+// whose tile was not cut have their output already.
+template <typename T>
+__global__ void __launch_bounds__(128)
+attn_rows_merge_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, RowsArgs a, RowsScratch sc,
+                       int* __restrict__ status) {
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= (long long)a.T * a.H) return;
+    const int t = (int)(row / a.H), h = (int)(row % a.H), g = h / a.G;
+    if (t >= cu_q[a.B]) return;                                    // a row behind the last sequence
+    int lo = 0, hi = a.B;                                          // the last sequence that begins at or before t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (cu_q[mid] <= t) lo = mid; else hi = mid;
+    }
+    RowUnit u;
+    u.b = lo;
+    u.s = seq_shape(cu_q, kv_len, lo, a, status);
+    if (u.s.n_q == 0) return;
+    const RowInfo info = sc.info[lo];
+    const int pr = (t - u.s.q_begin) * a.G + h % a.G;
+    u.tile = pr / a.tile_rows;
+    u.cp = info.cp;
+    u.seq_chunks = (u.s.pages + u.cp - 1) / u.cp;
+    const int n = (u.tile_pages(a) + u.cp - 1) / u.cp;
+    if (n <= 1) return;
+    const long long unit = info.unit0 + (long long)(u.s.tiles - 1 - u.tile) * u.seq_chunks;
+    auto at = [&](int c) { return ((unit + c) * a.KV + g) * a.tile_rows + pr % a.tile_rows; };
+    float mx = -INFINITY;
+    for (int c = lane; c < n; c += 32) mx = fmaxf(mx, sc.ml[at(c)].x);
+    mx = warp_max(mx);
+    const float m_use = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f;
+    for (int c = lane; c < n; c += 32) {
+        const float2 ml = sc.ml[at(c)];
+        l += ml.y * exp2f(ml.x - m_use);
+    }
+    l = warp_sum(l);
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    for (int col = lane * 4; col < a.HD; col += 128) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int c = 0; c < n; c++) {
+            const long long i = at(c);
+            const float w = exp2f(sc.ml[i].x - m_use);
+            const float4 y = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
+            x.x = fmaf(w, y.x, x.x);
+            x.y = fmaf(w, y.y, x.y);
+            x.z = fmaf(w, y.z, x.z);
+            x.w = fmaf(w, y.w, x.w);
+        }
+        T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
+        o[0] = from_f32<T>(x.x * inv);
+        o[1] = from_f32<T>(x.y * inv);
+        o[2] = from_f32<T>(x.z * inv);
+        o[3] = from_f32<T>(x.w * inv);
+    }
+    if (lane == 0 && sc.lse != nullptr) sc.lse[(size_t)t * a.H + h] = l == 0.f ? -INFINITY : m_use + log2f(l);
+}
+
+template <typename T, int TY, int TX, int NC>
+int go(const void* q, void* out, const RowsArgs& a, const void* k, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
+       const long long* masks, RowsScratch s, int* status, cudaStream_t stream) {
+    constexpr int R = 4 * TY;
+    const size_t smem = (size_t)R * (a.HD + 4) * 4 + (size_t)R * (KT + 4) * 4 + 4 * (size_t)KT * pitch_of<T>(a.HD) * sizeof(T);
+    auto kern = attn_rows_kernel<T, TY, TX, NC>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
+    const dim3 grid((unsigned)row_units_max(a), a.KV);
+    kern<<<grid, TY * TX, smem, stream>>>((const T*)q, (T*)out, (const T*)k, (const T*)v, cu_q, kv_len, pt, masks, a, s, status);
+    return mynah_check_launch("attn_rows");
+}
+
+template <typename T>
+int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
+         const long long* masks, RowsScratch s, int* status, cudaStream_t stream) {
+#define ROWS_GO(TY, TX, NC) return go<T, TY, TX, NC>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream)
+    if (a.tile_rows == 16) {
+        if (a.HD <= 128) ROWS_GO(4, 32, 1);
+        ROWS_GO(4, 32, 2);
+    }
+    if (a.HD <= 64) ROWS_GO(16, 16, 1);
+    if (a.HD <= 128) ROWS_GO(16, 16, 2);
+    ROWS_GO(16, 16, 4);
+#undef ROWS_GO
+}
+
+}  // namespace
+
+long long rows_scratch_floats(const RowsArgs& a) {
+    const long long rows = a.target > 0 ? row_units_max(a) * a.KV * a.tile_rows : 0;     // uncut tiles leave nothing
+    return 2ll * a.B + 4 + rows * (a.HD + 2);
+}
+
+RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
+    const long long rows = a.target > 0 ? row_units_max(a) * a.KV * a.tile_rows : 0;
+    RowsScratch s;
+    s.o = scratch;                                                 // 16-byte rows first
+    s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
+    s.info = reinterpret_cast<RowInfo*>(scratch + rows * (a.HD + 2));
+    s.lse = lse;
+    return s;
+}
+
+bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
+    const int sms = mynah_sm_count();
+    const bool tc = aligned && rows_tcgen05_takes(dtype, a.H, a.KV, a.HD);
+    if (tc) {
+        a.tile_rows = 128 / a.G * a.G;
+    } else {
+        a.tile_rows = (long long)max_q_len * a.G <= 16 ? 16 : 64;
+    }
+    a.min_pages = 2;
+    a.target = 2 * sms;
+    // A step whose tiles alone fill the device twice over: its keys are not cut, and nothing has to be joined.
+    if ((long long)a.T * a.G / a.tile_rows * a.KV >= 2ll * a.target) a.target = 0;
+    return tc;
+}
+
+int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, const void* k, const void* v, const int* cu_q,
+                        const int* kv_len, PageTable pt, const long long* masks, RowsScratch s, int* status, cudaStream_t stream) {
+    if (dtype == MYNAH_F32) return pick<float>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
+    return pick<bf16>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
+}
+
+int launch_rows_merge(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, RowsScratch s, int* status,
+                      cudaStream_t stream) {
+    const long long rows = (long long)a.T * a.H;
+    const unsigned grid = (unsigned)((rows + 3) / 4);
+    if (dtype == MYNAH_F32) attn_rows_merge_kernel<float><<<grid, 128, 0, stream>>>((float*)out, cu_q, kv_len, a, s, status);
+    else attn_rows_merge_kernel<bf16><<<grid, 128, 0, stream>>>((bf16*)out, cu_q, kv_len, a, s, status);
+    return mynah_check_launch("attn_rows_merge");
+}
+
+// Floats of scratch for mynah_attn_tree, whichever kernel takes the call.
+MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype) {
+    if (T <= 0 || B <= 0 || KV <= 0 || H % KV != 0 || H <= 0 || HD <= 0) return 0;
+    long long need = 0;
+    for (int aligned = 0; aligned < 2; aligned++) {
+        RowsArgs a{};
+        a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = H / KV;
+        rows_plan(a, dtype, max_q_len, aligned != 0);
+        const long long n = rows_scratch_floats(a);
+        if (n > need) need = n;
+    }
+    return need;
+}
+
+// What mynah_attn_tree and mynah_attn_mass check and launch alike.
+int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs a, int max_q_len, const void* k_cache, const void* v_cache,
+                  const int* cu_q, const int* kv_len, PageTable pt, const long long* masks, float* scratch, long long scratch_floats,
+                  float* lse, int* status, cudaStream_t stream) {
+    MYNAH_REQUIRE(dtype == MYNAH_F32 || dtype == MYNAH_BF16, "%s: dtype %d is neither float32 nor bfloat16", who, dtype);
+    MYNAH_REQUIRE(a.KV > 0 && a.H > 0 && a.H % a.KV == 0 && a.KV <= 65535, "%s: %d heads over %d kv heads", who, a.H, a.KV);
+    MYNAH_REQUIRE(a.HD > 0 && a.HD % 8 == 0 && a.HD <= MAX_HEAD, "%s: head_dim %d is no multiple of 8 up to %d", who, a.HD, MAX_HEAD);
+    const int es = dtype == MYNAH_F32 ? 4 : 2;
+    MYNAH_REQUIRE(a.ldq >= a.H * a.HD && a.ldo >= a.H * a.HD, "%s: rows of %d and %d values for %d heads of %d", who, a.ldq, a.ldo, a.H, a.HD);
+    MYNAH_REQUIRE(((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0, "%s: the cache must be 16-byte aligned", who);
+    MYNAH_REQUIRE((long long)a.T * a.G < (1ll << 30), "%s: %d rows of %d heads a kv head are too many", who, a.T, a.G);
+    MYNAH_REQUIRE(status != nullptr && scratch != nullptr && ((uintptr_t)scratch & 15) == 0, "%s: a status word and 16-byte aligned scratch are required", who);
+    const bool aligned = ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0 && (long long)a.ldq * es % 16 == 0 && (long long)a.ldo * es % 16 == 0;
+    const bool tc = rows_plan(a, dtype, max_q_len, aligned);
+    const long long need = rows_scratch_floats(a);
+    MYNAH_REQUIRE(scratch_floats >= need, "%s: scratch holds %lld floats, %lld are needed", who, scratch_floats, need);
+    MYNAH_REQUIRE(row_units_max(a) < (1ll << 31), "%s: launch too large", who);
+    const RowsScratch s = rows_scratch(a, scratch, lse);
+    const int rc = tc ? launch_rows_tcgen05(q, out, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream)
+                      : launch_rows_generic(q, out, dtype, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream);
+    if (rc != 0 || a.target == 0) return rc;
+    return launch_rows_merge(out, dtype, a, cu_q, kv_len, s, status, stream);
+}
+
+// q [T, ldq] and out [T, ldo], head h in columns [h * HD, (h + 1) * HD); k_cache, v_cache [n_pages, KV, 64, HD], which hold the
+// step's own rows already; cu_q [B + 1], kv_len [B]; masks [T, words]: bit j of a token's words says that it sees the step's row
+// j of its sequence. scale 0: 1 / sqrt(HD). Rows of out behind the last sequence are left as they are.
+MYNAH_API int mynah_attn_tree(const void* q, void* out, int dtype, int T, int B, int max_q_len, int H, int KV, int HD, int ldq, int ldo,
+                              const void* k_cache, const void* v_cache, const int* cu_q, const int* kv_len,
+                              const int* page_indptr, const int* page_ids, const int* page_base, int n_pages,
+                              const long long* masks, int words, float scale, float* scratch, long long scratch_floats, int* status,
+                              cudaStream_t stream) {
+    if (T <= 0 || B <= 0) return 0;
+    MYNAH_REQUIRE(masks != nullptr && words > 0, "attn_tree: mask words are required");
+    MYNAH_REQUIRE(scale >= 0.f, "attn_tree: the score scale %g is negative", scale);
+    RowsArgs a{};
+    a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = KV > 0 ? H / KV : 0, a.ldq = ldq, a.ldo = ldo, a.words = words;
+    a.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
+    return attn_rows_run("attn_tree", q, out, dtype, a, max_q_len, k_cache, v_cache, cu_q, kv_len,
+                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, status, stream);
+}

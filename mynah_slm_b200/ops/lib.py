@@ -26,6 +26,10 @@ _lib: ctypes.CDLL | None = None
 
 P = c_void_p
 _SIGNATURES: dict[str, list] = {
+    "mynah_attn_tree": [P, P] + [c_int] * 9 + [P, P, P, P, P, P, P, c_int, P, c_int, c_float, P, c_longlong, P, P],
+    "mynah_attn_mass": [P, P, P] + [c_int] * 9 + [P, P, P, P, P, P, P, c_int, c_int, c_float, P, c_longlong, P, P],
+    "mynah_cache_evict": [P, P, P] + [c_int] * 6 + [P, P, P, P, c_int, P, P, P] + [c_int] * 4 + [P, P, P, P],
+    "mynah_tree_commit": [P, P, P, c_int, c_int, c_int, P, P, P, P, P, c_int, P, P] + [c_int] * 4 + [P, P, P, P, P],
     "mynah_embed_gather": [P, c_int, P, P, c_int, c_int, c_int, c_float, P],
     "mynah_rmsnorm": [P, P, P, c_int, P, P, c_int, c_int, c_int, c_float, c_float, P],
     "mynah_residual_add": [P, P, c_int, c_longlong, c_float, P],
@@ -212,6 +216,10 @@ def load() -> ctypes.CDLL:
     lib.mynah_retention_scratch_floats.argtypes = [c_int] * 6 + [P]
     lib.mynah_gated_memory_scratch_floats.restype = c_longlong
     lib.mynah_gated_memory_scratch_floats.argtypes = [c_int] * 9
+    lib.mynah_attn_tree_scratch_floats.restype = c_longlong
+    lib.mynah_attn_tree_scratch_floats.argtypes = [c_int] * 7
+    lib.mynah_attn_mass_scratch_floats.restype = c_longlong
+    lib.mynah_attn_mass_scratch_floats.argtypes = [c_int] * 8
     lib.mynah_moe_grouped_rows.restype = c_int
     lib.mynah_moe_grouped_rows.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
     lib.mynah_moe_max_tiles.restype = c_int

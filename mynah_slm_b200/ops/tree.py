@@ -1,0 +1,163 @@
+"""Trees of drafted tokens over the paged cache: the attention of a step that brings a tree for every sequence, and the
+acceptance of a tree's path with the move of its rows.
+
+A step that checks drafted tokens brings, for each sequence, a tree: row 0 is the token that was sampled last, every other row
+hangs on an earlier row (`parents`, -1 for none). All rows' keys and values are written to the cache behind what it holds, row
+past + i for the tree's row i, but rotated for their positions, past + depth. Every row attends to what was held and to its
+ancestors. What the model then chooses behind every row decides which path goes on (`tree_commit`): the path's rows move to
+past + 0, 1, 2, ..., where a sequence that had taken the tokens one by one would have them.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from ..cache.pages import PAGE_TOKENS
+from . import lib
+from .kernels import MAX_HEAD_DIM, PageTableView
+from .lib import KernelError, call, code, stream_ptr
+
+
+def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> tuple[np.ndarray, np.ndarray]:
+    """What a step needs to know of a tree given as every row's parent (an earlier row, or -1): (depths int32 [n], mask words
+    int64 [n, words]); bit j of row i's words (bit j % 64 of word j // 64) says that row j is row i or an ancestor of it."""
+    n = len(parents)
+    need = max(1, -(-n // 64))
+    words = need if words is None else int(words)
+    if words < need:
+        raise KernelError(f"tree_rows: {words} mask words for a tree of {n} rows, {need} are needed")
+    depth = np.zeros((n,), dtype=np.int32)
+    bits = np.zeros((n, words), dtype=np.uint64)
+    for i, p in enumerate(parents):
+        p = int(p)
+        if not -1 <= p < i:
+            raise KernelError(f"tree_rows: row {i} hangs on row {p}, which is not before it")
+        if p >= 0:
+            depth[i] = depth[p] + 1
+            bits[i] = bits[p]
+        bits[i, i // 64] |= np.uint64(1) << np.uint64(i % 64)
+    return depth, bits.view(np.int64)
+
+
+def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor,
+               v_cache: torch.Tensor, pages: PageTableView, scale: float) -> None:
+    """What the attention of a few rows a sequence asks of its arguments."""
+    dev = q.device
+    if not q.is_cuda or dev.index != torch.cuda.current_device():
+        raise KernelError(f"{who}: q is not on the current CUDA device")
+    if KV < 1 or H < 1 or H % KV:
+        raise KernelError(f"{who}: {H} heads over {KV} kv heads")
+    if HD < 1 or HD % 8 or HD > MAX_HEAD_DIM:
+        raise KernelError(f"{who}: head_dim {HD} is no multiple of 8 up to {MAX_HEAD_DIM}")
+    if not 0.0 <= scale < float("inf"):
+        raise KernelError(f"{who}: the score scale {scale} is not a positive number, nor 0 for 1 / sqrt(head_dim)")
+    code(q.dtype)
+    for t, name in ((q, "q"), (out, "the output")):
+        if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] < H * HD or (t.shape[0] > 1 and t.stride(0) < H * HD):
+            raise KernelError(f"{who}: {name} must be rows of at least {H * HD} values, one row behind the other")
+        if t.dtype != q.dtype or t.device != dev:
+            raise KernelError(f"{who}: {name} is {t.dtype} on {t.device}, q {q.dtype} on {dev}")
+    if out.shape[0] < q.shape[0]:
+        raise KernelError(f"{who}: {out.shape[0]} output rows for {q.shape[0]} rows")
+    for t, name in ((k_cache, "K cache"), (v_cache, "V cache")):
+        if t.dtype != q.dtype or t.device != dev or not t.is_contiguous() or t.dim() != 4 or t.shape[1:] != (KV, PAGE_TOKENS, HD) \
+                or t.shape[0] < pages.n_pages:
+            raise KernelError(f"{who}: the {name} must be contiguous [{pages.n_pages}, {KV}, {PAGE_TOKENS}, {HD}] of q's type and device, "
+                              f"got {tuple(t.shape)} {t.dtype}")
+    if ctx.B < 0 or ctx.max_q_len < 0:
+        raise KernelError(f"{who}: {ctx.B} sequences of up to {ctx.max_q_len} rows")
+    check_lists(who, dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
+
+
+def check_lists(who: str, dev, B: int, cu_q: Optional[torch.Tensor], kv_len: torch.Tensor, pages: PageTableView, status: torch.Tensor) -> None:
+    for t, n, name in ((cu_q, B + 1, "cu_q"), (kv_len, B, "kv_len"), (pages.indptr, B + 1, "the page lists' bounds"),
+                       (pages.base, B, "the page lists' first pages"), (pages.ids, 0, "the page lists"), (status, 1, "the status word")):
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or t.device != dev or t.numel() < n or not t.is_contiguous():
+            raise KernelError(f"{who}: {name} must be at least {n} contiguous int32 on {dev}")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def row_scratch(who: str, scratch: Optional[torch.Tensor], need: int, dev) -> torch.Tensor:
+    if scratch is None:
+        return torch.empty((need,), dtype=torch.float32, device=dev)
+    if scratch.dtype != torch.float32 or scratch.device != dev or not scratch.is_contiguous() or scratch.numel() < need:
+        raise KernelError(f"{who}: scratch must be at least {need} contiguous float32 on {dev}")
+    return scratch
+
+
+def attn_tree_scratch_floats(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dtype: torch.dtype) -> int:
+    return int(lib.load().mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, code(dtype)))
+
+
+def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              pages: PageTableView, masks: torch.Tensor, scale: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
+    """Attention of a step's rows over the paged cache, which holds the rows' own keys and values already: with past = kv_len -
+    n_q, row i of a sequence sees every cached row below past, and row past + j where bit j of its mask words is set (`tree_rows`
+    makes the words of a tree; any other mask will do, a row that sees nothing gives zeros). Query head h reads kv head
+    h // (H / KV). `q` and `out` are rows with head h in columns [h HD, (h + 1) HD), and may be wider; rows of `out` behind the
+    last sequence are left as they are. masks: int64 [T, words]; rows of a tree beyond 64 * words are seen by nobody. scale 0:
+    1 / sqrt(HD). ctx: the step's description (B, max_q_len, cu_q, kv_len, status). Rows of the cache that a row does not see
+    have no influence on it, whatever they hold. float32 and bfloat16, heads of any multiple of 8 up to 256; bfloat16 heads of 64
+    and 128 run on the tensor cores. `scratch`: attn_tree_scratch_floats fp32 words, taken from torch's allocator unless given."""
+    check_rows("attn_tree", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
+    T = q.shape[0]
+    if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] < T or masks.shape[1] < 1 or not masks.is_contiguous() \
+            or masks.device != q.device:
+        raise KernelError(f"attn_tree: the masks must be contiguous int64 [{T}, words] on {q.device}, got {tuple(masks.shape)} {masks.dtype}")
+    if T == 0 or ctx.B == 0:
+        return
+    dt = code(q.dtype)
+    L = lib.load()
+    scratch = row_scratch("attn_tree", scratch, L.mynah_attn_tree_scratch_floats(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), q.device)
+    call("mynah_attn_tree", q.data_ptr(), out.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q), _row_stride(out),
+         k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(),
+         pages.base.data_ptr(), pages.n_pages, masks.data_ptr(), masks.shape[1], float(scale), scratch.data_ptr(), scratch.numel(),
+         ctx.status.data_ptr(), stream_ptr())
+
+
+def check_layers(who: str, k_caches: torch.Tensor, v_caches: torch.Tensor, pages: PageTableView) -> None:
+    for t, name in ((k_caches, "K"), (v_caches, "V")):
+        if not t.is_cuda or t.device.index != torch.cuda.current_device():
+            raise KernelError(f"{who}: the {name} cache is not on the current CUDA device")
+        if t.dim() != 5 or not t.is_contiguous() or t.shape[3] != PAGE_TOKENS or t.shape[1] != pages.n_pages:
+            raise KernelError(f"{who}: the {name} cache must be contiguous [layers, {pages.n_pages}, kv heads, {PAGE_TOKENS}, head], got {tuple(t.shape)}")
+    if v_caches.shape[:4] != k_caches.shape[:4] or v_caches.dtype != k_caches.dtype or v_caches.device != k_caches.device:
+        raise KernelError(f"{who}: K cache {tuple(k_caches.shape)} {k_caches.dtype} and V cache {tuple(v_caches.shape)} {v_caches.dtype} do not go together")
+
+
+def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tensor, ctx, k_caches: torch.Tensor, v_caches: torch.Tensor,
+                pages: PageTableView) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The path of every sequence's tree that the model's choices accept, and the move of its rows in all layers, in one launch.
+
+    tokens, parents, chosen: int32 [T], the step's tokens, every row's parent within its sequence (-1: none; a parent that is
+    not an earlier row counts as none), and the token chosen behind every row (the most likely one, or one drawn). From a
+    sequence's row 0 on, a row goes on to its lowest child whose token was chosen behind it. Cached row past + path[i] becomes
+    row past + i in every layer of k_caches, v_caches [layers, n_pages, kv heads, 64, head] (a storage group of the cache), past =
+    kv_len - n_q. Returns int32 (path [T]: the path's rows from every sequence's first place on, -1 behind them; count [B]; next
+    [B]: what was chosen behind the path's last row). A sequence without rows has count 0 and next -1. Trees of up to 4,096 rows;
+    ctx.max_q_len is the longest one's (a longer one is refused through the status word, with count 0)."""
+    check_layers("tree_commit", k_caches, v_caches, pages)
+    dev = k_caches.device
+    T = tokens.numel()
+    for t, name in ((tokens, "tokens"), (parents, "parents"), (chosen, "chosen tokens")):
+        if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.numel() < T or not t.is_contiguous():
+            raise KernelError(f"tree_commit: {name} must be {T} contiguous int32 on {dev}")
+    if not 0 <= ctx.max_q_len <= 4096:
+        raise KernelError(f"tree_commit: trees of {ctx.max_q_len} rows, 4096 are the most")
+    check_lists("tree_commit", dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
+    out = torch.empty((T + 2 * ctx.B,), dtype=torch.int32, device=dev)
+    path, count, after = out[:T], out[T:T + ctx.B], out[T + ctx.B:]
+    E, _, KV, _, HD = k_caches.shape
+    es = k_caches.element_size()
+    call("mynah_tree_commit", tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), T, ctx.B, ctx.max_q_len, ctx.cu_q.data_ptr(),
+         ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, k_caches.data_ptr(),
+         v_caches.data_ptr(), E, KV, HD * es, v_caches.shape[4] * es, path.data_ptr(), count.data_ptr(), after.data_ptr(),
+         ctx.status.data_ptr(), stream_ptr())
+    return path, count, after
