@@ -8,9 +8,10 @@
 // the resident operand and the step's packed rows going by: a key's sum stays with its thread, no two CTAs add to the same
 // word, and the order of the sum does not depend on timing. Sums are fp32.
 //
-// Long steps are cut over their rows too (units of `rt` row tiles, as in row_units.cuh): the cut pieces' sums are left in
-// scratch and added in order by a second launch.
-#include "attn_rows.cuh"
+// Long steps are cut over their rows too (attn_mass.cuh): the cut pieces' sums are left in scratch and added in order by a
+// second launch. This file holds the general kernel (fp32, and bfloat16 heads that the tensor-core kernel does not take), that
+// second launch and the entry points.
+#include "attn_mass.cuh"
 
 #include <math.h>
 
@@ -19,96 +20,6 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
                   float* lse, int* status, cudaStream_t stream);
 
 namespace {
-
-// Units of the sums: a unit is `keys` cached rows of one sequence and `rt` of its row tiles of `rows` packed rows.
-struct MassArgs {
-    RowsArgs r;
-    int keys, rows;
-    int target;                       // units to aim at over all kv heads; 0: rows are never cut
-};
-
-struct MassUnit {
-    int b, kt, piece, pieces, rt, unit0;
-    SeqShape s;
-};
-
-__device__ __forceinline__ int mass_ktiles(const SeqShape& s, const MassArgs& a) { return s.n_q > 0 ? (s.kvl + a.keys - 1) / a.keys : 0; }
-__device__ __forceinline__ int mass_rtiles(const SeqShape& s, const MassArgs& a) { return (s.n_q * a.r.G + a.rows - 1) / a.rows; }
-
-__device__ __forceinline__ int mass_rt(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const MassArgs& a, int* status) {
-    if (a.target == 0) return 1 << 28;
-    const int lane = threadIdx.x & 31;
-    long long work = 0;
-    for (int b0 = 0; b0 < a.r.B; b0 += 32) {
-        if (b0 + lane < a.r.B) {
-            const SeqShape s = seq_shape(cu_q, kv_len, b0 + lane, a.r, status);
-            work += (long long)mass_ktiles(s, a) * mass_rtiles(s, a);
-        }
-    }
-    work = warp_sum_ll(work);
-    return (int)max(1ll, (work * a.r.KV + a.target - 1) / a.target);
-}
-
-// Finds unit `flat`, like find_row_unit: a sequence's units lie together, key tiles ascending (the first keys have the most
-// rows above them), a key tile's pieces one after the other.
-__device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const MassArgs& a, int flat,
-                                               MassUnit& u, int* status) {
-    __shared__ int found_s[3];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) {
-        const int rt = mass_rt(cu_q, kv_len, a, status);
-        int fb = -1, base = 0, first = 0;
-        for (int b0 = 0; b0 < a.r.B && fb < 0; b0 += 32) {
-            int n = 0;
-            if (b0 + lane < a.r.B) {
-                const SeqShape s = seq_shape(cu_q, kv_len, b0 + lane, a.r, status);
-                n = mass_ktiles(s, a) * ((mass_rtiles(s, a) + rt - 1) / rt);
-            }
-            int incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            const int excl = incl - n;
-            const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && flat >= base + excl && flat < base + incl);
-            if (hit != 0u) {
-                const int src = __ffs(hit) - 1;
-                fb = b0 + src;
-                first = base + __shfl_sync(0xffffffffu, excl, src);
-            }
-            base += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (lane == 0) {
-            found_s[0] = fb;
-            found_s[1] = first;
-            found_s[2] = rt;
-        }
-    }
-    __syncthreads();
-    u.b = found_s[0];
-    if (u.b < 0) return false;
-    u.unit0 = found_s[1];
-    u.rt = found_s[2];
-    u.s = seq_shape(cu_q, kv_len, u.b, a.r, status);
-    u.pieces = (mass_rtiles(u.s, a) + u.rt - 1) / u.rt;
-    const int at = flat - u.unit0;
-    u.kt = at / u.pieces;
-    u.piece = at % u.pieces;
-    return true;
-}
-
-// The first row tile with a token that sees the key tile's first key.
-__device__ __forceinline__ int mass_first_tile(const MassUnit& u, const MassArgs& a) {
-    const int tok = max(0, u.kt * a.keys - (u.s.kvl - u.s.n_q));
-    return tok * a.r.G / a.rows;
-}
-
-// Where a key's sum lies, or -1.
-__device__ __forceinline__ long long mass_at(const PageTable& pt, int b, int key, int KV, int g) {
-    const int page = page_of(pt, b, key);
-    return page < 0 ? -1 : ((long long)page * KV + g) * PAGE_TOKENS + key % PAGE_TOKENS;
-}
 
 __device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 four_of(const bf16* p) {
@@ -131,7 +42,7 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
     __shared__ float lse_s[GR];
     MassUnit u;
     if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
-    const int g = blockIdx.y, G = a.r.G, past = u.s.kvl - u.s.n_q, key0 = u.kt * GK, n_rows = u.s.n_q * G;
+    const int g = blockIdx.y, G = a.r.G, past = u.s.kvl - u.s.n_q, key0 = u.kt0 * GK, n_rows = u.s.n_q * G;
     const int tiles = mass_rtiles(u.s, a);
     const int r0 = max(u.piece * u.rt, mass_first_tile(u, a)), r1 = (int)min((long long)tiles, (long long)(u.piece + 1) * u.rt);
     if (r0 >= r1) return;                                          // no token of this piece sees the page
@@ -152,7 +63,7 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
         }
         if (threadIdx.x < GR) {
             const int pr = rt * GR + threadIdx.x;
-            lse_s[threadIdx.x] = pr < n_rows ? lse[(size_t)(u.s.q_begin + pr / G) * a.r.H + g * G + pr % G] : 0.f;
+            lse_s[threadIdx.x] = pr < n_rows ? lse[((size_t)g * a.r.T + u.s.q_begin) * G + pr] : 0.f;
         }
         __syncthreads();
         float s[4][2];
@@ -207,7 +118,7 @@ __global__ void attn_mass_add_kernel(float* __restrict__ mass, const float* __re
     // the units of key tile n of the step: unit numbers are found as the first launch's were, from the tile's first piece on
     if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
     if (u.piece != 0 || u.pieces <= 1) return;                     // one CTA a key tile; uncut tiles are done
-    const int g = blockIdx.y, past = u.s.kvl - u.s.n_q, key = u.kt * a.keys + threadIdx.x;
+    const int g = blockIdx.y, past = u.s.kvl - u.s.n_q, key = u.kt0 * a.keys + threadIdx.x;
     if (threadIdx.x >= a.keys || key >= u.s.kvl) return;
     const long long at = mass_at(pt, u.b, key, a.r.KV, g);
     if (at < 0) return;                                            // reported by the first launch
@@ -217,22 +128,31 @@ __global__ void attn_mass_add_kernel(float* __restrict__ mass, const float* __re
     mass[at] = sum;
 }
 
-// Most units (of one kv head) for `n_ids` pages of all sequences.
-long long mass_units_max(const MassArgs& a, int n_ids) {
-    const long long kt = ceil_div_ll((long long)n_ids * PAGE_TOKENS, a.keys) + a.r.B;
-    return kt + (a.target > 0 ? ceil_div(a.target, a.r.KV) : 0);
+int launch_mass_generic(const void* q, const void* k, const float* lse, float* mass, float* part, int dtype, const int* cu_q,
+                        const int* kv_len, PageTable pt, const MassArgs& a, dim3 grid, int* status, cudaStream_t stream) {
+    const size_t smem = (size_t)(GK + GR) * (a.r.HD + 4) * sizeof(float);
+    auto kf = attn_mass_kernel<float>;
+    auto kb = attn_mass_kernel<bf16>;
+    const cudaError_t e = dtype == MYNAH_F32 ? cudaFuncSetAttribute(kf, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
+                                             : cudaFuncSetAttribute(kb, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
+    if (dtype == MYNAH_F32) kf<<<grid, 256, smem, stream>>>((const float*)q, (const float*)k, lse, mass, part, cu_q, kv_len, pt, a, status);
+    else kb<<<grid, 256, smem, stream>>>((const bf16*)q, (const bf16*)k, lse, mass, part, cu_q, kv_len, pt, a, status);
+    return mynah_check_launch("attn_mass");
 }
 
-void mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
-    a.keys = GK;
-    a.rows = GR;
-    a.target = 4 * mynah_sm_count();
-    if ((long long)max_q_len * a.r.G <= a.rows) a.target = 0;      // one row tile a sequence: nothing to cut
-    (void)dtype, (void)aligned;
+// Which kernel takes the sums, and its tiles.
+bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
+    const bool tc = aligned && mass_tcgen05_takes(dtype, a.r.H, a.r.KV, a.r.HD);
+    a.keys = tc ? 128 : GK;
+    a.rows = tc ? 128 / a.r.G * a.r.G : GR;
+    a.by_keys = (long long)max_q_len * a.r.G <= a.rows;
+    a.target = (tc ? 4 : (a.by_keys ? 0 : 4)) * mynah_sm_count();
+    return tc;
 }
 
 long long mass_scratch(const MassArgs& a, int n_ids) {
-    return (long long)a.r.T * a.r.H + 4 + (a.target > 0 ? mass_units_max(a, n_ids) * a.r.KV * a.keys : 0);
+    return (long long)a.r.T * a.r.H + 4 + (a.target > 0 && !a.by_keys ? mass_units_max(a, n_ids) * a.r.KV * a.keys : 0);
 }
 
 }  // namespace
@@ -271,7 +191,7 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
     const bool aligned = ((uintptr_t)q & 15) == 0 && (long long)ldq * es % 16 == 0;
     MassArgs a{};
     a.r = r;
-    mass_plan(a, dtype, aligned, max_q_len);
+    const bool tc = mass_plan(a, dtype, aligned, max_q_len);
     const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids);
     MYNAH_REQUIRE(scratch_floats >= need, "attn_mass: scratch holds %lld floats, %lld are needed", scratch_floats, need);
     const long long attn = (mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dtype) + 3) & ~3ll;
@@ -281,18 +201,14 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
     const int rc = attn_rows_run("attn_mass", q, out, dtype, r, max_q_len, k_cache, v_cache, cu_q, kv_len, pt, nullptr, scratch, attn, lse, status, stream);
     if (rc != 0) return rc;
     const long long units = mass_units_max(a, n_ids);
-    MYNAH_REQUIRE(units < (1ll << 31), "attn_mass: launch too large");
+    MYNAH_REQUIRE(units * KV < (1ll << 31) && KV <= 65535, "attn_mass: launch too large");
     const dim3 grid((unsigned)units, KV);
-    const size_t smem = (size_t)(GK + GR) * (HD + 4) * sizeof(float);
-    auto kf = attn_mass_kernel<float>;
-    auto kb = attn_mass_kernel<bf16>;
-    const cudaError_t e = dtype == MYNAH_F32 ? cudaFuncSetAttribute(kf, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
-                                             : cudaFuncSetAttribute(kb, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
-    if (dtype == MYNAH_F32) kf<<<grid, 256, smem, stream>>>((const float*)q, (const float*)k_cache, lse, mass, part, cu_q, kv_len, pt, a, status);
-    else kb<<<grid, 256, smem, stream>>>((const bf16*)q, (const bf16*)k_cache, lse, mass, part, cu_q, kv_len, pt, a, status);
-    if (mynah_check_launch("attn_mass")) return -1;
-    if (a.target == 0) return 0;
+    if (tc) {
+        if (launch_mass_tcgen05(q, k_cache, lse, mass, part, cu_q, kv_len, pt, a, n_ids, status, stream)) return -1;
+    } else if (launch_mass_generic(q, k_cache, lse, mass, part, dtype, cu_q, kv_len, pt, a, grid, status, stream)) {
+        return -1;
+    }
+    if (a.by_keys) return 0;                                       // nothing was cut over its rows
     attn_mass_add_kernel<<<grid, a.keys, 0, stream>>>(mass, part, cu_q, kv_len, pt, a, status);
     return mynah_check_launch("attn_mass_add");
 }

@@ -229,7 +229,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
                     const int col = 4 * tx + 4 * TX * c + e;
                     if (col < HD) o[col] = from_f32<T>(acc[i][c][e] * inv);
                 }
-            if (tx == 0 && sc.lse != nullptr) sc.lse[(size_t)(u.s.q_begin + tok) * a.H + h] = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
+            if (tx == 0 && sc.lse != nullptr) sc.lse[((size_t)g * a.T + u.s.q_begin) * a.G + pr] = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
         } else {
             float* o = sc.o + (slot * a.tile_rows + r) * HD;
 #pragma unroll
@@ -300,7 +300,7 @@ attn_rows_merge_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const 
         o[2] = from_f32<T>(x.z * inv);
         o[3] = from_f32<T>(x.w * inv);
     }
-    if (lane == 0 && sc.lse != nullptr) sc.lse[(size_t)t * a.H + h] = l == 0.f ? -INFINITY : m_use + log2f(l);
+    if (lane == 0 && sc.lse != nullptr) sc.lse[((size_t)g * a.T + t) * a.G + h % a.G] = l == 0.f ? -INFINITY : m_use + log2f(l);
 }
 
 template <typename T, int TY, int TX, int NC>

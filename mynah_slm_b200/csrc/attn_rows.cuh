@@ -8,7 +8,7 @@ struct RowsScratch {
     RowInfo* info;                    // [B]
     float2* ml;                       // [units][KV][tile_rows]: reference maximum (base 2, scaled) and sum
     float* o;                         // [units][KV][tile_rows][HD], not normalised
-    float* lse;                       // [T][H]: log2 of the sum of 2^score, -inf for a row that sees nothing; null: not wanted
+    float* lse;                       // [KV][T][G]: log2 of the sum of 2^score, -inf for a row that sees nothing; null: not wanted
 };
 
 // fp32 words of scratch that attention of this shape needs (without lse), and how it is laid out.

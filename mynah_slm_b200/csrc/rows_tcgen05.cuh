@@ -1,0 +1,58 @@
+// What the tcgen05 kernels on packed rows share: operand and instruction descriptors, paired fp32 arithmetic, the queries' tensor map.
+#pragma once
+#include "tcgen05.cuh"
+
+namespace tc5 {
+
+constexpr int HALF_BYTES = 128 * 128; // 128 rows of 128 bytes: one 64-column half of a tile
+constexpr int PAGE_BYTES = PAGE_TOKENS * 128;
+
+// K-major operand, 128-byte swizzle, groups of 8 rows 1024 bytes apart.
+static __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major operand: a row of 128 bytes holds 64 MN elements of one k; groups of 8 k 1024 bytes apart, the next 64 MN elements
+// `lbo` bytes further on.
+static __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulator, bf16 operands, M = 128, N = n; b_mn: B is MN-major.
+static __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+static __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+static __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
+    asm("{ .reg .b64 ra, rb, rc, rd;\n\t mov.b64 ra, {%2, %3};\n\t mov.b64 rb, {%4, %4};\n\t mov.b64 rc, {%5, %5};\n\t"
+        " fma.rn.f32x2 rd, ra, rb, rc;\n\t mov.b64 {%0, %1}, rd; }"
+        : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+static __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
+    asm("{ .reg .b64 ra, rb;\n\t mov.b64 ra, {%0, %1};\n\t mov.b64 rb, {%2, %3};\n\t add.rn.f32x2 ra, ra, rb;\n\t mov.b64 {%0, %1}, ra; }"
+        : "+f"(x0), "+f"(x1) : "f"(a0), "f"(a1));
+}
+static __device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+static __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// q as [T][H][HD] with a row pitch of ld elements; boxes of 64 columns x G heads x `tokens` tokens, 128-byte swizzle.
+static inline int make_map_rows(CUtensorMap* map, const void* q, long long T, int H, int HD, int G, int ld, int tokens) {
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return mynah_fail("tensor map: the driver does not provide cuTensorMapEncodeTiled");
+    const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)H, (cuuint64_t)T};
+    const cuuint64_t strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)ld * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)tokens};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return mynah_fail("tensor map: cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return 0;
+}
+
+}  // namespace tc5
