@@ -147,6 +147,7 @@ bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
     a.keys = tc ? 128 : GK;
     a.rows = tc ? 128 / a.r.G * a.r.G : GR;
     a.by_keys = (long long)max_q_len * a.r.G <= a.rows;
+    a.r.tile_rows = a.rows;
     a.target = (tc ? 4 : (a.by_keys ? 0 : 4)) * mynah_sm_count();
     return tc;
 }

@@ -5,11 +5,11 @@
 //   s_ihr = scale * q_ih . k_gr,   w = softmax over the visible r,   out_ih = sum_r w_ihr v_gr      (g = h / (H / KV))
 //
 // with past = kv_len - n_q. A token that sees nothing gives zeros. The query heads of a kv head are rows of one problem, so a
-// page is read once for all of them; the keys of a tile are cut into chunks that run side by side, each with its own running
-// maximum and sum, and joined by a second launch where a tile has more than one (row_units.cuh has the rule).
+// page is read once for all of them; the keys are shared out among the CTAs in equal ranges, each with its own running maximum
+// and sum, and a second launch joins what was cut (row_units.cuh has the rule).
 //
-// This file holds the general kernel (fp32, and bfloat16 heads that the tensor-core kernel does not take), the joining of
-// chunks, and the entry points.
+// This file holds the general kernel (fp32, and bfloat16 heads that the tensor-core kernel does not take), the joining, and
+// the entry points.
 #include "attn_rows.cuh"
 
 #include <math.h>
@@ -52,20 +52,21 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     T* k_s = reinterpret_cast<T*>(p_s + R * (KT + 4));             // [2][KT][kp]
     T* v_s = k_s + 2 * KT * kp;                                    // [2][KT][kp]
     __shared__ int bad_s;
+    __shared__ RowWalk walk_s;
 
-    RowUnit u;
+    if (threadIdx.x < 32) find_range(cu_q, kv_len, a, &walk_s, sc.info, status);
+    __syncthreads();
+    RowWalk u = walk_s;
+    if (u.b < 0) return;
+    const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
+    do {
+    const int g = u.g, n_rows = u.rows(a), past = u.past(), row0 = u.tile * a.tile_rows;
+    const int pg0 = u.pg0, pg1 = u.pg1;
     if (threadIdx.x == 0) bad_s = 0;
-    if (!find_row_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
-    const int g = blockIdx.y, n_rows = u.rows(a), past = u.past(), row0 = u.tile * a.tile_rows;
-    const int pages = u.tile_pages(a), pg0 = u.chunk * u.cp, pg1 = min(pages, pg0 + u.cp);
-    const int n_chunks = (pages + u.cp - 1) / u.cp;
-    if (threadIdx.x == 0 && g == 0 && u.tile == u.s.tiles - 1 && u.chunk == 0) sc.info[u.b] = RowInfo{u.unit0, u.cp};
-    if (u.chunk >= n_chunks) return;                               // a causal tile that ends before this chunk
-    // every page of the chunk must be there: a chunk that lacks one counts as keys that nobody sees
+    __syncthreads();                                               // (the segment before is done with shared memory)
+    // every page of the segment must be there: one that lacks a page counts as keys that nobody sees
     for (int p = pg0 + (int)threadIdx.x; p < pg1; p += THREADS)
         if (page_of(pt, u.b, p * PAGE_TOKENS) < 0) bad_s = 1;
-
-    const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
     for (int i = threadIdx.x; i < R * HD; i += THREADS) {
         const int r = i / HD, d = i % HD;
         float x = 0.f;
@@ -213,13 +214,14 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         __syncthreads();                                           // the stage and the weights are free again
     }
 
-    const long long slot = (long long)blockIdx.x * a.KV + g;
+    const long long slot = (long long)blockIdx.x * 2 + u.place();
+    const bool whole = u.whole();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int r = ty + TY * i;
         if (r >= n_rows) continue;
         const int pr = row0 + r, tok = pr / a.G, h = g * a.G + pr % a.G;
-        if (n_chunks == 1) {
+        if (whole) {
             const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);    // a NaN stays one
             T* o = out + (size_t)(u.s.q_begin + tok) * a.ldo + (size_t)h * HD;
 #pragma unroll
@@ -240,14 +242,16 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
             if (tx == 0) sc.ml[slot * a.tile_rows + r] = make_float2(m[i], l[i]);
         }
     }
+    } while (u.next(cu_q, kv_len, a, status));
 }
 
-// Joins the chunks of a cut tile: with M = max m_c, out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c. A warp a row; rows
-// whose tile was not cut have their output already.
+// Joins the segments of a cut item: with M = max m_c, out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c. A warp a row; rows
+// of items that were not cut have their output already.
 template <typename T>
 __global__ void __launch_bounds__(128)
 attn_rows_merge_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, RowsArgs a, RowsScratch sc,
                        int* __restrict__ status) {
+    griddep_wait();
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= (long long)a.T * a.H) return;
@@ -258,19 +262,27 @@ attn_rows_merge_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const 
         const int mid = (lo + hi) / 2;
         if (cu_q[mid] <= t) lo = mid; else hi = mid;
     }
-    RowUnit u;
-    u.b = lo;
-    u.s = seq_shape(cu_q, kv_len, lo, a, status);
-    if (u.s.n_q == 0) return;
-    const RowInfo info = sc.info[lo];
-    const int pr = (t - u.s.q_begin) * a.G + h % a.G;
-    u.tile = pr / a.tile_rows;
-    u.cp = info.cp;
-    u.seq_chunks = (u.s.pages + u.cp - 1) / u.cp;
-    const int n = (u.tile_pages(a) + u.cp - 1) / u.cp;
+    const SeqShape s = seq_shape(cu_q, kv_len, lo, a, status);
+    const int pr = (t - s.q_begin) * a.G + h % a.G, tile = pr / a.tile_rows;
+    if (pr < 0 || tile >= s.tiles) return;
+    // where the item lies on the line, and the CTAs that had a part of it
+    long long from, pages = tile_pages(s, tile, a);
+    if (a.causal && s.tiles > 1) {
+        long long all = 0, before = 0;
+        for (int i = lane; i < s.tiles; i += 32) {
+            const int p = tile_pages(s, i, a);
+            all += p;
+            if (i < tile) before += p;
+        }
+        from = warp_sum_ll(all) * g + warp_sum_ll(before);
+    } else {
+        from = ((long long)g * s.tiles + tile) * s.pages;
+    }
+    from += sc.info[lo];
+    const long long range = sc.info[a.B], c0 = from / range;
+    const int n = (int)((from + pages - 1) / range - c0) + 1;
     if (n <= 1) return;
-    const long long unit = info.unit0 + (long long)(u.s.tiles - 1 - u.tile) * u.seq_chunks;
-    auto at = [&](int c) { return ((unit + c) * a.KV + g) * a.tile_rows + pr % a.tile_rows; };
+    auto at = [&](int c) { return ((c0 + c) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + pr % a.tile_rows; };
     float mx = -INFINITY;
     for (int c = lane; c < n; c += 32) mx = fmaxf(mx, sc.ml[at(c)].x);
     mx = warp_max(mx);
@@ -311,8 +323,7 @@ int go(const void* q, void* out, const RowsArgs& a, const void* k, const void* v
     auto kern = attn_rows_kernel<T, TY, TX, NC>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
-    const dim3 grid((unsigned)row_units_max(a), a.KV);
-    kern<<<grid, TY * TX, smem, stream>>>((const T*)q, (T*)out, (const T*)k, (const T*)v, cu_q, kv_len, pt, masks, a, s, status);
+    kern<<<a.ctas, TY * TX, smem, stream>>>((const T*)q, (T*)out, (const T*)k, (const T*)v, cu_q, kv_len, pt, masks, a, s, status);
     return mynah_check_launch("attn_rows");
 }
 
@@ -333,32 +344,28 @@ int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void*
 }  // namespace
 
 long long rows_scratch_floats(const RowsArgs& a) {
-    const long long rows = a.target > 0 ? row_units_max(a) * a.KV * a.tile_rows : 0;     // uncut tiles leave nothing
-    return 2ll * a.B + 4 + rows * (a.HD + 2);
+    return 2ll * a.ctas * a.tile_rows * (a.HD + 2) + 2ll * (a.B + 1) + 4;
 }
 
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
-    const long long rows = a.target > 0 ? row_units_max(a) * a.KV * a.tile_rows : 0;
+    const long long rows = 2ll * a.ctas * a.tile_rows;
     RowsScratch s;
     s.o = scratch;                                                 // 16-byte rows first
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
-    s.info = reinterpret_cast<RowInfo*>(scratch + rows * (a.HD + 2));
+    s.info = reinterpret_cast<long long*>(scratch + rows * (a.HD + 2));
     s.lse = lse;
     return s;
 }
 
 bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
-    const int sms = mynah_sm_count();
     const bool tc = aligned && rows_tcgen05_takes(dtype, a.H, a.KV, a.HD);
     if (tc) {
         a.tile_rows = 128 / a.G * a.G;
     } else {
         a.tile_rows = (long long)max_q_len * a.G <= 16 ? 16 : 64;
     }
-    a.min_pages = 2;
-    a.target = 2 * sms;
-    // A step whose tiles alone fill the device twice over: its keys are not cut, and nothing has to be joined.
-    if ((long long)a.T * a.G / a.tile_rows * a.KV >= 2ll * a.target) a.target = 0;
+    a.min_range = 2;
+    a.ctas = 2 * mynah_sm_count();                                 // both kernels have two CTAs an SM
     return tc;
 }
 
@@ -371,9 +378,11 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
 int launch_rows_merge(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, RowsScratch s, int* status,
                       cudaStream_t stream) {
     const long long rows = (long long)a.T * a.H;
-    const unsigned grid = (unsigned)((rows + 3) / 4);
-    if (dtype == MYNAH_F32) attn_rows_merge_kernel<float><<<grid, 128, 0, stream>>>((float*)out, cu_q, kv_len, a, s, status);
-    else attn_rows_merge_kernel<bf16><<<grid, 128, 0, stream>>>((bf16*)out, cu_q, kv_len, a, s, status);
+    const dim3 grid((unsigned)((rows + 3) / 4));
+    const cudaError_t e = dtype == MYNAH_F32
+        ? launch_behind(attn_rows_merge_kernel<float>, grid, dim3(128), 0, stream, (float*)out, cu_q, kv_len, a, s, status)
+        : launch_behind(attn_rows_merge_kernel<bf16>, grid, dim3(128), 0, stream, (bf16*)out, cu_q, kv_len, a, s, status);
+    if (e != cudaSuccess) return mynah_fail("attn_rows_merge: %s", cudaGetErrorString(e));
     return mynah_check_launch("attn_rows_merge");
 }
 
@@ -407,11 +416,10 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
     const bool tc = rows_plan(a, dtype, max_q_len, aligned);
     const long long need = rows_scratch_floats(a);
     MYNAH_REQUIRE(scratch_floats >= need, "%s: scratch holds %lld floats, %lld are needed", who, scratch_floats, need);
-    MYNAH_REQUIRE(row_units_max(a) < (1ll << 31), "%s: launch too large", who);
     const RowsScratch s = rows_scratch(a, scratch, lse);
     const int rc = tc ? launch_rows_tcgen05(q, out, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream)
                       : launch_rows_generic(q, out, dtype, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream);
-    if (rc != 0 || a.target == 0) return rc;
+    if (rc != 0) return rc;
     return launch_rows_merge(out, dtype, a, cu_q, kv_len, s, status, stream);
 }
 

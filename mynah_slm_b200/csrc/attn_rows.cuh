@@ -3,11 +3,11 @@
 #pragma once
 #include "row_units.cuh"
 
-// Partial results of a cut tile, and what every launch of one call reads.
+// Partial results of cut items, and what every launch of one call reads.
 struct RowsScratch {
-    RowInfo* info;                    // [B]
-    float2* ml;                       // [units][KV][tile_rows]: reference maximum (base 2, scaled) and sum
-    float* o;                         // [units][KV][tile_rows][HD], not normalised
+    long long* info;                  // [B + 1]: where every sequence begins on the line, the range
+    float2* ml;                       // [CTAs][2][tile_rows]: reference maximum (base 2, scaled) and sum
+    float* o;                         // [CTAs][2][tile_rows][HD], not normalised
     float* lse;                       // [KV][T][G]: log2 of the sum of 2^score, -inf for a row that sees nothing; null: not wanted
 };
 
@@ -15,7 +15,7 @@ struct RowsScratch {
 long long rows_scratch_floats(const RowsArgs& a);
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse);
 
-// Fills tile_rows, min_pages and target for the kernel that takes these sizes; `tc` says which.
+// Fills tile_rows, min_range and ctas; true where the tcgen05 kernel takes the call.
 bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned);
 
 int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, const void* k, const void* v, const int* cu_q,
@@ -30,4 +30,21 @@ __device__ __forceinline__ float ex2_f(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// A launch that may begin while the kernel before it on the stream finishes; the kernel waits for that one's results itself
+// (griddep_wait) before it touches anything.
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }

@@ -1,12 +1,18 @@
-// How attention of a few rows a sequence over a paged cache is cut into units of work, for the kernels of attn_rows.cu and
+// How attention of a few rows a sequence over a paged cache is shared out among CTAs, for the kernels of attn_rows.cu and
 // attn_rows_tcgen05.cu.
 //
 // The query heads that share a kv head are rows of one problem: packed row r of a sequence is token r / G, head r % G of the
-// group (G = H / KV). A tile is `tile_rows` packed rows, a chunk `cp` pages of the sequence's keys, a unit one chunk of one tile
-// (and, in the grid's second dimension, one kv head). Every CTA works the units out from the step's description on the device,
-// so a captured launch serves whatever lengths its replays bring: cp is such that all units together are about `target`, and
-// the grid is sized for the most units that the step's rows can make (units() on the host). A sequence of many pages has many
-// chunks, a short one a single unit, whatever the other sequences are.
+// group (G = H / KV). A tile is `tile_rows` packed rows; an item is one tile against all keys it may see, for one kv head; its
+// length is the number of those keys' pages. All items of the step lie one behind the other (by sequence, kv head, tile) on a
+// line, and CTA c takes the `range` pages from c * range on, whatever items they belong to: every CTA has the same number of
+// pages, however ragged the batch. A piece of an item that a CTA has on its own is a segment. An item that one CTA has whole is
+// finished there; of the others every CTA leaves its segment's maximum, sum and unnormalised output in scratch (at most two a
+// CTA: one that began before its range, one that goes on behind it), and a second launch joins them.
+//
+// Everything is worked out on the device from the step's description, so a captured launch serves whatever lengths its replays
+// bring. Against chunks of equal pages per sequence, whose last chunks are short and whose number is no multiple of what the
+// device holds, equal ranges took 8 trees of 24 tokens behind 2,050 rows from 41 to TREE8 us and 16 of 64 behind 8,191 from 216
+// to TREE16 (with the smaller key tiles that came with them).
 #pragma once
 #include "layout.cuh"
 
@@ -14,18 +20,12 @@ struct RowsArgs {
     int T, B, H, KV, HD, G;
     int ldq, ldo;
     int tile_rows;                    // packed rows a tile
-    int min_pages;                    // pages a chunk at least
-    int target;                       // units to aim at, over all kv heads; 0: a tile's keys are never cut
+    int min_range;                    // pages a CTA at least
+    int ctas;                         // CTAs of the launch
     int causal;                       // 1: token i sees rows <= past + i; 0: the mask words
     int words;                        // mask words a token
     float scale_log2;                 // score scale * log2(e)
 };
-
-// Most units (of one kv head) that a step can make: tiles * ceil(pages / cp) <= tiles * pages / cp + tiles.
-static inline long long row_units_max(const RowsArgs& a) {
-    const long long tiles = ceil_div_ll((long long)a.T * a.G, a.tile_rows) + a.B;
-    return tiles + (a.target > 0 ? ceil_div(a.target, a.KV) : 0);
-}
 
 struct SeqShape {
     int q_begin, n_q, kvl, tiles, pages;
@@ -44,25 +44,59 @@ __device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, cons
         if (s.n_q != 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
         s.n_q = 0;
     }
-    s.tiles = (int)(((long long)s.n_q * a.G + a.tile_rows - 1) / a.tile_rows);
+    s.tiles = (s.n_q * a.G + a.tile_rows - 1) / a.tile_rows;
     s.pages = s.n_q > 0 ? (s.kvl + PAGE_TOKENS - 1) / PAGE_TOKENS : 0;
     return s;
 }
 
-struct RowUnit {
-    int b, tile, chunk;
-    int unit0;                        // the first unit of the sequence; unit0 + tile * seq_chunks + chunk is this one
-    int seq_chunks;                   // units a tile of this sequence has room for
-    int cp;                           // pages a chunk
+// Pages that some row of a tile may see: all, or up to the tile's last token.
+__device__ __forceinline__ int tile_pages(const SeqShape& s, int tile, const RowsArgs& a) {
+    if (!a.causal) return s.pages;
+    const int last = (min(s.n_q * a.G, (tile + 1) * a.tile_rows) - 1) / a.G;
+    return (s.kvl - s.n_q + last) / PAGE_TOKENS + 1;
+}
+
+// Pages of the sequence's tiles together, for one kv head.
+__device__ __forceinline__ long long seq_pages(const SeqShape& s, const RowsArgs& a) {
+    if (!a.causal || s.tiles <= 1) return (long long)s.tiles * s.pages;
+    long long n = 0;
+    for (int t = 0; t < s.tiles; t++) n += tile_pages(s, t, a);
+    return n;
+}
+
+// Where a CTA is on the line, and the segment it is at: pages [pg0, pg1) of item (b, g, tile).
+struct RowWalk {
+    int b, g, tile, pg0, pg1;
+    int item_pages;
+    long long left;                   // pages of the range that are left, this segment's among them
     SeqShape s;
 
     __device__ __forceinline__ int past() const { return s.kvl - s.n_q; }
     __device__ __forceinline__ int rows(const RowsArgs& a) const { return min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows); }
-    // pages that some row of the tile may see: all, or up to the tile's last token
-    __device__ __forceinline__ int tile_pages(const RowsArgs& a) const {
-        if (!a.causal) return s.pages;
-        const int last = (min(s.n_q * a.G, (tile + 1) * a.tile_rows) - 1) / a.G;
-        return (past() + last) / PAGE_TOKENS + 1;
+    __device__ __forceinline__ bool whole() const { return pg0 == 0 && pg1 == item_pages; }
+    // which of a CTA's two places in scratch a segment of a cut item takes
+    __device__ __forceinline__ int place() const { return pg0 > 0 ? 0 : 1; }
+    __device__ __forceinline__ void set(const RowsArgs& a) {
+        item_pages = tile_pages(s, tile, a);
+        pg1 = (int)min((long long)item_pages, pg0 + left);
+    }
+    // The next segment of the range; false when there is none.
+    __device__ __forceinline__ bool next(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, int* status) {
+        left -= pg1 - pg0;
+        if (left <= 0) return false;
+        pg0 = 0;
+        if (++tile == s.tiles) {
+            tile = 0;
+            if (++g == a.KV) {
+                g = 0;
+                do {
+                    if (++b >= a.B) return false;
+                    s = seq_shape(cu_q, kv_len, b, a, status);
+                } while (s.n_q == 0);
+            }
+        }
+        set(a);
+        return true;
     }
 };
 
@@ -71,74 +105,65 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-
-// Finds unit number `flat` (the units of a sequence lie together, its last tile first, so that the longest work of a causal step
-// starts first); false when the step has fewer. Warp 0 does the sums, 32 sequences at a time; every thread of the CTA must call
-// this (it synchronises the CTA).
-__device__ __forceinline__ bool find_row_unit(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, int flat,
-                                              RowUnit& u, int* status) {
-    __shared__ int found_s[4];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) {
-        int cp = 1 << 28;
-        if (a.target > 0) {
-            long long work = 0;
-            for (int b0 = 0; b0 < a.B; b0 += 32) {
-                const int b = b0 + lane;
-                if (b < a.B) {
-                    const SeqShape s = seq_shape(cu_q, kv_len, b, a, status);
-                    work += (long long)s.tiles * s.pages;
-                }
-            }
-            work = warp_sum_ll(work);
-            cp = (int)max((long long)a.min_pages, (work * a.KV + a.target - 1) / a.target);
-        }
-        int fb = -1, base = 0, first = 0;
-        for (int b0 = 0; b0 < a.B && fb < 0; b0 += 32) {
-            const int b = b0 + lane;
-            int n = 0;
-            if (b < a.B) {
-                const SeqShape s = seq_shape(cu_q, kv_len, b, a, status);
-                n = s.tiles * ((s.pages + cp - 1) / cp);
-            }
-            int incl = n;
+__device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {      // sum over the lanes up to this one
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            const int excl = incl - n;
-            const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && flat >= base + excl && flat < base + incl);
-            if (hit != 0u) {
-                const int src = __ffs(hit) - 1;
-                fb = b0 + src;
-                first = base + __shfl_sync(0xffffffffu, excl, src);
-            }
-            base += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (lane == 0) {
-            found_s[0] = fb;
-            found_s[1] = first;
-            found_s[2] = cp;
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
     }
-    __syncthreads();
-    u.b = found_s[0];
-    if (u.b < 0) return false;
-    u.unit0 = found_s[1];
-    u.cp = found_s[2];
-    u.s = seq_shape(cu_q, kv_len, u.b, a, status);
-    u.seq_chunks = (u.s.pages + u.cp - 1) / u.cp;
-    const int at = flat - u.unit0;
-    u.tile = u.s.tiles - 1 - at / u.seq_chunks;
-    u.chunk = at % u.seq_chunks;
-    return true;
+    return v;
 }
 
-// What a unit's CTA leaves for the merge, per sequence: where its units begin, their pages a chunk.
-struct RowInfo {
-    int unit0, cp;
-};
+// The start of this CTA's range, for one whole warp; `at` is set by lane 0 (b < 0: nothing to do). CTA 0 leaves where every
+// sequence begins on the line, and the range, for the second launch: info[b], info[B].
+__device__ __forceinline__ void find_range(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, RowWalk* at,
+                                           long long* info, int* status) {
+    const int lane = threadIdx.x & 31;
+    long long total = 0, own = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        own = 0;
+        if (b0 + lane < a.B) own = seq_pages(seq_shape(cu_q, kv_len, b0 + lane, a, status), a) * a.KV;
+        total += warp_sum_ll(own);
+    }
+    const long long range = max((long long)a.min_range, (total + a.ctas - 1) / a.ctas);
+    const long long from = range * blockIdx.x;
+    if (lane == 0) at->b = -1;
+    if (blockIdx.x == 0 && lane == 0) info[a.B] = range;
+    __syncwarp();
+    if (from >= total) return;
+    long long base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        if (a.B > 32) {                                        // (of up to 32 sequences every lane still has its own)
+            own = 0;
+            if (b0 + lane < a.B) own = seq_pages(seq_shape(cu_q, kv_len, b0 + lane, a, status), a) * a.KV;
+        }
+        const long long incl = warp_scan_ll(own, lane), excl = incl - own;
+        if (blockIdx.x == 0 && b0 + lane < a.B) info[b0 + lane] = base + excl;
+        if (own > 0 && from >= base + excl && from < base + incl) {
+            RowWalk w;
+            w.b = b0 + lane;
+            w.s = seq_shape(cu_q, kv_len, w.b, a, status);
+            const long long each = own / a.KV;
+            long long r = from - base - excl;
+            w.g = (int)(r / each);
+            r %= each;
+            if (a.causal) {
+                w.tile = 0;
+                for (int p; r >= (p = tile_pages(w.s, w.tile, a)); w.tile++) r -= p;
+            } else {
+                w.tile = (int)(r / w.s.pages);
+                r %= w.s.pages;
+            }
+            w.pg0 = (int)r;
+            w.left = range;
+            w.set(a);
+            *at = w;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+        if (blockIdx.x != 0 && from < base) break;
+    }
+    __syncwarp();
+}
 
 // Which of the 64 keys from key0 (a multiple of 64) on token `tok` of a sequence sees: bit e for key key0 + e. Held rows (below
 // past) are seen by all; of the step's own rows, those up to the token's own (causal), or those whose bits are set in the
