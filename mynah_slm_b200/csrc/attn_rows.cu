@@ -266,23 +266,24 @@ attn_rows_merge_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const 
     const int pr = (t - s.q_begin) * a.G + h % a.G, tile = pr / a.tile_rows;
     if (pr < 0 || tile >= s.tiles) return;
     // where the item lies on the line, and the CTAs that had a part of it
-    long long from, pages = tile_pages(s, tile, a);
-    if (a.causal && s.tiles > 1) {
+    const int item = tile / a.group, items = seq_items(s, a);
+    long long from;
+    if (a.causal && items > 1) {
         long long all = 0, before = 0;
-        for (int i = lane; i < s.tiles; i += 32) {
-            const int p = tile_pages(s, i, a);
+        for (int i = lane; i < items; i += 32) {
+            const int p = item_pages(s, i, a);
             all += p;
-            if (i < tile) before += p;
+            if (i < item) before += p;
         }
         from = warp_sum_ll(all) * g + warp_sum_ll(before);
     } else {
-        from = ((long long)g * s.tiles + tile) * s.pages;
+        from = ((long long)g * items + item) * s.pages;
     }
     from += sc.info[lo];
     const long long range = sc.info[a.B], c0 = from / range;
-    const int n = (int)((from + pages - 1) / range - c0) + 1;
-    if (n <= 1) return;
-    auto at = [&](int c) { return ((c0 + c) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + pr % a.tile_rows; };
+    const int n = (int)((from + tile_pages(s, tile, a) - 1) / range - c0) + 1;
+    if (n <= 1) return;                                            // not cut
+    auto at = [&](int c) { return (((c0 + c) * a.group + tile % a.group) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + pr % a.tile_rows; };
     float mx = -INFINITY;
     for (int c = lane; c < n; c += 32) mx = fmaxf(mx, sc.ml[at(c)].x);
     mx = warp_max(mx);
@@ -323,7 +324,7 @@ int go(const void* q, void* out, const RowsArgs& a, const void* k, const void* v
     auto kern = attn_rows_kernel<T, TY, TX, NC>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
-    kern<<<a.ctas, TY * TX, smem, stream>>>((const T*)q, (T*)out, (const T*)k, (const T*)v, cu_q, kv_len, pt, masks, a, s, status);
+    kern<<<a.ctas * a.group, TY * TX, smem, stream>>>((const T*)q, (T*)out, (const T*)k, (const T*)v, cu_q, kv_len, pt, masks, a, s, status);
     return mynah_check_launch("attn_rows");
 }
 
@@ -344,11 +345,11 @@ int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void*
 }  // namespace
 
 long long rows_scratch_floats(const RowsArgs& a) {
-    return 2ll * a.ctas * a.tile_rows * (a.HD + 2) + 2ll * (a.B + 1) + 4;
+    return 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2) + 2ll * (a.B + 1) + 4;
 }
 
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
-    const long long rows = 2ll * a.ctas * a.tile_rows;
+    const long long rows = 2ll * a.ctas * a.group * a.tile_rows;
     RowsScratch s;
     s.o = scratch;                                                 // 16-byte rows first
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
@@ -366,6 +367,16 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     }
     a.min_range = 2;
     a.ctas = 2 * mynah_sm_count();                                 // both kernels have two CTAs an SM
+    a.group = 1;
+    if (tc) {
+        // As many tiles side by side as the step's sequences have on average (a sequence of fewer leaves CTAs idle), up to 8. Prompts
+        // of many tiles are bound by their products and their pages stay in L2 anyway: one by one.
+        const long long rows = (long long)a.T * a.G, each = (long long)a.B * a.tile_rows;
+        const long long most = ((long long)max_q_len * a.G + a.tile_rows - 1) / a.tile_rows, mean = (rows + each / 2) / each;
+        a.group = (int)(mean <= 1 || (a.causal && mean > 8) ? 1 : mean > 8 ? 8 : mean);
+        if (a.group > most && most >= 1) a.group = (int)most;
+        a.ctas /= a.group;
+    }
     return tc;
 }
 

@@ -372,7 +372,7 @@ int go(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cons
     auto kern = attn_rows_tcgen05_kernel<HD>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
-    kern<<<a.ctas, THREADS, smem, stream>>>(mq, mk, mv, (const bf16*)v, cu_q, kv_len, pt, masks, a, (bf16*)out, s, status);
+    kern<<<a.ctas * a.group, THREADS, smem, stream>>>(mq, mk, mv, (const bf16*)v, cu_q, kv_len, pt, masks, a, (bf16*)out, s, status);
     return mynah_check_launch("attn_rows");
 }
 

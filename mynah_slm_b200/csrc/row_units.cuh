@@ -10,7 +10,9 @@
 // CTA: one that began before its range, one that goes on behind it), and a second launch joins them.
 //
 // Everything is worked out on the device from the step's description, so a captured launch serves whatever lengths its replays
-// bring. Against chunks of equal pages per sequence, whose last chunks are short and whose number is no multiple of what the
+// bring. Where sequences have several tiles, `group` CTAs side by side take the same pages for `group` tiles (an item is then
+// that many tiles), so that a page comes from memory once and from L2 for the others: 16 trees of 64 tokens with four heads a kv
+// head (two tiles each) behind 8,191 rows read 1.05 GB one tile after the other, 0.54 GB together. Against chunks of equal pages per sequence, whose last chunks are short and whose number is no multiple of what the
 // device holds, equal ranges took 8 trees of 24 tokens behind 2,050 rows from 41 to TREE8 us and 16 of 64 behind 8,191 from 216
 // to TREE16 (with the smaller key tiles that came with them).
 #pragma once
@@ -21,7 +23,8 @@ struct RowsArgs {
     int ldq, ldo;
     int tile_rows;                    // packed rows a tile
     int min_range;                    // pages a CTA at least
-    int ctas;                         // CTAs of the launch
+    int ctas;                         // ranges that the line is cut into; the launch has ctas * group CTAs
+    int group;                        // tiles an item, each a CTA's
     int causal;                       // 1: token i sees rows <= past + i; 0: the mask words
     int words;                        // mask words a token
     float scale_log2;                 // score scale * log2(e)
@@ -56,46 +59,60 @@ __device__ __forceinline__ int tile_pages(const SeqShape& s, int tile, const Row
     return (s.kvl - s.n_q + last) / PAGE_TOKENS + 1;
 }
 
-// Pages of the sequence's tiles together, for one kv head.
+__device__ __forceinline__ int seq_items(const SeqShape& s, const RowsArgs& a) { return (s.tiles + a.group - 1) / a.group; }
+// Pages of an item: of its last tile, which sees the most.
+__device__ __forceinline__ int item_pages(const SeqShape& s, int item, const RowsArgs& a) {
+    return tile_pages(s, min(s.tiles, (item + 1) * a.group) - 1, a);
+}
+// Pages of the sequence's items together, for one kv head.
 __device__ __forceinline__ long long seq_pages(const SeqShape& s, const RowsArgs& a) {
-    if (!a.causal || s.tiles <= 1) return (long long)s.tiles * s.pages;
+    const int items = seq_items(s, a);
+    if (!a.causal || items <= 1) return (long long)items * s.pages;
     long long n = 0;
-    for (int t = 0; t < s.tiles; t++) n += tile_pages(s, t, a);
+    for (int i = 0; i < items; i++) n += item_pages(s, i, a);
     return n;
 }
 
-// Where a CTA is on the line, and the segment it is at: pages [pg0, pg1) of item (b, g, tile).
+// Where a CTA is on the line, and the segment it is at: pages [pg0, pg1) of one tile of item (b, g, item).
 struct RowWalk {
-    int b, g, tile, pg0, pg1;
-    int item_pages;
+    int b, g, item, tile, pg0, pg1;
+    int from, to;                     // the item's pages in this range
+    int pages;                        // that the tile may see
     long long left;                   // pages of the range that are left, this segment's among them
     SeqShape s;
 
     __device__ __forceinline__ int past() const { return s.kvl - s.n_q; }
     __device__ __forceinline__ int rows(const RowsArgs& a) const { return min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows); }
-    __device__ __forceinline__ bool whole() const { return pg0 == 0 && pg1 == item_pages; }
+    __device__ __forceinline__ bool whole() const { return pg0 == 0 && pg1 == pages; }
     // which of a CTA's two places in scratch a segment of a cut item takes
-    __device__ __forceinline__ int place() const { return pg0 > 0 ? 0 : 1; }
-    __device__ __forceinline__ void set(const RowsArgs& a) {
-        item_pages = tile_pages(s, tile, a);
-        pg1 = (int)min((long long)item_pages, pg0 + left);
+    __device__ __forceinline__ int place() const { return from > 0 ? 0 : 1; }
+    // Whether this CTA has a part of the item at `from`: its tile exists and sees a page of the range.
+    __device__ __forceinline__ bool set(const RowsArgs& a) {
+        to = (int)min((long long)item_pages(s, item, a), from + left);
+        tile = a.group == 1 ? item : item * a.group + (int)blockIdx.x % a.group;
+        if (tile >= s.tiles) return false;
+        pages = tile_pages(s, tile, a);
+        pg0 = from;
+        pg1 = min(to, pages);
+        return pg0 < pg1;
     }
     // The next segment of the range; false when there is none.
     __device__ __forceinline__ bool next(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, int* status) {
-        left -= pg1 - pg0;
-        if (left <= 0) return false;
-        pg0 = 0;
-        if (++tile == s.tiles) {
-            tile = 0;
-            if (++g == a.KV) {
-                g = 0;
-                do {
-                    if (++b >= a.B) return false;
-                    s = seq_shape(cu_q, kv_len, b, a, status);
-                } while (s.n_q == 0);
+        do {
+            left -= to - from;
+            if (left <= 0) return false;
+            from = 0;
+            if (++item == seq_items(s, a)) {
+                item = 0;
+                if (++g == a.KV) {
+                    g = 0;
+                    do {
+                        if (++b >= a.B) return false;
+                        s = seq_shape(cu_q, kv_len, b, a, status);
+                    } while (s.n_q == 0);
+                }
             }
-        }
-        set(a);
+        } while (!set(a));
         return true;
     }
 };
@@ -114,7 +131,7 @@ __device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {      
     return v;
 }
 
-// The start of this CTA's range, for one whole warp; `at` is set by lane 0 (b < 0: nothing to do). CTA 0 leaves where every
+// The start of this CTA's range, for one whole warp, into `at` (b < 0: nothing to do). CTA 0 leaves where every
 // sequence begins on the line, and the range, for the second launch: info[b], info[B].
 __device__ __forceinline__ void find_range(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, RowWalk* at,
                                            long long* info, int* status) {
@@ -126,7 +143,7 @@ __device__ __forceinline__ void find_range(const int* __restrict__ cu_q, const i
         total += warp_sum_ll(own);
     }
     const long long range = max((long long)a.min_range, (total + a.ctas - 1) / a.ctas);
-    const long long from = range * blockIdx.x;
+    const long long from = range * (blockIdx.x / a.group);
     if (lane == 0) at->b = -1;
     if (blockIdx.x == 0 && lane == 0) info[a.B] = range;
     __syncwarp();
@@ -148,16 +165,15 @@ __device__ __forceinline__ void find_range(const int* __restrict__ cu_q, const i
             w.g = (int)(r / each);
             r %= each;
             if (a.causal) {
-                w.tile = 0;
-                for (int p; r >= (p = tile_pages(w.s, w.tile, a)); w.tile++) r -= p;
+                w.item = 0;
+                for (int p; r >= (p = item_pages(w.s, w.item, a)); w.item++) r -= p;
             } else {
-                w.tile = (int)(r / w.s.pages);
+                w.item = (int)(r / w.s.pages);
                 r %= w.s.pages;
             }
-            w.pg0 = (int)r;
+            w.from = (int)r;
             w.left = range;
-            w.set(a);
-            *at = w;
+            if (w.set(a) || w.next(cu_q, kv_len, a, status)) *at = w;
         }
         base += __shfl_sync(0xffffffffu, incl, 31);
         if (blockIdx.x != 0 && from < base) break;
