@@ -158,7 +158,7 @@ long long mass_scratch(const MassArgs& a, int n_ids) {
 
 }  // namespace
 
-MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype);
+long long attn_rows_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int causal);
 
 // Floats of scratch for mynah_attn_mass, whichever kernels take the call.
 MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int n_ids) {
@@ -171,7 +171,7 @@ MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, 
         const long long n = mass_scratch(a, n_ids);
         if (n > need) need = n;
     }
-    return ((mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dtype) + 3) & ~3ll) + need;
+    return attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1) + need;
 }
 
 // As mynah_attn_tree with causal rows, and mass [n_pages, KV, 64] fp32. n_ids: entries of page_ids (no fewer than the
@@ -195,7 +195,7 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
     const bool tc = mass_plan(a, dtype, aligned, max_q_len);
     const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids);
     MYNAH_REQUIRE(scratch_floats >= need, "attn_mass: scratch holds %lld floats, %lld are needed", scratch_floats, need);
-    const long long attn = (mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dtype) + 3) & ~3ll;
+    const long long attn = attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1);
     float* lse = scratch + attn;
     float* part = lse + (((long long)T * H + 3) & ~3ll);
     const PageTable pt{page_indptr, page_ids, page_base, n_pages};

@@ -54,7 +54,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     __shared__ int bad_s;
     __shared__ RowWalk walk_s;
 
-    if (threadIdx.x < 32) find_range(cu_q, kv_len, a, &walk_s, sc.info, status);
+    if (threadIdx.x < 32) find_range(cu_q, kv_len, a, &walk_s, sc.starts, status);
     __syncthreads();
     RowWalk u = walk_s;
     if (u.b < 0) return;
@@ -245,75 +245,61 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     } while (u.next(cu_q, kv_len, a, status));
 }
 
-// Joins the segments of a cut item: with M = max m_c, out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c. A warp a row; rows
-// of items that were not cut have their output already.
+// Joins the segments of a cut item: with M = max m_c, out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c. Range c's CTAs
+// (blockIdx.x = c) take the item that the range begins inside of, if the item's first pages are in the range before (each cut
+// item has one such range). A warp a row; JOIN_CTAS CTAs share an item's rows. Few numbers and short chains of loads: it is
+// bound by its launch and three dependent reads (where the range begins, the segments' maxima, their rows, from L2).
+constexpr int JOIN_CTAS = 8, JOIN_WARPS = 4;
 template <typename T>
-__global__ void __launch_bounds__(128)
-attn_rows_merge_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, RowsArgs a, RowsScratch sc,
-                       int* __restrict__ status) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32)
+attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, RowsArgs a, RowsScratch sc,
+                      int* __restrict__ status) {
     griddep_wait();
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= (long long)a.T * a.H) return;
-    const int t = (int)(row / a.H), h = (int)(row % a.H), g = h / a.G;
-    if (t >= cu_q[a.B]) return;                                    // a row behind the last sequence
-    int lo = 0, hi = a.B;                                          // the last sequence that begins at or before t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (cu_q[mid] <= t) lo = mid; else hi = mid;
-    }
-    const SeqShape s = seq_shape(cu_q, kv_len, lo, a, status);
-    const int pr = (t - s.q_begin) * a.G + h % a.G, tile = pr / a.tile_rows;
-    if (pr < 0 || tile >= s.tiles) return;
-    // where the item lies on the line, and the CTAs that had a part of it
-    const int item = tile / a.group, items = seq_items(s, a);
-    long long from;
-    if (a.causal && items > 1) {
-        long long all = 0, before = 0;
-        for (int i = lane; i < items; i += 32) {
-            const int p = item_pages(s, i, a);
-            all += p;
-            if (i < item) before += p;
+    const int cta = blockIdx.x / a.group + 1, sub = blockIdx.x % a.group;       // (range 0 begins inside of nothing)
+    const RowStart at = sc.starts[cta];
+    const int range = sc.starts[a.ctas].from;
+    if (at.b < 0 || at.from == 0 || at.from > range) return;
+    const SeqShape s = seq_shape(cu_q, kv_len, at.b, a, status);
+    const int tile = at.item * a.group + sub;
+    if (tile >= s.tiles) return;
+    const int pages = tile_pages(s, tile, a);
+    if (pages <= at.from) return;                                  // this tile ends before the cut: it was whole
+    const int n = 2 + (pages - at.from - 1) / range;               // segments
+    const int lane = threadIdx.x & 31, rows = min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows);
+    for (int row = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5); row < rows; row += JOIN_CTAS * JOIN_WARPS) {
+        const int pr = tile * a.tile_rows + row, t = s.q_begin + pr / a.G, h = at.g * a.G + pr % a.G;
+        auto slot = [&](int c) { return ((long long)((cta - 1 + c) * a.group + sub) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + row; };
+        float mx = -INFINITY;
+        for (int c = lane; c < n; c += 32) mx = fmaxf(mx, sc.ml[slot(c)].x);
+        mx = warp_max(mx);
+        const float m_use = mx == -INFINITY ? 0.f : mx;
+        float l = 0.f;
+        for (int c = lane; c < n; c += 32) {
+            const float2 ml = sc.ml[slot(c)];
+            l += ml.y * exp2f(ml.x - m_use);
         }
-        from = warp_sum_ll(all) * g + warp_sum_ll(before);
-    } else {
-        from = ((long long)g * items + item) * s.pages;
-    }
-    from += sc.info[lo];
-    const long long range = sc.info[a.B], c0 = from / range;
-    const int n = (int)((from + tile_pages(s, tile, a) - 1) / range - c0) + 1;
-    if (n <= 1) return;                                            // not cut
-    auto at = [&](int c) { return (((c0 + c) * a.group + tile % a.group) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + pr % a.tile_rows; };
-    float mx = -INFINITY;
-    for (int c = lane; c < n; c += 32) mx = fmaxf(mx, sc.ml[at(c)].x);
-    mx = warp_max(mx);
-    const float m_use = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f;
-    for (int c = lane; c < n; c += 32) {
-        const float2 ml = sc.ml[at(c)];
-        l += ml.y * exp2f(ml.x - m_use);
-    }
-    l = warp_sum(l);
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    for (int col = lane * 4; col < a.HD; col += 128) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = warp_sum(l);
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a NaN stays one
+        for (int col = lane * 4; col < a.HD; col += 128) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int c = 0; c < n; c++) {
-            const long long i = at(c);
-            const float w = exp2f(sc.ml[i].x - m_use);
-            const float4 y = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
-            x.x = fmaf(w, y.x, x.x);
-            x.y = fmaf(w, y.y, x.y);
-            x.z = fmaf(w, y.z, x.z);
-            x.w = fmaf(w, y.w, x.w);
+            for (int c = 0; c < n; c++) {
+                const long long i = slot(c);
+                const float w = exp2f(sc.ml[i].x - m_use);
+                const float4 y = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
+                x.x = fmaf(w, y.x, x.x);
+                x.y = fmaf(w, y.y, x.y);
+                x.z = fmaf(w, y.z, x.z);
+                x.w = fmaf(w, y.w, x.w);
+            }
+            T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
+            o[0] = from_f32<T>(x.x * inv);
+            o[1] = from_f32<T>(x.y * inv);
+            o[2] = from_f32<T>(x.z * inv);
+            o[3] = from_f32<T>(x.w * inv);
         }
-        T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
-        o[0] = from_f32<T>(x.x * inv);
-        o[1] = from_f32<T>(x.y * inv);
-        o[2] = from_f32<T>(x.z * inv);
-        o[3] = from_f32<T>(x.w * inv);
+        if (lane == 0 && sc.lse != nullptr) sc.lse[((size_t)at.g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m_use + log2f(l);
     }
-    if (lane == 0 && sc.lse != nullptr) sc.lse[((size_t)g * a.T + t) * a.G + h % a.G] = l == 0.f ? -INFINITY : m_use + log2f(l);
 }
 
 template <typename T, int TY, int TX, int NC>
@@ -345,7 +331,7 @@ int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void*
 }  // namespace
 
 long long rows_scratch_floats(const RowsArgs& a) {
-    return 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2) + 2ll * (a.B + 1) + 4;
+    return 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2) + 4ll * (a.ctas + 1);
 }
 
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
@@ -353,28 +339,33 @@ RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
     RowsScratch s;
     s.o = scratch;                                                 // 16-byte rows first
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
-    s.info = reinterpret_cast<long long*>(scratch + rows * (a.HD + 2));
+    s.starts = reinterpret_cast<RowStart*>(scratch + rows * (a.HD + 2));
     s.lse = lse;
     return s;
 }
 
 bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     const bool tc = aligned && rows_tcgen05_takes(dtype, a.H, a.KV, a.HD);
-    if (tc) {
-        a.tile_rows = 128 / a.G * a.G;
-    } else {
-        a.tile_rows = (long long)max_q_len * a.G <= 16 ? 16 : 64;
-    }
     a.min_range = 2;
-    a.ctas = 2 * mynah_sm_count();                                 // both kernels have two CTAs an SM
     a.group = 1;
-    if (tc) {
-        // As many tiles side by side as the step's sequences have on average (a sequence of fewer leaves CTAs idle), up to 8. Prompts
-        // of many tiles are bound by their products and their pages stay in L2 anyway: one by one.
-        const long long rows = (long long)a.T * a.G, each = (long long)a.B * a.tile_rows;
-        const long long most = ((long long)max_q_len * a.G + a.tile_rows - 1) / a.tile_rows, mean = (rows + each / 2) / each;
-        a.group = (int)(mean <= 1 || (a.causal && mean > 8) ? 1 : mean > 8 ? 8 : mean);
-        if (a.group > most && most >= 1) a.group = (int)most;
+    a.two = 0;
+    a.ctas = 2 * mynah_sm_count();                                 // two CTAs an SM
+    if (!tc) {
+        a.tile_rows = (long long)max_q_len * a.G <= 16 ? 16 : 64;
+        return false;
+    }
+    a.tile_rows = 128 / a.G * a.G;
+    // Tiles that the step's sequences have on average. From one and a half on a CTA takes two; beyond that as many side by side
+    // as there are (up to eight; a sequence of fewer leaves CTAs idle). Prompts of many tiles are bound by their products and
+    // their pages stay in L2 anyway: one item after the other.
+    const long long rows = (long long)a.T * a.G, each = (long long)a.B * a.tile_rows;
+    if ((long long)max_q_len * a.G > a.tile_rows && 2 * rows >= 3 * each) {
+        a.two = 1;
+        a.tile_rows *= 2;
+        a.ctas /= 2;
+        const long long most = ((long long)max_q_len * a.G + a.tile_rows - 1) / a.tile_rows, mean = (rows + each) / (2 * each);
+        a.group = (int)(mean <= 1 || (a.causal && mean > 4) ? 1 : mean > 4 ? 4 : mean);
+        if (a.group > most) a.group = (int)most;
         a.ctas /= a.group;
     }
     return tc;
@@ -386,29 +377,32 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
     return pick<bf16>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
 }
 
-int launch_rows_merge(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, RowsScratch s, int* status,
-                      cudaStream_t stream) {
-    const long long rows = (long long)a.T * a.H;
-    const dim3 grid((unsigned)((rows + 3) / 4));
+int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, RowsScratch s, int* status,
+                     cudaStream_t stream) {
+    if (a.ctas <= 1) return 0;                                     // one range: nothing is cut
+    const dim3 grid((a.ctas - 1) * a.group, JOIN_CTAS), block(JOIN_WARPS * 32);
     const cudaError_t e = dtype == MYNAH_F32
-        ? launch_behind(attn_rows_merge_kernel<float>, grid, dim3(128), 0, stream, (float*)out, cu_q, kv_len, a, s, status)
-        : launch_behind(attn_rows_merge_kernel<bf16>, grid, dim3(128), 0, stream, (bf16*)out, cu_q, kv_len, a, s, status);
-    if (e != cudaSuccess) return mynah_fail("attn_rows_merge: %s", cudaGetErrorString(e));
-    return mynah_check_launch("attn_rows_merge");
+        ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, a, s, status)
+        : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, a, s, status);
+    if (e != cudaSuccess) return mynah_fail("attn_rows_join: %s", cudaGetErrorString(e));
+    return mynah_check_launch("attn_rows_join");
 }
 
-// Floats of scratch for mynah_attn_tree, whichever kernel takes the call.
-MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype) {
+// Floats of scratch for the attention, whichever kernel takes the call.
+long long attn_rows_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int causal) {
     if (T <= 0 || B <= 0 || KV <= 0 || H % KV != 0 || H <= 0 || HD <= 0) return 0;
     long long need = 0;
     for (int aligned = 0; aligned < 2; aligned++) {
         RowsArgs a{};
-        a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = H / KV;
+        a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = H / KV, a.causal = causal;
         rows_plan(a, dtype, max_q_len, aligned != 0);
         const long long n = rows_scratch_floats(a);
         if (n > need) need = n;
     }
-    return need;
+    return (need + 3) & ~3ll;
+}
+MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype) {
+    return attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 0);
 }
 
 // What mynah_attn_tree and mynah_attn_mass check and launch alike.
@@ -431,7 +425,7 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
     const int rc = tc ? launch_rows_tcgen05(q, out, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream)
                       : launch_rows_generic(q, out, dtype, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream);
     if (rc != 0) return rc;
-    return launch_rows_merge(out, dtype, a, cu_q, kv_len, s, status, stream);
+    return launch_rows_join(out, dtype, a, cu_q, kv_len, s, status, stream);
 }
 
 // q [T, ldq] and out [T, ldo], head h in columns [h * HD, (h + 1) * HD); k_cache, v_cache [n_pages, KV, 64, HD], which hold the

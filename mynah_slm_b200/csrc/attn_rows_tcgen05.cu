@@ -4,16 +4,20 @@
 //
 //   warp 0     one lane brings a tile's queries (a box of 64 columns x the group's heads x the tile's tokens lands as the packed
 //              rows) and the pages' K and V with TMA (128-byte swizzle), in rings that run on from segment to segment;
-//   warp 1     one lane issues tcgen05.mma: S = Q.K^T into tensor memory (two buffers), and O += P.V with P read from tensor
-//              memory and V as an MN-major operand in shared memory;
-//   warps 2-5  the softmax, a thread a row: 64 scores in registers, O rescaled only when the reference maximum has to grow by
+//   warp 1     issues S = Q.K^T into tensor memory (two buffers),
+//   warp 2     O += P.V, P read from tensor memory and V as an MN-major operand in shared memory: two warps, because an issuer
+//              that waits for weights keeps the tensor cores from the next scores (one warp for both took 2,200 clocks a page of
+//              two tiles, these TWOWARPS). Both run whole, with one elected lane at the instructions: under `lane == 0` every
+//              descriptor went through vector registers and a product took 85 clocks to issue, under elect.sync 55;
+//   warps 3-6  the softmax, a thread a row: 64 scores in registers, O rescaled only when the reference maximum has to grow by
 //              more than 2^8, weights written back over the scores as bfloat16 (half a step is lost, as much as the output's own
 //              rounding loses; their sum is of the unrounded ones in fp32). Warps whose rows do not exist only keep step.
 //
-// Two CTAs an SM (98 KB of tiles, 256 columns of tensor memory each): one's softmax runs under the other's products and its
-// start and end under the other's pages. Bound by the bytes of K and V while a tile has few rows; a page takes the tensor cores
-// about 640 clocks whatever the rows (Q.K^T of 64 columns waits for shared memory), the exponentials of 128 rows 512, its share
-// of the memory's time is 1,400.
+// NT = 1: one tile, two CTAs an SM (98 KB and 256 columns of tensor memory each): one's softmax runs under the other's products
+// and its start and end under the other's pages. NT = 2: two tiles of 128 rows on the same pages, with warps 7-10 for the second,
+// one CTA an SM: a page is brought into shared memory once for 256 rows. Bound by the bytes of K and V while there are few rows;
+// a page takes the tensor cores about 640 clocks a tile whatever its rows (Q.K^T of 64 columns waits for shared memory), the
+// exponentials of 128 rows 512, its share of the memory's time is 1,400.
 //
 // A key that a row must not see gets the score -inf by a select, so its K cannot matter. Its V could: a weight of zero times a
 // NaN is a NaN. So in pages where some row does not see some key the values are looked through: rows that nobody sees are
@@ -32,65 +36,66 @@ using namespace tc5;
 
 constexpr int BQ = 128;               // packed rows a tile at most (the lanes of tensor memory)
 constexpr int KEYS = PAGE_TOKENS;     // keys a step
-constexpr int THREADS = 192;
-template <int HD> constexpr int STAGES = HD == 128 ? 2 : 4;          // of K and of V
+template <int HD, int NT> constexpr int STAGES = HD == 128 ? 2 * NT : 4 * NT;       // of K and of V
 
 // Which of two packed bfloat16 are not finite, as a mask over their bits.
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
     return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(THREADS, 2)
+template <int HD, int NT>
+__global__ void __launch_bounds__(96 + 128 * NT, 3 - NT)
 attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const bf16* __restrict__ v_cache, const int* __restrict__ cu_q,
                          const int* __restrict__ kv_len, PageTable pt, const long long* __restrict__ masks, RowsArgs a,
                          bf16* __restrict__ out, RowsScratch sc, int* __restrict__ status) {
-    constexpr int HALVES = HD / 64, NS = STAGES<HD>;
+    constexpr int HALVES = HD / 64, NS = STAGES<HD, NT>;
     constexpr int PAGE_TILE = HALVES * PAGE_BYTES;             // one page of K or of V
-    constexpr int TMEM_COLS = 256, O_COL = 2 * KEYS;           // two score buffers, the output behind them
+    constexpr int TMEM_COLS = 256 * NT, O_COL = 2 * KEYS * NT; // two score buffers a tile, the outputs behind them
+    constexpr int Q_TILE = HALVES * HALF_BYTES;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* q_s = smem;
-    unsigned char* k_s = q_s + HALVES * HALF_BYTES;            // NS stages
+    unsigned char* k_s = q_s + NT * Q_TILE;                    // NS stages
     unsigned char* v_s = k_s + NS * PAGE_TILE;                 // NS stages
     uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + NS * PAGE_TILE);
-    const uint32_t k_full = smem_u32(bars), v_full = smem_u32(bars + 4), k_free = smem_u32(bars + 8), v_free = smem_u32(bars + 12);   // [NS]
-    const uint32_t s_full = smem_u32(bars + 16), p_full = smem_u32(bars + 18);       // [2]: scores ready, weights ready
-    const uint32_t q_full = smem_u32(bars + 20), q_free = smem_u32(bars + 21);       // once a segment
-    const uint32_t o_done = smem_u32(bars + 22);               // once a page: the output has it
-    const uint32_t o_last = smem_u32(bars + 23), o_free = smem_u32(bars + 24);       // once a segment: output whole, output read
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-    int* flags = reinterpret_cast<int*>(bars + 26);            // [0], [1]: 1 + the last segment (even, odd) in which a value that is
+    const uint32_t k_full = smem_u32(bars), v_full = smem_u32(bars + 8), k_free = smem_u32(bars + 16), v_free = smem_u32(bars + 24);   // [NS]
+    const uint32_t s_full = smem_u32(bars + 32), p_full = smem_u32(bars + 36);       // [NT][2]: scores ready, weights ready
+    const uint32_t q_full = smem_u32(bars + 40), q_free = smem_u32(bars + 41);       // once a segment
+    const uint32_t p_free = smem_u32(bars + 42);               // [NT][2]: the output has the page, its buffer is free
+    const uint32_t o_free = smem_u32(bars + 46);               // once a segment: the outputs have been read
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 47);
+    int* flags = reinterpret_cast<int*>(bars + 48);            // [0], [1]: 1 + the last segment (even, odd) in which a value that is
                                                                // not finite was zeroed; [2 .. 9]: the same for missing pages, by
                                                                // segment % 8 (the producer is up to three segments ahead)
     __shared__ RowWalk walk_s;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        find_range(cu_q, kv_len, a, &walk_s, sc.info, status);
+        find_range(cu_q, kv_len, a, &walk_s, sc.starts, status);
     } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else if (threadIdx.x == 64) {
+    } else if (threadIdx.x == 96) {
         for (int i = 0; i < NS; i++) {
             mbar_init(k_full + 8 * i, 1);
             mbar_init(v_full + 8 * i, 1);
             mbar_init(k_free + 8 * i, 1);
             mbar_init(v_free + 8 * i, 1);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 2 * NT; i++) {
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 4);                      // one arrival per softmax warp
+            mbar_init(p_full + 8 * i, 4);                      // one arrival per softmax warp of the tile
+            mbar_init(p_free + 8 * i, 1);
         }
         mbar_init(q_full, 1);
         mbar_init(q_free, 1);
-        mbar_init(o_done, 1);
-        mbar_init(o_last, 1);
-        mbar_init(o_free, 4);
+        mbar_init(o_free, 4 * NT);
         for (int i = 0; i < 10; i++) flags[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
+    } else if (threadIdx.x == 64) {
+        for (const CUtensorMap* m : {&map_q, &map_k, &map_v}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -98,8 +103,10 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t tmem_base = *tmem_slot;
     RowWalk u = walk_s;
     const bool any = u.b >= 0;
+    const int tile_rows = a.tile_rows / NT;                    // of one tile; a tile exists if the CTA's rows reach it
 
-    // Page number i of the CTA (over all segments) uses stage i % NS of K and V, in that stage's use i / NS, and score buffer i & 1.
+    // Page number i of the CTA (over all segments) uses stage i % NS of K and V, in that stage's use i / NS; the pages of a tile number
+    // c use its score buffer c & 1.
     if (warp == 0) {
         if (lane == 0 && any) {                                // ---- TMA producer
             int i = 0, seg = 0, k_issued = 0, v_issued = 0, q_issued = 0;
@@ -122,10 +129,13 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     k_issued = i + 1;
                     if (p == u.pg0) {
                         if (seg > 0 && !mbar_wait(q_free, (seg - 1) & 1)) { ok = false; break; }
-                        mbar_expect_tx(q_full, HALVES * a.tile_rows * 128);
+                        const int nt = NT == 1 || u.rows(a) <= tile_rows ? 1 : NT;
+                        mbar_expect_tx(q_full, nt * HALVES * tile_rows * 128);
+                        for (int x = 0; x < nt; x++)
 #pragma unroll
-                        for (int hf = 0; hf < HALVES; hf++)
-                            tma_load_3d(smem_u32(q_s + hf * HALF_BYTES), &map_q, hf * 64, u.g * a.G, u.s.q_begin + u.tile * a.tile_rows / a.G, q_full);
+                            for (int hf = 0; hf < HALVES; hf++)
+                                tma_load_3d(smem_u32(q_s + x * Q_TILE + hf * HALF_BYTES), &map_q, hf * 64, u.g * a.G,
+                                            u.s.q_begin + (u.tile * a.tile_rows + x * tile_rows) / a.G, q_full);
                         q_issued = seg + 1;
                     }
                     if (i >= NS && !mbar_wait(v_free + 8 * st, prev)) { ok = false; break; }
@@ -144,74 +154,109 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int j = max(0, v_issued - NS); j < v_issued; j++) mbar_wait(v_full + 8 * (j % NS), (j / NS) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0 && any) {                                // ---- MMA issuer
-            constexpr uint32_t idesc_s = idesc(KEYS, false), idesc_o = idesc(HD, true);
-            const uint32_t t_o = tmem_base + O_COL;
-            const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
-            auto scores = [&](int i, bool last) {              // S[i & 1] = Q . K_i^T
-                const int st = i % NS;
-#pragma unroll
-                for (int k = 0; k < HD / 16; k++)
-                    tc_mma(tmem_base + (i & 1) * KEYS, desc_k_major(q_addr + (k / 4) * HALF_BYTES + (k % 4) * 32),
-                           desc_k_major(k_addr + st * PAGE_TILE + (k / 4) * PAGE_BYTES + (k % 4) * 32), idesc_s, k != 0);
-                tc_commit(s_full + 8 * (i & 1));
-                tc_commit(k_free + 8 * st);
-                if (last) tc_commit(q_free);
-            };
+        if (any) {                                             // ---- scores: S = Q . K^T
+            constexpr uint32_t idesc_s = idesc(KEYS, false);
+            const bool leader = elect_one();
+            const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s);
+            int c[NT] = {};                                    // pages of each tile so far
             int i = 0, seg = 0;
             bool ok = true;
             do {
-                const int n = u.pg1 - u.pg0;
-                ok = mbar_wait(q_full, seg & 1) && mbar_wait(k_full + 8 * (i % NS), (i / NS) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                scores(i, n == 1);
-                for (int j = 0; j < n; j++, i++) {
+                const int n = u.pg1 - u.pg0, nt = NT == 1 || u.rows(a) <= tile_rows ? 1 : NT;
+                ok = warp_wait(q_full, seg & 1);
+                for (int j = 0; j < n && ok; j++, i++) {
                     const int st = i % NS;
-                    if (j + 1 < n) {                           // the next page's scores, while the softmax works on this one. Their
-                        // buffer held the weights of page i - 1; the product that read them was issued before.
-                        ok = mbar_wait(k_full + 8 * ((i + 1) % NS), ((i + 1) / NS) & 1);
+                    ok = warp_wait(k_full + 8 * st, (i / NS) & 1);
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        if (x >= nt || !ok) break;
+                        const int buf = c[x] & 1;
+                        // the buffer held the weights of the page before the last
+                        ok = c[x] < 2 || warp_wait(p_free + 8 * (2 * x + buf), ((c[x] >> 1) & 1) ^ 1);
                         if (!ok) break;
                         tc_fence_after();
-                        scores(i + 1, j + 2 == n);
-                    }
-                    ok = mbar_wait(p_full + 8 * (i & 1), (i >> 1) & 1) && mbar_wait(v_full + 8 * st, (i / NS) & 1) &&
-                         (j > 0 || seg == 0 || mbar_wait(o_free, (seg - 1) & 1));       // the segment before has been read out
-                    if (!ok) break;
-                    tc_fence_after();
+                        if (leader) {
 #pragma unroll
-                    for (int k = 0; k < KEYS / 16; k++)        // 16 keys a step: 8 columns of packed weights, 16 rows of V
-                        tc_mma_ts(t_o, tmem_base + (i & 1) * KEYS + k * 8, desc_mn_major(v_addr + st * PAGE_TILE + k * 16 * 128, PAGE_BYTES),
-                                  idesc_o, (j | k) != 0);
-                    tc_commit(v_free + 8 * st);
-                    tc_commit(o_done);
-                    // A segment's last product has a barrier of its own: behind it a warp may be two phases of o_done ahead of the
-                    // slowest, where a wait for a parity would be answered by the phase before.
-                    if (j + 1 == n) tc_commit(o_last);
+                            for (int k = 0; k < HD / 16; k++)
+                                tc_mma(tmem_base + (2 * x + buf) * KEYS, desc_k_major(q_addr + x * Q_TILE + (k / 4) * HALF_BYTES + (k % 4) * 32),
+                                       desc_k_major(k_addr + st * PAGE_TILE + (k / 4) * PAGE_BYTES + (k % 4) * 32), idesc_s, k != 0);
+                            tc_commit(s_full + 8 * (2 * x + buf));
+                        }
+                        __syncwarp();
+                        c[x]++;
+                    }
+                    if (!ok) break;
+                    if (leader) {
+                        tc_commit(k_free + 8 * st);
+                        if (j + 1 == n) tc_commit(q_free);
+                    }
+                    __syncwarp();
                 }
                 seg++;
             } while (ok && u.next(cu_q, kv_len, a, status));
-            if (!ok) atomicOr(status, MYNAH_ST_TIMEOUT);
+            if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
+        }
+    } else if (warp == 2) {
+        if (any) {                                             // ---- outputs: O += P . V
+            constexpr uint32_t idesc_o = idesc(HD, true);
+            const bool leader = elect_one();
+            const uint32_t v_addr = smem_u32(v_s);
+            int c[NT] = {};
+            int i = 0, seg = 0;
+            bool ok = true;
+            do {
+                const int n = u.pg1 - u.pg0, nt = NT == 1 || u.rows(a) <= tile_rows ? 1 : NT;
+                if (seg > 0) ok = warp_wait(o_free, (seg - 1) & 1);            // the segment before has been read out
+                for (int j = 0; j < n && ok; j++, i++) {
+                    const int st = i % NS;
+                    ok = warp_wait(v_full + 8 * st, (i / NS) & 1);
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {             // (the first tile's warps have looked through V before they hand over)
+                        if (x >= nt || !ok) break;
+                        const int buf = c[x] & 1;
+                        ok = warp_wait(p_full + 8 * (2 * x + buf), (c[x] >> 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (leader) {
+#pragma unroll
+                            for (int k = 0; k < KEYS / 16; k++)        // 16 keys a step: 8 columns of packed weights, 16 rows of V
+                                tc_mma_ts(tmem_base + O_COL + x * HD, tmem_base + (2 * x + buf) * KEYS + k * 8,
+                                          desc_mn_major(v_addr + st * PAGE_TILE + k * 16 * 128, PAGE_BYTES), idesc_o, (j | k) != 0);
+                            tc_commit(p_free + 8 * (2 * x + buf));
+                        }
+                        __syncwarp();
+                        c[x]++;
+                    }
+                    if (!ok) break;
+                    if (leader) tc_commit(v_free + 8 * st);
+                    __syncwarp();
+                }
+                seg++;
+            } while (ok && u.next(cu_q, kv_len, a, status));
+            if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
         }
     } else if (any) {
         // ---- softmax: a warp reads the lane quadrant (warp % 4) of tensor memory, a thread a row
-        const int quad = warp & 3, row = quad * 32 + lane;
-        const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16), t_o = t_row + O_COL;
-        int i = 0, seg = 0;
+        const int mine = (warp - 3) >> 2, quad = warp & 3, row = quad * 32 + lane;       // (of its own tile)
+        const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + mine * 2 * KEYS;
+        const uint32_t t_o = tmem_base + ((uint32_t)(quad * 32) << 16) + O_COL + mine * HD;
+        const uint32_t s_mine = s_full + 16 * mine, p_mine = p_full + 16 * mine, f_mine = p_free + 16 * mine;
+        int i = 0, c_own = 0, seg = 0;
         bool ok = true;
         do {
-            const int n = u.pg1 - u.pg0, n_rows = u.rows(a), past = u.past(), row0 = u.tile * a.tile_rows, kvl = u.s.kvl;
-            const bool works = quad * 32 < n_rows;
-            const int first_tok = row0 / a.G, tok = (row0 + row) / a.G;            // of the sequence
+            const int n = u.pg1 - u.pg0, past = u.past(), kvl = u.s.kvl;
+            const int row0 = u.tile * a.tile_rows + mine * tile_rows, n_rows = max(0, min(tile_rows, u.rows(a) - mine * tile_rows));
+            const bool there = NT == 1 || n_rows > 0, works = quad * 32 < n_rows;
+            const int first_tok = u.tile * a.tile_rows / a.G, tok = (row0 + row) / a.G;            // of the sequence
             const long long* words = masks + (size_t)(u.s.q_begin + min(tok, u.s.n_q - 1)) * a.words;
-            // Is there a key in the page that some row of the tile must not see?
+            // Is there a key in the page that some row of the CTA must not see?
             auto masked = [&](int key0) { return key0 + KEYS > kvl || (a.causal ? key0 + KEYS - 1 > past + first_tok : key0 + KEYS > past); };
             float m_ref = -INFINITY, l = 0.f;                  // the maximum that the sums are scaled by; the sum
-            for (int j = 0; j < n && ok; j++, i++) {
-                const int st = i % NS, key0 = (u.pg0 + j) * KEYS;
-                const uint32_t t_s = t_row + (i & 1) * KEYS;
+            for (int j = 0; j < n && ok && there; j++, i++, c_own++) {
+                const int st = i % NS, key0 = (u.pg0 + j) * KEYS, buf = c_own & 1;
+                const uint32_t t_s = t_row + buf * KEYS;
                 const bool mask = masked(key0);
-                if (!warp_wait(s_full + 8 * (i & 1), (i >> 1) & 1)) { ok = false; break; }
+                if (!warp_wait(s_mine + 8 * buf, (c_own >> 1) & 1)) { ok = false; break; }
                 tc_fence_after();
                 if (works) {
                     float s[KEYS];
@@ -240,10 +285,10 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
                     // O is touched only when some row of the warp has to be rescaled; then the product of the page before must have
-                    // finished. (The scores of page i were issued behind the product of page i - 2, so o_done has at least that
-                    // phase behind it, and the wait below cannot be answered by an older one.)
+                    // finished. (That page's scores were issued behind the product of the page two before it, in the same buffer:
+                    // the wait below cannot be answered by an older phase.)
                     if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                        if (!warp_wait(o_done, (i - 1) & 1)) { ok = false; break; }
+                        if (!warp_wait(f_mine + 8 * (buf ^ 1), ((c_own - 1) >> 1) & 1)) { ok = false; break; }
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < HD / 32; c++) {
@@ -269,7 +314,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     tc_wait_st();
                     l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
                 }
-                if (mask) {                                    // look through V: a thread a key's row of 64 columns
+                if (mask && mine == 0) {                       // look through V: a thread a key's row of 64 columns
                     if (!warp_wait(v_full + 8 * st, (i / NS) & 1)) { ok = false; break; }
                     const int key = row & 63, hf = row >> 6;
                     if (hf < HALVES) {
@@ -294,10 +339,11 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * (i & 1));
+                if (lane == 0) mbar_arrive(p_mine + 8 * buf);
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");     // what any warp found in V is known to all
-            if (ok && !warp_wait(o_last, seg & 1)) ok = false;
+            if (!there) i += n;
+            asm volatile("bar.sync 1, %0;" ::"n"(128 * NT) : "memory");       // what any warp found in V is known to all
+            if (ok && there && !warp_wait(f_mine + 8 * ((c_own - 1) & 1), ((c_own - 1) >> 1) & 1)) ok = false;      // the last page is in
             if (ok) {
                 tc_fence_after();
                 const bool poison = *(volatile int*)(flags + (seg & 1)) == seg + 1, lost = *(volatile int*)(flags + 2 + (seg & 7)) == seg + 1;
@@ -306,7 +352,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;      // a NaN stays one
                 const int h = u.g * a.G + (row0 + row) % a.G;
                 const size_t t = (size_t)u.s.q_begin + tok;
-                const long long slot = ((long long)blockIdx.x * 2 + u.place()) * a.tile_rows + row;
+                const long long slot = ((long long)blockIdx.x * 2 + u.place()) * a.tile_rows + mine * tile_rows + row;
                 if (works) {
 #pragma unroll 1
                     for (int c = 0; c < HD / 32; c++) {
@@ -365,14 +411,14 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
 }
 
-template <int HD>
+template <int HD, int NT>
 int go(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
        const long long* masks, const RowsArgs& a, void* out, RowsScratch s, int* status, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)(HD / 64) * (HALF_BYTES + 2 * STAGES<HD> * PAGE_BYTES) + 256 + 1024;
-    auto kern = attn_rows_tcgen05_kernel<HD>;
+    constexpr size_t smem = (size_t)(HD / 64) * (NT * HALF_BYTES + 2 * STAGES<HD, NT> * PAGE_BYTES) + 448 + 1024;
+    auto kern = attn_rows_tcgen05_kernel<HD, NT>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
-    kern<<<a.ctas * a.group, THREADS, smem, stream>>>(mq, mk, mv, (const bf16*)v, cu_q, kv_len, pt, masks, a, (bf16*)out, s, status);
+    kern<<<a.ctas * a.group, 96 + 128 * NT, smem, stream>>>(mq, mk, mv, (const bf16*)v, cu_q, kv_len, pt, masks, a, (bf16*)out, s, status);
     return mynah_check_launch("attn_rows");
 }
 
@@ -388,9 +434,15 @@ int launch_rows_tcgen05(const void* q, void* out, const RowsArgs& a, const void*
     MYNAH_REQUIRE(rows < (1ll << 31), "attn_rows: launch too large");
     if (pt.n_pages == 0) return mynah_fail("attn_rows: a cache without pages");
     CUtensorMap mq, mk, mv;
-    if (make_map_rows(&mq, q, a.T, a.H, a.HD, a.G, a.ldq, a.tile_rows / a.G)) return -1;
+    if (make_map_rows(&mq, q, a.T, a.H, a.HD, a.G, a.ldq, a.tile_rows / (a.two ? 2 : 1) / a.G)) return -1;
     if (make_map(&mk, k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, a.HD, a.HD, PAGE_TOKENS, 64)) return -1;
     if (make_map(&mv, v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, a.HD, a.HD, PAGE_TOKENS, 64)) return -1;
-    if (a.HD == 128) return go<128>(mq, mk, mv, v, cu_q, kv_len, pt, masks, a, out, s, status, stream);
-    return go<64>(mq, mk, mv, v, cu_q, kv_len, pt, masks, a, out, s, status, stream);
+#define ROWS_GO(HD, NT) return go<HD, NT>(mq, mk, mv, v, cu_q, kv_len, pt, masks, a, out, s, status, stream)
+    if (a.two) {
+        if (a.HD == 128) ROWS_GO(128, 2);
+        ROWS_GO(64, 2);
+    }
+    if (a.HD == 128) ROWS_GO(128, 1);
+    ROWS_GO(64, 1);
+#undef ROWS_GO
 }

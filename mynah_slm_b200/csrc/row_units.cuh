@@ -7,7 +7,9 @@
 // line, and CTA c takes the `range` pages from c * range on, whatever items they belong to: every CTA has the same number of
 // pages, however ragged the batch. A piece of an item that a CTA has on its own is a segment. An item that one CTA has whole is
 // finished there; of the others every CTA leaves its segment's maximum, sum and unnormalised output in scratch (at most two a
-// CTA: one that began before its range, one that goes on behind it), and a second launch joins them.
+// CTA: one that began before its range, one that goes on behind it), and a second launch joins them: an item that is cut is cut
+// at the start of some range, so there is one CTA (and its helpers) of that launch for every range, which finds there what the
+// range's own CTA wrote down of its start.
 //
 // Everything is worked out on the device from the step's description, so a captured launch serves whatever lengths its replays
 // bring. Where sequences have several tiles, `group` CTAs side by side take the same pages for `group` tiles (an item is then
@@ -22,6 +24,7 @@ struct RowsArgs {
     int T, B, H, KV, HD, G;
     int ldq, ldo;
     int tile_rows;                    // packed rows a tile
+    int two;                          // 1: the tcgen05 kernel's tile is two of its own
     int min_range;                    // pages a CTA at least
     int ctas;                         // ranges that the line is cut into; the launch has ctas * group CTAs
     int group;                        // tiles an item, each a CTA's
@@ -117,6 +120,11 @@ struct RowWalk {
     }
 };
 
+// Where a range begins: what the joining launch goes by. from > 0: inside item (b, g, item).
+struct RowStart {
+    int b, g, item, from;             // b < 0: behind the end of the line
+};
+
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -130,53 +138,68 @@ __device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {      
     }
     return v;
 }
+// Quotients of numbers that hardly ever need 64 bits.
+__device__ __forceinline__ long long div_ll(long long x, long long y) {
+    return ((x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
+}
 
-// The start of this CTA's range, for one whole warp, into `at` (b < 0: nothing to do). CTA 0 leaves where every
-// sequence begins on the line, and the range, for the second launch: info[b], info[B].
+// The start of this CTA's range, for one whole warp, into `at` (b < 0: nothing to do) and, for the joining launch, starts[range];
+// starts[ctas].from is the length of a range.
 __device__ __forceinline__ void find_range(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, RowWalk* at,
-                                           long long* info, int* status) {
-    const int lane = threadIdx.x & 31;
+                                           RowStart* starts, int* status) {
+    const int lane = threadIdx.x & 31, cta = blockIdx.x / a.group;
+    const bool writes = a.group == 1 || blockIdx.x % a.group == 0;
     long long total = 0, own = 0;
+    SeqShape s;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         own = 0;
-        if (b0 + lane < a.B) own = seq_pages(seq_shape(cu_q, kv_len, b0 + lane, a, status), a) * a.KV;
+        if (b0 + lane < a.B) {
+            s = seq_shape(cu_q, kv_len, b0 + lane, a, status);
+            own = seq_pages(s, a) * a.KV;
+        }
         total += warp_sum_ll(own);
     }
-    const long long range = max((long long)a.min_range, (total + a.ctas - 1) / a.ctas);
-    const long long from = range * (blockIdx.x / a.group);
-    if (lane == 0) at->b = -1;
-    if (blockIdx.x == 0 && lane == 0) info[a.B] = range;
+    const long long range = max((long long)a.min_range, div_ll(total + a.ctas - 1, a.ctas));
+    const long long from = range * cta;
+    if (lane == 0) {
+        at->b = -1;
+        if (writes && from >= total) starts[cta] = RowStart{-1, 0, 0, 0};
+        if (blockIdx.x == 0) starts[a.ctas] = RowStart{0, 0, 0, (int)min(range, 0x7fffffffll)};
+    }
     __syncwarp();
     if (from >= total) return;
     long long base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         if (a.B > 32) {                                        // (of up to 32 sequences every lane still has its own)
             own = 0;
-            if (b0 + lane < a.B) own = seq_pages(seq_shape(cu_q, kv_len, b0 + lane, a, status), a) * a.KV;
+            if (b0 + lane < a.B) {
+                s = seq_shape(cu_q, kv_len, b0 + lane, a, status);
+                own = seq_pages(s, a) * a.KV;
+            }
         }
         const long long incl = warp_scan_ll(own, lane), excl = incl - own;
-        if (blockIdx.x == 0 && b0 + lane < a.B) info[b0 + lane] = base + excl;
         if (own > 0 && from >= base + excl && from < base + incl) {
             RowWalk w;
             w.b = b0 + lane;
-            w.s = seq_shape(cu_q, kv_len, w.b, a, status);
-            const long long each = own / a.KV;
-            long long r = from - base - excl;
-            w.g = (int)(r / each);
-            r %= each;
+            w.s = s;
+            const long long each = div_ll(own, a.KV);
+            long long x = from - base - excl;
+            w.g = (int)div_ll(x, each);
+            x -= w.g * each;
             if (a.causal) {
                 w.item = 0;
-                for (int p; r >= (p = item_pages(w.s, w.item, a)); w.item++) r -= p;
+                for (int p; x >= (p = item_pages(s, w.item, a)); w.item++) x -= p;
             } else {
-                w.item = (int)(r / w.s.pages);
-                r %= w.s.pages;
+                w.item = (int)div_ll(x, s.pages);
+                x -= (long long)w.item * s.pages;
             }
-            w.from = (int)r;
+            w.from = (int)x;
             w.left = range;
+            if (writes) starts[cta] = RowStart{w.b, w.g, w.item, w.from};
             if (w.set(a) || w.next(cu_q, kv_len, a, status)) *at = w;
         }
         base += __shfl_sync(0xffffffffu, incl, 31);
-        if (blockIdx.x != 0 && from < base) break;
+        if (from < base) break;
     }
     __syncwarp();
 }
