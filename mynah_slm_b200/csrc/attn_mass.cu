@@ -41,7 +41,7 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
     float* q_s = k_s + GK * p;                                     // [GR][p]
     __shared__ float lse_s[GR];
     MassUnit u;
-    if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
+    if (!find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x, u, status)) return;
     const int g = blockIdx.y, G = a.r.G, past = u.s.kvl - u.s.n_q, key0 = u.kt0 * GK, n_rows = u.s.n_q * G;
     const int tiles = mass_rtiles(u.s, a);
     const int r0 = max(u.piece * u.rt, mass_first_tile(u, a)), r1 = (int)min((long long)tiles, (long long)(u.piece + 1) * u.rt);
@@ -116,7 +116,7 @@ __global__ void attn_mass_add_kernel(float* __restrict__ mass, const float* __re
                                      const int* __restrict__ kv_len, PageTable pt, MassArgs a, int* __restrict__ status) {
     MassUnit u;
     // the units of key tile n of the step: unit numbers are found as the first launch's were, from the tile's first piece on
-    if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x, u, status)) return;
+    if (!find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x, u, status)) return;
     if (u.piece != 0 || u.pieces <= 1) return;                     // one CTA a key tile; uncut tiles are done
     const int g = blockIdx.y, past = u.s.kvl - u.s.n_q, key = u.kt0 * a.keys + threadIdx.x;
     if (threadIdx.x >= a.keys || key >= u.s.kvl) return;

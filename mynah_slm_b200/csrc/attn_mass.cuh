@@ -24,7 +24,7 @@ __device__ __forceinline__ int mass_rtiles(const SeqShape& s, const MassArgs& a)
 
 // Finds unit `flat`, like find_row_unit: a sequence's units lie together, key tiles ascending (the first keys have the most rows
 // above them), a key tile's pieces one after the other.
-__device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const MassArgs& a, int flat,
+__device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt, const MassArgs& a, int flat,
                                                MassUnit& u, int* status) {
     __shared__ int found_s[3];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -34,7 +34,7 @@ __device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, con
             long long work = 0;
             for (int b0 = 0; b0 < a.r.B; b0 += 32) {
                 if (b0 + lane < a.r.B) {
-                    const SeqShape s = seq_shape(cu_q, kv_len, b0 + lane, a.r, status);
+                    const SeqShape s = seq_shape(cu_q, kv_len, pt, b0 + lane, a.r, status);
                     work += (long long)mass_ktiles(s, a) * mass_rtiles(s, a);
                 }
             }
@@ -45,7 +45,7 @@ __device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, con
         for (int b0 = 0; b0 < a.r.B && fb < 0; b0 += 32) {
             int n = 0;
             if (b0 + lane < a.r.B) {
-                const SeqShape s = seq_shape(cu_q, kv_len, b0 + lane, a.r, status);
+                const SeqShape s = seq_shape(cu_q, kv_len, pt, b0 + lane, a.r, status);
                 const int kt = mass_ktiles(s, a);
                 n = a.by_keys ? (kt + each - 1) / each : kt * ((mass_rtiles(s, a) + each - 1) / each);
             }
@@ -75,7 +75,7 @@ __device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, con
     if (u.b < 0) return false;
     u.unit0 = found_s[1];
     const int each = found_s[2], at = flat - u.unit0;
-    u.s = seq_shape(cu_q, kv_len, u.b, a.r, status);
+    u.s = seq_shape(cu_q, kv_len, pt, u.b, a.r, status);
     if (a.by_keys) {
         u.rt = 1 << 28;
         u.piece = 0;

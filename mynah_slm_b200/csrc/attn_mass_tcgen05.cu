@@ -45,7 +45,7 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     MassUnit u;
-    if (!find_mass_unit(cu_q, kv_len, a, blockIdx.x / a.r.KV, u, status)) return;
+    if (!find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x / a.r.KV, u, status)) return;
     const int g = blockIdx.x % a.r.KV, G = a.r.G, past = u.s.kvl - u.s.n_q, n_rows = u.s.n_q * G;
     const int r0 = max(u.piece * u.rt, a.by_keys ? 0 : mass_first_tile(u, a));
     const int r1 = (int)min((long long)mass_rtiles(u.s, a), (long long)(u.piece + 1) * u.rt);

@@ -19,6 +19,12 @@ namespace {
 constexpr int KT = 32;               // keys a tile of the general kernel
 constexpr int MAX_HEAD = 256;
 
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 __device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 four_of(const bf16* p) {
     const uint2 w = *reinterpret_cast<const uint2*>(p);
@@ -54,7 +60,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     __shared__ int bad_s;
     __shared__ RowWalk walk_s;
 
-    if (threadIdx.x < 32) find_range(cu_q, kv_len, a, &walk_s, sc.starts, status);
+    if (threadIdx.x < 32) find_start(cu_q, kv_len, pt, a, &walk_s, sc.starts, status);
     __syncthreads();
     RowWalk u = walk_s;
     if (u.b < 0) return;
@@ -66,7 +72,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     __syncthreads();                                               // (the segment before is done with shared memory)
     // every page of the segment must be there: one that lacks a page counts as keys that nobody sees
     for (int p = pg0 + (int)threadIdx.x; p < pg1; p += THREADS)
-        if (page_of(pt, u.b, p * PAGE_TOKENS) < 0) bad_s = 1;
+        if (page_at(pt, u.s, p) < 0) bad_s = 1;
     for (int i = threadIdx.x; i < R * HD; i += THREADS) {
         const int r = i / HD, d = i % HD;
         float x = 0.f;
@@ -83,7 +89,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     const int first_tok = row0 / a.G;
     const int t0 = bad ? 0 : pg0 * (PAGE_TOKENS / KT), t1 = bad ? 0 : min(pg1 * (PAGE_TOKENS / KT), (u.s.kvl + KT - 1) / KT);
     auto bring = [&](int t, int st) {
-        const int page = page_of(pt, u.b, t * KT);
+        const int page = page_at(pt, u.s, t / (PAGE_TOKENS / KT));
         const size_t base = (((size_t)page * a.KV + g) * PAGE_TOKENS + (t * KT) % PAGE_TOKENS) * HD;
         const int per_row = HD * (int)sizeof(T) / 16;
         for (int i = threadIdx.x; i < KT * per_row; i += THREADS) {
@@ -242,63 +248,65 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
             if (tx == 0) sc.ml[slot * a.tile_rows + r] = make_float2(m[i], l[i]);
         }
     }
-    } while (u.next(cu_q, kv_len, a, status));
+    } while (u.next(cu_q, kv_len, pt, a, status));
 }
 
-// Joins the segments of a cut item: with M = max m_c, out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c. Range c's CTAs
-// (blockIdx.x = c) take the item that the range begins inside of, if the item's first pages are in the range before (each cut
-// item has one such range). A warp a row; JOIN_CTAS CTAs share an item's rows. Few numbers and short chains of loads: it is
-// bound by its launch and three dependent reads (where the range begins, the segments' maxima, their rows, from L2).
-constexpr int JOIN_CTAS = 8, JOIN_WARPS = 4;
+// Joins the segments of a cut item, running over them with the maximum so far as the softmax does over keys. CTA c's helpers
+// (blockIdx.x = c - 1) take the item that CTA c begins inside of, if the item's first pages are CTA c - 1's (each cut item has
+// one such CTA). A warp a row. Bound by its start behind the attention and three dependent reads (where the CTA begins, the
+// sequence's numbers, then the segments' maxima and rows together, from L2).
+constexpr int JOIN_WARPS = 4, JOIN_ROWS = 2 * JOIN_WARPS;          // rows a CTA
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
-attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, RowsArgs a, RowsScratch sc,
+attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, RowsScratch sc,
                       int* __restrict__ status) {
     griddep_wait();
-    const int cta = blockIdx.x / a.group + 1, sub = blockIdx.x % a.group;       // (range 0 begins inside of nothing)
+    const int cta = blockIdx.x / a.group + 1, sub = blockIdx.x % a.group;       // (CTA 0 begins inside of nothing)
     const RowStart at = sc.starts[cta];
-    const int range = sc.starts[a.ctas].from;
-    if (at.b < 0 || at.from == 0 || at.from > range) return;
-    const SeqShape s = seq_shape(cu_q, kv_len, at.b, a, status);
+    if (at.b < 0 || at.from == 0 || at.from > at.each) return;
+    const SeqShape s = seq_shape(cu_q, kv_len, pt, at.b, a, status);
     const int tile = at.item * a.group + sub;
     if (tile >= s.tiles) return;
     const int pages = tile_pages(s, tile, a);
     if (pages <= at.from) return;                                  // this tile ends before the cut: it was whole
-    const int n = 2 + (pages - at.from - 1) / range;               // segments
+    const int n = 2 + (pages - at.from - 1) / at.each;             // segments
     const int lane = threadIdx.x & 31, rows = min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows);
-    for (int row = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5); row < rows; row += JOIN_CTAS * JOIN_WARPS) {
+    for (int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5); row < min(rows, ((int)blockIdx.y + 1) * JOIN_ROWS); row += JOIN_WARPS) {
         const int pr = tile * a.tile_rows + row, t = s.q_begin + pr / a.G, h = at.g * a.G + pr % a.G;
         auto slot = [&](int c) { return ((long long)((cta - 1 + c) * a.group + sub) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + row; };
-        float mx = -INFINITY;
-        for (int c = lane; c < n; c += 32) mx = fmaxf(mx, sc.ml[slot(c)].x);
-        mx = warp_max(mx);
-        const float m_use = mx == -INFINITY ? 0.f : mx;
-        float l = 0.f;
-        for (int c = lane; c < n; c += 32) {
-            const float2 ml = sc.ml[slot(c)];
-            l += ml.y * exp2f(ml.x - m_use);
-        }
-        l = warp_sum(l);
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a NaN stays one
         for (int col = lane * 4; col < a.HD; col += 128) {
+            float m = -INFINITY, l = 0.f;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int c = 0; c < n; c++) {
-                const long long i = slot(c);
-                const float w = exp2f(sc.ml[i].x - m_use);
-                const float4 y = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
-                x.x = fmaf(w, y.x, x.x);
-                x.y = fmaf(w, y.y, x.y);
-                x.z = fmaf(w, y.z, x.z);
-                x.w = fmaf(w, y.w, x.w);
+            for (int c0 = 0; c0 < n; c0 += 4) {
+                float2 ml[4];
+                float4 y[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const long long i = slot(min(c0 + c, n - 1));
+                    ml[c] = sc.ml[i];
+                    y[c] = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (c0 + c >= n) break;
+                    const float m_new = max_or_nan(m, ml[c].x), m_use = m_new == -INFINITY ? 0.f : m_new;
+                    const float u = exp2f(m - m_use), w = exp2f(ml[c].x - m_use);
+                    m = m_new;
+                    l = fmaf(l, u, ml[c].y * w);
+                    x.x = fmaf(x.x, u, y[c].x * w);
+                    x.y = fmaf(x.y, u, y[c].y * w);
+                    x.z = fmaf(x.z, u, y[c].z * w);
+                    x.w = fmaf(x.w, u, y[c].w * w);
+                }
             }
+            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a NaN stays one
             T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
             o[0] = from_f32<T>(x.x * inv);
             o[1] = from_f32<T>(x.y * inv);
             o[2] = from_f32<T>(x.z * inv);
             o[3] = from_f32<T>(x.w * inv);
+            if (col == 0 && sc.lse != nullptr) sc.lse[((size_t)at.g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m + log2f(l);
         }
-        if (lane == 0 && sc.lse != nullptr) sc.lse[((size_t)at.g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m_use + log2f(l);
     }
 }
 
@@ -331,7 +339,7 @@ int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void*
 }  // namespace
 
 long long rows_scratch_floats(const RowsArgs& a) {
-    return 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2) + 4ll * (a.ctas + 1);
+    return 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2) + (long long)(sizeof(RowStart) / 4) * a.ctas;
 }
 
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
@@ -346,12 +354,14 @@ RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
 
 bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     const bool tc = aligned && rows_tcgen05_takes(dtype, a.H, a.KV, a.HD);
+    const long long longest = (long long)max_q_len * a.G;          // packed rows of the longest sequence
     a.min_range = 2;
     a.group = 1;
     a.two = 0;
     a.ctas = 2 * mynah_sm_count();                                 // two CTAs an SM
     if (!tc) {
-        a.tile_rows = (long long)max_q_len * a.G <= 16 ? 16 : 64;
+        a.tile_rows = longest <= 16 ? 16 : 64;
+        a.most_rows = (int)(longest < a.tile_rows ? longest : a.tile_rows);
         return false;
     }
     a.tile_rows = 128 / a.G * a.G;
@@ -359,15 +369,16 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     // as there are (up to eight; a sequence of fewer leaves CTAs idle). Prompts of many tiles are bound by their products and
     // their pages stay in L2 anyway: one item after the other.
     const long long rows = (long long)a.T * a.G, each = (long long)a.B * a.tile_rows;
-    if ((long long)max_q_len * a.G > a.tile_rows && 2 * rows >= 3 * each) {
+    if (longest > a.tile_rows && 2 * rows >= 3 * each) {
         a.two = 1;
         a.tile_rows *= 2;
         a.ctas /= 2;
-        const long long most = ((long long)max_q_len * a.G + a.tile_rows - 1) / a.tile_rows, mean = (rows + each) / (2 * each);
+        const long long most = (longest + a.tile_rows - 1) / a.tile_rows, mean = (rows + each) / (2 * each);
         a.group = (int)(mean <= 1 || (a.causal && mean > 4) ? 1 : mean > 4 ? 4 : mean);
         if (a.group > most) a.group = (int)most;
         a.ctas /= a.group;
     }
+    a.most_rows = (int)(longest < a.tile_rows ? longest : a.tile_rows);
     return tc;
 }
 
@@ -377,13 +388,13 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
     return pick<bf16>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
 }
 
-int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, RowsScratch s, int* status,
+int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int* status,
                      cudaStream_t stream) {
-    if (a.ctas <= 1) return 0;                                     // one range: nothing is cut
-    const dim3 grid((a.ctas - 1) * a.group, JOIN_CTAS), block(JOIN_WARPS * 32);
+    if (a.ctas <= 1) return 0;                                     // one CTA: nothing is cut
+    const dim3 grid((a.ctas - 1) * a.group, ceil_div(a.most_rows, JOIN_ROWS)), block(JOIN_WARPS * 32);
     const cudaError_t e = dtype == MYNAH_F32
-        ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, a, s, status)
-        : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, a, s, status);
+        ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, pt, a, s, status)
+        : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, pt, a, s, status);
     if (e != cudaSuccess) return mynah_fail("attn_rows_join: %s", cudaGetErrorString(e));
     return mynah_check_launch("attn_rows_join");
 }
@@ -425,7 +436,7 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
     const int rc = tc ? launch_rows_tcgen05(q, out, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream)
                       : launch_rows_generic(q, out, dtype, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream);
     if (rc != 0) return rc;
-    return launch_rows_join(out, dtype, a, cu_q, kv_len, s, status, stream);
+    return launch_rows_join(out, dtype, a, cu_q, kv_len, pt, s, status, stream);
 }
 
 // q [T, ldq] and out [T, ldo], head h in columns [h * HD, (h + 1) * HD); k_cache, v_cache [n_pages, KV, 64, HD], which hold the

@@ -5,7 +5,7 @@
 
 // Partial results of cut items, and what every launch of one call reads.
 struct RowsScratch {
-    RowStart* starts;                 // [ctas + 1]: where every range begins, and a range's length
+    RowStart* starts;                 // [ctas]: where every CTA begins
     float2* ml;                       // [CTAs][2][tile_rows]: reference maximum (base 2, scaled) and sum
     float* o;                         // [CTAs][2][tile_rows][HD], not normalised
     float* lse;                       // [KV][T][G]: log2 of the sum of 2^score, -inf for a row that sees nothing; null: not wanted
@@ -22,7 +22,7 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
                         const int* kv_len, PageTable pt, const long long* masks, RowsScratch s, int* status, cudaStream_t stream);
 int launch_rows_tcgen05(const void* q, void* out, const RowsArgs& a, const void* k, const void* v, const int* cu_q,
                         const int* kv_len, PageTable pt, const long long* masks, RowsScratch s, int* status, cudaStream_t stream);
-int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, RowsScratch s, int* status,
+int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int* status,
                      cudaStream_t stream);
 bool rows_tcgen05_takes(int dtype, int H, int KV, int HD);
 

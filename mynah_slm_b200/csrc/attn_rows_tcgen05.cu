@@ -36,6 +36,7 @@ using namespace tc5;
 
 constexpr int BQ = 128;               // packed rows a tile at most (the lanes of tensor memory)
 constexpr int KEYS = PAGE_TOKENS;     // keys a step
+constexpr int STAGE_PITCH = 20;       // floats: rows of 80 bytes, whose 16-byte pieces meet no bank twice in eight lanes
 template <int HD, int NT> constexpr int STAGES = HD == 128 ? 2 * NT : 4 * NT;       // of K and of V
 
 // Which of two packed bfloat16 are not finite, as a mask over their bits.
@@ -58,7 +59,8 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     unsigned char* q_s = smem;
     unsigned char* k_s = q_s + NT * Q_TILE;                    // NS stages
     unsigned char* v_s = k_s + NS * PAGE_TILE;                 // NS stages
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + NS * PAGE_TILE);
+    float* stage_s = reinterpret_cast<float*>(v_s + NS * PAGE_TILE);       // [softmax warps][32 rows][16 columns]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stage_s + NT * 4 * 32 * STAGE_PITCH);
     const uint32_t k_full = smem_u32(bars), v_full = smem_u32(bars + 8), k_free = smem_u32(bars + 16), v_free = smem_u32(bars + 24);   // [NS]
     const uint32_t s_full = smem_u32(bars + 32), p_full = smem_u32(bars + 36);       // [NT][2]: scores ready, weights ready
     const uint32_t q_full = smem_u32(bars + 40), q_free = smem_u32(bars + 41);       // once a segment
@@ -72,7 +74,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        find_range(cu_q, kv_len, a, &walk_s, sc.starts, status);
+        find_start(cu_q, kv_len, pt, a, &walk_s, sc.starts, status);
     } else if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -115,7 +117,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 for (int p = u.pg0; p < u.pg1; p++, i++) {
                     const int st = i % NS;
                     const uint32_t prev = ((i / NS) & 1) ^ 1;  // parity of the stage's use before this one
-                    int page = page_of(pt, u.b, p * PAGE_TOKENS);
+                    int page = page_at(pt, u.s, p);
                     if (page < 0) {                            // the segment will count as keys that nobody sees
                         atomicOr(status, MYNAH_ST_PAGE_RANGE);
                         *(volatile int*)(flags + 2 + (seg & 7)) = seg + 1;
@@ -146,7 +148,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     v_issued = i + 1;
                 }
                 seg++;
-            } while (ok && u.next(cu_q, kv_len, a, status));
+            } while (ok && u.next(cu_q, kv_len, pt, a, status));
             if (!ok) atomicOr(status, MYNAH_ST_TIMEOUT);
             // whatever was started still lands in this CTA's shared memory: wait for it before leaving (bounded)
             if (q_issued > 0) mbar_wait(q_full, (q_issued - 1) & 1);
@@ -193,7 +195,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     __syncwarp();
                 }
                 seg++;
-            } while (ok && u.next(cu_q, kv_len, a, status));
+            } while (ok && u.next(cu_q, kv_len, pt, a, status));
             if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
         }
     } else if (warp == 2) {
@@ -232,7 +234,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     __syncwarp();
                 }
                 seg++;
-            } while (ok && u.next(cu_q, kv_len, a, status));
+            } while (ok && u.next(cu_q, kv_len, pt, a, status));
             if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
         }
     } else if (any) {
@@ -350,47 +352,55 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const bool whole = u.whole();
                 if (lost) m_ref = -INFINITY, l = 0.f;          // a page was missing: nothing counts
                 const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;      // a NaN stays one
-                const int h = u.g * a.G + (row0 + row) % a.G;
-                const size_t t = (size_t)u.s.q_begin + tok;
-                const long long slot = ((long long)blockIdx.x * 2 + u.place()) * a.tile_rows + mine * tile_rows + row;
+                const long long slot0 = ((long long)blockIdx.x * 2 + u.place()) * a.tile_rows + mine * tile_rows;      // of the tile
                 if (works) {
+                    float* mine_s = stage_s + (warp - 3) * 32 * STAGE_PITCH;           // this warp's rows, 16 columns at a time
+                    const int rows_here = min(32, n_rows - quad * 32);
+                    // where the four rows that this lane writes a part of begin (four lanes a row, 4 of 16 columns each)
+                    size_t to[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int pr = row0 + quad * 32 + e * 8 + (lane >> 2);
+                        to[e] = (whole ? (size_t)(u.s.q_begin + pr / a.G) * a.ldo + (size_t)(u.g * a.G + pr % a.G) * HD
+                                       : (size_t)(slot0 + quad * 32 + e * 8 + (lane >> 2)) * HD) + (lane & 3) * 4;
+                    }
 #pragma unroll 1
-                    for (int c = 0; c < HD / 32; c++) {
-                        uint32_t r[32];
-                        tc_ld32(t_o + c * 32, r);
-                        if (row < n_rows) {
-                            if (lost) {
+                    for (int c = 0; c < HD / 16; c++) {
+                        uint32_t r[16];
+                        tc_ld16(t_o + c * 16, r);
+                        if (lost) {
 #pragma unroll
-                                for (int e = 0; e < 32; e++) r[e] = 0u;
-                            } else if (poison) {                   // the values that were zeroed, to the rows that see them
-                                for (int key = u.pg0 * KEYS; key < min(u.pg1 * KEYS, kvl); key++) {
-                                    if (!masked(key & ~63) || !((visible64(key & ~63, kvl, past, tok, a.causal, words, a.words) >> (key & 63)) & 1ull)) continue;
-                                    const bf16* vr = v_cache + (((size_t)page_of(pt, u.b, key) * a.KV + u.g) * PAGE_TOKENS + key % PAGE_TOKENS) * HD + c * 32;
+                            for (int e = 0; e < 16; e++) r[e] = 0u;
+                        } else if (poison && row < n_rows) {   // the values that were zeroed, to the rows that see them
+                            for (int key = u.pg0 * KEYS; key < min(u.pg1 * KEYS, kvl); key++) {
+                                if (!masked(key & ~63) || !((visible64(key & ~63, kvl, past, tok, a.causal, words, a.words) >> (key & 63)) & 1ull)) continue;
+                                const bf16* vr = v_cache + (((size_t)page_at(pt, u.s, key / PAGE_TOKENS) * a.KV + u.g) * PAGE_TOKENS + key % PAGE_TOKENS) * HD + c * 16;
 #pragma unroll
-                                    for (int e = 0; e < 32; e++) {
-                                        const float x = __bfloat162float(vr[e]);
-                                        if (!isfinite(x)) r[e] = __float_as_uint(__uint_as_float(r[e]) + x);
-                                    }
+                                for (int e = 0; e < 16; e++) {
+                                    const float x = __bfloat162float(vr[e]);
+                                    if (!isfinite(x)) r[e] = __float_as_uint(__uint_as_float(r[e]) + x);
                                 }
                             }
-                            if (whole) {
-                                uint4* o = reinterpret_cast<uint4*>(out + t * a.ldo + (size_t)h * HD + c * 32);
+                        }
 #pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    o[e] = make_uint4(pack2(__uint_as_float(r[8 * e]) * inv, __uint_as_float(r[8 * e + 1]) * inv),
-                                                      pack2(__uint_as_float(r[8 * e + 2]) * inv, __uint_as_float(r[8 * e + 3]) * inv),
-                                                      pack2(__uint_as_float(r[8 * e + 4]) * inv, __uint_as_float(r[8 * e + 5]) * inv),
-                                                      pack2(__uint_as_float(r[8 * e + 6]) * inv, __uint_as_float(r[8 * e + 7]) * inv));
-                            } else {
-                                uint4* o = reinterpret_cast<uint4*>(sc.o + slot * HD + c * 32);
+                        for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * inv);
+                        __syncwarp();                          // (the columns before have been read)
 #pragma unroll
-                                for (int e = 0; e < 8; e++) o[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                        for (int e = 0; e < 4; e++)
+                            *reinterpret_cast<uint4*>(mine_s + lane * STAGE_PITCH + 4 * e) = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int rr = e * 8 + (lane >> 2);
+                            if (rr < rows_here) {
+                                const float4 x = *reinterpret_cast<const float4*>(mine_s + rr * STAGE_PITCH + (lane & 3) * 4);
+                                if (whole) *reinterpret_cast<uint2*>(out + to[e] + c * 16) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
+                                else *reinterpret_cast<float4*>(sc.o + to[e] + c * 16) = x;
                             }
                         }
-                        __syncwarp();
                     }
                     if (row < n_rows) {
-                        if (!whole) sc.ml[slot] = make_float2(m_ref, l);
+                        if (!whole) sc.ml[slot0 + row] = make_float2(m_ref, l);
                         else if (sc.lse != nullptr) sc.lse[((size_t)u.g * a.T + u.s.q_begin) * a.G + row0 + row] = l == 0.f ? -INFINITY : m_ref + log2f(l);
                     }
                 }
@@ -399,7 +409,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if (lane == 0) mbar_arrive(o_free);
             }
             seg++;
-        } while (u.next(cu_q, kv_len, a, status));             // (a warp that has given up goes on to keep the others' barriers)
+        } while (u.next(cu_q, kv_len, pt, a, status));             // (a warp that has given up goes on to keep the others' barriers)
         if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
     }
     griddep_launch_late();
@@ -414,7 +424,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 template <int HD, int NT>
 int go(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
        const long long* masks, const RowsArgs& a, void* out, RowsScratch s, int* status, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)(HD / 64) * (NT * HALF_BYTES + 2 * STAGES<HD, NT> * PAGE_BYTES) + 448 + 1024;
+    constexpr size_t smem = (size_t)(HD / 64) * (NT * HALF_BYTES + 2 * STAGES<HD, NT> * PAGE_BYTES) + NT * 4 * 32 * STAGE_PITCH * 4 + 448 + 1024;
     auto kern = attn_rows_tcgen05_kernel<HD, NT>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));

@@ -3,20 +3,24 @@
 //
 // The query heads that share a kv head are rows of one problem: packed row r of a sequence is token r / G, head r % G of the
 // group (G = H / KV). A tile is `tile_rows` packed rows; an item is one tile against all keys it may see, for one kv head; its
-// length is the number of those keys' pages. All items of the step lie one behind the other (by sequence, kv head, tile) on a
-// line, and CTA c takes the `range` pages from c * range on, whatever items they belong to: every CTA has the same number of
-// pages, however ragged the batch. A piece of an item that a CTA has on its own is a segment. An item that one CTA has whole is
-// finished there; of the others every CTA leaves its segment's maximum, sum and unnormalised output in scratch (at most two a
-// CTA: one that began before its range, one that goes on behind it), and a second launch joins them: an item that is cut is cut
-// at the start of some range, so there is one CTA (and its helpers) of that launch for every range, which finds there what the
-// range's own CTA wrote down of its start.
+// length is the number of those keys' pages. What a CTA takes of an item is a segment. There are two ways:
+//
+//   pieces  every item is cut into pieces of equal numbers of pages, of `each` at most, a CTA a piece. `each` is the least that
+//           leaves no more pieces than CTAs. One segment a CTA, but items that do not divide well leave CTAs idle.
+//   line    all items lie one behind the other (by sequence, kv head, item), and CTA c takes the `range` pages from c * range on:
+//           every CTA has the same number of pages, however ragged the batch, but a range that reaches from one item into the
+//           next is two segments, and most items are cut.
+//
+// The line is taken where `each` exceeds `range` by more than a segment and a join cost (LINE_COST pages). 8 trees of 24 tokens
+// behind 2,050 rows, 16 heads: PIECES8; a decode step of 64 sequences of 3,000 rows, 32 heads: LINE64. An item that one CTA has
+// whole is finished there; of the others every CTA leaves its segment's maximum, sum and unnormalised output in scratch (at
+// most two a CTA: one whose item began before, one whose item goes on), and a second launch joins them: there is one CTA (and
+// its helpers) of that launch for every CTA of the first, which finds there what that one wrote down of its start.
 //
 // Everything is worked out on the device from the step's description, so a captured launch serves whatever lengths its replays
 // bring. Where sequences have several tiles, `group` CTAs side by side take the same pages for `group` tiles (an item is then
 // that many tiles), so that a page comes from memory once and from L2 for the others: 16 trees of 64 tokens with four heads a kv
-// head (two tiles each) behind 8,191 rows read 1.05 GB one tile after the other, 0.54 GB together. Against chunks of equal pages per sequence, whose last chunks are short and whose number is no multiple of what the
-// device holds, equal ranges took 8 trees of 24 tokens behind 2,050 rows from 41 to TREE8 us and 16 of 64 behind 8,191 from 216
-// to TREE16 (with the smaller key tiles that came with them).
+// head (two tiles each) behind 8,191 rows read 1.05 GB one tile after the other, 0.54 GB together.
 #pragma once
 #include "layout.cuh"
 
@@ -24,6 +28,7 @@ struct RowsArgs {
     int T, B, H, KV, HD, G;
     int ldq, ldo;
     int tile_rows;                    // packed rows a tile
+    int most_rows;                    // of one tile that the step's longest sequence fills
     int two;                          // 1: the tcgen05 kernel's tile is two of its own
     int min_range;                    // pages a CTA at least
     int ctas;                         // ranges that the line is cut into; the launch has ctas * group CTAs
@@ -35,15 +40,20 @@ struct RowsArgs {
 
 struct SeqShape {
     int q_begin, n_q, kvl, tiles, pages;
+    int list0, list1;                 // its page list: entries [list0, list1), the first one for logical page `first`
+    int first;
 };
 
 // A sequence's numbers. Bounds that cannot be (rows outside the step, fewer keys than rows) count as a sequence without rows
 // and are reported.
-__device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, const int* __restrict__ kv_len, int b, const RowsArgs& a,
-                                              int* status) {
+__device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt, int b,
+                                              const RowsArgs& a, int* status) {
     SeqShape s;
     s.q_begin = cu_q[b];
     const int end = cu_q[b + 1];
+    s.list0 = pt.indptr[b];
+    s.list1 = pt.indptr[b + 1];
+    s.first = pt.base[b];
     s.n_q = end - s.q_begin;
     s.kvl = kv_len[b];
     if (s.n_q <= 0 || s.q_begin < 0 || end > a.T || s.kvl < s.n_q) {
@@ -53,6 +63,14 @@ __device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, cons
     s.tiles = (s.n_q * a.G + a.tile_rows - 1) / a.tile_rows;
     s.pages = s.n_q > 0 ? (s.kvl + PAGE_TOKENS - 1) / PAGE_TOKENS : 0;
     return s;
+}
+
+// The physical page of a sequence's logical page, or -1.
+__device__ __forceinline__ int page_at(const PageTable& pt, const SeqShape& s, int page) {
+    const int at = s.list0 + page - s.first;
+    if (at < s.list0 || at >= s.list1) return -1;
+    const int id = pt.ids[at];
+    return id >= 0 && id < pt.n_pages ? id : -1;
 }
 
 // Pages that some row of a tile may see: all, or up to the tile's last token.
@@ -81,7 +99,7 @@ struct RowWalk {
     int b, g, item, tile, pg0, pg1;
     int from, to;                     // the item's pages in this range
     int pages;                        // that the tile may see
-    long long left;                   // pages of the range that are left, this segment's among them
+    long long left;                   // pages that are left of what this CTA takes, this segment's among them
     SeqShape s;
 
     __device__ __forceinline__ int past() const { return s.kvl - s.n_q; }
@@ -100,7 +118,8 @@ struct RowWalk {
         return pg0 < pg1;
     }
     // The next segment of the range; false when there is none.
-    __device__ __forceinline__ bool next(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, int* status) {
+    __device__ __forceinline__ bool next(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt, const RowsArgs& a,
+                                         int* status) {
         do {
             left -= to - from;
             if (left <= 0) return false;
@@ -111,7 +130,7 @@ struct RowWalk {
                     g = 0;
                     do {
                         if (++b >= a.B) return false;
-                        s = seq_shape(cu_q, kv_len, b, a, status);
+                        s = seq_shape(cu_q, kv_len, pt, b, a, status);
                     } while (s.n_q == 0);
                 }
             }
@@ -120,15 +139,22 @@ struct RowWalk {
     }
 };
 
-// Where a range begins: what the joining launch goes by. from > 0: inside item (b, g, item).
+// Where a CTA begins: what the joining launch goes by. from > 0: inside item (b, g, item), of which a CTA has `each` pages.
 struct RowStart {
-    int b, g, item, from;             // b < 0: behind the end of the line
+    int b, g, item, from;             // b < 0: nothing
+    int each, pad[3];
 };
+constexpr int LINE_COST = 16;
 
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+// The same where no lane has more than 2^26, which is all but always.
+__device__ __forceinline__ long long warp_sum_small(long long v) {
+    if (__all_sync(0xffffffffu, v < (1ll << 26))) return (long long)__reduce_add_sync(0xffffffffu, (unsigned)v);
+    return warp_sum_ll(v);
 }
 __device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {      // sum over the lanes up to this one
 #pragma unroll
@@ -143,60 +169,102 @@ __device__ __forceinline__ long long div_ll(long long x, long long y) {
     return ((x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
 }
 
-// The start of this CTA's range, for one whole warp, into `at` (b < 0: nothing to do) and, for the joining launch, starts[range];
-// starts[ctas].from is the length of a range.
-__device__ __forceinline__ void find_range(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const RowsArgs& a, RowWalk* at,
-                                           RowStart* starts, int* status) {
+// Pieces of one kv head's items of a sequence.
+__device__ __forceinline__ int seq_pieces(const SeqShape& s, int each, const RowsArgs& a) {
+    const int items = seq_items(s, a);
+    if (!a.causal || items <= 1) return items * ((s.pages + each - 1) / each);
+    int n = 0;
+    for (int i = 0; i < items; i++) n += (item_pages(s, i, a) + each - 1) / each;
+    return n;
+}
+
+// The start of this CTA, for one whole warp, into `at` (b < 0: nothing to do) and, for the joining launch, starts[CTA].
+__device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt,
+                                           const RowsArgs& a, RowWalk* at, RowStart* starts, int* status) {
     const int lane = threadIdx.x & 31, cta = blockIdx.x / a.group;
     const bool writes = a.group == 1 || blockIdx.x % a.group == 0;
     long long total = 0, own = 0;
     SeqShape s;
+    s.tiles = s.pages = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         own = 0;
         if (b0 + lane < a.B) {
-            s = seq_shape(cu_q, kv_len, b0 + lane, a, status);
+            s = seq_shape(cu_q, kv_len, pt, b0 + lane, a, status);
             own = seq_pages(s, a) * a.KV;
         }
-        total += warp_sum_ll(own);
+        total += warp_sum_small(own);
     }
     const long long range = max((long long)a.min_range, div_ll(total + a.ctas - 1, a.ctas));
-    const long long from = range * cta;
-    if (lane == 0) {
-        at->b = -1;
-        if (writes && from >= total) starts[cta] = RowStart{-1, 0, 0, 0};
-        if (blockIdx.x == 0) starts[a.ctas] = RowStart{0, 0, 0, (int)min(range, 0x7fffffffll)};
+    // Pieces, for up to 32 sequences: the least `each` of range .. range + LINE_COST that makes no more pieces than there are CTAs.
+    int each = 0;
+    if (a.B <= 32 && range < (1 << 20)) {
+        int lo = (int)range, hi = (int)range + LINE_COST + 1;
+        while (lo < hi) {                                      // hi: fits, or is beyond what pays
+            const int mid = (lo + hi) / 2;
+            const bool fits = warp_sum_small(s.tiles > 0 ? (long long)seq_pieces(s, mid, a) * a.KV : 0) <= a.ctas;
+            if (fits) hi = mid; else lo = mid + 1;
+        }
+        if (lo <= (int)range + LINE_COST) each = lo;
     }
+    if (lane == 0) at->b = -1;
     __syncwarp();
-    if (from >= total) return;
-    long long base = 0;
+    long long base = 0, pieces = 0;
+    if (each > 0) {
+        pieces = s.tiles > 0 ? (long long)seq_pieces(s, each, a) * a.KV : 0;
+        total = warp_sum_small(pieces);
+    }
+    const long long from = each > 0 ? cta : range * cta;       // in pieces, or in pages
+    if (from >= total) {
+        if (lane == 0 && writes) starts[cta].b = -1;
+        return;
+    }
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         if (a.B > 32) {                                        // (of up to 32 sequences every lane still has its own)
             own = 0;
             if (b0 + lane < a.B) {
-                s = seq_shape(cu_q, kv_len, b0 + lane, a, status);
+                s = seq_shape(cu_q, kv_len, pt, b0 + lane, a, status);
                 own = seq_pages(s, a) * a.KV;
             }
         }
-        const long long incl = warp_scan_ll(own, lane), excl = incl - own;
-        if (own > 0 && from >= base + excl && from < base + incl) {
+        const long long mine = each > 0 ? pieces : own, incl = warp_scan_ll(mine, lane), excl = incl - mine;
+        if (mine > 0 && from >= base + excl && from < base + incl) {
             RowWalk w;
             w.b = b0 + lane;
             w.s = s;
-            const long long each = div_ll(own, a.KV);
+            const long long head = div_ll(mine, a.KV);         // one kv head's
             long long x = from - base - excl;
-            w.g = (int)div_ll(x, each);
-            x -= w.g * each;
-            if (a.causal) {
-                w.item = 0;
-                for (int p; x >= (p = item_pages(s, w.item, a)); w.item++) x -= p;
+            w.g = (int)div_ll(x, head);
+            x -= w.g * head;
+            w.item = 0;
+            if (each > 0) {
+                int p = item_pages(s, 0, a), n = (p + each - 1) / each;
+                if (!a.causal) {
+                    w.item = (int)x / n;
+                    x -= (long long)w.item * n;
+                } else {
+                    while (x >= n) {
+                        x -= n;
+                        p = item_pages(s, ++w.item, a);
+                        n = (p + each - 1) / each;
+                    }
+                }
+                w.left = (p + n - 1) / n;                      // pieces of one size
+                w.from = (int)(x * w.left);
             } else {
-                w.item = (int)div_ll(x, s.pages);
-                x -= (long long)w.item * s.pages;
+                w.left = range;
+                if (!a.causal) {
+                    w.item = (int)div_ll(x, s.pages);
+                    x -= (long long)w.item * s.pages;
+                } else {
+                    for (int p; x >= (p = item_pages(s, w.item, a)); w.item++) x -= p;
+                }
+                w.from = (int)x;
             }
-            w.from = (int)x;
-            w.left = range;
-            if (writes) starts[cta] = RowStart{w.b, w.g, w.item, w.from};
-            if (w.set(a) || w.next(cu_q, kv_len, a, status)) *at = w;
+            if (writes) starts[cta] = RowStart{w.b, w.g, w.item, w.from, (int)min(w.left, 0x7fffffffll)};
+            // (a piece is one segment: what is left of it when the item ends is nobody's)
+            const bool has = w.set(a);
+            if (each > 0) w.left = w.to - w.from;
+            if (has || w.next(cu_q, kv_len, pt, a, status)) *at = w;
         }
         base += __shfl_sync(0xffffffffu, incl, 31);
         if (from < base) break;
