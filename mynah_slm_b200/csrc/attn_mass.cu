@@ -148,6 +148,8 @@ bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
     a.rows = tc ? 128 / a.r.G * a.r.G : GR;
     a.by_keys = (long long)max_q_len * a.r.G <= a.rows;
     a.r.tile_rows = a.rows;
+    a.r.group = a.r.ctas = 1;
+    a.r.finish();
     a.target = (tc ? 4 : (a.by_keys ? 0 : 4)) * mynah_sm_count();
     return tc;
 }

@@ -20,7 +20,7 @@ struct MassUnit {
 };
 
 __device__ __forceinline__ int mass_ktiles(const SeqShape& s, const MassArgs& a) { return s.n_q > 0 ? (s.kvl + a.keys - 1) / a.keys : 0; }
-__device__ __forceinline__ int mass_rtiles(const SeqShape& s, const MassArgs& a) { return (s.n_q * a.r.G + a.rows - 1) / a.rows; }
+__device__ __forceinline__ int mass_rtiles(const SeqShape& s, const MassArgs& a) { return a.r.by_tile.div(s.n_q * a.r.G + a.rows - 1); }
 
 // Finds unit `flat`, like find_row_unit: a sequence's units lie together, key tiles ascending (the first keys have the most rows
 // above them), a key tile's pieces one after the other.

@@ -46,7 +46,7 @@ template <typename T> __host__ __device__ constexpr int pitch_of(int HD) { retur
 // what arithmetic does. K and V come KT keys at a time by asynchronous copies, two tiles in flight.
 // 16-row tiles (TY = 4, TX = 32) are for the few rows of decode steps and small trees, 64-row tiles (TY = TX = 16) for the rest.
 template <typename T, int TY, int TX, int NC>
-__global__ void __launch_bounds__(TY * TX)
+__global__ void __launch_bounds__(TY * TX, 2)
 attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
                  const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, const long long* __restrict__ masks,
                  RowsArgs a, RowsScratch sc, int* __restrict__ status) {
@@ -77,8 +77,8 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         const int r = i / HD, d = i % HD;
         float x = 0.f;
         if (r < n_rows) {
-            const int pr = row0 + r;
-            x = to_f32(q[(size_t)(u.s.q_begin + pr / a.G) * a.ldq + (size_t)(g * a.G + pr % a.G) * HD + d]);
+            const int pr = row0 + r, tok = a.by_G.div(pr);
+            x = to_f32(q[(size_t)(u.s.q_begin + tok) * a.ldq + (size_t)(g * a.G + pr - tok * a.G) * HD + d]);
         }
         q_s[r * qp + d] = x;
     }
@@ -86,7 +86,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     const bool bad = bad_s != 0;
     if (bad && threadIdx.x == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
 
-    const int first_tok = row0 / a.G;
+    const int first_tok = a.by_G.div(row0);
     const int t0 = bad ? 0 : pg0 * (PAGE_TOKENS / KT), t1 = bad ? 0 : min(pg1 * (PAGE_TOKENS / KT), (u.s.kvl + KT - 1) / KT);
     auto bring = [&](int t, int st) {
         const int page = page_at(pt, u.s, t / (PAGE_TOKENS / KT));
@@ -149,7 +149,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         const bool need_mask = key0 + KT > u.s.kvl || (a.causal ? key0 + KT - 1 > past + first_tok : key0 + KT > past);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = ty + TY * i, pr = row0 + r, tok = pr / a.G;
+            const int r = ty + TY * i, pr = row0 + r, tok = a.by_G.div(pr);
             uint32_t seen = 0xffffffffu;
             if (need_mask) {
                 const unsigned long long vis = r < n_rows ? visible64(key0 & ~63, u.s.kvl, past, tok, a.causal, masks + (size_t)(u.s.q_begin + tok) * a.words, a.words) : 0ull;
@@ -226,7 +226,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     for (int i = 0; i < 4; i++) {
         const int r = ty + TY * i;
         if (r >= n_rows) continue;
-        const int pr = row0 + r, tok = pr / a.G, h = g * a.G + pr % a.G;
+        const int pr = row0 + r, tok = a.by_G.div(pr), h = g * a.G + pr - tok * a.G;
         if (whole) {
             const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);    // a NaN stays one
             T* o = out + (size_t)(u.s.q_begin + tok) * a.ldo + (size_t)h * HD;
@@ -255,13 +255,14 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
 // (blockIdx.x = c - 1) take the item that CTA c begins inside of, if the item's first pages are CTA c - 1's (each cut item has
 // one such CTA). A warp a row. Bound by its start behind the attention and three dependent reads (where the CTA begins, the
 // sequence's numbers, then the segments' maxima and rows together, from L2).
-constexpr int JOIN_WARPS = 4, JOIN_ROWS = 2 * JOIN_WARPS;          // rows a CTA
+constexpr int JOIN_WARPS = 8, JOIN_ROWS = JOIN_WARPS;              // rows a CTA
+constexpr int JOIN_AHEAD = 8;                                      // segments asked for at once
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, RowsScratch sc,
                       int* __restrict__ status) {
     griddep_wait();
-    const int cta = blockIdx.x / a.group + 1, sub = blockIdx.x % a.group;       // (CTA 0 begins inside of nothing)
+    const int cta = a.by_group.div(blockIdx.x) + 1, sub = a.by_group.mod(blockIdx.x);       // (CTA 0 begins inside of nothing)
     const RowStart at = sc.starts[cta];
     if (at.b < 0 || at.from == 0 || at.from > at.each) return;
     const SeqShape s = seq_shape(cu_q, kv_len, pt, at.b, a, status);
@@ -269,28 +270,30 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
     if (tile >= s.tiles) return;
     const int pages = tile_pages(s, tile, a);
     if (pages <= at.from) return;                                  // this tile ends before the cut: it was whole
-    const int n = 2 + (pages - at.from - 1) / at.each;             // segments
+    const int n = 2 + quotient(pages - at.from - 1, at.each);      // segments
     const int lane = threadIdx.x & 31, rows = min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows);
-    for (int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5); row < min(rows, ((int)blockIdx.y + 1) * JOIN_ROWS); row += JOIN_WARPS) {
-        const int pr = tile * a.tile_rows + row, t = s.q_begin + pr / a.G, h = at.g * a.G + pr % a.G;
+    const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
+    if (row < rows) {
+        const int pr = tile * a.tile_rows + row, tok = a.by_G.div(pr), t = s.q_begin + tok, h = at.g * a.G + pr - tok * a.G;
         auto slot = [&](int c) { return ((long long)((cta - 1 + c) * a.group + sub) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + row; };
         for (int col = lane * 4; col < a.HD; col += 128) {
             float m = -INFINITY, l = 0.f;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c0 = 0; c0 < n; c0 += 4) {
-                float2 ml[4];
-                float4 y[4];
+#pragma unroll 1
+            for (int c0 = 0; c0 < n; c0 += JOIN_AHEAD) {
+                float2 ml[JOIN_AHEAD];
+                float4 y[JOIN_AHEAD];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < JOIN_AHEAD; c++) {
                     const long long i = slot(min(c0 + c, n - 1));
                     ml[c] = sc.ml[i];
                     y[c] = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
                 }
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    if (c0 + c >= n) break;
+                for (int c = 0; c < JOIN_AHEAD; c++) {
+                    if (c0 + c >= n) ml[c] = make_float2(-INFINITY, 0.f);      // (the last segment again: no weight)
                     const float m_new = max_or_nan(m, ml[c].x), m_use = m_new == -INFINITY ? 0.f : m_new;
-                    const float u = exp2f(m - m_use), w = exp2f(ml[c].x - m_use);
+                    const float u = ex2_f(m - m_use), w = ex2_f(ml[c].x - m_use);
                     m = m_new;
                     l = fmaf(l, u, ml[c].y * w);
                     x.x = fmaf(x.x, u, y[c].x * w);
@@ -362,6 +365,7 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     if (!tc) {
         a.tile_rows = longest <= 16 ? 16 : 64;
         a.most_rows = (int)(longest < a.tile_rows ? longest : a.tile_rows);
+        a.finish();
         return false;
     }
     a.tile_rows = 128 / a.G * a.G;
@@ -379,6 +383,7 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
         a.ctas /= a.group;
     }
     a.most_rows = (int)(longest < a.tile_rows ? longest : a.tile_rows);
+    a.finish();
     return tc;
 }
 

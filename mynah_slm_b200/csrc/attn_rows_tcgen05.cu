@@ -105,7 +105,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t tmem_base = *tmem_slot;
     RowWalk u = walk_s;
     const bool any = u.b >= 0;
-    const int tile_rows = a.tile_rows / NT;                    // of one tile; a tile exists if the CTA's rows reach it
+    const int tile_rows = NT == 2 ? a.tile_rows >> 1 : a.tile_rows;                    // of one tile; a tile exists if the CTA's rows reach it
 
     // Page number i of the CTA (over all segments) uses stage i % NS of K and V, in that stage's use i / NS; the pages of a tile number
     // c use its score buffer c & 1.
@@ -137,7 +137,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                             for (int hf = 0; hf < HALVES; hf++)
                                 tma_load_3d(smem_u32(q_s + x * Q_TILE + hf * HALF_BYTES), &map_q, hf * 64, u.g * a.G,
-                                            u.s.q_begin + (u.tile * a.tile_rows + x * tile_rows) / a.G, q_full);
+                                            u.s.q_begin + a.by_G.div(u.tile * a.tile_rows + x * tile_rows), q_full);
                         q_issued = seg + 1;
                     }
                     if (i >= NS && !mbar_wait(v_free + 8 * st, prev)) { ok = false; break; }
@@ -249,7 +249,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int n = u.pg1 - u.pg0, past = u.past(), kvl = u.s.kvl;
             const int row0 = u.tile * a.tile_rows + mine * tile_rows, n_rows = max(0, min(tile_rows, u.rows(a) - mine * tile_rows));
             const bool there = NT == 1 || n_rows > 0, works = quad * 32 < n_rows;
-            const int first_tok = u.tile * a.tile_rows / a.G, tok = (row0 + row) / a.G;            // of the sequence
+            const int first_tok = a.by_G.div(u.tile * a.tile_rows), tok = a.by_G.div(row0 + row);            // of the sequence
             const long long* words = masks + (size_t)(u.s.q_begin + min(tok, u.s.n_q - 1)) * a.words;
             // Is there a key in the page that some row of the CTA must not see?
             auto masked = [&](int key0) { return key0 + KEYS > kvl || (a.causal ? key0 + KEYS - 1 > past + first_tok : key0 + KEYS > past); };
@@ -360,8 +360,8 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     size_t to[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int pr = row0 + quad * 32 + e * 8 + (lane >> 2);
-                        to[e] = (whole ? (size_t)(u.s.q_begin + pr / a.G) * a.ldo + (size_t)(u.g * a.G + pr % a.G) * HD
+                        const int pr = row0 + quad * 32 + e * 8 + (lane >> 2), tk = a.by_G.div(pr);
+                        to[e] = (whole ? (size_t)(u.s.q_begin + tk) * a.ldo + (size_t)(u.g * a.G + pr - tk * a.G) * HD
                                        : (size_t)(slot0 + quad * 32 + e * 8 + (lane >> 2)) * HD) + (lane & 3) * 4;
                     }
 #pragma unroll 1

@@ -5,8 +5,9 @@
 // group (G = H / KV). A tile is `tile_rows` packed rows; an item is one tile against all keys it may see, for one kv head; its
 // length is the number of those keys' pages. What a CTA takes of an item is a segment. There are two ways:
 //
-//   pieces  every item is cut into pieces of equal numbers of pages, of `each` at most, a CTA a piece. `each` is the least that
-//           leaves no more pieces than CTAs. One segment a CTA, but items that do not divide well leave CTAs idle.
+//   pieces  every item is cut into pieces of equal numbers of pages, of `each` at most, a CTA a piece. The longest item has as
+//           many pieces as all items can have with a CTA for each. One segment a CTA, but shorter items and numbers that do not
+//           divide well leave CTAs idle.
 //   line    all items lie one behind the other (by sequence, kv head, item), and CTA c takes the `range` pages from c * range on:
 //           every CTA has the same number of pages, however ragged the batch, but a range that reaches from one item into the
 //           next is two segments, and most items are cut.
@@ -17,12 +18,26 @@
 // most two a CTA: one whose item began before, one whose item goes on), and a second launch joins them: there is one CTA (and
 // its helpers) of that launch for every CTA of the first, which finds there what that one wrote down of its start.
 //
-// Everything is worked out on the device from the step's description, so a captured launch serves whatever lengths its replays
+// Everything is worked out on the device from the step's description (in few instructions: a CTA's first trip through any code
+// waits for that code, about 0.3 us for every 128 bytes of it, which is most of what a small call takes), so a captured launch serves whatever lengths its replays
 // bring. Where sequences have several tiles, `group` CTAs side by side take the same pages for `group` tiles (an item is then
 // that many tiles), so that a page comes from memory once and from L2 for the others: 16 trees of 64 tokens with four heads a kv
 // head (two tiles each) behind 8,191 rows read 1.05 GB one tile after the other, 0.54 GB together.
 #pragma once
 #include "layout.cuh"
+
+// Quotient of x < 2^31 and a divisor that the host knows: multiply and shift.
+struct FastDiv {
+    uint32_t by, mul;
+    int shift;
+    static FastDiv of(int d) {
+        int s = 0;
+        while ((1ll << s) < d) s++;                                // 2^s >= d: (2^(31 + s) / d rounded up) fits 32 bits and is exact below 2^31
+        return FastDiv{(uint32_t)d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+    }
+    __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(uint32_t)x * mul) >> shift); }
+    __device__ __forceinline__ int mod(int x) const { return x - div(x) * (int)by; }
+};
 
 struct RowsArgs {
     int T, B, H, KV, HD, G;
@@ -31,12 +46,27 @@ struct RowsArgs {
     int most_rows;                    // of one tile that the step's longest sequence fills
     int two;                          // 1: the tcgen05 kernel's tile is two of its own
     int min_range;                    // pages a CTA at least
-    int ctas;                         // ranges that the line is cut into; the launch has ctas * group CTAs
+    int ctas;                         // ranges that the line is cut into, or pieces; the launch has ctas * group CTAs
     int group;                        // tiles an item, each a CTA's
     int causal;                       // 1: token i sees rows <= past + i; 0: the mask words
     int words;                        // mask words a token
     float scale_log2;                 // score scale * log2(e)
+    FastDiv by_G, by_tile, by_group, by_KV, by_ctas;
+    void finish() {                   // once the numbers above stand
+        by_G = FastDiv::of(G), by_tile = FastDiv::of(tile_rows), by_group = FastDiv::of(group), by_KV = FastDiv::of(KV), by_ctas = FastDiv::of(ctas);
+    }
 };
+constexpr int LINE_COST = 16;
+// Most page visits of a step (pages of every tile's keys, over the kv heads) that the numbers below are made for: a prompt of a
+// million tokens and 32 heads. A step of more is refused through the status word.
+constexpr long long MAX_VISITS = 1ll << 30;
+
+// Quotient of two numbers of the device's, 0 <= x < 2^31, y > 0. Below 2^22 the fp32 quotient is off by less than one.
+__device__ __forceinline__ int quotient(int x, int y) {
+    if (x >= 1 << 22) return x / y;
+    const int q = (int)__fdividef((float)x, (float)y), r = x - q * y;
+    return q + (r >= y ? 1 : 0) - (r < 0 ? 1 : 0);
+}
 
 struct SeqShape {
     int q_begin, n_q, kvl, tiles, pages;
@@ -60,8 +90,8 @@ __device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, cons
         if (s.n_q != 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
         s.n_q = 0;
     }
-    s.tiles = (s.n_q * a.G + a.tile_rows - 1) / a.tile_rows;
-    s.pages = s.n_q > 0 ? (s.kvl + PAGE_TOKENS - 1) / PAGE_TOKENS : 0;
+    s.tiles = a.by_tile.div(s.n_q * a.G + a.tile_rows - 1);
+    s.pages = s.n_q > 0 ? (int)(((unsigned)s.kvl + PAGE_TOKENS - 1) / PAGE_TOKENS) : 0;
     return s;
 }
 
@@ -76,11 +106,11 @@ __device__ __forceinline__ int page_at(const PageTable& pt, const SeqShape& s, i
 // Pages that some row of a tile may see: all, or up to the tile's last token.
 __device__ __forceinline__ int tile_pages(const SeqShape& s, int tile, const RowsArgs& a) {
     if (!a.causal) return s.pages;
-    const int last = (min(s.n_q * a.G, (tile + 1) * a.tile_rows) - 1) / a.G;
+    const int last = a.by_G.div(min(s.n_q * a.G, (tile + 1) * a.tile_rows) - 1);
     return (s.kvl - s.n_q + last) / PAGE_TOKENS + 1;
 }
 
-__device__ __forceinline__ int seq_items(const SeqShape& s, const RowsArgs& a) { return (s.tiles + a.group - 1) / a.group; }
+__device__ __forceinline__ int seq_items(const SeqShape& s, const RowsArgs& a) { return a.by_group.div(s.tiles + a.group - 1); }
 // Pages of an item: of its last tile, which sees the most.
 __device__ __forceinline__ int item_pages(const SeqShape& s, int item, const RowsArgs& a) {
     return tile_pages(s, min(s.tiles, (item + 1) * a.group) - 1, a);
@@ -90,16 +120,17 @@ __device__ __forceinline__ long long seq_pages(const SeqShape& s, const RowsArgs
     const int items = seq_items(s, a);
     if (!a.causal || items <= 1) return (long long)items * s.pages;
     long long n = 0;
+#pragma unroll 1
     for (int i = 0; i < items; i++) n += item_pages(s, i, a);
     return n;
 }
 
-// Where a CTA is on the line, and the segment it is at: pages [pg0, pg1) of one tile of item (b, g, item).
+// Where a CTA is, and the segment it is at: pages [pg0, pg1) of one tile of item (b, g, item).
 struct RowWalk {
     int b, g, item, tile, pg0, pg1;
     int from, to;                     // the item's pages in this range
     int pages;                        // that the tile may see
-    long long left;                   // pages that are left of what this CTA takes, this segment's among them
+    int left;                         // pages that are left of what this CTA takes, this segment's among them
     SeqShape s;
 
     __device__ __forceinline__ int past() const { return s.kvl - s.n_q; }
@@ -109,8 +140,8 @@ struct RowWalk {
     __device__ __forceinline__ int place() const { return from > 0 ? 0 : 1; }
     // Whether this CTA has a part of the item at `from`: its tile exists and sees a page of the range.
     __device__ __forceinline__ bool set(const RowsArgs& a) {
-        to = (int)min((long long)item_pages(s, item, a), from + left);
-        tile = a.group == 1 ? item : item * a.group + (int)blockIdx.x % a.group;
+        to = min(item_pages(s, item, a), from + left);
+        tile = item * a.group + a.by_group.mod(blockIdx.x);
         if (tile >= s.tiles) return false;
         pages = tile_pages(s, tile, a);
         pg0 = from;
@@ -144,123 +175,110 @@ struct RowStart {
     int b, g, item, from;             // b < 0: nothing
     int each, pad[3];
 };
-constexpr int LINE_COST = 16;
 
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
-#pragma unroll
+#pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// The same where no lane has more than 2^26, which is all but always.
-__device__ __forceinline__ long long warp_sum_small(long long v) {
-    if (__all_sync(0xffffffffu, v < (1ll << 26))) return (long long)__reduce_add_sync(0xffffffffu, (unsigned)v);
-    return warp_sum_ll(v);
-}
-__device__ __forceinline__ long long warp_scan_ll(long long v, int lane) {      // sum over the lanes up to this one
-#pragma unroll
+__device__ __forceinline__ int warp_scan(int v, int lane) {        // sum over the lanes up to this one
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, v, o);
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += x;
     }
     return v;
-}
-// Quotients of numbers that hardly ever need 64 bits.
-__device__ __forceinline__ long long div_ll(long long x, long long y) {
-    return ((x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
-}
-
-// Pieces of one kv head's items of a sequence.
-__device__ __forceinline__ int seq_pieces(const SeqShape& s, int each, const RowsArgs& a) {
-    const int items = seq_items(s, a);
-    if (!a.causal || items <= 1) return items * ((s.pages + each - 1) / each);
-    int n = 0;
-    for (int i = 0; i < items; i++) n += (item_pages(s, i, a) + each - 1) / each;
-    return n;
 }
 
 // The start of this CTA, for one whole warp, into `at` (b < 0: nothing to do) and, for the joining launch, starts[CTA].
 __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt,
                                            const RowsArgs& a, RowWalk* at, RowStart* starts, int* status) {
-    const int lane = threadIdx.x & 31, cta = blockIdx.x / a.group;
-    const bool writes = a.group == 1 || blockIdx.x % a.group == 0;
-    long long total = 0, own = 0;
+    const int lane = threadIdx.x & 31, cta = a.by_group.div(blockIdx.x);
+    const bool writes = a.by_group.mod(blockIdx.x) == 0;
+    long long all = 0, own = 0;
+    int items = 0, longest = 0;
+    bool alike = true;                                             // every item of a sequence has its pages
     SeqShape s;
     s.tiles = s.pages = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         own = 0;
         if (b0 + lane < a.B) {
             s = seq_shape(cu_q, kv_len, pt, b0 + lane, a, status);
+            items = seq_items(s, a);
             own = seq_pages(s, a) * a.KV;
+            alike = !a.causal || items <= 1;
+            longest = s.pages;
         }
-        total += warp_sum_small(own);
+        all += own;
     }
-    const long long range = max((long long)a.min_range, div_ll(total + a.ctas - 1, a.ctas));
-    // Pieces, for up to 32 sequences: the least `each` of range .. range + LINE_COST that makes no more pieces than there are CTAs.
-    int each = 0;
-    if (a.B <= 32 && range < (1 << 20)) {
-        int lo = (int)range, hi = (int)range + LINE_COST + 1;
-        while (lo < hi) {                                      // hi: fits, or is beyond what pays
-            const int mid = (lo + hi) / 2;
-            const bool fits = warp_sum_small(s.tiles > 0 ? (long long)seq_pieces(s, mid, a) * a.KV : 0) <= a.ctas;
-            if (fits) hi = mid; else lo = mid + 1;
-        }
-        if (lo <= (int)range + LINE_COST) each = lo;
-    }
+    all = __all_sync(0xffffffffu, all < (1ll << 26)) ? (long long)__reduce_add_sync(0xffffffffu, (unsigned)all) : warp_sum_ll(all);
     if (lane == 0) at->b = -1;
-    __syncwarp();
-    long long base = 0, pieces = 0;
-    if (each > 0) {
-        pieces = s.tiles > 0 ? (long long)seq_pieces(s, each, a) * a.KV : 0;
-        total = warp_sum_small(pieces);
+    if (all > MAX_VISITS) {
+        if (lane == 0) atomicOr(status, MYNAH_ST_SPLIT_RANGE);
+        all = 0;
     }
-    const long long from = each > 0 ? cta : range * cta;       // in pieces, or in pages
-    if (from >= total) {
+    int total = (int)all;
+    const int range = max(a.min_range, a.by_ctas.div(total + a.ctas - 1));
+    // Pieces, for up to 32 sequences whose items are alike, where they pay.
+    int each = 0, n = 0;                                           // n: pieces of one of this lane's items
+    if (a.B <= 32 && __all_sync(0xffffffffu, alike)) {
+        const int lots = (int)__reduce_add_sync(0xffffffffu, (unsigned)items) * a.KV;
+        if (lots > 0 && lots <= a.ctas) {
+            longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
+            const int most = quotient(a.ctas, lots);
+            each = max(a.min_range, quotient(longest + most - 1, most));
+            if (each > range + LINE_COST) {
+                each = 0;
+            } else {
+                n = quotient(s.pages + each - 1, each);
+                own = (long long)(items * n) * a.KV;
+                total = (int)__reduce_add_sync(0xffffffffu, (unsigned)own);
+            }
+        }
+    }
+    const long long from64 = each > 0 ? cta : (long long)range * cta;      // in pieces, or in pages
+    __syncwarp();
+    if (from64 >= total) {
         if (lane == 0 && writes) starts[cta].b = -1;
         return;
     }
+    const int from = (int)from64;
+    int base = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-        if (a.B > 32) {                                        // (of up to 32 sequences every lane still has its own)
+        if (a.B > 32) {                                            // (of up to 32 sequences every lane still has its own)
             own = 0;
             if (b0 + lane < a.B) {
                 s = seq_shape(cu_q, kv_len, pt, b0 + lane, a, status);
                 own = seq_pages(s, a) * a.KV;
             }
         }
-        const long long mine = each > 0 ? pieces : own, incl = warp_scan_ll(mine, lane), excl = incl - mine;
-        if (mine > 0 && from >= base + excl && from < base + incl) {
+        const int mine = (int)own, incl = a.B == 1 ? mine : warp_scan(mine, lane);
+        int x = from - base - (incl - mine);                       // within this lane's sequence
+        if (x >= 0 && x < mine) {
             RowWalk w;
             w.b = b0 + lane;
             w.s = s;
-            const long long head = div_ll(mine, a.KV);         // one kv head's
-            long long x = from - base - excl;
-            w.g = (int)div_ll(x, head);
+            const int head = a.by_KV.div(mine);                    // one kv head's
+            w.g = quotient(x, head);
             x -= w.g * head;
             w.item = 0;
-            if (each > 0) {
-                int p = item_pages(s, 0, a), n = (p + each - 1) / each;
-                if (!a.causal) {
-                    w.item = (int)x / n;
-                    x -= (long long)w.item * n;
-                } else {
-                    while (x >= n) {
-                        x -= n;
-                        p = item_pages(s, ++w.item, a);
-                        n = (p + each - 1) / each;
-                    }
+            if (!a.causal) {
+                const int one = each > 0 ? n : s.pages;            // of one item
+                w.item = quotient(x, one);
+                x -= w.item * one;
+            } else if (each == 0) {
+                int p = item_pages(s, 0, a);
+#pragma unroll 1
+                while (x >= p) {
+                    x -= p;
+                    p = item_pages(s, ++w.item, a);
                 }
-                w.left = (p + n - 1) / n;                      // pieces of one size
-                w.from = (int)(x * w.left);
-            } else {
-                w.left = range;
-                if (!a.causal) {
-                    w.item = (int)div_ll(x, s.pages);
-                    x -= (long long)w.item * s.pages;
-                } else {
-                    for (int p; x >= (p = item_pages(s, w.item, a)); w.item++) x -= p;
-                }
-                w.from = (int)x;
             }
-            if (writes) starts[cta] = RowStart{w.b, w.g, w.item, w.from, (int)min(w.left, 0x7fffffffll)};
+            w.left = each > 0 ? quotient(s.pages + n - 1, n) : range;      // pieces of one size
+            w.from = each > 0 ? x * w.left : x;
+            if (writes) starts[cta] = RowStart{w.b, w.g, w.item, w.from, w.left};
             // (a piece is one segment: what is left of it when the item ends is nobody's)
             const bool has = w.set(a);
             if (each > 0) w.left = w.to - w.from;
