@@ -133,8 +133,9 @@ int launch_mass_generic(const void* q, const void* k, const float* lse, float* m
     const size_t smem = (size_t)(GK + GR) * (a.r.HD + 4) * sizeof(float);
     auto kf = attn_mass_kernel<float>;
     auto kb = attn_mass_kernel<bf16>;
-    const cudaError_t e = dtype == MYNAH_F32 ? cudaFuncSetAttribute(kf, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)
-                                             : cudaFuncSetAttribute(kb, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> opted_f{0}, opted_b{0};
+    constexpr size_t most = (size_t)(GK + GR) * (256 + 4) * sizeof(float);
+    const cudaError_t e = dtype == MYNAH_F32 ? shared_memory_once(kf, most, opted_f) : shared_memory_once(kb, most, opted_b);
     if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
     if (dtype == MYNAH_F32) kf<<<grid, 256, smem, stream>>>((const float*)q, (const float*)k, lse, mass, part, cu_q, kv_len, pt, a, status);
     else kb<<<grid, 256, smem, stream>>>((const bf16*)q, (const bf16*)k, lse, mass, part, cu_q, kv_len, pt, a, status);

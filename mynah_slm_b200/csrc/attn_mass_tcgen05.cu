@@ -233,7 +233,8 @@ int go(const CUtensorMap& mq, const CUtensorMap& mk, const float* lse, float* ma
        PageTable pt, const MassArgs& a, int n_ids, int* status, cudaStream_t stream) {
     constexpr size_t smem = 3 * (size_t)(HD / 64) * HALF_BYTES + 4 * 128 * sizeof(float) + 80 + 1024;
     auto kern = attn_mass_tcgen05_kernel<HD>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> opted{0};
+    const cudaError_t e = shared_memory_once(kern, smem, opted);
     if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
     kern<<<(unsigned)(mass_units_max(a, n_ids) * a.r.KV), THREADS, smem, stream>>>(mq, mk, lse, mass, part, cu_q, kv_len, pt, a, status);
     return mynah_check_launch("attn_mass");

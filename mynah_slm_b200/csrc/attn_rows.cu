@@ -18,6 +18,7 @@ namespace {
 
 constexpr int KT = 32;               // keys a tile of the general kernel
 constexpr int MAX_HEAD = 256;
+constexpr size_t MOST_SHARED = 226 * 1024;        // (heads of 256 and 64 rows in fp32 take 209 KB)
 
 __device__ __forceinline__ float max_or_nan(float a, float b) {
     float d;
@@ -319,7 +320,8 @@ int go(const void* q, void* out, const RowsArgs& a, const void* k, const void* v
     constexpr int R = 4 * TY;
     const size_t smem = (size_t)R * (a.HD + 4) * 4 + (size_t)R * (KT + 4) * 4 + 4 * (size_t)KT * pitch_of<T>(a.HD) * sizeof(T);
     auto kern = attn_rows_kernel<T, TY, TX, NC>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> opted{0};
+    const cudaError_t e = shared_memory_once(kern, MOST_SHARED, opted);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
     kern<<<a.ctas * a.group, TY * TX, smem, stream>>>((const T*)q, (T*)out, (const T*)k, (const T*)v, cu_q, kv_len, pt, masks, a, s, status);
     return mynah_check_launch("attn_rows");

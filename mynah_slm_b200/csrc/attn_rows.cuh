@@ -3,6 +3,8 @@
 #pragma once
 #include "row_units.cuh"
 
+#include <atomic>
+
 // Partial results of cut items, and what every launch of one call reads.
 struct RowsScratch {
     RowStart* starts;                 // [ctas]: where every CTA begins
@@ -30,6 +32,16 @@ __device__ __forceinline__ float ex2_f(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Lets a kernel use so much shared memory, once a device (`done` has a bit for each).
+template <typename K> static inline cudaError_t shared_memory_once(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1ull))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
 }
 
 // A launch that may begin while the kernel before it on the stream finishes; the kernel waits for that one's results itself

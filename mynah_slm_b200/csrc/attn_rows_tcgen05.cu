@@ -426,7 +426,8 @@ int go(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cons
        const long long* masks, const RowsArgs& a, void* out, RowsScratch s, int* status, cudaStream_t stream) {
     constexpr size_t smem = (size_t)(HD / 64) * (NT * HALF_BYTES + 2 * STAGES<HD, NT> * PAGE_BYTES) + NT * 4 * 32 * STAGE_PITCH * 4 + 448 + 1024;
     auto kern = attn_rows_tcgen05_kernel<HD, NT>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> opted{0};
+    const cudaError_t e = shared_memory_once(kern, smem, opted);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
     kern<<<a.ctas * a.group, 96 + 128 * NT, smem, stream>>>(mq, mk, mv, (const bf16*)v, cu_q, kv_len, pt, masks, a, (bf16*)out, s, status);
     return mynah_check_launch("attn_rows");

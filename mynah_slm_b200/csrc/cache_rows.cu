@@ -1,13 +1,14 @@
 // Rows of the paged cache that stay and rows that go: the eviction of the rows that gathered the least attention, and the
 // acceptance of a drafted tree's path. Both end in moving rows of K and V to lower rows of the same sequence, for all layers
 // that share the page lists, in one launch.
-#include "layout.cuh"
+#include "attn_rows.cuh"
 
 namespace {
 
 // ------------------------------------------------------------------ choosing
 
 constexpr int CH_THREADS = 512, CH_WARPS = CH_THREADS / 32;
+constexpr int CH_BITS = 11, CH_BINS = 1 << CH_BITS;       // of a word that one pass settles (the last pass: the ten that are left)
 
 // A sum's order as an unsigned word: greater sums have greater words, both zeros the same one, a NaN the greatest.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -22,15 +23,17 @@ struct EvictArgs {
 
 // One CTA for one (layer, sequence, kv head): the rows that stay, ascending. Of n > keep rows the first `first` and the last
 // `recent` stay anyway; of those between them the `need` = keep - first - recent with the greatest sums. The need-th greatest
-// word is found eight bits at a time (a histogram of the words that still agree with it in the bits above, the bin that holds
-// it, and so on: the words are read five times in all, from shared memory where they fit); then one walk over the rows in
-// order writes those above it, and of those equal to it the first ones.
+// word is found in three passes, 11, 11 and 10 bits (a histogram of the words that still agree with it in the bits above, the bin
+// that holds it, and so on); then every warp takes a run of rows, counts those above it and those equal to it, and, once it
+// knows the counts of the runs before, writes its own: those above, and the first of the equal ones. The words are read from
+// memory once where they fit shared memory. Bound by its chain of barriers and passes: 448 choices of 2,048 of 4,100 rows,
+// CHOOSE us.
 __global__ void __launch_bounds__(CH_THREADS)
 evict_choose_kernel(const float* __restrict__ mass, PageTable pt, const int* __restrict__ kv_len, EvictArgs a, int* __restrict__ kept,
                     int* __restrict__ new_len, int* __restrict__ status) {
     extern __shared__ uint32_t words_s[];
-    __shared__ int hist[256];
-    __shared__ int warp_s[CH_WARPS];
+    __shared__ int hist[CH_BINS];
+    __shared__ int warp_s[CH_WARPS], equal_s[CH_WARPS];
     __shared__ int found[2];
     const int unit = blockIdx.x, g = unit % a.KV, b = unit / a.KV % a.B, e = unit / a.KV / a.B;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -41,100 +44,121 @@ evict_choose_kernel(const float* __restrict__ mass, PageTable pt, const int* __r
         for (int i = tid; i < a.keep; i += CH_THREADS) out[i] = i < n ? i : -1;
         return;
     }
-    const float* m = mass + (size_t)e * a.n_pages * a.KV * PAGE_TOKENS;
+    const float* m = mass + ((size_t)e * a.n_pages * a.KV + g) * PAGE_TOKENS;
     const int lo = a.first, hi = n - a.recent, need = a.keep - a.first - a.recent;
     const bool cached = hi - lo <= a.cached;
+    const int list0 = pt.indptr[b] - pt.base[b], list_lo = pt.indptr[b], list_hi = pt.indptr[b + 1];
     bool bad = false;
     auto word_at = [&](int r) {
-        const int page = page_of(pt, b, r);
-        if (page < 0) {
+        const int at = list0 + r / PAGE_TOKENS;
+        int page = at >= list_lo && at < list_hi ? pt.ids[at] : -1;
+        if (page < 0 || page >= a.n_pages) {
             bad = true;
             return 0u;
         }
-        return order_of(m[((size_t)page * a.KV + g) * PAGE_TOKENS + r % PAGE_TOKENS]);
+        return order_of(m[(size_t)page * a.KV * PAGE_TOKENS + r % PAGE_TOKENS]);
     };
     auto word = [&](int r) { return cached ? words_s[r - lo] : word_at(r); };
-    if (cached)
+    for (int i = tid; i < CH_BINS; i += CH_THREADS) hist[i] = 0;
+    if (cached && need > 0) {
+#pragma unroll 8
         for (int r = lo + tid; r < hi; r += CH_THREADS) words_s[r - lo] = word_at(r);
+    }
     uint32_t prefix = 0;
     int left = need;                                       // the left-th greatest among the words with this prefix is sought
-    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+    for (int pass = 0; pass < 3 && need > 0; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u, mask = pass == 2 ? 1023u : 2047u;
+        __syncthreads();                                   // (words and empty bins)
+#pragma unroll 4
         for (int r = lo + tid; r < hi; r += CH_THREADS) {
             const uint32_t w = word(r);
-            if ((w & above) == prefix) atomicAdd(&hist[(w >> shift) & 255], 1);
+            if ((w & above) == prefix) atomicAdd(&hist[(w >> shift) & mask], 1);
         }
         __syncthreads();
-        if (warp == 0) {                                   // bins from the greatest down, eight a lane
-            int own[8], sum = 0;
+        // bins from the greatest down, four a thread
+        int own[4], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                own[i] = hist[255 - (lane * 8 + i)];
-                sum += own[i];
-            }
-            int incl = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
-            }
-            int before = incl - sum;
-            if (before < left && incl >= left) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (before < left && before + own[i] >= left) {
-                        found[0] = 255 - (lane * 8 + i);
-                        found[1] = left - before;
-                        break;
-                    }
-                    before += own[i];
-                }
-            }
+        for (int i = 0; i < 4; i++) {
+            own[i] = hist[CH_BINS - 1 - (tid * 4 + i)];
+            sum += own[i];
         }
-        __syncthreads();
-        prefix |= (uint32_t)found[0] << shift;
-        left = found[1];
-        __syncthreads();
-    }
-    // `left` of the words equal to `prefix` stay, the first ones. A row's place: those above before it, the equal ones before it
-    // up to `left`, and the rows that stay anyway; counted over the CTA, a slab of rows at a time.
-    int above0 = 0, equal0 = 0;                            // before this slab
-    for (int r0 = 0; r0 < n; r0 += CH_THREADS) {
-        const int r = r0 + tid;
-        bool sure = false, equal = false;
-        if (r < n) {
-            if (r < lo || r >= hi) sure = true;
-            else if (need > 0) {
-                const uint32_t w = word(r);
-                sure = w > prefix;
-                equal = w == prefix;
-            }
-        }
-        const unsigned bs = __ballot_sync(0xffffffffu, sure), be = __ballot_sync(0xffffffffu, equal), under = (1u << lane) - 1u;
-        if (lane == 0) warp_s[warp] = __popc(bs) | __popc(be) << 16;
-        __syncthreads();
-        int s = lane < CH_WARPS ? warp_s[lane] : 0;        // (counts of a slab stay below 2^16)
-        int incl = s;
+        int incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        const int total = __shfl_sync(0xffffffffu, incl, 31), mine = __shfl_sync(0xffffffffu, incl - s, warp);
-        const int sb = above0 + (mine & 0xffff) + __popc(bs & under), eb = equal0 + (mine >> 16) + __popc(be & under);
-        if (sure || (equal && eb < left)) out[sb + min(eb, left)] = r;
-        above0 += total & 0xffff;
-        equal0 += total >> 16;
+        if (lane == 31) warp_s[warp] = incl;
         __syncthreads();
+        int before = incl - sum;
+        for (int i = 0; i < warp; i++) before += warp_s[i];
+        if (before < left && before + sum >= left) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (before < left && before + own[i] >= left) {
+                    found[0] = CH_BINS - 1 - (tid * 4 + i);
+                    found[1] = left - before;
+                    break;
+                }
+                before += own[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) hist[CH_BINS - 1 - (tid * 4 + i)] = 0;
+        __syncthreads();
+        prefix |= (uint32_t)found[0] << shift;
+        left = found[1];
+    }
+    // `left` of the words equal to `prefix` stay, the first ones. A row's place: those above before it, the equal ones before it
+    // up to `left`, and the rows that stay anyway.
+    const int run = (n + CH_THREADS - 1) / CH_THREADS * 32, r_begin = warp * run, r_end = min(n, r_begin + run);
+    auto kind = [&](int r, bool& sure, bool& equal) {
+        sure = equal = false;
+        if (r >= r_end) return;
+        if (r < lo || r >= hi) {
+            sure = true;
+        } else if (need > 0) {
+            const uint32_t w = word(r);
+            sure = w > prefix;
+            equal = w == prefix;
+        }
+    };
+    int n_sure = 0, n_equal = 0;
+    for (int r0 = r_begin; r0 < r_end; r0 += 32) {
+        bool sure, equal;
+        kind(r0 + lane, sure, equal);
+        n_sure += __popc(__ballot_sync(0xffffffffu, sure));
+        n_equal += __popc(__ballot_sync(0xffffffffu, equal));
+    }
+    __syncthreads();                                       // (warp_s is read above)
+    if (lane == 0) {
+        warp_s[warp] = n_sure;
+        equal_s[warp] = n_equal;
+    }
+    __syncthreads();
+    int sure0 = 0, equal0 = 0;
+    for (int i = 0; i < warp; i++) {
+        sure0 += warp_s[i];
+        equal0 += equal_s[i];
+    }
+    for (int r0 = r_begin; r0 < r_end; r0 += 32) {
+        bool sure, equal;
+        kind(r0 + lane, sure, equal);
+        const unsigned bs = __ballot_sync(0xffffffffu, sure), be = __ballot_sync(0xffffffffu, equal), under = (1u << lane) - 1u;
+        const int eb = equal0 + __popc(be & under);
+        if (sure || (equal && eb < left)) out[sure0 + __popc(bs & under) + min(eb, left)] = r0 + lane;
+        sure0 += __popc(bs);
+        equal0 += __popc(be);
     }
     if (bad) atomicOr(status, MYNAH_ST_PAGE_RANGE);
 }
 
 // -------------------------------------------------------------------- moving
 
-constexpr int MV_THREADS = 256, MV_UNROLL = 4;
+constexpr int MV_THREADS = 256, MV_UNROLL = 8;
+constexpr int MV_ROWS = MV_THREADS / 8 * MV_UNROLL;       // rows a step: eight lanes a row, 16 bytes a lane
+constexpr int MV_BATCH = 4 * MV_ROWS;                     // rows whose places are worked out together
 
 struct MoveArgs {
     int B, KV, n_pages, keep;
@@ -146,75 +170,88 @@ struct MoveArgs {
 // Rows kept[i] -> i of one (layer, sequence, kv head), one slice of up to 128 bytes of every row of K or of V, or the sums.
 // i <= kept[i], ascending. In the same pages a row is read before it is written over: a step's rows are all in registers, the
 // next step's already asked for, when the barrier lets the step's writes go; and a row that is written in a step is a source of
-// that step or of an earlier one. 128 rows a step in flight, 256 with the next.
+// that step or of an earlier one. Places are worked out 1,024 rows ahead, so that the copies wait for one read, not for the
+// choice, the page list and the row one behind the other (28 layers of 2 sequences, 2,048 rows of 8 heads of 128: 265 -> MOVE us).
 __global__ void __launch_bounds__(MV_THREADS)
 evict_move_kernel(uint4* __restrict__ k, uint4* __restrict__ v, float* __restrict__ mass, PageTable from, PageTable to,
                   const int* __restrict__ kv_len, const int* __restrict__ kept, MoveArgs a, int* __restrict__ status) {
+    __shared__ int src_s[2][MV_BATCH], dst_s[2][MV_BATCH];         // rows of the layer's storage, -1: none
     const int unit = blockIdx.x, g = unit % a.KV, b = unit / a.KV % a.B, e = unit / a.KV / a.B;
     const int held = max(0, kv_len[b]);
     const int n = min(held, a.keep);
     if (n == 0 || (a.same && held <= a.keep)) return;      // nothing moves
     const int* src = kept + (size_t)unit * a.keep;
-    const size_t page0 = (size_t)e * a.n_pages * a.KV + g;
+    const size_t row0 = (size_t)e * a.n_pages * a.KV * PAGE_TOKENS;        // the layer's first row
     bool bad = false;
-    // index of a row (of 64 a page) in a layer's storage, or -1
-    auto row_of = [&](const PageTable& pt, int r) -> long long {
+    // a row of the layer's storage, or -1 (the launch is refused where these do not fit 31 bits)
+    auto row_of = [&](const PageTable& pt, int r) {
         const int page = page_of(pt, b, r);
         if (page < 0) {
             bad = true;
             return -1;
         }
-        return (long long)(page0 + (size_t)page * a.KV) * PAGE_TOKENS + r % PAGE_TOKENS;
+        return (page * a.KV + g) * PAGE_TOKENS + r % PAGE_TOKENS;
+    };
+    auto places = [&](int i0, int buf) {
+#pragma unroll
+        for (int j = 0; j < MV_BATCH / MV_THREADS; j++) {
+            const int i = i0 + j * MV_THREADS + threadIdx.x;
+            src_s[buf][j * MV_THREADS + threadIdx.x] = i < n ? row_of(from, src[i]) : -1;
+            dst_s[buf][j * MV_THREADS + threadIdx.x] = i < n ? row_of(to, i) : -1;
+        }
     };
     const int sl = blockIdx.y;
     if (sl == a.k_slices + a.v_slices) {                   // the sums, a row a thread
-        float x[MV_UNROLL], y[MV_UNROLL];
-        constexpr int STEP = MV_THREADS * MV_UNROLL;
-        auto load = [&](int i0, float (&w)[MV_UNROLL]) {
+        float* t = mass + row0;
+        constexpr int EACH = MV_BATCH / MV_THREADS;
+        places(0, 0);
+        for (int i0 = 0, buf = 0; i0 < n; i0 += MV_BATCH, buf ^= 1) {
+            float x[EACH];
 #pragma unroll
-            for (int j = 0; j < MV_UNROLL; j++) {
-                const int i = i0 + j * MV_THREADS + threadIdx.x;
-                const long long s = i < n ? row_of(from, src[i]) : -1;
-                w[j] = s >= 0 ? mass[s] : 0.f;
+            for (int j = 0; j < EACH; j++) {               // (a thread reads the places that it wrote itself)
+                const int s = src_s[buf][j * MV_THREADS + threadIdx.x];
+                x[j] = s >= 0 ? t[s] : 0.f;
             }
-        };
-        load(0, x);
-        for (int i0 = 0; i0 < n; i0 += STEP) {
-            load(i0 + STEP, y);
+            places(i0 + MV_BATCH, buf ^ 1);
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < MV_UNROLL; j++) {
-                const int i = i0 + j * MV_THREADS + threadIdx.x;
-                const long long d = i < n ? row_of(to, i) : -1;
-                if (d >= 0) mass[d] = x[j];
-                x[j] = y[j];
+            for (int j = 0; j < EACH; j++) {
+                const int d = dst_s[buf][j * MV_THREADS + threadIdx.x];
+                if (d >= 0 && src_s[buf][j * MV_THREADS + threadIdx.x] >= 0) t[d] = x[j];
             }
         }
     } else {
         const bool is_k = sl < a.k_slices;
-        uint4* t = is_k ? k : v;
         const int pieces = is_k ? a.k_pieces : a.v_pieces, at = (is_k ? sl : sl - a.k_slices) * 8 + (threadIdx.x & 7);
+        uint4* t = (is_k ? k : v) + row0 * pieces + at;
         const bool on = at < pieces;
         const int row = threadIdx.x >> 3;
-        constexpr int ROWS = MV_THREADS / 8, STEP = ROWS * MV_UNROLL;
         uint4 x[MV_UNROLL], y[MV_UNROLL];
-        auto load = [&](int i0, uint4 (&w)[MV_UNROLL]) {
+        auto load = [&](int i0, uint4 (&w)[MV_UNROLL]) {   // the step from row i0 on
+            const int* s = src_s[(i0 / MV_BATCH) & 1] + i0 % MV_BATCH;
 #pragma unroll
             for (int j = 0; j < MV_UNROLL; j++) {
-                const int i = i0 + j * ROWS + row;
-                const long long s = i < n && on ? row_of(from, src[i]) : -1;
-                w[j] = s >= 0 ? t[s * pieces + at] : make_uint4(0u, 0u, 0u, 0u);
+                const int r = s[j * (MV_THREADS / 8) + row];
+                if (r >= 0 && on) w[j] = t[(size_t)r * pieces];
             }
         };
+        places(0, 0);
+        __syncthreads();
         load(0, x);
-        for (int i0 = 0; i0 < n; i0 += STEP) {
-            load(i0 + STEP, y);
+        for (int i0 = 0; i0 < n; i0 += MV_ROWS) {
+            // the next step's rows; in a batch's last step its successor's places first
+            if (i0 % MV_BATCH == MV_BATCH - MV_ROWS) {
+                places(i0 + MV_ROWS, ((i0 + MV_ROWS) / MV_BATCH) & 1);
+                __syncthreads();
+            }
+            if (i0 + MV_ROWS < n) load(i0 + MV_ROWS, y);
             __syncthreads();
+            const int* d = dst_s[(i0 / MV_BATCH) & 1] + i0 % MV_BATCH;
+            const int* s = src_s[(i0 / MV_BATCH) & 1] + i0 % MV_BATCH;
 #pragma unroll
             for (int j = 0; j < MV_UNROLL; j++) {
-                const int i = i0 + j * ROWS + row;
-                const long long d = i < n && on ? row_of(to, i) : -1;
-                if (d >= 0) t[d * pieces + at] = x[j];
+                const int q = j * (MV_THREADS / 8) + row, r = d[q];
+                if (r >= 0 && s[q] >= 0 && on) t[(size_t)r * pieces] = x[j];
                 x[j] = y[j];
             }
         }
@@ -325,14 +362,15 @@ MYNAH_API int mynah_cache_evict(void* k, void* v, float* mass, int E, int B, int
     MYNAH_REQUIRE(row_ok(k_bytes) && row_ok(v_bytes), "cache_evict: rows of %d and %d bytes are not whole 16-byte pieces", k_bytes, v_bytes);
     MYNAH_REQUIRE(((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0, "cache_evict: the cache must be 16-byte aligned");
     MYNAH_REQUIRE(keep > 0 && recent >= 0 && first >= 0 && (long long)recent + first <= keep, "cache_evict: keep %d, recent %d and first %d do not go together", keep, recent, first);
-    MYNAH_REQUIRE((long long)E * B * KV < (1ll << 31), "cache_evict: launch too large");
+    MYNAH_REQUIRE((long long)E * B * KV < (1ll << 31) && (long long)n_pages * KV * PAGE_TOKENS < (1ll << 31), "cache_evict: launch too large");
     MYNAH_REQUIRE(status != nullptr && kept != nullptr && new_len != nullptr && mass != nullptr, "cache_evict: outputs, sums and a status word are required");
     const PageTable from{page_indptr, page_ids, page_base, n_pages}, to{out_indptr, out_ids, out_base, n_pages};
     // words of up to 96 KB a CTA (two CTAs an SM) are kept in shared memory; longer rows are read again from L2
     const long long most = (long long)n_ids * PAGE_TOKENS;
     const int cached = (int)(most < 24576 ? most : 24576);
     const EvictArgs ea{E, B, KV, n_pages, keep, recent, first, cached};
-    const cudaError_t err = cudaFuncSetAttribute(evict_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cached * 4);
+    static std::atomic<unsigned long long> opted{0};
+    const cudaError_t err = shared_memory_once(evict_choose_kernel, 24576 * 4, opted);
     if (err != cudaSuccess) return mynah_fail("cache_evict: %s", cudaGetErrorString(err));
     evict_choose_kernel<<<(unsigned)(E * B * KV), CH_THREADS, (size_t)cached * 4, stream>>>(mass, from, kv_len, ea, kept, new_len, status);
     if (mynah_check_launch("evict_choose")) return -1;

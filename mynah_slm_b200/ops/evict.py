@@ -8,6 +8,7 @@ is, while the tokens that follow are rotated for their true positions.)
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -15,12 +16,17 @@ import torch
 from ..cache.pages import PAGE_TOKENS
 from . import lib
 from .kernels import PageTableView
-from .lib import KernelError, call, code, stream_ptr
+from .lib import KernelError, call, code, stream_on
 from .tree import _row_stride, check_layers, check_lists, check_rows, row_scratch
 
 
+@lru_cache(maxsize=256)
+def _mass_scratch(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dcode: int, n_ids: int) -> int:
+    return int(lib.load().mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dcode, n_ids))
+
+
 def attn_mass_scratch_floats(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dtype: torch.dtype, n_ids: int) -> int:
-    return int(lib.load().mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, code(dtype), n_ids))
+    return _mass_scratch(T, B, max_q_len, H, KV, HD, code(dtype), n_ids)
 
 
 def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor,
@@ -31,7 +37,7 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
     head's query heads give it, added to what it holds for rows that were there before the step, in place of it for the step's own
     (so nothing has to be cleared when a page is taken). Other rows' sums are left as they are. The order of the sums does not
     depend on timing."""
-    check_rows("attn_mass", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
+    dt = check_rows("attn_mass", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
     T = q.shape[0]
     if mass.dtype != torch.float32 or mass.device != q.device or not mass.is_contiguous() or mass.dim() != 3 \
             or mass.shape[1:] != (KV, PAGE_TOKENS) or mass.shape[0] < pages.n_pages:
@@ -39,14 +45,12 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
                           f"got {tuple(mass.shape)} {mass.dtype}")
     if T == 0 or ctx.B == 0:
         return
-    dt = code(q.dtype)
     n_ids = pages.ids.numel()
-    L = lib.load()
-    scratch = row_scratch("attn_mass", scratch, L.mynah_attn_mass_scratch_floats(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids), q.device)
+    scratch = row_scratch("attn_mass", scratch, _mass_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids), q.device)
     call("mynah_attn_mass", q.data_ptr(), out.data_ptr(), mass.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q),
          _row_stride(out), k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(),
          pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, n_ids, float(scale), scratch.data_ptr(), scratch.numel(),
-         ctx.status.data_ptr(), stream_ptr())
+         ctx.status.data_ptr(), stream_on(q.device.index))
 
 
 def cache_evict(k_caches: torch.Tensor, v_caches: torch.Tensor, masses: torch.Tensor, ctx, pages: PageTableView, keep: int, recent: int,
@@ -84,5 +88,5 @@ def cache_evict(k_caches: torch.Tensor, v_caches: torch.Tensor, masses: torch.Te
     call("mynah_cache_evict", k_caches.data_ptr(), v_caches.data_ptr(), masses.data_ptr(), E, ctx.B, KV, n_pages, HD * es,
          v_caches.shape[4] * es, ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(),
          pages.ids.numel(), out_pages.indptr.data_ptr(), out_pages.ids.data_ptr(), out_pages.base.data_ptr(), 1 if same else 0,
-         keep, recent, first, kept.data_ptr(), new_len.data_ptr(), ctx.status.data_ptr(), stream_ptr())
+         keep, recent, first, kept.data_ptr(), new_len.data_ptr(), ctx.status.data_ptr(), stream_on(dev.index))
     return kept, new_len

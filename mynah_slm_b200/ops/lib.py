@@ -302,6 +302,11 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_on(index: int) -> int:
+    """The current stream of a device by its index, without making a Stream object (3 us of a call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
 

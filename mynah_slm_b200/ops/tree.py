@@ -9,6 +9,7 @@ past + 0, 1, 2, ..., where a sequence that had taken the tokens one by one would
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import numpy as np
@@ -17,7 +18,10 @@ import torch
 from ..cache.pages import PAGE_TOKENS
 from . import lib
 from .kernels import MAX_HEAD_DIM, PageTableView
-from .lib import KernelError, call, code, stream_ptr
+from .lib import KernelError, call, code, stream_on
+
+_INF = float("inf")
+_I32 = torch.int32
 
 
 def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> tuple[np.ndarray, np.ndarray]:
@@ -42,42 +46,43 @@ def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> tuple[np.n
 
 
 def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor,
-               v_cache: torch.Tensor, pages: PageTableView, scale: float) -> None:
-    """What the attention of a few rows a sequence asks of its arguments."""
-    dev = q.device
+               v_cache: torch.Tensor, pages: PageTableView, scale: float) -> int:
+    """What the attention of a few rows a sequence asks of its arguments. Returns q's type code."""
+    dev, dt = q.device, q.dtype
     if not q.is_cuda or dev.index != torch.cuda.current_device():
         raise KernelError(f"{who}: q is not on the current CUDA device")
     if KV < 1 or H < 1 or H % KV:
         raise KernelError(f"{who}: {H} heads over {KV} kv heads")
     if HD < 1 or HD % 8 or HD > MAX_HEAD_DIM:
         raise KernelError(f"{who}: head_dim {HD} is no multiple of 8 up to {MAX_HEAD_DIM}")
-    if not 0.0 <= scale < float("inf"):
+    if not 0.0 <= scale < _INF:
         raise KernelError(f"{who}: the score scale {scale} is not a positive number, nor 0 for 1 / sqrt(head_dim)")
-    code(q.dtype)
-    for t, name in ((q, "q"), (out, "the output")):
-        if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] < H * HD or (t.shape[0] > 1 and t.stride(0) < H * HD):
-            raise KernelError(f"{who}: {name} must be rows of at least {H * HD} values, one row behind the other")
-        if t.dtype != q.dtype or t.device != dev:
-            raise KernelError(f"{who}: {name} is {t.dtype} on {t.device}, q {q.dtype} on {dev}")
-    if out.shape[0] < q.shape[0]:
-        raise KernelError(f"{who}: {out.shape[0]} output rows for {q.shape[0]} rows")
-    for t, name in ((k_cache, "K cache"), (v_cache, "V cache")):
-        if t.dtype != q.dtype or t.device != dev or not t.is_contiguous() or t.dim() != 4 or t.shape[1:] != (KV, PAGE_TOKENS, HD) \
-                or t.shape[0] < pages.n_pages:
-            raise KernelError(f"{who}: the {name} must be contiguous [{pages.n_pages}, {KV}, {PAGE_TOKENS}, {HD}] of q's type and device, "
-                              f"got {tuple(t.shape)} {t.dtype}")
+    dcode = code(dt)
+    width = H * HD
+    for t in (q, out):
+        shape = t.shape
+        if len(shape) != 2 or shape[1] < width or t.stride(1) != 1 or (shape[0] > 1 and t.stride(0) < width):
+            raise KernelError(f"{who}: q and the output must be rows of at least {width} values, one row behind the other, got "
+                              f"{tuple(shape)} with strides {t.stride()}")
+    if out.dtype != dt or out.device != dev or out.shape[0] < q.shape[0]:
+        raise KernelError(f"{who}: the output is {tuple(out.shape)} {out.dtype} on {out.device}, q {tuple(q.shape)} {dt} on {dev}")
+    cache = (KV, PAGE_TOKENS, HD)
+    for t in (k_cache, v_cache):
+        shape = t.shape
+        if t.dtype != dt or t.device != dev or len(shape) != 4 or shape[1:] != cache or shape[0] < pages.n_pages or not t.is_contiguous():
+            raise KernelError(f"{who}: the cache must be contiguous [{pages.n_pages}, {KV}, {PAGE_TOKENS}, {HD}] of q's type and device, "
+                              f"got {tuple(t.shape)} {t.dtype} on {t.device}")
     if ctx.B < 0 or ctx.max_q_len < 0:
         raise KernelError(f"{who}: {ctx.B} sequences of up to {ctx.max_q_len} rows")
     check_lists(who, dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
+    return dcode
 
 
 def check_lists(who: str, dev, B: int, cu_q: Optional[torch.Tensor], kv_len: torch.Tensor, pages: PageTableView, status: torch.Tensor) -> None:
-    for t, n, name in ((cu_q, B + 1, "cu_q"), (kv_len, B, "kv_len"), (pages.indptr, B + 1, "the page lists' bounds"),
-                       (pages.base, B, "the page lists' first pages"), (pages.ids, 0, "the page lists"), (status, 1, "the status word")):
-        if t is None:
-            continue
-        if t.dtype != torch.int32 or t.device != dev or t.numel() < n or not t.is_contiguous():
-            raise KernelError(f"{who}: {name} must be at least {n} contiguous int32 on {dev}")
+    for t, n in ((cu_q, B + 1), (kv_len, B), (pages.indptr, B + 1), (pages.base, B), (pages.ids, 0), (status, 1)):
+        if t is not None and (t.dtype != _I32 or t.device != dev or t.numel() < n or not t.is_contiguous()):
+            raise KernelError(f"{who}: cu_q, kv_len, the page lists and the status word must be contiguous int32 on {dev} for {B} sequences, "
+                              f"got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -86,14 +91,19 @@ def _row_stride(t: torch.Tensor) -> int:
 
 def row_scratch(who: str, scratch: Optional[torch.Tensor], need: int, dev) -> torch.Tensor:
     if scratch is None:
-        return torch.empty((need,), dtype=torch.float32, device=dev)
+        return torch.empty(need, dtype=torch.float32, device=dev)
     if scratch.dtype != torch.float32 or scratch.device != dev or not scratch.is_contiguous() or scratch.numel() < need:
         raise KernelError(f"{who}: scratch must be at least {need} contiguous float32 on {dev}")
     return scratch
 
 
+@lru_cache(maxsize=256)
+def _tree_scratch(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dcode: int) -> int:
+    return int(lib.load().mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dcode))
+
+
 def attn_tree_scratch_floats(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dtype: torch.dtype) -> int:
-    return int(lib.load().mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, code(dtype)))
+    return _tree_scratch(T, B, max_q_len, H, KV, HD, code(dtype))
 
 
 def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -106,30 +116,28 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
     1 / sqrt(HD). ctx: the step's description (B, max_q_len, cu_q, kv_len, status). Rows of the cache that a row does not see
     have no influence on it, whatever they hold. float32 and bfloat16, heads of any multiple of 8 up to 256; bfloat16 heads of 64
     and 128 run on the tensor cores. `scratch`: attn_tree_scratch_floats fp32 words, taken from torch's allocator unless given."""
-    check_rows("attn_tree", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
+    dt = check_rows("attn_tree", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
     T = q.shape[0]
     if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] < T or masks.shape[1] < 1 or not masks.is_contiguous() \
             or masks.device != q.device:
         raise KernelError(f"attn_tree: the masks must be contiguous int64 [{T}, words] on {q.device}, got {tuple(masks.shape)} {masks.dtype}")
     if T == 0 or ctx.B == 0:
         return
-    dt = code(q.dtype)
-    L = lib.load()
-    scratch = row_scratch("attn_tree", scratch, L.mynah_attn_tree_scratch_floats(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), q.device)
+    scratch = row_scratch("attn_tree", scratch, _tree_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), q.device)
     call("mynah_attn_tree", q.data_ptr(), out.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q), _row_stride(out),
          k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(),
          pages.base.data_ptr(), pages.n_pages, masks.data_ptr(), masks.shape[1], float(scale), scratch.data_ptr(), scratch.numel(),
-         ctx.status.data_ptr(), stream_ptr())
+         ctx.status.data_ptr(), stream_on(q.device.index))
 
 
 def check_layers(who: str, k_caches: torch.Tensor, v_caches: torch.Tensor, pages: PageTableView) -> None:
-    for t, name in ((k_caches, "K"), (v_caches, "V")):
-        if not t.is_cuda or t.device.index != torch.cuda.current_device():
-            raise KernelError(f"{who}: the {name} cache is not on the current CUDA device")
-        if t.dim() != 5 or not t.is_contiguous() or t.shape[3] != PAGE_TOKENS or t.shape[1] != pages.n_pages:
-            raise KernelError(f"{who}: the {name} cache must be contiguous [layers, {pages.n_pages}, kv heads, {PAGE_TOKENS}, head], got {tuple(t.shape)}")
-    if v_caches.shape[:4] != k_caches.shape[:4] or v_caches.dtype != k_caches.dtype or v_caches.device != k_caches.device:
-        raise KernelError(f"{who}: K cache {tuple(k_caches.shape)} {k_caches.dtype} and V cache {tuple(v_caches.shape)} {v_caches.dtype} do not go together")
+    ks, vs = k_caches.shape, v_caches.shape
+    if not k_caches.is_cuda or k_caches.device.index != torch.cuda.current_device():
+        raise KernelError(f"{who}: the cache is not on the current CUDA device")
+    if len(ks) != 5 or len(vs) != 5 or ks[1] != pages.n_pages or ks[3] != PAGE_TOKENS or ks[:4] != vs[:4] or k_caches.dtype != v_caches.dtype \
+            or k_caches.device != v_caches.device or not k_caches.is_contiguous() or not v_caches.is_contiguous():
+        raise KernelError(f"{who}: the cache must be contiguous [layers, {pages.n_pages}, kv heads, {PAGE_TOKENS}, head], got K {tuple(ks)} "
+                          f"{k_caches.dtype}, V {tuple(vs)} {v_caches.dtype}")
 
 
 def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tensor, ctx, k_caches: torch.Tensor, v_caches: torch.Tensor,
@@ -146,18 +154,18 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
     check_layers("tree_commit", k_caches, v_caches, pages)
     dev = k_caches.device
     T = tokens.numel()
-    for t, name in ((tokens, "tokens"), (parents, "parents"), (chosen, "chosen tokens")):
-        if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.numel() < T or not t.is_contiguous():
-            raise KernelError(f"tree_commit: {name} must be {T} contiguous int32 on {dev}")
+    for t in (tokens, parents, chosen):
+        if t.dtype != _I32 or t.device != dev or t.dim() != 1 or t.numel() < T or not t.is_contiguous():
+            raise KernelError(f"tree_commit: tokens, parents and chosen tokens must be {T} contiguous int32 on {dev}")
     if not 0 <= ctx.max_q_len <= 4096:
         raise KernelError(f"tree_commit: trees of {ctx.max_q_len} rows, 4096 are the most")
     check_lists("tree_commit", dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
-    out = torch.empty((T + 2 * ctx.B,), dtype=torch.int32, device=dev)
-    path, count, after = out[:T], out[T:T + ctx.B], out[T + ctx.B:]
+    path = torch.empty_like(tokens)
+    count, after = torch.empty((2, ctx.B), dtype=_I32, device=dev).unbind(0)
     E, _, KV, _, HD = k_caches.shape
     es = k_caches.element_size()
     call("mynah_tree_commit", tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), T, ctx.B, ctx.max_q_len, ctx.cu_q.data_ptr(),
          ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, k_caches.data_ptr(),
          v_caches.data_ptr(), E, KV, HD * es, v_caches.shape[4] * es, path.data_ptr(), count.data_ptr(), after.data_ptr(),
-         ctx.status.data_ptr(), stream_ptr())
+         ctx.status.data_ptr(), stream_on(dev.index))
     return path, count, after
