@@ -17,7 +17,7 @@
 
 int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs a, int max_q_len, const void* k_cache, const void* v_cache,
                   const int* cu_q, const int* kv_len, PageTable pt, const long long* masks, float* scratch, long long scratch_floats,
-                  float* lse, int* status, cudaStream_t stream);
+                  float* lse, float* scores, int score_rows, int n_ids, int* status, cudaStream_t stream);
 
 namespace {
 
@@ -142,6 +142,34 @@ int launch_mass_generic(const void* q, const void* k, const float* lse, float* m
     return mynah_check_launch("attn_mass");
 }
 
+// Sums from the scores that the attention has kept (steps of few rows a sequence, on the tensor cores): a thread a key, pages of
+// a sequence in turn. Bound by the scores' and the sums' bytes: a thirtieth of the keys' and values' for two rows a kv head.
+constexpr int SC_THREADS = 256, SC_PAGES = SC_THREADS / PAGE_TOKENS;
+__global__ void __launch_bounds__(SC_THREADS)
+attn_mass_scores_kernel(const float* __restrict__ scores, int score_rows, const float* __restrict__ lse, float* __restrict__ mass,
+                        const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, int entries, int* __restrict__ status) {
+    griddep_wait();
+    const int b = blockIdx.y;
+    const SeqShape s = seq_shape(cu_q, kv_len, pt, b, a, status);
+    const int rows = s.n_q * a.G, units = s.pages * a.KV, past = s.kvl - s.n_q, e = threadIdx.x % PAGE_TOKENS;
+    for (int u = blockIdx.x * SC_PAGES + threadIdx.x / PAGE_TOKENS; u < units; u += gridDim.x * SC_PAGES) {
+        const int lp = a.by_KV.div(u), g = u - lp * a.KV, key = lp * PAGE_TOKENS + e;
+        const int page = page_at(pt, s, lp);
+        if (page < 0 || key >= s.kvl || s.list0 + lp - s.first >= entries) continue;       // (the attention has reported a missing page)
+        const float* z = scores + (((size_t)(s.list0 + lp - s.first) * a.KV + g) * score_rows) * PAGE_TOKENS + e;
+        const float* l = lse + ((size_t)g * a.T + s.q_begin) * a.G;
+        float* m = mass + ((size_t)page * a.KV + g) * PAGE_TOKENS + e;
+        float sum = key < past ? *m : 0.f;
+#pragma unroll 4
+        for (int r = 0; r < rows; r++) sum += l[r] == -INFINITY ? 0.f : ex2_f(z[(size_t)r * PAGE_TOKENS] - l[r]);
+        *m = sum;
+    }
+}
+
+// Rows of a kv head up to which the attention keeps its scores for the sums rather than having the keys looked at again: they are
+// 256 bytes a row and page written and read, the keys of 128 columns 16 KB.
+constexpr int SCORE_ROWS = 8;
+
 // Which kernel takes the sums, and its tiles.
 bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
     const bool tc = aligned && mass_tcgen05_takes(dtype, a.r.H, a.r.KV, a.r.HD);
@@ -152,11 +180,14 @@ bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
     a.r.group = a.r.ctas = 1;
     a.r.finish();
     a.target = (tc ? 4 : (a.by_keys ? 0 : 4)) * mynah_sm_count();
+    a.score_rows = tc && (long long)max_q_len * a.r.G <= SCORE_ROWS ? max_q_len * a.r.G : 0;
     return tc;
 }
 
 long long mass_scratch(const MassArgs& a, int n_ids) {
-    return (long long)a.r.T * a.r.H + 4 + (a.target > 0 && !a.by_keys ? mass_units_max(a, n_ids) * a.r.KV * a.keys : 0);
+    const long long lse = ((long long)a.r.T * a.r.H + 3) & ~3ll;
+    if (a.score_rows > 0) return lse + (long long)n_ids * a.r.KV * a.score_rows * PAGE_TOKENS;
+    return lse + (a.target > 0 && !a.by_keys ? mass_units_max(a, n_ids) * a.r.KV * a.keys : 0);
 }
 
 }  // namespace
@@ -202,8 +233,19 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
     float* lse = scratch + attn;
     float* part = lse + (((long long)T * H + 3) & ~3ll);
     const PageTable pt{page_indptr, page_ids, page_base, n_pages};
-    const int rc = attn_rows_run("attn_mass", q, out, dtype, r, max_q_len, k_cache, v_cache, cu_q, kv_len, pt, nullptr, scratch, attn, lse, status, stream);
+    const int rc = attn_rows_run("attn_mass", q, out, dtype, r, max_q_len, k_cache, v_cache, cu_q, kv_len, pt, nullptr, scratch, attn, lse,
+                                 a.score_rows > 0 ? part : nullptr, a.score_rows, n_ids, status, stream);
     if (rc != 0) return rc;
+    if (a.score_rows > 0) {
+        MYNAH_REQUIRE(B <= 65535, "attn_mass: %d sequences are too many", B);
+        // about two units (four keys' threads each) a thread block and SM eight times over
+        const long long blocks = ceil_div_ll((long long)n_ids * KV, SC_PAGES), each = ceil_div_ll(blocks, B), most = ceil_div_ll(16ll * mynah_sm_count(), B);
+        const dim3 grid((unsigned)(each < 1 ? 1 : each < most ? each : most), B);
+        const cudaError_t e = launch_behind(attn_mass_scores_kernel, grid, dim3(SC_THREADS), 0, stream, (const float*)part, a.score_rows,
+                                            (const float*)lse, mass, cu_q, kv_len, pt, a.r, n_ids, status);
+        if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
+        return mynah_check_launch("attn_mass");
+    }
     const long long units = mass_units_max(a, n_ids);
     MYNAH_REQUIRE(units * KV < (1ll << 31) && KV <= 65535, "attn_mass: launch too large");
     const dim3 grid((unsigned)units, KV);

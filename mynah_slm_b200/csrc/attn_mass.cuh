@@ -10,6 +10,7 @@ struct MassArgs {
     int keys, rows;                   // cached rows a key tile, packed rows a row tile
     int by_keys;                      // 1: no sequence of the step has more than one row tile
     int target;                       // units to aim at over all kv heads; 0: a key tile a unit, rows are never cut
+    int score_rows;                   // > 0: the attention keeps its scores, of so many rows a kv head at most
 };
 
 struct MassUnit {

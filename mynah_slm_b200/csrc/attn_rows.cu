@@ -252,12 +252,29 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     } while (u.next(cu_q, kv_len, pt, a, status));
 }
 
+// Four values of a row; rows may begin anywhere.
+__device__ __forceinline__ void store4(float* o, float a, float b, float c, float d) {
+    if (((uintptr_t)o & 15) == 0) {
+        *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
+    } else {
+        o[0] = a, o[1] = b, o[2] = c, o[3] = d;
+    }
+}
+__device__ __forceinline__ void store4(bf16* o, float a, float b, float c, float d) {
+    if (((uintptr_t)o & 7) == 0) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+        *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    } else {
+        o[0] = from_f32<bf16>(a), o[1] = from_f32<bf16>(b), o[2] = from_f32<bf16>(c), o[3] = from_f32<bf16>(d);
+    }
+}
+
 // Joins the segments of a cut item, running over them with the maximum so far as the softmax does over keys. CTA c's helpers
 // (blockIdx.x = c - 1) take the item that CTA c begins inside of, if the item's first pages are CTA c - 1's (each cut item has
 // one such CTA). A warp a row. Bound by its start behind the attention and three dependent reads (where the CTA begins, the
 // sequence's numbers, then the segments' maxima and rows together, from L2).
-constexpr int JOIN_WARPS = 8, JOIN_ROWS = JOIN_WARPS;              // rows a CTA
-constexpr int JOIN_AHEAD = 8;                                      // segments asked for at once
+constexpr int JOIN_WARPS = 8, JOIN_HELPERS = 16;                   // warps of a CTA; CTAs that share an item's rows at most
+constexpr int JOIN_AHEAD = 4;                                      // segments asked for at once
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, RowsScratch sc,
@@ -273,8 +290,8 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
     if (pages <= at.from) return;                                  // this tile ends before the cut: it was whole
     const int n = 2 + quotient(pages - at.from - 1, at.each);      // segments
     const int lane = threadIdx.x & 31, rows = min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows);
-    const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
-    if (row < rows) {
+#pragma unroll 1
+    for (int row = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5); row < rows; row += gridDim.y * JOIN_WARPS) {
         const int pr = tile * a.tile_rows + row, tok = a.by_G.div(pr), t = s.q_begin + tok, h = at.g * a.G + pr - tok * a.G;
         auto slot = [&](int c) { return ((long long)((cta - 1 + c) * a.group + sub) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + row; };
         for (int col = lane * 4; col < a.HD; col += 128) {
@@ -286,13 +303,16 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
                 float4 y[JOIN_AHEAD];
 #pragma unroll
                 for (int c = 0; c < JOIN_AHEAD; c++) {
-                    const long long i = slot(min(c0 + c, n - 1));
-                    ml[c] = sc.ml[i];
-                    y[c] = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
+                    ml[c] = make_float2(-INFINITY, 0.f);           // (behind the last: no weight)
+                    y[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c0 + c < n) {
+                        const long long i = slot(c0 + c);
+                        ml[c] = sc.ml[i];
+                        y[c] = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
+                    }
                 }
 #pragma unroll
                 for (int c = 0; c < JOIN_AHEAD; c++) {
-                    if (c0 + c >= n) ml[c] = make_float2(-INFINITY, 0.f);      // (the last segment again: no weight)
                     const float m_new = max_or_nan(m, ml[c].x), m_use = m_new == -INFINITY ? 0.f : m_new;
                     const float u = ex2_f(m - m_use), w = ex2_f(ml[c].x - m_use);
                     m = m_new;
@@ -305,10 +325,7 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
             }
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a NaN stays one
             T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
-            o[0] = from_f32<T>(x.x * inv);
-            o[1] = from_f32<T>(x.y * inv);
-            o[2] = from_f32<T>(x.z * inv);
-            o[3] = from_f32<T>(x.w * inv);
+            store4(o, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
             if (col == 0 && sc.lse != nullptr) sc.lse[((size_t)at.g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m + log2f(l);
         }
     }
@@ -354,6 +371,8 @@ RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
     s.starts = reinterpret_cast<RowStart*>(scratch + rows * (a.HD + 2));
     s.lse = lse;
+    s.scores = nullptr;
+    s.score_rows = 0;
     return s;
 }
 
@@ -398,7 +417,7 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
 int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int* status,
                      cudaStream_t stream) {
     if (a.ctas <= 1) return 0;                                     // one CTA: nothing is cut
-    const dim3 grid((a.ctas - 1) * a.group, ceil_div(a.most_rows, JOIN_ROWS)), block(JOIN_WARPS * 32);
+    const dim3 grid((a.ctas - 1) * a.group, min(ceil_div(a.most_rows, JOIN_WARPS), JOIN_HELPERS)), block(JOIN_WARPS * 32);
     const cudaError_t e = dtype == MYNAH_F32
         ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, pt, a, s, status)
         : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, pt, a, s, status);
@@ -426,7 +445,7 @@ MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, 
 // What mynah_attn_tree and mynah_attn_mass check and launch alike.
 int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs a, int max_q_len, const void* k_cache, const void* v_cache,
                   const int* cu_q, const int* kv_len, PageTable pt, const long long* masks, float* scratch, long long scratch_floats,
-                  float* lse, int* status, cudaStream_t stream) {
+                  float* lse, float* scores, int score_rows, int n_ids, int* status, cudaStream_t stream) {
     MYNAH_REQUIRE(dtype == MYNAH_F32 || dtype == MYNAH_BF16, "%s: dtype %d is neither float32 nor bfloat16", who, dtype);
     MYNAH_REQUIRE(a.KV > 0 && a.H > 0 && a.H % a.KV == 0 && a.KV <= 65535, "%s: %d heads over %d kv heads", who, a.H, a.KV);
     MYNAH_REQUIRE(a.HD > 0 && a.HD % 8 == 0 && a.HD <= MAX_HEAD, "%s: head_dim %d is no multiple of 8 up to %d", who, a.HD, MAX_HEAD);
@@ -439,7 +458,10 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
     const bool tc = rows_plan(a, dtype, max_q_len, aligned);
     const long long need = rows_scratch_floats(a);
     MYNAH_REQUIRE(scratch_floats >= need, "%s: scratch holds %lld floats, %lld are needed", who, scratch_floats, need);
-    const RowsScratch s = rows_scratch(a, scratch, lse);
+    RowsScratch s = rows_scratch(a, scratch, lse);
+    s.scores = scores;
+    s.score_rows = score_rows;
+    s.entries = n_ids;
     const int rc = tc ? launch_rows_tcgen05(q, out, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream)
                       : launch_rows_generic(q, out, dtype, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream);
     if (rc != 0) return rc;
@@ -461,5 +483,5 @@ MYNAH_API int mynah_attn_tree(const void* q, void* out, int dtype, int T, int B,
     a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = KV > 0 ? H / KV : 0, a.ldq = ldq, a.ldo = ldo, a.words = words;
     a.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     return attn_rows_run("attn_tree", q, out, dtype, a, max_q_len, k_cache, v_cache, cu_q, kv_len,
-                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, status, stream);
+                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, nullptr, 0, 0, status, stream);
 }

@@ -10,6 +10,8 @@ struct RowsScratch {
     RowStart* starts;                 // [ctas]: where every CTA begins
     float2* ml;                       // [CTAs][2][tile_rows]: reference maximum (base 2, scaled) and sum
     float* o;                         // [CTAs][2][tile_rows][HD], not normalised
+    float* scores;                    // [entries of the page lists][KV][score_rows][64]: scores * scale_log2, -inf for unseen keys; null: not wanted
+    int score_rows, entries;          // (entries: of the page lists)
     float* lse;                       // [KV][T][G]: log2 of the sum of 2^score, -inf for a row that sees nothing; null: not wanted
 };
 

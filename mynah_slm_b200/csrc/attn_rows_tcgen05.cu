@@ -275,6 +275,14 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             s[32 + e] = (v1 >> e) & 1u ? s[32 + e] : -INFINITY;
                         }
                     }
+                    const int entry = u.s.list0 + u.pg0 + j - u.s.first;       // of the page lists
+                    if (sc.scores != nullptr && row < n_rows && entry >= u.s.list0 && entry < min(u.s.list1, sc.entries)) {
+                        // for the sums of the weights (one tile, of few rows)
+                        float4* to = reinterpret_cast<float4*>(sc.scores + (((size_t)entry * a.KV + u.g) * sc.score_rows + row0 + row) * KEYS);
+#pragma unroll
+                        for (int e = 0; e < KEYS; e += 4)
+                            to[e >> 2] = make_float4(s[e] * a.scale_log2, s[e + 1] * a.scale_log2, s[e + 2] * a.scale_log2, s[e + 3] * a.scale_log2);
+                    }
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int e = 0; e < KEYS; e += 2) mx4[(e >> 1) & 3] = max3(mx4[(e >> 1) & 3], s[e], s[e + 1]);

@@ -56,7 +56,7 @@ struct RowsArgs {
         by_G = FastDiv::of(G), by_tile = FastDiv::of(tile_rows), by_group = FastDiv::of(group), by_KV = FastDiv::of(KV), by_ctas = FastDiv::of(ctas);
     }
 };
-constexpr int LINE_COST = 16;
+constexpr int LINE_COST = 20;
 // Most page visits of a step (pages of every tile's keys, over the kv heads) that the numbers below are made for: a prompt of a
 // million tokens and 32 heads. A step of more is refused through the status word.
 constexpr long long MAX_VISITS = 1ll << 30;
