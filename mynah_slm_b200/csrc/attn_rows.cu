@@ -361,11 +361,11 @@ int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void*
 }  // namespace
 
 long long rows_scratch_floats(const RowsArgs& a) {
-    return 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2) + (long long)(sizeof(RowStart) / 4) * a.ctas;
+    return (a.whole_items ? 0 : 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2)) + (long long)(sizeof(RowStart) / 4) * a.ctas;
 }
 
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
-    const long long rows = 2ll * a.ctas * a.group * a.tile_rows;
+    const long long rows = a.whole_items ? 0 : 2ll * a.ctas * a.group * a.tile_rows;
     RowsScratch s;
     s.o = scratch;                                                 // 16-byte rows first
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
@@ -382,6 +382,7 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     a.min_range = 2;
     a.group = 1;
     a.two = 0;
+    a.whole_items = 0;
     a.ctas = 2 * mynah_sm_count();                                 // two CTAs an SM
     if (!tc) {
         a.tile_rows = longest <= 16 ? 16 : 64;
@@ -390,16 +391,18 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
         return false;
     }
     a.tile_rows = 128 / a.G * a.G;
-    // Tiles that the step's sequences have on average. From one and a half on a CTA takes two; beyond that as many side by side
-    // as there are (up to eight; a sequence of fewer leaves CTAs idle). Prompts of many tiles are bound by their products and
-    // their pages stay in L2 anyway: one item after the other.
     const long long rows = (long long)a.T * a.G, each = (long long)a.B * a.tile_rows;
-    if (longest > a.tile_rows && 2 * rows >= 3 * each) {
+    if (a.causal && rows / a.tile_rows * a.KV >= mynah_sm_count()) {
+        a.whole_items = 1;
+        a.ctas = (int)((rows / a.tile_rows + 1 + a.B) * a.KV);     // as many as the step's rows can make
+    } else if (longest > a.tile_rows && 2 * rows >= 3 * each) {
+        // From one and a half tiles a sequence on, on average, a CTA takes two; beyond that as many side by side as there are, up to
+        // eight tiles (a sequence of fewer leaves CTAs idle).
         a.two = 1;
         a.tile_rows *= 2;
         a.ctas /= 2;
         const long long most = (longest + a.tile_rows - 1) / a.tile_rows, mean = (rows + each) / (2 * each);
-        a.group = (int)(mean <= 1 || (a.causal && mean > 4) ? 1 : mean > 4 ? 4 : mean);
+        a.group = (int)(mean <= 1 ? 1 : mean > 4 ? 4 : mean);
         if (a.group > most) a.group = (int)most;
         a.ctas /= a.group;
     }
@@ -416,7 +419,7 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
 
 int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int* status,
                      cudaStream_t stream) {
-    if (a.ctas <= 1) return 0;                                     // one CTA: nothing is cut
+    if (a.ctas <= 1 || a.whole_items) return 0;                    // nothing is cut
     const dim3 grid((a.ctas - 1) * a.group, min(ceil_div(a.most_rows, JOIN_WARPS), JOIN_HELPERS)), block(JOIN_WARPS * 32);
     const cudaError_t e = dtype == MYNAH_F32
         ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, pt, a, s, status)

@@ -362,7 +362,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;      // a NaN stays one
                 const long long slot0 = ((long long)blockIdx.x * 2 + u.place()) * a.tile_rows + mine * tile_rows;      // of the tile
                 if (works) {
-                    float* mine_s = stage_s + (warp - 3) * 32 * STAGE_PITCH;           // this warp's rows, 16 columns at a time
+                    const uint32_t mine_s = smem_u32(stage_s) + (warp - 3) * 32 * STAGE_PITCH * 4;     // this warp's rows, 16 columns at a time
                     const int rows_here = min(32, n_rows - quad * 32);
                     // where the four rows that this lane writes a part of begin (four lanes a row, 4 of 16 columns each)
                     size_t to[4];
@@ -372,39 +372,47 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         to[e] = (whole ? (size_t)(u.s.q_begin + tk) * a.ldo + (size_t)(u.g * a.G + pr - tk * a.G) * HD
                                        : (size_t)(slot0 + quad * 32 + e * 8 + (lane >> 2)) * HD) + (lane & 3) * 4;
                     }
+                    // 64 columns at a time out of tensor memory (one wait for all), 16 at a time through shared memory
 #pragma unroll 1
-                    for (int c = 0; c < HD / 16; c++) {
-                        uint32_t r[16];
-                        tc_ld16(t_o + c * 16, r);
-                        if (lost) {
-#pragma unroll
-                            for (int e = 0; e < 16; e++) r[e] = 0u;
-                        } else if (poison && row < n_rows) {   // the values that were zeroed, to the rows that see them
+                    for (int c = 0; c < HD / 64; c++) {
+                        uint32_t r[64];
+                        tc_ld32_nowait(t_o + c * 64, reinterpret_cast<uint32_t(&)[32]>(r[0]));
+                        tc_ld32_nowait(t_o + c * 64 + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
+                        tc_wait_ld(reinterpret_cast<uint32_t(&)[32]>(r[0]));
+                        tc_wait_ld(reinterpret_cast<uint32_t(&)[32]>(r[32]));
+                        if (poison && !lost && row < n_rows) { // the values that were zeroed, to the rows that see them
+#pragma unroll 1
                             for (int key = u.pg0 * KEYS; key < min(u.pg1 * KEYS, kvl); key++) {
                                 if (!masked(key & ~63) || !((visible64(key & ~63, kvl, past, tok, a.causal, words, a.words) >> (key & 63)) & 1ull)) continue;
-                                const bf16* vr = v_cache + (((size_t)page_at(pt, u.s, key / PAGE_TOKENS) * a.KV + u.g) * PAGE_TOKENS + key % PAGE_TOKENS) * HD + c * 16;
+                                const bf16* vr = v_cache + (((size_t)page_at(pt, u.s, key / PAGE_TOKENS) * a.KV + u.g) * PAGE_TOKENS + key % PAGE_TOKENS) * HD + c * 64;
 #pragma unroll
-                                for (int e = 0; e < 16; e++) {
+                                for (int e = 0; e < 64; e++) {
                                     const float x = __bfloat162float(vr[e]);
                                     if (!isfinite(x)) r[e] = __float_as_uint(__uint_as_float(r[e]) + x);
                                 }
                             }
                         }
-#pragma unroll
-                        for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * inv);
-                        __syncwarp();                          // (the columns before have been read)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            *reinterpret_cast<uint4*>(mine_s + lane * STAGE_PITCH + 4 * e) = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
                         __syncwarp();
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int rr = e * 8 + (lane >> 2);
-                            if (rr < rows_here) {
-                                const float4 x = *reinterpret_cast<const float4*>(mine_s + rr * STAGE_PITCH + (lane & 3) * 4);
-                                if (whole) *reinterpret_cast<uint2*>(out + to[e] + c * 16) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
-                                else *reinterpret_cast<float4*>(sc.o + to[e] + c * 16) = x;
+                        for (int f = 0; f < 4; f++) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                float v[4];
+#pragma unroll
+                                for (int d = 0; d < 4; d++) v[d] = lost ? 0.f : __uint_as_float(r[16 * f + 4 * e + d]) * inv;
+                                st_shared(mine_s + (lane * STAGE_PITCH + 4 * e) * 4, make_float4(v[0], v[1], v[2], v[3]));
                             }
+                            __syncwarp();
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int rr = e * 8 + (lane >> 2);
+                                const float4 x = ld_shared(mine_s + (rr * STAGE_PITCH + (lane & 3) * 4) * 4);
+                                if (rr < rows_here) {
+                                    if (whole) *reinterpret_cast<uint2*>(out + to[e] + c * 64 + f * 16) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
+                                    else *reinterpret_cast<float4*>(sc.o + to[e] + c * 64 + f * 16) = x;
+                                }
+                            }
+                            __syncwarp();                      // (before the next columns go over these)
                         }
                     }
                     if (row < n_rows) {

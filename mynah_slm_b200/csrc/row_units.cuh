@@ -3,7 +3,9 @@
 //
 // The query heads that share a kv head are rows of one problem: packed row r of a sequence is token r / G, head r % G of the
 // group (G = H / KV). A tile is `tile_rows` packed rows; an item is one tile against all keys it may see, for one kv head; its
-// length is the number of those keys' pages. What a CTA takes of an item is a segment. There are two ways:
+// length is the number of those keys' pages. What a CTA takes of an item is a segment. There are three ways:
+//
+//   items   a CTA an item, the longest of every sequence first, nothing is cut: steps with enough tiles for that (prompts).
 //
 //   pieces  every item is cut into pieces of equal numbers of pages, of `each` at most, a CTA a piece. The longest item has as
 //           many pieces as all items can have with a CTA for each. One segment a CTA, but shorter items and numbers that do not
@@ -44,6 +46,7 @@ struct RowsArgs {
     int ldq, ldo;
     int tile_rows;                    // packed rows a tile
     int most_rows;                    // of one tile that the step's longest sequence fills
+    int whole_items;                  // 1: a CTA an item
     int two;                          // 1: the tcgen05 kernel's tile is two of its own
     int min_range;                    // pages a CTA at least
     int ctas;                         // ranges that the line is cut into, or pieces; the launch has ctas * group CTAs
@@ -206,7 +209,7 @@ __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const i
         if (b0 + lane < a.B) {
             s = seq_shape(cu_q, kv_len, pt, b0 + lane, a, status);
             items = seq_items(s, a);
-            own = seq_pages(s, a) * a.KV;
+            own = (a.whole_items ? items : seq_pages(s, a)) * a.KV;
             alike = !a.causal || items <= 1;
             longest = s.pages;
         }
@@ -222,7 +225,7 @@ __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const i
     const int range = max(a.min_range, a.by_ctas.div(total + a.ctas - 1));
     // Pieces, for up to 32 sequences whose items are alike, where they pay.
     int each = 0, n = 0;                                           // n: pieces of one of this lane's items
-    if (a.B <= 32 && __all_sync(0xffffffffu, alike)) {
+    if (!a.whole_items && a.B <= 32 && __all_sync(0xffffffffu, alike)) {
         const int lots = (int)__reduce_add_sync(0xffffffffu, (unsigned)items) * a.KV;
         if (lots > 0 && lots <= a.ctas) {
             longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
@@ -237,7 +240,7 @@ __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const i
             }
         }
     }
-    const long long from64 = each > 0 ? cta : (long long)range * cta;      // in pieces, or in pages
+    const long long from64 = each > 0 || a.whole_items ? cta : (long long)range * cta;       // in pieces, in items, or in pages
     __syncwarp();
     if (from64 >= total) {
         if (lane == 0 && writes) starts[cta].b = -1;
@@ -251,7 +254,7 @@ __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const i
             own = 0;
             if (b0 + lane < a.B) {
                 s = seq_shape(cu_q, kv_len, pt, b0 + lane, a, status);
-                own = seq_pages(s, a) * a.KV;
+                own = (a.whole_items ? seq_items(s, a) : seq_pages(s, a)) * a.KV;
             }
         }
         const int mine = (int)own, incl = a.B == 1 ? mine : warp_scan(mine, lane);
@@ -264,7 +267,11 @@ __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const i
             w.g = quotient(x, head);
             x -= w.g * head;
             w.item = 0;
-            if (!a.causal) {
+            if (a.whole_items) {
+                x = from - base - (incl - mine);
+                w.item = head - 1 - a.by_KV.div(x);                // (the last tile sees the most)
+                w.g = a.by_KV.mod(x);
+            } else if (!a.causal) {
                 const int one = each > 0 ? n : s.pages;            // of one item
                 w.item = quotient(x, one);
                 x -= w.item * one;
@@ -276,12 +283,12 @@ __device__ __forceinline__ void find_start(const int* __restrict__ cu_q, const i
                     p = item_pages(s, ++w.item, a);
                 }
             }
-            w.left = each > 0 ? quotient(s.pages + n - 1, n) : range;      // pieces of one size
-            w.from = each > 0 ? x * w.left : x;
+            w.left = a.whole_items ? s.pages : each > 0 ? quotient(s.pages + n - 1, n) : range;      // pieces of one size
+            w.from = a.whole_items ? 0 : each > 0 ? x * w.left : x;
             if (writes) starts[cta] = RowStart{w.b, w.g, w.item, w.from, w.left};
             // (a piece is one segment: what is left of it when the item ends is nobody's)
             const bool has = w.set(a);
-            if (each > 0) w.left = w.to - w.from;
+            if (each > 0 || a.whole_items) w.left = w.to - w.from;
             if (has || w.next(cu_q, kv_len, pt, a, status)) *at = w;
         }
         base += __shfl_sync(0xffffffffu, incl, 31);
