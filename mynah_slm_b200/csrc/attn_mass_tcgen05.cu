@@ -120,16 +120,18 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int i = max(0, issued - 2); i < issued; i++) mbar_wait(s_full + 8 * (i & 1), (i >> 1) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {                                       // ---- MMA issuer
-            constexpr uint32_t idesc_s = idesc(ROWS, false);
-            const uint32_t fix = smem_u32(fix_s), str = smem_u32(str_s);
-            bool ok = mbar_wait(f_full, 0);
-            for (int i = 0; i < n && ok; i++) {
-                const int st = i & 1;
-                ok = mbar_wait(s_full + 8 * st, (i >> 1) & 1) && (i < 2 || mbar_wait(d_free + 8 * st, ((i >> 1) & 1) ^ 1));
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t k_addr = a.by_keys ? str + st * TILE_BYTES : fix, q_addr = a.by_keys ? fix : str + st * TILE_BYTES;
+        // ---- MMA issuer (the whole warp runs, one elected lane issues: see attn_rows_tcgen05.cu)
+        constexpr uint32_t idesc_s = idesc(ROWS, false);
+        const bool leader = elect_one();
+        const uint32_t fix = smem_u32(fix_s), str = smem_u32(str_s);
+        bool ok = warp_wait(f_full, 0);
+        for (int i = 0; i < n && ok; i++) {
+            const int st = i & 1;
+            ok = warp_wait(s_full + 8 * st, (i >> 1) & 1) && (i < 2 || warp_wait(d_free + 8 * st, ((i >> 1) & 1) ^ 1));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t k_addr = a.by_keys ? str + st * TILE_BYTES : fix, q_addr = a.by_keys ? fix : str + st * TILE_BYTES;
+            if (leader) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
                     const uint32_t off = (k / 4) * HALF_BYTES + (k % 4) * 32;
@@ -137,8 +139,9 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
                 tc_commit(d_full + 8 * st);
             }
-            if (!ok) atomicOr(status, MYNAH_ST_TIMEOUT);
+            __syncwarp();
         }
+        if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
     } else if (warp == 10) {                                   // ---- lse
         bool ok = true;
         for (int i = 0; i < n && ok; i++) {
