@@ -27,7 +27,7 @@ struct EvictArgs {
 // that holds it, and so on); then every warp takes a run of rows, counts those above it and those equal to it, and, once it
 // knows the counts of the runs before, writes its own: those above, and the first of the equal ones. The words are read from
 // memory once where they fit shared memory. Bound by its chain of barriers and passes: 448 choices of 2,048 of 4,100 rows,
-// CHOOSE us.
+// 35 us.
 __global__ void __launch_bounds__(CH_THREADS)
 evict_choose_kernel(const float* __restrict__ mass, PageTable pt, const int* __restrict__ kv_len, EvictArgs a, int* __restrict__ kept,
                     int* __restrict__ new_len, int* __restrict__ status) {
@@ -156,25 +156,29 @@ evict_choose_kernel(const float* __restrict__ mass, PageTable pt, const int* __r
 
 // -------------------------------------------------------------------- moving
 
-constexpr int MV_THREADS = 256, MV_UNROLL = 8;
-constexpr int MV_ROWS = MV_THREADS / 8 * MV_UNROLL;       // rows a step: eight lanes a row, 16 bytes a lane
-constexpr int MV_BATCH = 4 * MV_ROWS;                     // rows whose places are worked out together
+constexpr int MV_THREADS = 256, MV_UNROLL = 4;
+constexpr int MV_BATCH = 512;                             // rows whose places are worked out together
 
 struct MoveArgs {
     int B, KV, n_pages, keep;
     int same;                         // 1: the rows go to lower rows of the same pages
     int k_pieces, v_pieces;           // 16-byte pieces a row
-    int k_slices, v_slices;           // slices of up to 8 pieces, each a CTA's
+    int k_slices, v_slices;           // slices of up to LANES pieces, each a CTA's
 };
 
-// Rows kept[i] -> i of one (layer, sequence, kv head), one slice of up to 128 bytes of every row of K or of V, or the sums.
+// Rows kept[i] -> i of one (layer, sequence, kv head), one slice of up to LANES * 16 bytes of every row of K or of V, or the sums.
 // i <= kept[i], ascending. In the same pages a row is read before it is written over: a step's rows are all in registers, the
 // next step's already asked for, when the barrier lets the step's writes go; and a row that is written in a step is a source of
-// that step or of an earlier one. Places are worked out 1,024 rows ahead, so that the copies wait for one read, not for the
-// choice, the page list and the row one behind the other (28 layers of 2 sequences, 2,048 rows of 8 heads of 128: 265 -> MOVE us).
+// that step or of an earlier one. Places are worked out 512 rows ahead, so that the copies wait for one read, not for the
+// choice, the page list and the row one behind the other. LANES: 16 (whole rows of 256 bytes: 28 layers of 2 sequences, 2,048 rows
+// of 8 heads of 128, 161 us of both launches' 198, against 329 with 4), or 4 where that would leave too few CTAs (one layer of one sequence, 512
+// rows of 700: both launches 12.3 against 14.4 us).
+template <int LANES>
 __global__ void __launch_bounds__(MV_THREADS)
 evict_move_kernel(uint4* __restrict__ k, uint4* __restrict__ v, float* __restrict__ mass, PageTable from, PageTable to,
                   const int* __restrict__ kv_len, const int* __restrict__ kept, MoveArgs a, int* __restrict__ status) {
+    constexpr int EACH_ROW = MV_THREADS / LANES, MV_ROWS = EACH_ROW * MV_UNROLL;       // rows at once, rows a step
+    static_assert(MV_BATCH % MV_ROWS == 0, "a batch is whole steps");
     __shared__ int src_s[2][MV_BATCH], dst_s[2][MV_BATCH];         // rows of the layer's storage, -1: none
     const int unit = blockIdx.x, g = unit % a.KV, b = unit / a.KV % a.B, e = unit / a.KV / a.B;
     const int held = max(0, kv_len[b]);
@@ -222,16 +226,16 @@ evict_move_kernel(uint4* __restrict__ k, uint4* __restrict__ v, float* __restric
         }
     } else {
         const bool is_k = sl < a.k_slices;
-        const int pieces = is_k ? a.k_pieces : a.v_pieces, at = (is_k ? sl : sl - a.k_slices) * 8 + (threadIdx.x & 7);
+        const int pieces = is_k ? a.k_pieces : a.v_pieces, at = (is_k ? sl : sl - a.k_slices) * LANES + threadIdx.x % LANES;
         uint4* t = (is_k ? k : v) + row0 * pieces + at;
         const bool on = at < pieces;
-        const int row = threadIdx.x >> 3;
+        const int row = threadIdx.x / LANES;
         uint4 x[MV_UNROLL], y[MV_UNROLL];
         auto load = [&](int i0, uint4 (&w)[MV_UNROLL]) {   // the step from row i0 on
             const int* s = src_s[(i0 / MV_BATCH) & 1] + i0 % MV_BATCH;
 #pragma unroll
             for (int j = 0; j < MV_UNROLL; j++) {
-                const int r = s[j * (MV_THREADS / 8) + row];
+                const int r = s[j * EACH_ROW + row];
                 if (r >= 0 && on) w[j] = t[(size_t)r * pieces];
             }
         };
@@ -250,7 +254,7 @@ evict_move_kernel(uint4* __restrict__ k, uint4* __restrict__ v, float* __restric
             const int* s = src_s[(i0 / MV_BATCH) & 1] + i0 % MV_BATCH;
 #pragma unroll
             for (int j = 0; j < MV_UNROLL; j++) {
-                const int q = j * (MV_THREADS / 8) + row, r = d[q];
+                const int q = j * EACH_ROW + row, r = d[q];
                 if (r >= 0 && s[q] >= 0 && on) t[(size_t)r * pieces] = x[j];
                 x[j] = y[j];
             }
@@ -375,9 +379,11 @@ MYNAH_API int mynah_cache_evict(void* k, void* v, float* mass, int E, int B, int
     evict_choose_kernel<<<(unsigned)(E * B * KV), CH_THREADS, (size_t)cached * 4, stream>>>(mass, from, kv_len, ea, kept, new_len, status);
     if (mynah_check_launch("evict_choose")) return -1;
     const int kp = k_bytes / 16, vp = v_bytes / 16;
-    const MoveArgs ma{B, KV, n_pages, keep, same, kp, vp, ceil_div(kp, 8), ceil_div(vp, 8)};
+    const int lanes = (long long)E * B * KV * (ceil_div(kp, 16) + ceil_div(vp, 16)) >= 2ll * mynah_sm_count() ? 16 : 4;
+    const MoveArgs ma{B, KV, n_pages, keep, same, kp, vp, ceil_div(kp, lanes), ceil_div(vp, lanes)};
     const dim3 grid((unsigned)(E * B * KV), ma.k_slices + ma.v_slices + 1);
-    evict_move_kernel<<<grid, MV_THREADS, 0, stream>>>((uint4*)k, (uint4*)v, mass, from, to, kv_len, kept, ma, status);
+    if (lanes == 16) evict_move_kernel<16><<<grid, MV_THREADS, 0, stream>>>((uint4*)k, (uint4*)v, mass, from, to, kv_len, kept, ma, status);
+    else evict_move_kernel<4><<<grid, MV_THREADS, 0, stream>>>((uint4*)k, (uint4*)v, mass, from, to, kv_len, kept, ma, status);
     return mynah_check_launch("evict_move");
 }
 
