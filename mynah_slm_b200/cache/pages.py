@@ -47,7 +47,7 @@ def _lib():
             "mynah_books_create": (P, [I, IP, I, I]), "mynah_books_destroy": (None, [P]),
             "mynah_books_open": (I, [P]), "mynah_books_close": (I, [P, I]), "mynah_books_length": (I, [P, I]),
             "mynah_books_pages_needed": (I, [P, I, I]), "mynah_books_reserve": (I, [P, I, I]),
-            "mynah_books_commit": (I, [P, I, I]), "mynah_books_held": (I, [P, I, I, IP, I, IP]),
+            "mynah_books_commit": (I, [P, I, I]), "mynah_books_shorten": (I, [P, I, I]), "mynah_books_held": (I, [P, I, I, IP, I, IP]),
             "mynah_books_live_slots": (I, [P, IP, I]), "mynah_books_pool": (P, [P, I]), "mynah_books_slots": (P, [P]),
             "mynah_step_fill": (I, [P, IP, IP, I, I, I, IP, I, IP, IP, IP, IP, IP, IP]),
             "mynah_decode_prepare": (I, [P, I, IP, IP, I, I, IP, IP, I, I, I, IP]),
@@ -226,6 +226,10 @@ class SequencePages:
         """The positions have been written: advance, and let windowed groups
         give back the pages no later query can see."""
         _check(_lib().mynah_books_commit(self._h, int(slot), int(n_new)))
+
+    def shorten(self, slot: int, n: int) -> None:
+        """The sequence holds its first n rows from now on (what else it held is gone); the pages behind them are free again."""
+        _check(_lib().mynah_books_shorten(self._h, int(slot), int(n)))
 
     # --------------------------------------------------------------- views
     def held(self, slot: int, group: int) -> tuple[list[int], int]:

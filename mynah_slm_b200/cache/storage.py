@@ -22,7 +22,7 @@ from .pages import PAGE_TOKENS, CacheError, SequencePages
 
 
 class Cache:
-    def __init__(self, plan, n_pages: int, max_seqs: int, dtype: torch.dtype, device):
+    def __init__(self, plan, n_pages: int, max_seqs: int, dtype: torch.dtype, device, masses: bool = False):
         self.plan = plan
         self.n_pages, self.max_seqs = n_pages, max_seqs
         self.pages = SequencePages(plan.groups, n_pages, max_seqs)
@@ -34,6 +34,8 @@ class Cache:
             self.keys.append(torch.empty((n, n_pages, g.kv_heads, PAGE_TOKENS, g.head_dim), dtype=dtype, device=device))
             vh = g.kv_heads if getattr(g, "v_heads", None) is None else g.v_heads
             self.values.append(torch.empty((n, n_pages, vh, PAGE_TOKENS, vd), dtype=dtype, device=device) if vd else None)
+        # where rows are evicted: the attention weight that every row has gathered, beside the keys
+        self.masses = [torch.zeros(k.shape[:4], dtype=torch.float32, device=device) for k in self.keys] if masses else None
         self._state_tensors: list[torch.Tensor] = []
 
         def make(req):
@@ -57,16 +59,17 @@ class Cache:
         self.views: list[CacheView] = []
         for i, e in enumerate(plan.entries):
             src = plan.entries[e.source] if e.source is not None else e
-            k = v = None
+            k = v = m = None
             if src.group is not None:
                 k = self.keys[src.group][src.index_in_group]
                 v = self.values[src.group][src.index_in_group] if self.values[src.group] is not None else None
+                m = self.masses[src.group][src.index_in_group] if self.masses is not None else None
             self.views.append(CacheView(group=src.group if src.group is not None else 0, k=k, v=v,
                                         writes=e.source is None, state=self.states.get(i),
-                                        block_state=self.block_states.get(i)))
+                                        block_state=self.block_states.get(i), mass=m))
 
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in [*self.keys, *self.values, *self._state_tensors] if t is not None)
+        return sum(t.numel() * t.element_size() for t in [*self.keys, *self.values, *(self.masses or ()), *self._state_tensors] if t is not None)
 
     def open(self) -> int:
         slot = self.pages.open()

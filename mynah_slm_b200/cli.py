@@ -4,7 +4,7 @@
     mynah-slm run (-m <model folder> | --random <config.json> [--weights-seed S]) --tokens 1,2,3
                   [-n 128] [--temp T] [--top-k K] [--top-p P] [--min-p M] [--seed S] [--repeat-penalty R]
                   [--no-stream] [--quiet] [--ctx N] [--dtype bfloat16|float32] [--batch B] [--ignore-eos]
-                  [--logits-out <file.npy>]
+                  [--logits-out <file.npy>] [--draft N] [--keep N]
     mynah-slm random -o <folder> --config <config.json> [--seed S] [--dtype bfloat16|float32]
     mynah-slm --version
 
@@ -17,6 +17,11 @@ counterpart: prompts are token ids, given with --tokens (repeatable: several
 prompts make a batch) or --tokens-file (one prompt per line). Generated ids
 go to stdout, one line per prompt; the timing line goes to stderr
 (src/timing.c:56-62), so stdout stays pipeable.
+
+--draft N checks up to N tokens a step that are drafted from the text so far
+(with --temp 0). --keep N bounds the rows that a sequence holds in the cache:
+beyond N it is cut to three quarters, keeping its first 4 rows, its last N / 4
+and those that gathered the most attention.
 
 --random <config.json> runs a model whose weights are made on the device from
 the configuration and a seed (--weights-seed, else --seed), without a folder.
@@ -61,14 +66,15 @@ def _write_logits(llm, prompts: list[list[int]], path: str) -> None:
 def cmd_run(argv: list[str]) -> int:
     o = {"model": None, "max_new": 128, "ctx": 0, "temp": 0.6, "top_k": 20, "top_p": 0.95, "min_p": 0.0, "seed": 0,
          "repeat_penalty": 1.0, "stream": True, "quiet": False, "dtype": "bfloat16", "ignore_eos": False,
-         "batch": 64, "device": "cuda:0", "random": None, "weights_seed": None, "logits_out": None}
+         "batch": 64, "device": "cuda:0", "random": None, "weights_seed": None, "logits_out": None, "draft": 0, "keep": 0}
     prompts: list[list[int]] = []
     i = 0
     valued = {"-m": ("model", str), "-n": ("max_new", int), "--ctx": ("ctx", int), "--temp": ("temp", float),
               "--top-k": ("top_k", int), "--top-p": ("top_p", float), "--min-p": ("min_p", float),
               "--seed": ("seed", int), "--repeat-penalty": ("repeat_penalty", float), "--dtype": ("dtype", str),
               "--batch": ("batch", int), "--device": ("device", str), "--random": ("random", str),
-              "--weights-seed": ("weights_seed", int), "--logits-out": ("logits_out", str)}
+              "--weights-seed": ("weights_seed", int), "--logits-out": ("logits_out", str), "--draft": ("draft", int),
+              "--keep": ("keep", int)}
     while i < len(argv):
         a = argv[i]
         if a in valued or a in ("--tokens", "--tokens-file"):
@@ -106,15 +112,21 @@ def cmd_run(argv: list[str]) -> int:
 
     from .engine.api import LLM
     longest = max(len(p) for p in prompts)
-    per_seq = o["ctx"] if o["ctx"] > 0 else longest + o["max_new"] + 8       # cli/main.c:264-265
+    if o["keep"] < 0 or 0 < o["keep"] < 16:
+        return _fail("--keep needs at least 16 rows")
+    per_seq = o["ctx"] if o["ctx"] > 0 else longest + o["max_new"] + 8 + o["draft"]       # cli/main.c:264-265
     per_seq = -(-per_seq // 64) * 64
     try:
         max_tokens = per_seq * min(len(prompts), o["batch"])
+        keep = None
+        if o["keep"]:
+            from .engine.engine import KeepRows
+            keep = KeepRows(o["keep"], o["keep"] * 3 // 4, o["keep"] // 4)
         if o["random"]:
             wseed = o["seed"] if o["weights_seed"] is None else o["weights_seed"]
-            llm = LLM.random(o["random"], seed=wseed, dtype=o["dtype"], max_tokens=max_tokens, device=o["device"])
+            llm = LLM.random(o["random"], seed=wseed, dtype=o["dtype"], max_tokens=max_tokens, device=o["device"], keep=keep)
         else:
-            llm = LLM(o["model"], dtype=o["dtype"], max_tokens=max_tokens, device=o["device"])
+            llm = LLM(o["model"], dtype=o["dtype"], max_tokens=max_tokens, device=o["device"], keep=keep)
         if o["logits_out"]:
             _write_logits(llm, prompts, o["logits_out"])
     except Exception as e:                                                    # noqa: BLE001 - report, as the reference does
@@ -133,7 +145,7 @@ def cmd_run(argv: list[str]) -> int:
     try:
         results = llm.generate(prompts, max_new=max_new, temp=o["temp"], top_k=o["top_k"], top_p=o["top_p"],
                                min_p=o["min_p"], seed=o["seed"], repeat_penalty=o["repeat_penalty"],
-                               ignore_eos=o["ignore_eos"], max_batch=o["batch"], callback=cb)
+                               ignore_eos=o["ignore_eos"], max_batch=o["batch"], callback=cb, draft=o["draft"])
     except Exception as e:                                                    # noqa: BLE001
         print(f"mynah-slm: {e}", file=sys.stderr)
         return 1

@@ -284,6 +284,24 @@ int mynah_books_commit(mynah_books* b, int slot, int n_new) {
     return 0;
 }
 
+int mynah_books_shorten(mynah_books* b, int slot, int n) {
+    auto it = b->live.find(slot);
+    if (it == b->live.end()) return fail("slot %d is not open", slot);
+    if (n < 0 || n > it->second.length) return fail("slot %d holds %d positions and cannot be cut to %d", slot, it->second.length, n);
+    for (size_t g = 0; g < b->pools.size(); g++)
+        if (b->windows[g] > 0) return fail("group %d keeps a window and cannot be cut", (int)g);
+    const int need = (n + PAGE - 1) / PAGE;
+    for (size_t g = 0; g < b->pools.size(); g++) {
+        Held& h = it->second.held[g];
+        const int more = (int)h.pages.size() - need;
+        if (more <= 0) continue;
+        if (pool_give_back(b->pools[g], h.pages.data() + need, more, slot)) return -1;
+        h.pages.resize(need);
+    }
+    it->second.length = n;
+    return 0;
+}
+
 int mynah_books_held(const mynah_books* b, int slot, int group, int32_t* pages_out, int cap, int32_t* base_out) {
     auto it = b->live.find(slot);
     if (it == b->live.end()) return fail("slot %d is not open", slot);

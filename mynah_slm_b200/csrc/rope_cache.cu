@@ -42,7 +42,7 @@ template <typename TA, typename TC>
 __global__ void __launch_bounds__(WARPS * 32)
 qk_norm_rope_store_kernel(TA* __restrict__ qkv, VecRef q_gain, VecRef k_gain,
                           const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-                          const int* __restrict__ tok_seq, const int* __restrict__ tok_pos,
+                          const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, const int* __restrict__ tok_row,
                           PageTable pt, TC* __restrict__ k_cache, TC* __restrict__ v_cache,
                           QkvArgs a, int* __restrict__ status) {
     __shared__ float stage[WARPS][MAX_HEAD_DIM];
@@ -63,12 +63,12 @@ qk_norm_rope_store_kernel(TA* __restrict__ qkv, VecRef q_gain, VecRef k_gain,
     TC* dst = nullptr;
     if (!is_q) {
         TC* cache = is_k ? k_cache : v_cache;
-        const int page = page_of(pt, seq, pos);
-        if (page < 0) {
+        const int at = tok_row != nullptr ? tok_row[t] : pos, page = page_of(pt, seq, at);
+        if (page < 0 || at < 0) {
             if (lane == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
             return;
         }
-        dst = cache + (((size_t)page * a.KV + kvh) * PAGE_TOKENS + pos % PAGE_TOKENS) * a.HD;
+        dst = cache + (((size_t)page * a.KV + kvh) * PAGE_TOKENS + at % PAGE_TOKENS) * a.HD;
     }
 
     if (!is_q && !is_k) {                                  // V: copy
@@ -128,7 +128,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(WARPS * 32, sizeof(T) == 2 ? 7 : 4)
 qk_norm_rope_store_fast_kernel(T* __restrict__ qkv, VecRef q_gain, VecRef k_gain,
                                const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-                               const int* __restrict__ tok_seq, const int* __restrict__ tok_pos,
+                               const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, const int* __restrict__ tok_row,
                                PageTable pt, T* __restrict__ k_cache, T* __restrict__ v_cache,
                                QkvArgs a, int hpw, int* __restrict__ status) {
     griddep_launch();
@@ -163,12 +163,12 @@ qk_norm_rope_store_fast_kernel(T* __restrict__ qkv, VecRef q_gain, VecRef k_gain
     const bool has_gain = q_gain.p != nullptr;
     size_t cache_row = 0;
     if (h1 > a.H) {                                        // some head of this warp goes to the cache
-        const int page = page_of(pt, seq, pos);
-        if (page < 0) {
+        const int at = tok_row != nullptr ? tok_row[t] : pos, page = page_of(pt, seq, at);
+        if (page < 0 || at < 0) {
             if (lane == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
             return;
         }
-        cache_row = (size_t)page * a.KV * PAGE_TOKENS + pos % PAGE_TOKENS;
+        cache_row = (size_t)page * a.KV * PAGE_TOKENS + at % PAGE_TOKENS;
     }
     for (int hb = h0; hb < h1; hb += BATCH * HPW) {
         if (hb != h0) {
@@ -206,7 +206,7 @@ qk_norm_rope_store_fast_kernel(T* __restrict__ qkv, VecRef q_gain, VecRef k_gain
 
 template <typename T>
 bool launch_fast(int HD, cudaStream_t stream, T* qkv, VecRef qg, VecRef kg, const float* cos_t,
-                 const float* sin_t, const int* tok_seq, const int* tok_pos, PageTable pt, T* kc, T* vc, QkvArgs a, int* status) {
+                 const float* sin_t, const int* tok_seq, const int* tok_pos, const int* tok_row, PageTable pt, T* kc, T* vc, QkvArgs a, int* status) {
     if (HD != 32 && HD != 64 && HD != 128 && HD != 256) return false;
     // heads per warp: one pass while the step is small (latency matters), up to eight passes when there are many tokens
     // (a warp's set-up, the token's position, page and rotation row, is then shared by more heads: 2,048 tokens of 32
@@ -220,10 +220,10 @@ bool launch_fast(int HD, cudaStream_t stream, T* qkv, VecRef qg, VecRef kg, cons
     const int groups = (heads + hpw - 1) / hpw;
     const unsigned blocks = (unsigned)ceil_div_ll((long long)a.T * groups, WARPS);
     switch (HD) {
-        case 32: mynah_launch(qk_norm_rope_store_fast_kernel<T, 32>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, kc, vc, a, hpw, status); return true;
-        case 64: mynah_launch(qk_norm_rope_store_fast_kernel<T, 64>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, kc, vc, a, hpw, status); return true;
-        case 128: mynah_launch(qk_norm_rope_store_fast_kernel<T, 128>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, kc, vc, a, hpw, status); return true;
-        default: mynah_launch(qk_norm_rope_store_fast_kernel<T, 256>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, kc, vc, a, hpw, status); return true;
+        case 32: mynah_launch(qk_norm_rope_store_fast_kernel<T, 32>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, kc, vc, a, hpw, status); return true;
+        case 64: mynah_launch(qk_norm_rope_store_fast_kernel<T, 64>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, kc, vc, a, hpw, status); return true;
+        case 128: mynah_launch(qk_norm_rope_store_fast_kernel<T, 128>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, kc, vc, a, hpw, status); return true;
+        default: mynah_launch(qk_norm_rope_store_fast_kernel<T, 256>, dim3(blocks), dim3(WARPS * 32), 0, stream, qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, kc, vc, a, hpw, status); return true;
     }
 }
 
@@ -239,12 +239,13 @@ MYNAH_API int mynah_rope_table(float* cos_t, float* sin_t, int n_pos, int rotary
     return mynah_check_launch("rope_table");
 }
 
-// dtype: type of qkv and of the cache (the 32-bit path keeps both in fp32).
-MYNAH_API int mynah_qk_norm_rope_store(
+// dtype: type of qkv and of the cache (the 32-bit path keeps both in fp32). tok_row: the cache's rows that the tokens' keys and
+// values are written to, where these are not their positions (null: the positions).
+MYNAH_API int mynah_qk_norm_rope_store_rows(
     void* qkv, int dtype, int T, int H, int KV, int HD, int ld,
     const void* q_gain, const void* k_gain, int gain_dtype, float eps,
     const float* cos_t, const float* sin_t, int rotary_dim, int n_pos,
-    const int* tok_seq, const int* tok_pos,
+    const int* tok_seq, const int* tok_pos, const int* tok_row,
     const int* page_indptr, const int* page_ids, const int* page_base, int n_pages,
     void* k_cache, void* v_cache, int* status, cudaStream_t stream) {
     if (T == 0) return 0;
@@ -262,18 +263,29 @@ MYNAH_API int mynah_qk_norm_rope_store(
     // the register-only kernel: the whole head rotated (or none of it), rows 16-byte aligned
     const bool fast_ok = (cos_t == nullptr || rotary_dim == HD) && ld % 8 == 0;
     if (fast_ok && dtype == MYNAH_F32 &&
-        launch_fast<float>(HD, stream, (float*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, (float*)k_cache, (float*)v_cache, a, status))
+        launch_fast<float>(HD, stream, (float*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, (float*)k_cache, (float*)v_cache, a, status))
         return mynah_check_launch("qk_norm_rope_store");
     if (fast_ok && dtype == MYNAH_BF16 &&
-        launch_fast<bf16>(HD, stream, (bf16*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, (bf16*)k_cache, (bf16*)v_cache, a, status))
+        launch_fast<bf16>(HD, stream, (bf16*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, (bf16*)k_cache, (bf16*)v_cache, a, status))
         return mynah_check_launch("qk_norm_rope_store");
     if (dtype == MYNAH_F32)
         mynah_launch(qk_norm_rope_store_kernel<float, float>, dim3(blocks), dim3(WARPS * 32), 0, stream,
-            (float*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, (float*)k_cache, (float*)v_cache, a, status);
+            (float*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, (float*)k_cache, (float*)v_cache, a, status);
     else if (dtype == MYNAH_BF16)
         mynah_launch(qk_norm_rope_store_kernel<bf16, bf16>, dim3(blocks), dim3(WARPS * 32), 0, stream,
-            (bf16*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, pt, (bf16*)k_cache, (bf16*)v_cache, a, status);
+            (bf16*)qkv, qg, kg, cos_t, sin_t, tok_seq, tok_pos, tok_row, pt, (bf16*)k_cache, (bf16*)v_cache, a, status);
     else
         return mynah_fail("qk_norm_rope_store: unsupported dtype %d", dtype);
     return mynah_check_launch("qk_norm_rope_store");
+}
+
+MYNAH_API int mynah_qk_norm_rope_store(
+    void* qkv, int dtype, int T, int H, int KV, int HD, int ld,
+    const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+    const float* cos_t, const float* sin_t, int rotary_dim, int n_pos,
+    const int* tok_seq, const int* tok_pos,
+    const int* page_indptr, const int* page_ids, const int* page_base, int n_pages,
+    void* k_cache, void* v_cache, int* status, cudaStream_t stream) {
+    return mynah_qk_norm_rope_store_rows(qkv, dtype, T, H, KV, HD, ld, q_gain, k_gain, gain_dtype, eps, cos_t, sin_t, rotary_dim, n_pos,
+                                         tok_seq, tok_pos, nullptr, page_indptr, page_ids, page_base, n_pages, k_cache, v_cache, status, stream);
 }

@@ -19,32 +19,47 @@ from typing import Callable, Optional, Sequence
 import torch
 
 from ..sampling.sampler import SamplingParams, stream_state
-from .engine import Engine, StepEntry
-from .generate import Request, Result, Timing, generate
+from ..cache.pages import PAGE_TOKENS
+from .draft import Lookup
+from .engine import Engine, KeepRows, StepEntry, TreeEntry
+from .generate import GenerationError, Request, Result, Timing, generate, tokens_held
 
 
 class EngineBackend:
     """`generate`'s view of an engine: prompts in one step, then one sampled
     token per sequence per step, host token ids in and out."""
 
-    def __init__(self, engine: Engine, params: SamplingParams):
+    def __init__(self, engine: Engine, params: SamplingParams, drafts: int = 0):
         self.engine = engine
         self.params = params
+        self.drafts = int(drafts)
+        self._lookups: dict[int, Lookup] = {}      # of the open sequences, where tokens are drafted
         self.max_positions = engine.spec.max_positions
         engine.sampler.set_params(params)
         self._host_rows: list[torch.Tensor] = []
         self._turn = 0
         self._to_start: list[tuple] = []
         # steps fed from the device are replayed graphs; MYNAH_RUN_AHEAD=0 keeps the step-by-step loop
-        self.runs_ahead = bool(engine.use_graphs and engine.graph_safe) and os.environ.get("MYNAH_RUN_AHEAD", "1") != "0"
+        self.runs_ahead = (bool(engine.use_graphs and engine.graph_safe) and os.environ.get("MYNAH_RUN_AHEAD", "1") != "0"
+                           and not self.drafts)
 
     def free_tokens(self) -> int:
         return self.engine.free_tokens()
+
+    def rows_held(self, prompt_len: int, max_new: int) -> int:
+        """Cache a request may come to hold: with drafts the rows of a step's tree too, with a bound no more than that (or its prompt)."""
+        most, keep = self.max_positions, self.engine.keep
+        if keep is not None:
+            n = max(prompt_len, min(prompt_len + max(max_new, 0), keep.limit + 1))
+            return -(-n // PAGE_TOKENS) * PAGE_TOKENS
+        return tokens_held(prompt_len, max_new, most) if not self.drafts else tokens_held(prompt_len, max_new + self.drafts, most)
 
     def open(self, request_index: int, prompt: Sequence[int]) -> int:
         slot = self.engine.open_sequence()
         # the generators and rings of a batch's slots are set in one go, when the batch's prompts run
         self._to_start.append((slot, stream_state(self.params.seed, request_index), prompt))
+        if self.drafts:
+            self._lookups[slot] = Lookup(prompt)
         return slot
 
     def _start_opened(self) -> None:
@@ -55,6 +70,7 @@ class EngineBackend:
 
     def close(self, slot: int) -> None:
         self._to_start = [t for t in self._to_start if t[0] != slot]
+        self._lookups.pop(slot, None)
         self.engine.close_sequence(slot)
 
     def prefill(self, slots: Sequence[int], prompts: Sequence[Sequence[int]]) -> list[int]:
@@ -70,6 +86,19 @@ class EngineBackend:
         self._start_opened()
         out = self.engine.decode_sampled(slots, tokens)
         return out[:len(slots)].cpu().tolist()
+
+    def decode_drafted(self, slots: Sequence[int], last: Sequence[int], rooms: Sequence[int]) -> list[list[int]]:
+        """One step over trees of drafted tokens (`Engine.step_tree`, the most likely tokens): every sequence gains at least one."""
+        entries = []
+        for s, t, room in zip(slots, last, rooms):
+            look = self._lookups[s]
+            look.extend([t])
+            entries.append(TreeEntry(s, *look.tree(min(self.drafts, room - 1))))
+        out = []
+        for s, r in zip(slots, self.engine.step_tree(entries)):
+            self._lookups[s].extend(r.tokens)
+            out.append([*r.tokens, r.next])
+        return out
 
     # A step that is not waited for: its tokens are copied to pinned host memory behind it on the stream, and an
     # event marks the copy's end, so that the next step can be launched (fed from this one's result on the device)
@@ -101,23 +130,25 @@ class _InFlight:
 
 class LLM:
     def __init__(self, model: str, dtype: str = "bfloat16", max_tokens: int = 65536, max_seqs: Optional[int] = None,
-                 device: str = "cuda:0", use_graphs: bool = True):
+                 device: str = "cuda:0", use_graphs: bool = True, keep: Optional[KeepRows] = None):
+        """`keep`: a bound on the rows that a sequence holds (`KeepRows`); those that gathered the least attention are evicted."""
         t0 = time.perf_counter()
         self.engine = Engine.from_folder(model, dtype=dtype, max_tokens=max_tokens, max_seqs=max_seqs,
-                                         device=device, use_graphs=use_graphs)
+                                         device=device, use_graphs=use_graphs, keep=keep)
         torch.cuda.synchronize()
         self.load_s = time.perf_counter() - t0
         self.last_timing: Optional[Timing] = None
 
     @classmethod
     def random(cls, config, seed: int = 0, dtype: str = "bfloat16", max_tokens: int = 65536,
-               max_seqs: Optional[int] = None, device: str = "cuda:0", use_graphs: bool = True) -> "LLM":
+               max_seqs: Optional[int] = None, device: str = "cuda:0", use_graphs: bool = True,
+               keep: Optional[KeepRows] = None) -> "LLM":
         """A model with random weights made on the device from `config` (a typed configuration, a config.json
         dictionary or the path of one) and `seed`; no file is written or read."""
         t0 = time.perf_counter()
         self = cls.__new__(cls)
         self.engine = Engine.random(config, seed=seed, dtype=dtype, max_tokens=max_tokens, max_seqs=max_seqs,
-                                    device=device, use_graphs=use_graphs)
+                                    device=device, use_graphs=use_graphs, keep=keep)
         torch.cuda.synchronize()
         self.load_s = time.perf_counter() - t0
         self.last_timing = None
@@ -131,15 +162,26 @@ class LLM:
                  top_p: float = 0.95, min_p: float = 0.0, seed: int = 0, repeat_penalty: float = 1.0,
                  freq_penalty: float = 0.0, presence_penalty: float = 0.0, penalty_window: int = 64,
                  stop_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False, max_batch: int = 64,
-                 callback: Optional[Callable[[int, int], int]] = None) -> list[Result]:
+                 callback: Optional[Callable[[int, int], int]] = None, draft: int = 0) -> list[Result]:
         """Generate for every prompt (a list of token ids each). `stop_ids`
         defaults to the model's stop set (config.json and generation_config.json);
-        `ignore_eos` empties it. Results are in the order of the prompts."""
+        `ignore_eos` empties it. Results are in the order of the prompts.
+
+        `draft` > 0: up to so many tokens a step are drafted from the sequence's own text and checked together (see
+        `engine/draft.py`, `Engine.step_tree`). The tokens are those of greedy decoding up to rounding (a step of several rows sums
+        in another order than a step of one), so it goes with temp 0 and no penalties."""
+        if draft < 0 or draft > 1024:
+            raise GenerationError(f"{draft} drafted tokens a step: 0 to 1024")
+        if draft and (temp > 0 or repeat_penalty != 1.0 or freq_penalty != 0.0 or presence_penalty != 0.0):
+            raise GenerationError("drafted tokens are checked against the most likely ones: temp 0 and no penalties")
         params = SamplingParams(temp=temp, top_k=top_k, top_p=top_p, min_p=min_p, repeat_penalty=repeat_penalty,
                                 freq_penalty=freq_penalty, presence_penalty=presence_penalty,
                                 penalty_window=penalty_window, seed=seed)
         stop = () if ignore_eos else (self.eos_token_ids if stop_ids is None else tuple(stop_ids))
-        backend = EngineBackend(self.engine, params)
+        if draft and (self.engine.keep is not None or not self.engine.rows_apart):
+            raise GenerationError("tokens can be drafted only where every layer is grouped-query attention over all positions, nothing else is "
+                                  "kept and no rows are evicted")
+        backend = EngineBackend(self.engine, params, draft)
         timing = Timing(load_s=self.load_s, device_name=torch.cuda.get_device_name(self.engine.device))
         reqs = [Request(list(p), max_new) for p in prompts]
         out = generate(backend, reqs, stop_ids=stop, max_batch=max_batch, callback=callback, timing=timing)

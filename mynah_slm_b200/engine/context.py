@@ -14,6 +14,10 @@ that a step costs one host-to-device copy:
   want    [W]    rows whose logits are wanted
   per storage group: indptr [B+1], base [B], ids [n_ids]   (the page lists)
 
+In a step whose tokens' rows of the cache are not their positions (drafted trees, a cache whose rows are evicted) there is also
+
+  tok_row [T]    row of the sequence's cache that the token's key and value are written to
+
 `StepLayout` fixes the offsets for given capacities; `StepContext` is the set
 of device views that parts and kernels read.
 """
@@ -38,6 +42,7 @@ class StepLayout:
     B: int
     W: int
     ids_cap: list[int]          # capacity of each group's page-id list
+    apart: bool = False         # with tok_row
 
     def __post_init__(self):
         off = 0
@@ -50,6 +55,9 @@ class StepLayout:
             for name, n in ((f"indptr{g}", self.B + 1), (f"base{g}", self.B), (f"ids{g}", cap)):
                 self.off[name] = (off, n)
                 off += _pad4(max(n, 1))
+        if self.apart:
+            self.off["tok_row"] = (off, self.T)
+            off += _pad4(max(self.T, 1))
         self.size = off
         # the same offsets as arrays, for the native packing routine (cache/pages.py: fill_step)
         names = ["tokens", "tok_seq", "tok_pos", "cu_q", "kv_len", "slots", "want"]
@@ -80,6 +88,9 @@ class StepContext:
     decode_splits: int
     status: torch.Tensor
     act_dtype: torch.dtype
+    # rows of the cache, where they are not the positions; the rows' mask words, in a step that brings drafted trees
+    tok_row: Optional[torch.Tensor] = None
+    tree_masks: Optional[torch.Tensor] = None
     # host-side copies for parts that plan on the host (toy parts, tests)
     host_q_lens: Optional[list[int]] = None
     host_past: Optional[list[int]] = None
@@ -96,4 +107,4 @@ def device_context(layout: StepLayout, dev_buf: torch.Tensor, n_pages: list[int]
     return StepContext(T=layout.T, B=layout.B, tokens=v("tokens"), tok_seq=v("tok_seq"), tok_pos=v("tok_pos"),
                        cu_q=v("cu_q"), kv_len=v("kv_len"), slots=v("slots"), want=v("want"), pages=pages,
                        max_q_len=max_q_len, is_decode=is_decode, decode_splits=decode_splits, status=status,
-                       act_dtype=act_dtype)
+                       act_dtype=act_dtype, tok_row=v("tok_row") if layout.apart else None)

@@ -53,6 +53,35 @@ class StepEntry:
     want: Sequence[int] = ()        # places among `tokens` whose logits are wanted
 
 
+@dataclass
+class TreeEntry:
+    """A sequence's drafted tree in a step that checks it: row 0 is the token that was sampled last, every other row a drafted token
+    behind an earlier row (`parents`, -1 for row 0)."""
+    slot: int
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
+@dataclass
+class TreeResult:
+    tokens: list                    # the accepted drafted tokens, in order (row 0 is not among them)
+    next: int                       # what was chosen behind the last of them
+
+
+@dataclass(frozen=True)
+class KeepRows:
+    """A bound on the rows that a sequence holds: a sequence that holds more than `limit` after a step is cut to `keep` rows in every
+    layer and kv head: its `first` first, its `recent` last, and between them those that gathered the most attention."""
+    limit: int
+    keep: int
+    recent: int
+    first: int = 4
+
+    def __post_init__(self):
+        if not 0 < self.keep <= self.limit or self.recent < 0 or self.first < 0 or self.recent + self.first > self.keep:
+            raise EngineError(f"a cache of up to {self.limit} rows cannot be cut to {self.keep} with {self.first} first and {self.recent} recent ones")
+
+
 class Runtime:
     """Device-wide things that parts share: the compute type, lookup tables
     built once, scratch memory, and the status word kernels report through."""
@@ -147,6 +176,15 @@ class _Staging:
 
 
 @dataclass
+class _Lists:
+    """What an operator over sequences' rows reads of the step's description (see StepContext)."""
+    B: int
+    kv_len: torch.Tensor
+    pages: object
+    status: torch.Tensor
+
+
+@dataclass
 class _DecodeGraph:
     bucket: int
     layout: StepLayout
@@ -207,7 +245,7 @@ def _prompt_rows_bucket(T: int) -> int:
 class Engine:
     def __init__(self, spec: ModelSpec, checkpoint: Checkpoint, dtype="bfloat16", max_tokens: int = 4096,
                  max_seqs: Optional[int] = None, device="cuda:0", use_graphs: bool = True,
-                 penalty_window: int = 64):
+                 penalty_window: int = 64, keep: Optional[KeepRows] = None):
         if isinstance(dtype, str):
             if dtype not in DTYPES:
                 raise EngineError(f"dtype {dtype!r} is not one of {sorted(DTYPES)}")
@@ -225,7 +263,8 @@ class Engine:
         self.model = Model(spec)
         self.n_pages = max(1, -(-int(max_tokens) // PAGE_TOKENS))
         # no sequence outgrows the cache, so position tables need not reach further than its pages do
-        self.runtime = Runtime(self.device, dtype, min(spec.max_positions, self.n_pages * PAGE_TOKENS))
+        # (one whose rows are evicted goes on behind what it has given up)
+        self.runtime = Runtime(self.device, dtype, spec.max_positions if keep is not None else min(spec.max_positions, self.n_pages * PAGE_TOKENS))
         from ..weights.random_init import RandomWeights, fill_into
         if isinstance(checkpoint, RandomWeights):
             fill_into(self.model.tensor_specs(), checkpoint, self.runtime)
@@ -235,7 +274,11 @@ class Engine:
             if not part.tensor_specs():
                 part.bind({}, self.runtime)
         self.max_seqs = int(max_seqs) if max_seqs else min(self.n_pages, 1024)
-        self.cache = Cache(self.model.cache_plan(), self.n_pages, self.max_seqs, dtype, self.device)
+        self.keep = keep
+        if keep is not None and not self.rows_apart:
+            raise EngineError("rows can be evicted only where every layer is grouped-query attention over all positions and nothing else is kept")
+        self.cache = Cache(self.model.cache_plan(), self.n_pages, self.max_seqs, dtype, self.device, masses=keep is not None)
+        self._dropped: dict[int, int] = {}         # positions of every open sequence that were evicted
         self.n_groups = len(self.cache.plan.groups)
         self.sampler = SamplerState(self.max_seqs, self.device, penalty_window)
         self.sampler.set_params(SamplingParams.greedy())
@@ -255,7 +298,7 @@ class Engine:
                                for e in self.model.schedule]
         self._feeds_embedding = any(e.add_embedding for e in self.model.schedule)
         # decode steps of a few rows run all layers in one launch, where the model's layers are of the kind it takes
-        self.decode_layers = DecodeLayers.plan(self.model, self.cache, self.runtime)
+        self.decode_layers = DecodeLayers.plan(self.model, self.cache, self.runtime) if keep is None else None
         self.launches = 0                          # kernels of this package launched (see count_launches)
         self.vocab_size = spec.vocab_size
 
@@ -293,13 +336,26 @@ class Engine:
         starts empty."""
         slot = self.cache.open()
         self.sampler.reset_slot(slot)
+        self._dropped[slot] = 0
         return slot
 
     def close_sequence(self, slot: int) -> None:
         self.cache.close(slot)
 
     def length(self, slot: int) -> int:
+        """Rows that the sequence holds (as many as its positions unless rows were evicted)."""
         return self.cache.pages.length[slot]
+
+    def positions(self, slot: int) -> int:
+        """Tokens that the sequence has run so far."""
+        return self.cache.pages.length[slot] + self._dropped.get(slot, 0)
+
+    @property
+    def rows_apart(self) -> bool:
+        """Whether the model can run where the cache's rows are not the tokens' positions (drafted trees, eviction)."""
+        m = self.model
+        return (all(getattr(l.mixer, "rows_apart", False) and l.state_request() is None for l in m.layers)
+                and all(e.cache_from is None for e in m.schedule) and m.embedding.state_request() is None)
 
     def free_tokens(self) -> int:
         return min(p.n_free for p in self.cache.pages.pools) * PAGE_TOKENS
@@ -328,8 +384,8 @@ class Engine:
             for w in e.want:
                 if not 0 <= int(w) < n:
                     raise EngineError(f"wanted place {w} lies outside the {n} tokens of slot {e.slot}")
-            if self.cache.pages.length[e.slot] + n > self.spec.max_positions:
-                raise EngineError(f"slot {e.slot} would grow to {self.cache.pages.length[e.slot] + n} positions, "
+            if self.positions(e.slot) + n > self.spec.max_positions:
+                raise EngineError(f"slot {e.slot} would grow to {self.positions(e.slot) + n} positions, "
                                   f"the model allows {self.spec.max_positions}")
 
     @staticmethod
@@ -340,10 +396,19 @@ class Engine:
     def _fill(self, buf_np: np.ndarray, layout: StepLayout, entries: Sequence[StepEntry], with_want: bool = True):
         """Write the batch description into a host buffer (packed by the native host runtime). Returns
         (max_q_len, want_count)."""
-        return self.cache.pages.fill_step(
+        out = self.cache.pages.fill_step(
             buf_np, layout.offsets_array, layout.T, layout.B, layout.W, layout.ids_cap_array,
             [e.slot for e in entries], [e.tokens for e in entries],
             [e.want for e in entries] if with_want else None)
+        if layout.apart:
+            self._set_rows(buf_np, layout, [e.slot for e in entries], [len(e.tokens) for e in entries])
+        return out
+
+    def _set_rows(self, buf_np: np.ndarray, layout: StepLayout, slots: Sequence[int], counts: Sequence[int]) -> None:
+        """The books count a sequence's rows; a token's position lies as much further on as rows were evicted."""
+        pos, n = layout.view(buf_np, "tok_pos"), int(sum(counts))
+        layout.view(buf_np, "tok_row")[:] = pos
+        pos[:n] += np.repeat(np.asarray([self._dropped.get(s, 0) for s in slots], dtype=np.int32), counts)
 
     # ------------------------------------------------------------- forward
     def _forward(self, ctx: StepContext, want_rows: Optional[torch.Tensor], taps: Optional[dict] = None) -> torch.Tensor:
@@ -423,6 +488,102 @@ class Engine:
                 out = self._eager_step(entries, is_decode)
         for e in entries:
             pages.commit(e.slot, len(e.tokens))
+        self._evict([e.slot for e in entries])
+        return out
+
+    # ------------------------------------------------------------- eviction
+    def _evict(self, slots: Sequence[int]) -> None:
+        """Cuts the sequences that hold more rows than they may, in all layers, in place."""
+        if self.keep is None:
+            return
+        from ..ops import evict
+        pages, k = self.cache.pages, self.keep
+        over = [s for s in slots if pages.length[s] > k.limit]
+        if not over:
+            return
+        for g in range(self.n_groups):
+            ctx = self._lists(over, g)
+            evict.cache_evict(self.cache.keys[g], self.cache.values[g], self.cache.masses[g], ctx, ctx.pages, k.keep, k.recent, k.first)
+        for s in over:
+            self._dropped[s] = self._dropped.get(s, 0) + pages.length[s] - k.keep
+            pages.shorten(s, k.keep)
+
+    def _lists(self, slots: Sequence[int], group: int) -> "_Lists":
+        """Lengths and page lists of some sequences on the device."""
+        pages = self.cache.pages
+        held = [pages.held(s, group) for s in slots]
+        n = len(slots)
+        words = [pages.length[s] for s in slots] + [0]
+        for ids, _ in held:
+            words.append(words[-1] + len(ids))
+        words += [base for _, base in held]
+        words += [p for ids, _ in held for p in ids]
+        host, hi = self._staging.get(len(words))
+        host.numpy()[:len(words)] = words
+        dev = torch.empty((len(words),), dtype=torch.int32, device=self.device)
+        dev.copy_(host[:len(words)], non_blocking=True)
+        self._staging.sent(hi)
+        return _Lists(n, dev[:n], kernels.PageTableView(dev[n:2 * n + 1], dev[3 * n + 1:], dev[2 * n + 1:3 * n + 1], self.n_pages), self.runtime.status)
+
+    # --------------------------------------------------------- drafted trees
+    def step_tree(self, entries: Sequence[TreeEntry], choose=None) -> list[TreeResult]:
+        """Checks drafted tokens: one step over the trees of `entries`, whose accepted paths the sequences go on behind.
+
+        Every row of a tree attends to what its sequence holds and to its ancestors, at the position of its depth, as it would if
+        its path had been taken token by token. `choose(logits [rows, vocab]) -> int32 [rows]` says what follows every row (by
+        default the most likely token). From row 0 on, a row goes on to its lowest child whose token was chosen behind it; the
+        rows of that path stay in the cache, row 0 among them, the others' keys and values are given up. Returns what every
+        sequence has gained: the accepted drafted tokens and what was chosen behind the last of them (which is not in the cache
+        yet: it is row 0 of the sequence's next tree, or the next step's token)."""
+        from ..ops import tree
+        if self.keep is not None or not self.rows_apart:
+            raise EngineError("trees can be checked only where every layer is grouped-query attention over all positions, nothing else is kept "
+                              "and no rows are evicted")
+        self._validate([StepEntry(e.slot, e.tokens) for e in entries])
+        longest = max(len(e.tokens) for e in entries)
+        if longest > 4096:
+            raise EngineError(f"a tree of {longest} tokens, 4096 are the most")
+        words = -(-longest // 64)
+        rows = []
+        for e in entries:
+            if len(e.parents) != len(e.tokens) or e.parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(e.parents) if i):
+                raise EngineError(f"the tree of slot {e.slot} is not one: row 0 has the parent -1, every other row an earlier row")
+            rows.append(tree.tree_rows(e.parents, words))
+        pages = self.cache.pages
+        for e in entries:
+            pages.reserve(e.slot, len(e.tokens))
+        T, B = sum(len(e.tokens) for e in entries), len(entries)
+        layout = StepLayout(T=T, B=B, W=1, ids_cap=[sum(pages.n_held(e.slot, g) for e in entries) for g in range(self.n_groups)], apart=True)
+        extra = layout.size + (layout.size & 1)               # behind the description: the masks, 8-byte aligned, and the parents
+        n_words = 2 * T * words
+        host, hi = self._staging.get(extra + n_words + T)
+        host_np = host.numpy()
+        max_q, _ = self._fill(host_np, layout, [StepEntry(e.slot, e.tokens) for e in entries], with_want=False)
+        past = np.repeat([pages.length[e.slot] for e in entries], [len(e.tokens) for e in entries])
+        layout.view(host_np, "tok_pos")[:T] = past + np.concatenate([d for d, _ in rows])
+        host_np[extra:extra + n_words] = np.concatenate([w for _, w in rows]).reshape(-1).view(np.int32)
+        host_np[extra + n_words:extra + n_words + T] = np.concatenate([np.asarray(e.parents, dtype=np.int32) for e in entries])
+        dev = torch.empty((extra + n_words + T,), dtype=torch.int32, device=self.device)
+        dev.copy_(host[:extra + n_words + T], non_blocking=True)
+        self._staging.sent(hi)
+        ctx = device_context(layout, dev, [self.n_pages] * self.n_groups, max_q, False, 1, self.runtime.status, self.dtype)
+        ctx.tree_masks = dev[extra:extra + n_words].view(torch.int64).view(T, words)
+        self._host_fields(ctx, [StepEntry(e.slot, e.tokens) for e in entries])
+        logits = self._forward(ctx, None)
+        chosen = kernels.argmax(logits) if choose is None else choose(logits)
+        if chosen.dtype != torch.int32 or tuple(chosen.shape) != (T,):
+            raise EngineError(f"choose: {T} int32 tokens are wanted, got {tuple(chosen.shape)} {chosen.dtype}")
+        for g in range(self.n_groups):
+            path, count, after = tree.tree_commit(ctx.tokens, dev[extra + n_words:], chosen.contiguous(), ctx, self.cache.keys[g], self.cache.values[g],
+                                                  ctx.pages[g])
+        got = torch.cat([path, count, after]).cpu().tolist()
+        self.check_status()
+        out, at = [], 0
+        for b, e in enumerate(entries):
+            n, steps = len(e.tokens), got[T + b]
+            pages.commit(e.slot, steps)
+            out.append(TreeResult([int(e.tokens[i]) for i in got[at + 1:at + steps]], got[T + B + b]))
+            at += n
         return out
 
     # --------------------------------------------------------- prompt graphs
@@ -448,7 +609,7 @@ class Engine:
             self._prompt_seen[key] = seen + 1
             if seen == 0:
                 return None                                   # once: run as it is; twice: worth a graph
-            layout = StepLayout(T=key[0], B=key[1], W=key[2], ids_cap=list(key[3]))
+            layout = StepLayout(T=key[0], B=key[1], W=key[2], ids_cap=list(key[3]), apart=self.keep is not None)
             meta = torch.zeros((layout.size,), dtype=torch.int32, device=self.device)
             ctx = device_context(layout, meta, [self.n_pages] * self.n_groups, key[0], False, 1, self.runtime.status, self.dtype)
             g = _PromptGraph(layout, meta, ctx)
@@ -500,7 +661,7 @@ class Engine:
         wants = [(b, int(w)) for b, e in enumerate(entries) for w in e.want]
         ids_cap = [sum(len(self.cache.pages.held(e.slot, g)[0]) for e in entries) for g in range(self.n_groups)]
         # wanted rows are normalised once each; duplicates are expanded afterwards
-        layout = StepLayout(T=T, B=B, W=max(len(wants), 1), ids_cap=ids_cap)
+        layout = StepLayout(T=T, B=B, W=max(len(wants), 1), ids_cap=ids_cap, apart=self.keep is not None)
         host, hi = self._staging.get(layout.size)
         max_q, n_want = self._fill(host.numpy(), layout, entries)
         want_np = layout.view(host.numpy(), "want")[:n_want]
@@ -563,7 +724,7 @@ class Engine:
         if g is not None:
             return g
         cap = min(bucket * max_pages_seq, self.n_pages + bucket)
-        layout = StepLayout(T=bucket, B=bucket, W=1, ids_cap=[cap] * self.n_groups)
+        layout = StepLayout(T=bucket, B=bucket, W=1, ids_cap=[cap] * self.n_groups, apart=self.keep is not None)
         meta = torch.zeros((layout.size,), dtype=torch.int32, device=self.device)
         ctx = device_context(layout, meta, [self.n_pages] * self.n_groups, 1, True, splits, self.runtime.status, self.dtype)
         g = _DecodeGraph(bucket, layout, meta, ctx, splits)
@@ -668,6 +829,11 @@ class Engine:
                 if "cache is full" in str(e):
                     raise
                 raise EngineError(str(e)) from None
+            if g.layout.apart:
+                for s in slots_a.tolist():
+                    if self.positions(s) >= self.spec.max_positions:
+                        raise EngineError(f"slot {s} would outgrow the model's {self.spec.max_positions} positions")
+                self._set_rows(host.numpy(), g.layout, slots_a.tolist(), [1] * len(slots_a))
             g.meta.copy_(host[:g.layout.size], non_blocking=True)
             self._staging.sent(hi)
             if feed is not None:
@@ -679,6 +845,7 @@ class Engine:
                     g.ctx.tokens[:n].copy_(prev[torch.tensor(list(rows), dtype=torch.int64, device=self.device)])
             out = self._run_graph(g, "sample", 1)
             pages.commit_many(slots_a, 1)
+            self._evict(slots_a.tolist())
             return out
         entries = [StepEntry(s, (int(t),)) for s, t in zip(slots, tokens)]
         self._validate(entries)
@@ -689,6 +856,7 @@ class Engine:
         out = self.sampler.sample(logits, slots_t)
         for e in entries:
             pages.commit(e.slot, 1)
+        self._evict([e.slot for e in entries])
         return out
 
     def decode_loop(self, slots: Sequence[int], tokens: Sequence[int], n_steps: int) -> torch.Tensor:
@@ -697,6 +865,8 @@ class Engine:
         of the last step (device). Used where only throughput is wanted."""
         if not (self.use_graphs and self.graph_safe):
             raise EngineError("decode_loop needs CUDA graphs")
+        if self.keep is not None:
+            raise EngineError("decode_loop leaves no room for evictions between its steps")
         entries = [StepEntry(s, (int(t),)) for s, t in zip(slots, tokens)]
         self._validate(entries)
         pages = self.cache.pages

@@ -90,6 +90,10 @@ class Backend(Protocol):
     #       tokens are `tokens` (host ids) or, with feed = (handle of the step before, rows), row rows[i] of that
     #       step's result, taken on the device;
     #   decode_collect(handle) -> list[int]                      waits for that step and returns its tokens.
+    # Optional, with `drafts = n > 0` (and runs_ahead False): steps that check drafted tokens and may gain several at once.
+    #   decode_drafted(slots, last, rooms) -> list[list[int]]    goes on behind `last` (every sequence's last token, which is not in
+    #       the cache yet); sequence i may gain at most rooms[i] tokens; returns what every one gained, at least one token.
+    # Optional: rows_held(prompt_len, max_new) -> int, the cache that a request may come to hold where that is not `tokens_held`.
 
 
 class GenerationError(RuntimeError):
@@ -102,7 +106,8 @@ def tokens_held(prompt_len: int, max_new: int, max_positions: int) -> int:
     return -(-n // PAGE_TOKENS) * PAGE_TOKENS
 
 
-def plan_batches(requests: Sequence[Request], max_batch: int, budget_tokens: int, max_positions: int) -> list[list[int]]:
+def plan_batches(requests: Sequence[Request], max_batch: int, budget_tokens: int, max_positions: int,
+                 rows_held: Optional[Callable[[int, int], int]] = None) -> list[list[int]]:
     """Split the requests, in order, into batches that fit the batch size and
     the cache. Requests with nothing to generate are not scheduled."""
     if max_batch < 1:
@@ -118,7 +123,7 @@ def plan_batches(requests: Sequence[Request], max_batch: int, budget_tokens: int
                                   f"{max_positions} positions")
         if r.max_new <= 0:
             continue
-        need = tokens_held(len(r.tokens), r.max_new, max_positions)
+        need = tokens_held(len(r.tokens), r.max_new, max_positions) if rows_held is None else rows_held(len(r.tokens), r.max_new)
         if need > budget_tokens:
             raise GenerationError(f"request {i} may hold {need} tokens of cache, the engine has {budget_tokens}")
         if cur and (len(cur) >= max_batch or used + need > budget_tokens):
@@ -175,7 +180,7 @@ def generate(backend: Backend, requests: Sequence[Request], stop_ids: Sequence[i
         live.next_token = tok
         return True
 
-    for batch in plan_batches(requests, max_batch, budget, backend.max_positions):
+    for batch in plan_batches(requests, max_batch, budget, backend.max_positions, getattr(backend, "rows_held", None)):
         live = [_Live(i, backend.open(i, requests[i].tokens)) for i in batch]
         try:
             t0 = time.perf_counter()
@@ -224,6 +229,19 @@ def generate(backend: Backend, requests: Sequence[Request], stop_ids: Sequence[i
                                 backend.close(l.slot)
                     rows = [l for _, l in ahead]
                     handle = nxt
+            while live and getattr(backend, "drafts", 0):
+                rooms = [min(requests[l.index].max_new - results[l.index].produced, backend.max_positions - l.length) for l in live]
+                gained = backend.decode_drafted([l.slot for l in live], [l.next_token for l in live], rooms)
+                going = []
+                for l, toks in zip(live, gained):
+                    for tok in toks:
+                        l.length += 1
+                        if not accept(l, int(tok)):
+                            backend.close(l.slot)
+                            break
+                    else:
+                        going.append(l)
+                live = going
             while live:
                 toks = backend.decode([l.slot for l in live], [l.next_token for l in live])
                 going = []

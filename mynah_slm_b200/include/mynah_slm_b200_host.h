@@ -62,6 +62,7 @@ int mynah_books_length(const mynah_books*, int slot);                           
 int mynah_books_pages_needed(const mynah_books*, int slot, int n_new);
 int mynah_books_reserve(mynah_books*, int slot, int n_new);                      /* pages for n_new more positions, in every group or in none */
 int mynah_books_commit(mynah_books*, int slot, int n_new);                       /* the positions are written; windowed groups give pages back */
+int mynah_books_shorten(mynah_books*, int slot, int n);                          /* the first n rows stay; pages behind them are given back */
 int mynah_books_held(const mynah_books*, int slot, int group, int32_t* pages_out, int cap, int32_t* base_out);   /* count */
 int mynah_books_live_slots(const mynah_books*, int32_t* out, int cap);           /* count, ascending */
 const mynah_pool* mynah_books_pool(const mynah_books*, int group);

@@ -316,8 +316,13 @@ def qk_norm_rope_store(qkv: torch.Tensor, H: int, KV: int, HD: int,
                        cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], rotary_dim: int,
                        tok_seq: torch.Tensor, tok_pos: torch.Tensor, pages: PageTableView,
                        k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
-                       status: torch.Tensor) -> None:
+                       status: torch.Tensor, tok_row: Optional[torch.Tensor] = None) -> None:
+    """`tok_row`: the cache's rows that the tokens' keys and values are written to, where these are not their positions."""
     _chk(qkv, "qkv", dim=2)
+    if tok_row is not None:
+        _chk(tok_row, "rows of the cache", torch.int32, 1)
+        if tok_row.numel() < qkv.shape[0]:
+            raise KernelError(f"qk_norm_rope_store: {tok_row.numel()} rows of the cache for {qkv.shape[0]} tokens")
     T, ld = qkv.shape
     if (q_gain is None) != (k_gain is None):
         raise KernelError("qk_norm_rope_store: q and k gains go together")
@@ -337,10 +342,10 @@ def qk_norm_rope_store(qkv: torch.Tensor, H: int, KV: int, HD: int,
             raise KernelError("qk_norm_rope_store: the cache and the activations differ in dtype")
         if tuple(k_cache.shape[1:]) != (KV, PAGE_TOKENS, HD):
             raise KernelError(f"qk_norm_rope_store: cache pages are {tuple(k_cache.shape[1:])}, expected {(KV, PAGE_TOKENS, HD)}")
-    call("mynah_qk_norm_rope_store", ptr(qkv), code(qkv.dtype), T, H, KV, HD, ld,
+    call("mynah_qk_norm_rope_store_rows", ptr(qkv), code(qkv.dtype), T, H, KV, HD, ld,
          ptr(q_gain), ptr(k_gain), gd, float(eps),
          ptr(cos), ptr(sin), rotary_dim, n_pos,
-         ptr(tok_seq), ptr(tok_pos),
+         ptr(tok_seq), ptr(tok_pos), ptr(tok_row),
          ptr(pages.indptr), ptr(pages.ids), ptr(pages.base), pages.n_pages,
          ptr(k_cache), ptr(v_cache), ptr(status), stream_ptr())
 

@@ -31,6 +31,12 @@ from .base import (CacheView, KVRequest, Mixer, TensorSpec, build_part, register
 class GQAttention(Mixer):
     accepts_normed = True        # its first product can compute the norm on its way
 
+    @property
+    def rows_apart(self) -> bool:
+        """Whether the layer can run where the cache's rows are not the tokens' positions: steps of drafted trees, a cache whose rows
+        are evicted. A window goes by positions, which the cached rows do not tell then."""
+        return self.window is None and self.position.fusable and type(self).forward is GQAttention.forward
+
     def __init__(self, spec: PartSpec):
         super().__init__(spec)
         self.D = int(spec["hidden_size"])
@@ -94,6 +100,8 @@ class GQAttention(Mixer):
         writes = cache.writes
         pages = ctx.pages[cache.group]
         from ..ops import attention_dispatch, gemm_bf16
+        if ctx.tok_row is not None:
+            return self._forward_apart(h, ctx, cache)
         w_in = self.w_qkv if writes else self.w_q
         if not ctx.is_decode and self.position.fusable and self.runtime.act_dtype == torch.bfloat16:
             cos, sin, rot = self.position.fused_tables()
@@ -141,6 +149,23 @@ class GQAttention(Mixer):
                                       self.runtime.attn_counters(ctx.B * KV))
         else:
             attention_dispatch.prefill(qkv, out, ctx, H, KV, HD, cache.k, cache.v, pages, self.window or 0)
+        return kernels.linear(out, self.w_o)
+
+    def _forward_apart(self, h: torch.Tensor, ctx, cache: CacheView) -> torch.Tensor:
+        """The same layer in a step that gives its rows of the cache: the tokens of drafted trees, each of which sees what was held
+        and its ancestors, or causal tokens whose attention also adds up what every cached row gets (`cache.mass`)."""
+        from ..ops import evict, tree
+        H, KV, HD = self.H, self.KV, self.HD
+        pages = ctx.pages[cache.group]
+        qkv = kernels.linear(h, self.w_qkv)
+        cos, sin, rot = self.position.fused_tables()
+        kernels.qk_norm_rope_store(qkv, H, KV, HD, self.q_gain, self.k_gain, self.qk_eps, cos, sin, rot, ctx.tok_seq, ctx.tok_pos, pages,
+                                   cache.k, cache.v, ctx.status, ctx.tok_row)
+        out = torch.empty((h.shape[0], H * HD), dtype=qkv.dtype, device=qkv.device)
+        if ctx.tree_masks is not None:
+            tree.attn_tree(qkv, out, ctx, H, KV, HD, cache.k, cache.v, pages, ctx.tree_masks)
+        else:
+            evict.attn_mass(qkv, out, cache.mass, ctx, H, KV, HD, cache.k, cache.v, pages)
         return kernels.linear(out, self.w_o)
 
 

@@ -109,6 +109,8 @@ class CacheView:
        several states by name gets a dictionary of such tensors.
     block_state: the same for the state that the layer's block asked for (a
        dictionary by name), or None.
+    mass: in a cache whose rows are evicted, the attention weight that every
+       row of k has gathered, fp32 [n_pages, kv_heads, 64]; else None.
     """
     group: Optional[int] = None
     k: Optional[torch.Tensor] = None
@@ -116,6 +118,7 @@ class CacheView:
     writes: bool = True
     state: Any = None
     block_state: Any = None
+    mass: Optional[torch.Tensor] = None
 
 
 # ------------------------------------------------------------------- parts
