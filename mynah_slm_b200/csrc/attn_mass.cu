@@ -52,18 +52,29 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
         return;
     }
     const T* k = k_cache + ((size_t)page * a.r.KV + g) * PAGE_TOKENS * HD;
-    for (int i = threadIdx.x * 4; i < GK * HD; i += 256 * 4) *reinterpret_cast<float4*>(k_s + i / HD * p + i % HD) = four_of(k + i);
+    const int quads = HD >> 2;
+    for (int i = threadIdx.x; i < GK * quads; i += 256) {
+        const int r = a.r.by_quads.div(i);
+        *reinterpret_cast<float4*>(k_s + r * p + (i - r * quads) * 4) = four_of(k + i * 4);
+    }
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int rt = r0; rt < r1; rt++) {
         __syncthreads();
-        for (int i = threadIdx.x; i < GR * HD; i += 256) {
-            const int r = i / HD, d = i % HD, pr = rt * GR + r;
-            q_s[r * p + d] = pr < n_rows ? to_f32(q[(size_t)(u.s.q_begin + pr / G) * a.r.ldq + (size_t)(g * G + pr % G) * HD + d]) : 0.f;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < GR * quads; i += 256) {
+            const int r = a.r.by_quads.div(i), d = (i - r * quads) * 4, pr = rt * GR + r, tok = a.r.by_G.div(pr);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (pr < n_rows) {
+                const T* at = q + (size_t)(u.s.q_begin + tok) * a.r.ldq + (size_t)(g * G + pr - tok * G) * HD + d;
+                x = a.r.q_aligned ? four_of(at) : make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
+            }
+            *reinterpret_cast<float4*>(q_s + r * p + d) = x;
         }
         if (threadIdx.x < GR) {
             const int pr = rt * GR + threadIdx.x;
-            lse_s[threadIdx.x] = pr < n_rows ? lse[((size_t)g * a.r.T + u.s.q_begin) * G + pr] : 0.f;
+            const float z = pr < n_rows ? lse[((size_t)g * a.r.T + u.s.q_begin) * G + pr] : 0.f;
+            lse_s[threadIdx.x] = z == -INFINITY ? INFINITY : z;    // a row that saw nothing gives no weight
         }
         __syncthreads();
         float s[4][2];
@@ -89,7 +100,7 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
         for (int j = 0; j < 2; j++) {
             const int r = tx + 16 * j, pr = rt * GR + r;
             if (pr >= n_rows) continue;
-            const int last = past + pr / G;                        // the last key that the row sees
+            const int last = past + a.r.by_G.div(pr);                        // the last key that the row sees
             const float z = lse_s[r];
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -151,7 +162,7 @@ attn_mass_scores_kernel(const float* __restrict__ scores, int score_rows, const 
     griddep_wait();
     const int b = blockIdx.y;
     const SeqShape s = seq_shape(cu_q, kv_len, pt, b, a, status);
-    const int rows = s.n_q * a.G, units = s.pages * a.KV, past = s.kvl - s.n_q, e = threadIdx.x % PAGE_TOKENS;
+    const int rows = min(s.n_q * a.G, score_rows), units = s.pages * a.KV, past = s.kvl - s.n_q, e = threadIdx.x % PAGE_TOKENS;
     for (int u = blockIdx.x * SC_PAGES + threadIdx.x / PAGE_TOKENS; u < units; u += gridDim.x * SC_PAGES) {
         const int lp = a.by_KV.div(u), g = u - lp * a.KV, key = lp * PAGE_TOKENS + e;
         const int page = page_at(pt, s, lp);
@@ -178,6 +189,7 @@ bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
     a.by_keys = (long long)max_q_len * a.r.G <= a.rows;
     a.r.tile_rows = a.rows;
     a.r.group = a.r.ctas = 1;
+    a.r.q_aligned = aligned;
     a.r.finish();
     a.target = (tc ? 4 : (a.by_keys ? 0 : 4)) * mynah_sm_count();
     a.score_rows = tc && (long long)max_q_len * a.r.G <= SCORE_ROWS ? max_q_len * a.r.G : 0;
@@ -227,6 +239,7 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
     MassArgs a{};
     a.r = r;
     const bool tc = mass_plan(a, dtype, aligned, max_q_len);
+    MYNAH_REQUIRE(a.score_rows == 0 || B <= 65535, "attn_mass: %d sequences are too many", B);
     const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids);
     MYNAH_REQUIRE(scratch_floats >= need, "attn_mass: scratch holds %lld floats, %lld are needed", scratch_floats, need);
     const long long attn = attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1);
@@ -237,7 +250,6 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
                                  a.score_rows > 0 ? part : nullptr, a.score_rows, n_ids, status, stream);
     if (rc != 0) return rc;
     if (a.score_rows > 0) {
-        MYNAH_REQUIRE(B <= 65535, "attn_mass: %d sequences are too many", B);
         // about two units (four keys' threads each) a thread block and SM eight times over
         const long long blocks = ceil_div_ll((long long)n_ids * KV, SC_PAGES), each = ceil_div_ll(blocks, B), most = ceil_div_ll(16ll * mynah_sm_count(), B);
         const dim3 grid((unsigned)(each < 1 ? 1 : each < most ? each : most), B);

@@ -42,9 +42,11 @@ template <typename T> __host__ __device__ constexpr int pitch_of(int HD) { retur
 
 // TY x TX threads; thread (ty, tx) has the packed rows ty + TY * i (i < 4) of the tile, for the scores the keys tx + TX * j of
 // KT, for the output the columns 4 * tx + 4 * TX * c. fp32 throughout, products and sums as written (FFMA). The row's maximum
-// and sum are kept by every thread of the row. A weight of an unseen key is stored as -1, and such keys are left out of the
-// output by a select: what lies in an unseen row of V (a stale NaN, an infinity) cannot reach a result, while a seen one does
-// what arithmetic does. K and V come KT keys at a time by asynchronous copies, two tiles in flight.
+// and sum are kept by every thread of the row. An unseen key has the weight 0; in a tile that holds unseen keys and a value
+// that is not finite (a stale row, an infinity) it is stored as -1, and such keys are left out of the output by a select:
+// what lies in an unseen row of V cannot reach a result, while a seen one does what arithmetic does (the select everywhere in
+// masked tiles, and the queries read one by one: 30.5 us against 26.7 for 3 trees of 19 in fp32 behind 1,021 rows). K and V come KT
+// keys at a time by asynchronous copies, two tiles in flight.
 // 16-row tiles (TY = 4, TX = 32) are for the few rows of decode steps and small trees, 64-row tiles (TY = TX = 16) for the rest.
 template <typename T, int TY, int TX, int NC>
 __global__ void __launch_bounds__(TY * TX, 2)
@@ -74,14 +76,17 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     // every page of the segment must be there: one that lacks a page counts as keys that nobody sees
     for (int p = pg0 + (int)threadIdx.x; p < pg1; p += THREADS)
         if (page_at(pt, u.s, p) < 0) bad_s = 1;
-    for (int i = threadIdx.x; i < R * HD; i += THREADS) {
-        const int r = i / HD, d = i % HD;
-        float x = 0.f;
+    // the tile's queries, four values a thread (one by one where rows are not aligned); rows that are not there are zero
+    const int quads = HD >> 2;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < R * quads; i += THREADS) {
+        const int r = a.by_quads.div(i), d = (i - r * quads) * 4, pr = row0 + r, tok = a.by_G.div(pr);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < n_rows) {
-            const int pr = row0 + r, tok = a.by_G.div(pr);
-            x = to_f32(q[(size_t)(u.s.q_begin + tok) * a.ldq + (size_t)(g * a.G + pr - tok * a.G) * HD + d]);
+            const T* at = q + (size_t)(u.s.q_begin + tok) * a.ldq + (size_t)(g * a.G + pr - tok * a.G) * HD + d;
+            x = a.q_aligned ? four_of(at) : make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
         }
-        q_s[r * qp + d] = x;
+        *reinterpret_cast<float4*>(q_s + r * qp + d) = x;
     }
     __syncthreads();
     const bool bad = bad_s != 0;
@@ -120,9 +125,21 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         } else {
             copies_wait<0>();
         }
-        __syncthreads();
         const T* ks = k_s + st * KT * kp;
         const T* vs = v_s + st * KT * kp;
+        const int key0 = t * KT;
+        // is there a key in the tile that some row of the tile must not see?
+        const bool need_mask = key0 + KT > u.s.kvl || (a.causal ? key0 + KT - 1 > past + first_tok : key0 + KT > past);
+        __syncthreads();
+        bool odd = false;                                          // and then a value that is not finite (or a stale row)?
+        if (need_mask) {
+            for (int i = threadIdx.x; i < KT * quads; i += THREADS) {
+                const int r = a.by_quads.div(i);
+                const float4 x = four_of(vs + r * kp + (i - r * quads) * 4);
+                odd |= !(fabsf(x.x) <= 3e38f && fabsf(x.y) <= 3e38f && fabsf(x.z) <= 3e38f && fabsf(x.w) <= 3e38f);
+            }
+            odd = __syncthreads_or(odd);
+        }
         float s[4][KJ];
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -145,9 +162,6 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
                     s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
                 }
         }
-        const int key0 = t * KT;
-        // is there a key in the tile that some row of the tile must not see?
-        const bool need_mask = key0 + KT > u.s.kvl || (a.causal ? key0 + KT - 1 > past + first_tok : key0 + KT > past);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = ty + TY * i, pr = row0 + r, tok = a.by_G.div(pr);
@@ -174,7 +188,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
                 const bool in = (seen >> (tx + TX * j)) & 1u;
                 const float p = exp2f(s[i][j] - m_use);
                 if (in) sum += p;
-                p_s[r * (KT + 4) + tx + TX * j] = in ? p : -1.f;
+                p_s[r * (KT + 4) + tx + TX * j] = in ? p : odd ? -1.f : 0.f;
             }
 #pragma unroll
             for (int o = TX / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -197,7 +211,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
                     const int col = 4 * tx + 4 * TX * c;
                     if (col >= HD) continue;
                     const float4 x = four_of(vs + (kk + e4) * kp + col);
-                    if (need_mask) {
+                    if (odd) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const float w = p[i][e4];
@@ -379,7 +393,10 @@ RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
 bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     const bool tc = aligned && rows_tcgen05_takes(dtype, a.H, a.KV, a.HD);
     const long long longest = (long long)max_q_len * a.G;          // packed rows of the longest sequence
-    a.min_range = 2;
+    // A page is little for the tensor cores and 20,000 clocks of FFMA for 64 rows: there every further CTA helps (3 trees of 19 in
+    // fp32 behind 1,021 rows: 33.7 us with two pages a CTA at least, 30.5 with one; 8 trees of 24 on the tensor cores: the same).
+    a.min_range = tc ? 2 : 1;
+    a.q_aligned = aligned;
     a.group = 1;
     a.two = 0;
     a.whole_items = 0;

@@ -7,7 +7,7 @@
 //   warp 1     issues S = Q.K^T into tensor memory (two buffers),
 //   warp 2     O += P.V, P read from tensor memory and V as an MN-major operand in shared memory: two warps, because an issuer
 //              that waits for weights keeps the tensor cores from the next scores (one warp for both took 2,200 clocks a page of
-//              two tiles, these TWOWARPS). Both run whole, with one elected lane at the instructions: under `lane == 0` every
+//              two tiles, these 2,100). Both run whole, with one elected lane at the instructions: under `lane == 0` every
 //              descriptor went through vector registers and a product took 85 clocks to issue, under elect.sync 55;
 //   warps 3-6  the softmax, a thread a row: 64 scores in registers, O rescaled only when the reference maximum has to grow by
 //              more than 2^8, weights written back over the scores as bfloat16 (half a step is lost, as much as the output's own
@@ -276,7 +276,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                     const int entry = u.s.list0 + u.pg0 + j - u.s.first;       // of the page lists
-                    if (sc.scores != nullptr && row < n_rows && entry >= u.s.list0 && entry < min(u.s.list1, sc.entries)) {
+                    if (sc.scores != nullptr && row0 + row < sc.score_rows && row < n_rows && entry >= u.s.list0 && entry < min(u.s.list1, sc.entries)) {
                         // for the sums of the weights (one tile, of few rows)
                         float4* to = reinterpret_cast<float4*>(sc.scores + (((size_t)entry * a.KV + u.g) * sc.score_rows + row0 + row) * KEYS);
 #pragma unroll

@@ -14,17 +14,22 @@
 //           every CTA has the same number of pages, however ragged the batch, but a range that reaches from one item into the
 //           next is two segments, and most items are cut.
 //
-// The line is taken where `each` exceeds `range` by more than a segment and a join cost (LINE_COST pages). 8 trees of 24 tokens
-// behind 2,050 rows, 16 heads: PIECES8; a decode step of 64 sequences of 3,000 rows, 32 heads: LINE64. An item that one CTA has
-// whole is finished there; of the others every CTA leaves its segment's maximum, sum and unnormalised output in scratch (at
-// most two a CTA: one whose item began before, one whose item goes on), and a second launch joins them: there is one CTA (and
-// its helpers) of that launch for every CTA of the first, which finds there what that one wrote down of its start.
+// The line is taken where `each` exceeds `range` by more than a segment and a join cost (LINE_COST pages), and for more sequences
+// than a warp has lanes. Pieces against line: 8 trees of 24 tokens behind up to 2,050 rows, 16 heads (9 pages each, a range of 8)
+// 29.7 us against 33.9; 16 trees of 8, one behind 800 rows, 15 behind 500 (7 and 4) 22.5 against 22.7; behind 1,600 and 500 rows
+// (13 and 4) 26.7 against 24.1, behind 8,000 and 500 (63 and 7) 73.9 against 30.9; 24 trees of 8 behind 1,600 rows (26 and 17)
+// 43.5 both, behind 9,000 (141 and 92) 165 against 149.
+//
+// An item that one CTA has whole is finished there; of the others every CTA leaves its segment's maximum, sum and unnormalised
+// output in scratch (at most two a CTA: one whose item began before, one whose item goes on), and a second launch joins them:
+// there is one CTA (and its helpers) of that launch for every CTA of the first, which finds there what that one wrote down of its
+// start.
 //
 // Everything is worked out on the device from the step's description (in few instructions: a CTA's first trip through any code
-// waits for that code, about 0.3 us for every 128 bytes of it, which is most of what a small call takes), so a captured launch serves whatever lengths its replays
-// bring. Where sequences have several tiles, `group` CTAs side by side take the same pages for `group` tiles (an item is then
-// that many tiles), so that a page comes from memory once and from L2 for the others: 16 trees of 64 tokens with four heads a kv
-// head (two tiles each) behind 8,191 rows read 1.05 GB one tile after the other, 0.54 GB together.
+// waits for that code, about 0.3 us for every 128 bytes of it, which is most of what a small call takes), so a captured launch
+// serves whatever lengths its replays bring. Where sequences have several tiles, `group` CTAs side by side take the same pages for
+// `group` tiles (an item is then that many tiles), so that a page comes from memory once and from L2 for the others: 16 trees of
+// 64 tokens with four heads a kv head (two tiles each) behind 8,191 rows read 1.05 GB one tile after the other, 0.54 GB together.
 #pragma once
 #include "layout.cuh"
 
@@ -54,12 +59,14 @@ struct RowsArgs {
     int causal;                       // 1: token i sees rows <= past + i; 0: the mask words
     int words;                        // mask words a token
     float scale_log2;                 // score scale * log2(e)
-    FastDiv by_G, by_tile, by_group, by_KV, by_ctas;
+    int q_aligned;                    // 1: q's rows are whole 16-byte pieces
+    FastDiv by_G, by_tile, by_group, by_KV, by_ctas, by_quads;
     void finish() {                   // once the numbers above stand
         by_G = FastDiv::of(G), by_tile = FastDiv::of(tile_rows), by_group = FastDiv::of(group), by_KV = FastDiv::of(KV), by_ctas = FastDiv::of(ctas);
+        by_quads = FastDiv::of(HD >= 4 ? HD / 4 : 1);
     }
 };
-constexpr int LINE_COST = 20;
+constexpr int LINE_COST = 6;
 // Most page visits of a step (pages of every tile's keys, over the kv heads) that the numbers below are made for: a prompt of a
 // million tokens and 32 heads. A step of more is refused through the status word.
 constexpr long long MAX_VISITS = 1ll << 30;

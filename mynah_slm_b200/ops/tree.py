@@ -161,7 +161,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
         raise KernelError(f"tree_commit: trees of {ctx.max_q_len} rows, 4096 are the most")
     check_lists("tree_commit", dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
     path = torch.empty_like(tokens)
-    count, after = torch.empty((2, ctx.B), dtype=_I32, device=dev).unbind(0)
+    count, after = tokens.new_empty(ctx.B), tokens.new_empty(ctx.B)
     E, _, KV, _, HD = k_caches.shape
     es = k_caches.element_size()
     call("mynah_tree_commit", tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), T, ctx.B, ctx.max_q_len, ctx.cu_q.data_ptr(),
