@@ -36,7 +36,7 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
     mass [n_pages, KV, 64] fp32 gets, at every cached row of the step's sequences, the weight that the step's rows and the kv
     head's query heads give it, added to what it holds for rows that were there before the step, in place of it for the step's own
     (so nothing has to be cleared when a page is taken). Other rows' sums are left as they are. The order of the sums does not
-    depend on timing."""
+    depend on timing, provided that no page is in two sequences' lists (a shared page's sums would be written by both)."""
     dt = check_rows("attn_mass", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
     T = q.shape[0]
     if mass.dtype != torch.float32 or mass.device != q.device or not mass.is_contiguous() or mass.dim() != 3 \
@@ -59,7 +59,7 @@ def cache_evict(k_caches: torch.Tensor, v_caches: torch.Tensor, masses: torch.Te
     `first` rows and the last `recent` stay, and of those between them the keep - first - recent with the greatest sums (the lower
     row where sums are equal; a NaN counts as the greatest). The rows that stay become rows 0, 1, 2, ..., in order, with their
     sums: in the same pages, or in those of `out_pages`, whose lists must have no page in common with `pages`' (sequences of no
-    more than `keep` rows are then copied whole).
+    more than `keep` rows are then copied whole). No page may be in two sequences' lists, unless its rows go to `out_pages`.
 
     k_caches, v_caches [layers, n_pages, kv heads, 64, head], masses [layers, n_pages, kv heads, 64] fp32, ctx.kv_len: the rows
     held. Returns int32 (kept [layers, B, kv heads, keep]: the rows that stayed, ascending, -1 behind them; kv_len [B])."""

@@ -61,11 +61,13 @@ def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: in
     width = H * HD
     for t in (q, out):
         shape = t.shape
-        if len(shape) != 2 or shape[1] < width or t.stride(1) != 1 or (shape[0] > 1 and t.stride(0) < width):
+        if len(shape) != 2 or shape[1] < width or t.stride(1) != 1 or (shape[0] > 1 and not width <= t.stride(0) < 1 << 31):
             raise KernelError(f"{who}: q and the output must be rows of at least {width} values, one row behind the other, got "
                               f"{tuple(shape)} with strides {t.stride()}")
     if out.dtype != dt or out.device != dev or out.shape[0] < q.shape[0]:
         raise KernelError(f"{who}: the output is {tuple(out.shape)} {out.dtype} on {out.device}, q {tuple(q.shape)} {dt} on {dev}")
+    if q.data_ptr() == out.data_ptr() and q.shape[0]:
+        raise KernelError(f"{who}: the output lies over q, which is read until the end")
     cache = (KV, PAGE_TOKENS, HD)
     for t in (k_cache, v_cache):
         shape = t.shape

@@ -1,0 +1,225 @@
+"""Attention of a few rows a sequence at lengths and batches where the work is cut in every way (pieces, a line, whole items, several
+tiles side by side), caches that pass 32-bit offsets, and calls that run at once; against the definitions in 64 bits."""
+import random
+
+import pytest
+import torch
+
+from plain import rows as plain
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _masks(trees):
+    from mynah_slm_b200.ops.tree import tree_rows
+    words = max(-(-len(t) // 64) for t in trees)
+    return torch.cat([torch.from_numpy(tree_rows(t, words)[1].copy()) for t in trees if t])
+
+
+def _tree(n, rng):
+    return [-1 if i == 0 else max(0, i - 1 - int(rng.random() ** 2 * 6)) for i in range(n)]
+
+
+def _case(seed, rows, past, H, KV, HD, dtype):
+    g = torch.Generator().manual_seed(seed)
+    step = plain.make_step(rows, past, DEV, g)
+    d = torch.Generator(device=DEV).manual_seed(seed)
+    q = torch.randn((sum(rows), H * HD), generator=d, device=DEV).to(dtype)
+    k, v = (torch.randn((step.pages.n_pages, KV, 64, HD), generator=d, device=DEV).to(dtype) for _ in range(2))
+    return step, q, k, v
+
+
+def _attention(step, q, k, v, H, scale, sees, p_bits, acc):
+    """`plain.attention` for many rows at once: the same formulas and bounds, in 64 bits on the device."""
+    KV, HD = k.shape[1], k.shape[3]
+    G = H // KV
+    out = torch.zeros((q.shape[0], H, HD), dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(out)
+    sums, room, at = [], [], 0
+    for b, (n, p) in enumerate(zip(step.q_lens, step.past)):
+        held, pages = p + n, torch.tensor(step.lists[b], device=DEV)
+        total, slack = (torch.zeros((KV, held), dtype=torch.float64, device=DEV) for _ in range(2))
+        for g in range(KV):
+            if n == 0:
+                break
+            kk, vv = (c[pages, g].reshape(-1, HD)[:held].double() for c in (k, v))
+            qq = q[at:at + n, g * G * HD:(g + 1) * G * HD].double().view(n * G, HD)
+            seen = sees[b].to(DEV).repeat_interleave(G, 0)
+            w = torch.softmax((qq @ kk.T * scale).masked_fill(~seen, float("-inf")), 1)
+            A = (qq.abs() @ kk.abs().T * scale).masked_fill(~seen, 0.0).amax(1, keepdim=True)
+            N = seen.sum(1, keepdim=True)
+            rel = (HD + 2) * acc * A * 2 + 8 * acc * (A + 8) + 2.0 ** -20 + (N + 16) * acc
+            out[at:at + n, g * G:(g + 1) * G] = (w @ vv).view(n, G, HD)
+            bound[at:at + n, g * G:(g + 1) * G] = ((w @ vv.abs()) * (rel + p_bits + N * acc)).view(n, G, HD)
+            total[g], slack[g] = w.sum(0), (w * (rel + (n * G + 4) * acc)).sum(0)
+        sums.append(total)
+        room.append(slack)
+        at += n
+    return out, bound, sums, room
+
+
+def _agrees(step, q, k, v, H, KV, HD, dtype, out, sees, mass=None, got=None):
+    tc = dtype == BF16 and HD in (64, 128)
+    ref, bound, sums, slack = _attention(step, q, k, v, H, HD ** -0.5, sees, 2.0 ** -8 if tc else 0.0, 2 * plain.F32 if tc else plain.F32)
+    last = 2.0 ** -8 if dtype == BF16 else plain.F32
+    tol = bound + last * (ref.abs() + bound) + 1e-37
+    off = (out.double().view(ref.shape) - ref).abs()
+    assert (off <= tol).all(), f"worst {float((off / tol).nan_to_num(1e9).max()):.2f} of the bound"
+    if mass is None:
+        return
+    want, room = mass.double().clone(), torch.zeros(mass.shape, dtype=torch.float64, device=DEV)
+    for b, (n, p) in enumerate(zip(step.q_lens, step.past)):
+        if n == 0:
+            continue
+        held, pages = p + n, torch.tensor(step.lists[b], device=DEV)
+        r = torch.arange(held, device=DEV)
+        at = (pages[r // 64], slice(None), r % 64)
+        old = torch.where((r < p)[:, None], mass[at].double(), 0.0)
+        want[at] = old + sums[b].T
+        room[at] = slack[b].T + plain.F32 * 4 * want[at]
+    off = (got.double() - want).abs()
+    assert (off <= room).all(), f"sums: worst {float((off / (room + 1e-300)).nan_to_num(1e9).max()):.2f} of the bound"
+
+
+TREES = [  # rows, past, H, KV, HD: what is cut
+    ([8] + [6] * 15, [6000] + [300] * 15, 8, 4, 128),                       # a line under 32 sequences
+    ([1 + b % 9 for b in range(45)], [(b * 397) % 2100 for b in range(45)], 8, 2, 64),      # a line of more than 32
+    ([200, 90, 0, 256], [3000, 700, 50, 64], 8, 2, 128),                    # tiles by twos, side by side
+    ([300, 10], [129, 2000], 16, 2, 64),
+    ([600], [1500], 8, 1, 128),                                             # five tiles, and ten words of masks
+    ([8], [30000], 4, 1, 128),                                              # one item, a piece a CTA
+    ([2, 3], [20000, 64], 1, 1, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("case", TREES, ids=lambda c: f"{len(c[0])}seq-{c[0][0]}x{c[1][0]}-{c[2]}:{c[3]}x{c[4]}")
+def test_tree_attention_however_it_is_cut(case, dtype):
+    from mynah_slm_b200.ops import tree
+    rows, past, H, KV, HD = case
+    rng = random.Random(len(rows))
+    step, q, k, v = _case(2, rows, past, H, KV, HD, dtype)
+    masks = _masks([_tree(n, rng) for n in rows])
+    out = torch.zeros_like(q)
+    tree.attn_tree(q, out, step, H, KV, HD, k, v, step.pages, masks.to(DEV))
+    assert step.status.item() == 0
+    sees, at = [], 0
+    for n, p in zip(rows, past):
+        j = torch.arange(n)
+        own = ((masks[at:at + n][:, j // 64] >> (j % 64)) & 1).bool() if n else torch.zeros((0, 0), dtype=torch.bool)
+        sees.append(torch.cat([torch.ones((n, p), dtype=torch.bool), own], 1))
+        at += n
+    _agrees(step, q, k, v, H, KV, HD, dtype, out, sees)
+
+
+STEPS = [
+    ([700, 1500, 40], [0, 100, 900], 16, 8, 128),                           # whole items
+    ([300, 5, 1], [4000, 50, 9], 4, 2, 128),                                # several tiles of different lengths on a line
+    ([20] * 40, [(b * 211) % 900 for b in range(40)], 8, 2, 64),            # more than 32 sequences, sums by keys
+    ([1] * 50, [(b * 631) % 4000 for b in range(50)], 8, 2, 128),           # sums from kept scores
+    ([1], [40000], 8, 1, 64),
+    ([90, 33], [5000, 2], 10, 2, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("case", STEPS, ids=lambda c: f"{len(c[0])}seq-{c[0][0]}x{c[1][0]}-{c[2]}:{c[3]}x{c[4]}")
+def test_sums_however_they_are_cut(case, dtype):
+    from mynah_slm_b200.ops import evict
+    rows, past, H, KV, HD = case
+    step, q, k, v = _case(3, rows, past, H, KV, HD, dtype)
+    mass = torch.rand((step.pages.n_pages, KV, 64), device=DEV) * 3
+    got, out = mass.clone(), torch.zeros_like(q)
+    evict.attn_mass(q, out, got, step, H, KV, HD, k, v, step.pages)
+    assert step.status.item() == 0
+    _agrees(step, q, k, v, H, KV, HD, dtype, out, plain.causal(step), mass, got)
+
+
+def test_caches_that_pass_32_bit_offsets():
+    """2,150 pages of 128 kv heads: 2.25 * 10^9 values. The sequences lie in the last pages and in the first ones."""
+    from mynah_slm_b200.ops import evict, tree
+    KV, HD, n_pages, rows, past = 128, 128, 2150, [5, 3], [300, 200]
+    g = torch.Generator().manual_seed(1)
+    lists = [[n_pages - 1 - i for i in range(5)], [3, 0, n_pages - 9, 7]]
+    step = plain.make_step(rows, past, DEV, g, lists=lists)
+    step.pages.n_pages = n_pages
+    used = sorted(p for l in lists for p in l)
+    k, v = (torch.empty((n_pages, KV, 64, HD), dtype=BF16, device=DEV) for _ in range(2))
+    d = torch.Generator(device=DEV).manual_seed(1)
+    for p in used:
+        for c in (k, v):
+            c[p] = torch.randn((KV, 64, HD), generator=d, device=DEV).to(BF16)
+    q = torch.randn((8, KV * HD), generator=d, device=DEV).to(BF16)
+    trees = [[-1, 0, 0, 1, 3], [-1, 0, 1]]
+    masks = _masks(trees)
+    small = torch.tensor(used, device=DEV)
+    where = {p: i for i, p in enumerate(used)}
+    near = plain.make_step(rows, past, DEV, g, lists=[[where[p] for p in l] for l in lists])
+    near.pages.n_pages = len(used)
+    kn, vn = k[small].contiguous(), v[small].contiguous()
+    out, want = torch.zeros_like(q), torch.zeros_like(q)
+    tree.attn_tree(q, out, step, KV, KV, HD, k, v, step.pages, masks.to(DEV))
+    tree.attn_tree(q, want, near, KV, KV, HD, kn, vn, near.pages, masks.to(DEV))
+    assert step.status.item() == 0 and torch.equal(out, want)
+    mass = torch.rand((n_pages, KV, 64), device=DEV)
+    mn = mass[small].contiguous()
+    evict.attn_mass(q, out, mass, step, KV, KV, HD, k, v, step.pages)
+    evict.attn_mass(q, want, mn, near, KV, KV, HD, kn, vn, near.pages)
+    assert step.status.item() == 0 and torch.equal(out, want) and torch.equal(mass[small], mn)
+    tokens = torch.tensor([9, 4, 5, 6, 7, 1, 2, 3], dtype=torch.int32, device=DEV)
+    parents = torch.tensor(trees[0] + trees[1], dtype=torch.int32, device=DEV)
+    chosen = torch.tensor([5, 0, 8, 0, 0, 2, 3, 4], dtype=torch.int32, device=DEV)
+    far = tree.tree_commit(tokens, parents, chosen, step, k[None], v[None], step.pages)
+    ref = tree.tree_commit(tokens, parents, chosen, near, kn[None], vn[None], near.pages)
+    assert all(torch.equal(a, b) for a, b in zip(far, ref)) and far[1].tolist() == [2, 3]
+    assert torch.equal(k[small], kn) and torch.equal(v[small], vn)
+    kept, after = evict.cache_evict(k[None], v[None], mass[None], step, step.pages, 150, 40, 3)
+    kept_n, after_n = evict.cache_evict(kn[None], vn[None], mn[None], near, near.pages, 150, 40, 3)
+    assert step.status.item() == 0 and torch.equal(kept, kept_n) and torch.equal(after, after_n)
+    assert torch.equal(k[small], kn) and torch.equal(v[small], vn) and torch.equal(mass[small], mn)
+
+
+def test_calls_at_once_on_two_streams_and_two_graphs():
+    """Every call has a workspace of its own: calls that run at once, and graphs captured one after the other and replayed at once,
+    give the bits that each gives alone."""
+    from mynah_slm_b200.ops import evict, tree
+    H, KV, HD = 8, 4, 128
+    rng = random.Random(5)
+    jobs = []
+    for s, (rows, past) in enumerate((([24] * 4, [1500, 900, 30, 2000]), ([8] * 8, [700] * 8))):
+        step, q, k, v = _case(30 + s, rows, past, H, KV, HD, BF16)
+        masks = _masks([_tree(n, rng) for n in rows]).to(DEV)
+        mass = torch.rand((step.pages.n_pages, KV, 64), device=DEV)
+
+        def run(step=step, q=q, k=k, v=v, masks=masks, mass=mass):
+            a, b, m = torch.zeros_like(q), torch.zeros_like(q), mass.clone()
+            tree.attn_tree(q, a, step, H, KV, HD, k, v, step.pages, masks)
+            evict.attn_mass(q, b, m, step, H, KV, HD, k, v, step.pages)
+            return a, b, m
+        jobs.append((run, [t.clone() for t in run()], step))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(10):
+        got = []
+        for (run, _, _), st in zip(jobs, streams):
+            with torch.cuda.stream(st):
+                got.append(run())
+        torch.cuda.synchronize()
+        for outs, (_, want, step) in zip(got, jobs):
+            assert step.status.item() == 0 and all(torch.equal(x, y) for x, y in zip(outs, want))
+    graphs = []
+    for (run, _, _), st in zip(jobs, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs = run()
+        graphs.append((graph, outs))
+    for _ in range(10):
+        for (graph, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs), (_, want, step) in zip(graphs, jobs):
+            assert step.status.item() == 0 and all(torch.equal(x, y) for x, y in zip(outs, want))

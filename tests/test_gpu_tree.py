@@ -256,6 +256,7 @@ def test_attn_tree_refuses():
     bad(q=q.float())
     bad(out=out[:2])
     bad(q=q[:, ::2])
+    bad(out=q)
     bad(H=3)
     bad(KV=0)
     bad(HD=60)
