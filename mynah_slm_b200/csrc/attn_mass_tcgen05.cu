@@ -3,8 +3,10 @@
 // The products are taken transposed, S^T = K.Q^T with 128 keys as the rows of the accumulator and up to 128 packed rows as its
 // columns: a key is then a lane of tensor memory, and its sum stays in one thread's register (two threads a key, one for each
 // half of the columns) without any exchange between lanes. w = 2^(s scale log2(e) - lse) needs one multiply-add, one
-// exponential and one addition an element; the exponentials (16 a clock and SM) bound it: 2,048 tokens of 16 heads, causal, are
-// 34 million, 7.5 us on 148 SMs.
+// exponential and one addition an element; the exponentials (16 a clock and SM) bound it: a product of 128 x 128 scores takes an
+// SM 1,024 clocks of them, measured 1,600 in long prompts (8,000 tokens of 32 heads, 370 us; with the selects of masked tiles in
+// every tile 424; a quarter of the exponentials as polynomials 342, not kept for their range and size). 2,048 tokens of 16 heads
+// are 34 million scores, 7.5 us, and take 30: units of unequal length, and 4 us until a CTA's first product.
 //
 //   warp 0      one lane loads by TMA: one operand stays (a key tile against many row tiles, or a sequence's only row tile
 //               against several key tiles), the other streams through two stages;
@@ -36,7 +38,7 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* fix_s = smem;                               // the operand that stays
     unsigned char* str_s = smem + TILE_BYTES;                  // [2] the one that streams
-    float* lse_s = reinterpret_cast<float*>(str_s + 2 * TILE_BYTES);       // [2][ROWS]
+    float* lse_s = reinterpret_cast<float*>(str_s + 2 * TILE_BYTES);       // [2][ROWS] minus the rows' lse
     float* xch = lse_s + 2 * ROWS;                             // [2][KEYS] the second group's sums
     uint64_t* bars = reinterpret_cast<uint64_t*>(xch + 2 * KEYS);
     const uint32_t f_full = smem_u32(bars), s_full = smem_u32(bars + 1), d_full = smem_u32(bars + 3), d_free = smem_u32(bars + 5);
@@ -154,7 +156,7 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int r = e * 32 + lane;
                 float x = INFINITY;
                 if (r < a.rows && row0 + r < n_rows) x = lse[((size_t)g * a.r.T + u.s.q_begin) * G + row0 + r];
-                lse_s[st * ROWS + r] = x == -INFINITY ? INFINITY : x;
+                lse_s[st * ROWS + r] = x == -INFINITY ? -INFINITY : -x;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(l_full + 8 * st);
@@ -180,23 +182,31 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const bool mask = max(0, ktile(i) * KEYS + KEYS - 1 - past) * G > row0 || n_rows - row0 < a.rows;
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    float v[32];
-                    tc_ld32(t_row + st * ROWS + c * 32, reinterpret_cast<uint32_t(&)[32]>(v));
+                    float w[32];
+                    tc_ld32(t_row + st * ROWS + c * 32, reinterpret_cast<uint32_t(&)[32]>(w));
                     const float4* z4 = reinterpret_cast<const float4*>(lse_s + st * ROWS + grp * 64 + c * 32);
+                    if (!mask) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 z = z4[e >> 2];
-                        float p[4];
-                        p[0] = ex2_f(fmaf(v[e], a.r.scale_log2, -z.x));
-                        p[1] = ex2_f(fmaf(v[e + 1], a.r.scale_log2, -z.y));
-                        p[2] = ex2_f(fmaf(v[e + 2], a.r.scale_log2, -z.z));
-                        p[3] = ex2_f(fmaf(v[e + 3], a.r.scale_log2, -z.w));
-                        if (mask) {
-#pragma unroll
-                            for (int f = 0; f < 4; f++) p[f] = (c * 32 + e + f >= lo && c * 32 + e + f < hi) ? p[f] : 0.f;
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 z = z4[e >> 2];
+                            float x[4];
+                            fma2v(x[0], x[1], w[e], w[e + 1], a.r.scale_log2, z.x, z.y);
+                            fma2v(x[2], x[3], w[e + 2], w[e + 3], a.r.scale_log2, z.z, z.w);
+                            add2(sum4[0], sum4[1], ex2_f(x[0]), ex2_f(x[1]));
+                            add2(sum4[2], sum4[3], ex2_f(x[2]), ex2_f(x[3]));
                         }
-                        add2(sum4[0], sum4[1], p[0], p[1]);
-                        add2(sum4[2], sum4[3], p[2], p[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 z = z4[e >> 2];
+                            float x[4];
+                            fma2v(x[0], x[1], w[e], w[e + 1], a.r.scale_log2, z.x, z.y);
+                            fma2v(x[2], x[3], w[e + 2], w[e + 3], a.r.scale_log2, z.z, z.w);
+#pragma unroll
+                            for (int f = 0; f < 4; f++) x[f] = (c * 32 + e + f >= lo && c * 32 + e + f < hi) ? ex2_f(x[f]) : 0.f;
+                            add2(sum4[0], sum4[1], x[0], x[1]);
+                            add2(sum4[2], sum4[3], x[2], x[3]);
+                        }
                     }
                 }
                 tc_fence_before();

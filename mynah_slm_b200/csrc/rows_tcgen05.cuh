@@ -42,6 +42,11 @@ static __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, floa
         " fma.rn.f32x2 rd, ra, rb, rc;\n\t mov.b64 {%0, %1}, rd; }"
         : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c));
 }
+static __device__ __forceinline__ void fma2v(float& x0, float& x1, float a0, float a1, float b, float c0, float c1) {
+    asm("{ .reg .b64 ra, rb, rc, rd;\n\t mov.b64 ra, {%2, %3};\n\t mov.b64 rb, {%4, %4};\n\t mov.b64 rc, {%5, %6};\n\t"
+        " fma.rn.f32x2 rd, ra, rb, rc;\n\t mov.b64 {%0, %1}, rd; }"
+        : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
+}
 static __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
     asm("{ .reg .b64 ra, rb;\n\t mov.b64 ra, {%0, %1};\n\t mov.b64 rb, {%2, %3};\n\t add.rn.f32x2 ra, ra, rb;\n\t mov.b64 {%0, %1}, ra; }"
         : "+f"(x0), "+f"(x1) : "f"(a0), "f"(a1));
