@@ -26,9 +26,10 @@ struct EvictArgs {
 // word is found in three passes, 11, 11 and 10 bits (a histogram of the words that still agree with it in the bits above, the bin
 // that holds it, and so on); then every warp takes a run of rows, counts those above it and those equal to it, and, once it
 // knows the counts of the runs before, writes its own: those above, and the first of the equal ones. The words are read from
-// memory once where they fit shared memory. Bound by its chain of barriers and passes: 448 choices of 2,048 of 4,100 rows,
-// 35 us.
-__global__ void __launch_bounds__(CH_THREADS)
+// memory once where they fit shared memory. Bound by its chain of barriers and passes, so four CTAs an SM (32 registers a thread):
+// 448 choices of 2,048 of 4,100 rows 27.5 us, against 35 with two (64 registers), which are 5% faster for rows beyond shared
+// memory (48 choices of 8,192 of 20,000: 96 and 101 us); with 256 threads 30 and 167.
+__global__ void __launch_bounds__(CH_THREADS, 4)
 evict_choose_kernel(const float* __restrict__ mass, PageTable pt, const int* __restrict__ kv_len, EvictArgs a, int* __restrict__ kept,
                     int* __restrict__ new_len, int* __restrict__ status) {
     extern __shared__ uint32_t words_s[];
@@ -171,8 +172,8 @@ struct MoveArgs {
 // next step's already asked for, when the barrier lets the step's writes go; and a row that is written in a step is a source of
 // that step or of an earlier one. Places are worked out 512 rows ahead, so that the copies wait for one read, not for the
 // choice, the page list and the row one behind the other. LANES: 16 (whole rows of 256 bytes: 28 layers of 2 sequences, 2,048 rows
-// of 8 heads of 128, 161 us of both launches' 198, against 329 with 4), or 4 where that would leave too few CTAs (one layer of one sequence, 512
-// rows of 700: both launches 12.3 against 14.4 us).
+// of 8 heads of 128, 160 us of both launches' 194, against 329 with 4), or 4 where that would leave too few CTAs (one layer of one
+// sequence, 512 rows of 700: both launches 12.3 against 14.4 us).
 template <int LANES>
 __global__ void __launch_bounds__(MV_THREADS)
 evict_move_kernel(uint4* __restrict__ k, uint4* __restrict__ v, float* __restrict__ mass, PageTable from, PageTable to,
