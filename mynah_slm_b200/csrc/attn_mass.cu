@@ -41,7 +41,9 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
     float* q_s = k_s + GK * p;                                     // [GR][p]
     __shared__ float lse_s[GR];
     MassUnit u;
-    if (!find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x, u, status)) return;
+    const bool any = find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x, u, status);
+    griddep_wait();
+    if (!any) return;
     const int g = blockIdx.y, G = a.r.G, past = u.s.kvl - u.s.n_q, key0 = u.kt0 * GK, n_rows = u.s.n_q * G;
     const int tiles = mass_rtiles(u.s, a);
     const int r0 = max(u.piece * u.rt, mass_first_tile(u, a)), r1 = (int)min((long long)tiles, (long long)(u.piece + 1) * u.rt);
@@ -120,6 +122,7 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
             *m = key < past ? *m + sum[i] : sum[i];
         }
     }
+    griddep_launch_late();
 }
 
 // Adds the pieces of every key's sum in order. A thread a key of a key tile; key tiles are numbered sequence by sequence.
@@ -127,7 +130,9 @@ __global__ void attn_mass_add_kernel(float* __restrict__ mass, const float* __re
                                      const int* __restrict__ kv_len, PageTable pt, MassArgs a, int* __restrict__ status) {
     MassUnit u;
     // the units of key tile n of the step: unit numbers are found as the first launch's were, from the tile's first piece on
-    if (!find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x, u, status)) return;
+    const bool any = find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x, u, status);
+    griddep_wait();
+    if (!any) return;
     if (u.piece != 0 || u.pieces <= 1) return;                     // one CTA a key tile; uncut tiles are done
     const int g = blockIdx.y, past = u.s.kvl - u.s.n_q, key = u.kt0 * a.keys + threadIdx.x;
     if (threadIdx.x >= a.keys || key >= u.s.kvl) return;
@@ -146,10 +151,11 @@ int launch_mass_generic(const void* q, const void* k, const float* lse, float* m
     auto kb = attn_mass_kernel<bf16>;
     static std::atomic<unsigned long long> opted_f{0}, opted_b{0};
     constexpr size_t most = (size_t)(GK + GR) * (256 + 4) * sizeof(float);
-    const cudaError_t e = dtype == MYNAH_F32 ? shared_memory_once(kf, most, opted_f) : shared_memory_once(kb, most, opted_b);
+    cudaError_t e = dtype == MYNAH_F32 ? shared_memory_once(kf, most, opted_f) : shared_memory_once(kb, most, opted_b);
+    if (e == cudaSuccess)
+        e = dtype == MYNAH_F32 ? launch_behind(kf, grid, dim3(256), smem, stream, (const float*)q, (const float*)k, lse, mass, part, cu_q, kv_len, pt, a, status)
+                               : launch_behind(kb, grid, dim3(256), smem, stream, (const bf16*)q, (const bf16*)k, lse, mass, part, cu_q, kv_len, pt, a, status);
     if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
-    if (dtype == MYNAH_F32) kf<<<grid, 256, smem, stream>>>((const float*)q, (const float*)k, lse, mass, part, cu_q, kv_len, pt, a, status);
-    else kb<<<grid, 256, smem, stream>>>((const bf16*)q, (const bf16*)k, lse, mass, part, cu_q, kv_len, pt, a, status);
     return mynah_check_launch("attn_mass");
 }
 
@@ -267,6 +273,7 @@ MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, 
         return -1;
     }
     if (a.by_keys) return 0;                                       // nothing was cut over its rows
-    attn_mass_add_kernel<<<grid, a.keys, 0, stream>>>(mass, part, cu_q, kv_len, pt, a, status);
+    const cudaError_t e = launch_behind(attn_mass_add_kernel, grid, dim3(a.keys), 0, stream, mass, (const float*)part, cu_q, kv_len, pt, a, status);
+    if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
     return mynah_check_launch("attn_mass_add");
 }

@@ -47,7 +47,9 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     MassUnit u;
-    if (!find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x / a.r.KV, u, status)) return;
+    const bool any = find_mass_unit(cu_q, kv_len, pt, a, blockIdx.x / a.r.KV, u, status);
+    griddep_wait();
+    if (!any) return;
     const int g = blockIdx.x % a.r.KV, G = a.r.G, past = u.s.kvl - u.s.n_q, n_rows = u.s.n_q * G;
     const int r0 = max(u.piece * u.rt, a.by_keys ? 0 : mass_first_tile(u, a));
     const int r1 = (int)min((long long)mass_rtiles(u.s, a), (long long)(u.piece + 1) * u.rt);
@@ -233,6 +235,7 @@ attn_mass_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         if (!ok && lane == 0) atomicOr(status, MYNAH_ST_TIMEOUT);
     }
+    griddep_launch_late();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -249,7 +252,9 @@ int go(const CUtensorMap& mq, const CUtensorMap& mk, const float* lse, float* ma
     static std::atomic<unsigned long long> opted{0};
     const cudaError_t e = shared_memory_once(kern, smem, opted);
     if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
-    kern<<<(unsigned)(mass_units_max(a, n_ids) * a.r.KV), THREADS, smem, stream>>>(mq, mk, lse, mass, part, cu_q, kv_len, pt, a, status);
+    const dim3 grid((unsigned)(mass_units_max(a, n_ids) * a.r.KV));
+    const cudaError_t err = launch_behind(kern, grid, dim3(THREADS), smem, stream, mq, mk, lse, mass, part, cu_q, kv_len, pt, a, status);
+    if (err != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(err));
     return mynah_check_launch("attn_mass");
 }
 

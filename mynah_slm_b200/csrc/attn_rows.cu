@@ -264,6 +264,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         }
     }
     } while (u.next(cu_q, kv_len, pt, a, status));
+    griddep_launch_late();
 }
 
 // Four values of a row; rows may begin anywhere.
@@ -343,6 +344,7 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
             if (col == 0 && sc.lse != nullptr) sc.lse[((size_t)at.g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m + log2f(l);
         }
     }
+    griddep_launch_late();
 }
 
 template <typename T, int TY, int TX, int NC>

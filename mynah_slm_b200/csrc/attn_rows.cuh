@@ -46,8 +46,8 @@ template <typename K> static inline cudaError_t shared_memory_once(K kernel, siz
     return e;
 }
 
-// A launch that may begin while the kernel before it on the stream finishes; the kernel waits for that one's results itself
-// (griddep_wait) before it touches anything.
+// A launch that may begin while the kernel before it on the stream finishes; every CTA of it waits for that one (griddep_wait), so
+// that it cannot end first, and before the wait it reads only what was there before both (the step's description, the page lists).
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
