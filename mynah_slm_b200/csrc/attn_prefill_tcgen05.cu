@@ -154,6 +154,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const uint32_t s_full = smem_u32(bars + 5), v_free = smem_u32(bars + 7);
     const uint32_t p_full = smem_u32(bars + 9), o_done = smem_u32(bars + 11), x_full = smem_u32(bars + 12);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+    const uint32_t o_last = smem_u32(bars + 15);               // the last tile's product: one phase
     float* xch = reinterpret_cast<float*>(bars + 16);          // [2 buffers][2 groups][128 rows]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -192,6 +193,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             mbar_init(x_full + 8 * i, 8);
         }
         mbar_init(o_done, 1);
+        mbar_init(o_last, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
@@ -303,6 +305,7 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                               idesc_o, (j | k) != 0);
                 tc_commit(v_free + 8 * st);
                 tc_commit(o_done);
+                if (j + 1 == n_tiles) tc_commit(o_last);
                 STAMP(j, 4);
                 if (NS == 1 && j + 1 < n_tiles) {              // one score buffer: the next scores overwrite these probabilities,
                     ok = mbar_wait(k_full, use_of(j + 1));     // so they are issued behind the product that reads them
@@ -499,7 +502,9 @@ attn_prefill_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             if (!warp_wait(x_full + 8 * st, (n_tiles >> 1) & 1)) ok = false;
             else l += xch[(st * 2 + (grp ^ 1)) * BQ + row];
         }
-        if (ok && !warp_wait(o_done, (n_tiles - 1) & 1)) ok = false;
+        // (Not o_done: with the last tile's scores and weights done, the product of the tile before it may still wait for its V, and
+        // a wait for o_done's last phase would be answered by the phase two before it.)
+        if (ok && !warp_wait(o_last, 0)) ok = false;
         if (ok) {
             tc_fence_after();
             // the term without a key counts 2^(0 - m), or 2^(sink log2(e) - m); where that overflows, the keys' share of the softmax is zero
