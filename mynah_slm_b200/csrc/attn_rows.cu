@@ -405,7 +405,7 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
     a.ctas = 2 * mynah_sm_count();                                 // two CTAs an SM
     if (!tc) {
         a.tile_rows = longest <= 16 ? 16 : 64;
-        a.most_rows = (int)(longest < a.tile_rows ? longest : a.tile_rows);
+        a.most_rows = (int)(longest < 1 ? 1 : longest < a.tile_rows ? longest : a.tile_rows);      // (a step may be all padding)
         a.finish();
         return false;
     }
@@ -425,7 +425,7 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
         if (a.group > most) a.group = (int)most;
         a.ctas /= a.group;
     }
-    a.most_rows = (int)(longest < a.tile_rows ? longest : a.tile_rows);
+    a.most_rows = (int)(longest < 1 ? 1 : longest < a.tile_rows ? longest : a.tile_rows);      // (a step may be all padding)
     a.finish();
     return tc;
 }

@@ -46,7 +46,7 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
     if T == 0 or ctx.B == 0:
         return
     n_ids = pages.ids.numel()
-    scratch = row_scratch("attn_mass", scratch, _mass_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids), q.device)
+    scratch = row_scratch("attn_mass", scratch, _mass_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids), ctx.status)
     call("mynah_attn_mass", q.data_ptr(), out.data_ptr(), mass.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q),
          _row_stride(out), k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(),
          pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, n_ids, float(scale), scratch.data_ptr(), scratch.numel(),
@@ -81,8 +81,7 @@ def cache_evict(k_caches: torch.Tensor, v_caches: torch.Tensor, masses: torch.Te
         if out_pages.n_pages != n_pages:
             raise KernelError(f"cache_evict: the out pages are of a pool of {out_pages.n_pages}, the pages of one of {n_pages}")
     es = k_caches.element_size()
-    kept = torch.empty((E, ctx.B, KV, keep), dtype=torch.int32, device=dev)
-    new_len = torch.empty((ctx.B,), dtype=torch.int32, device=dev)
+    kept, new_len = ctx.kv_len.new_empty((E, ctx.B, KV, keep)), ctx.kv_len.new_empty(ctx.B)
     if E == 0 or ctx.B == 0:
         return kept, new_len
     call("mynah_cache_evict", k_caches.data_ptr(), v_caches.data_ptr(), masses.data_ptr(), E, ctx.B, KV, n_pages, HD * es,

@@ -91,9 +91,10 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def row_scratch(who: str, scratch: Optional[torch.Tensor], need: int, dev) -> torch.Tensor:
+def row_scratch(who: str, scratch: Optional[torch.Tensor], need: int, status: torch.Tensor) -> torch.Tensor:
+    dev = status.device
     if scratch is None:
-        return torch.empty(need, dtype=torch.float32, device=dev)
+        return status.new_empty(need)                          # (32-bit words; torch.empty takes a us more)
     if scratch.dtype != torch.float32 or scratch.device != dev or not scratch.is_contiguous() or scratch.numel() < need:
         raise KernelError(f"{who}: scratch must be at least {need} contiguous float32 on {dev}")
     return scratch
@@ -125,7 +126,7 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
         raise KernelError(f"attn_tree: the masks must be contiguous int64 [{T}, words] on {q.device}, got {tuple(masks.shape)} {masks.dtype}")
     if T == 0 or ctx.B == 0:
         return
-    scratch = row_scratch("attn_tree", scratch, _tree_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), q.device)
+    scratch = row_scratch("attn_tree", scratch, _tree_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), ctx.status)
     call("mynah_attn_tree", q.data_ptr(), out.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q), _row_stride(out),
          k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(),
          pages.base.data_ptr(), pages.n_pages, masks.data_ptr(), masks.shape[1], float(scale), scratch.data_ptr(), scratch.numel(),
@@ -162,8 +163,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
     if not 0 <= ctx.max_q_len <= 4096:
         raise KernelError(f"tree_commit: trees of {ctx.max_q_len} rows, 4096 are the most")
     check_lists("tree_commit", dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
-    path = torch.empty_like(tokens)
-    count, after = tokens.new_empty(ctx.B), tokens.new_empty(ctx.B)
+    path, count, after = tokens.new_empty(T), tokens.new_empty(ctx.B), tokens.new_empty(ctx.B)       # (torch.empty takes a us more)
     E, _, KV, _, HD = k_caches.shape
     es = k_caches.element_size()
     call("mynah_tree_commit", tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), T, ctx.B, ctx.max_q_len, ctx.cu_q.data_ptr(),

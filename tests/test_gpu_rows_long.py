@@ -92,6 +92,7 @@ TREES = [  # rows, past, H, KV, HD: what is cut
     ([600], [1500], 8, 1, 128),                                             # five tiles, and ten words of masks
     ([8], [30000], 4, 1, 128),                                              # one item, a piece a CTA
     ([2, 3], [20000, 64], 1, 1, 64),
+    ([5, 2], [300, 70], 100, 1, 64),                                        # a token a tile
 ]
 
 
@@ -136,6 +137,23 @@ def test_sums_however_they_are_cut(case, dtype):
     evict.attn_mass(q, out, got, step, H, KV, HD, k, v, step.pages)
     assert step.status.item() == 0
     _agrees(step, q, k, v, H, KV, HD, dtype, out, plain.causal(step), mass, got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_a_step_of_nothing_but_padding(dtype):
+    """Sequences without rows in the step, and rows of q behind the last one: nothing is written."""
+    from mynah_slm_b200.ops import evict, tree
+    H, KV, HD = 4, 2, 64
+    step, _, k, v = _case(4, [0, 0], [100, 0], H, KV, HD, dtype)
+    q, out = torch.randn((6, H * HD), device=DEV).to(dtype), torch.full((6, H * HD), 7.0, dtype=dtype, device=DEV)
+    mass = torch.rand((step.pages.n_pages, KV, 64), device=DEV)
+    before = mass.clone()
+    tree.attn_tree(q, out, step, H, KV, HD, k, v, step.pages, torch.zeros((6, 1), dtype=torch.int64, device=DEV))
+    evict.attn_mass(q, out, mass, step, H, KV, HD, k, v, step.pages)
+    assert step.status.item() == 0 and (out == 7.0).all() and torch.equal(mass, before)
+    ids = torch.zeros(6, dtype=torch.int32, device=DEV)
+    path, count, after = tree.tree_commit(ids, ids, ids, step, k[None], v[None], step.pages)
+    assert step.status.item() == 0 and count.tolist() == [0, 0] and after.tolist() == [-1, -1]
 
 
 def test_caches_that_pass_32_bit_offsets():
