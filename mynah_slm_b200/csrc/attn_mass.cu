@@ -228,10 +228,24 @@ MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, 
 
 // As mynah_attn_tree with causal rows, and mass [n_pages, KV, 64] fp32. n_ids: entries of page_ids (no fewer than the
 // sequences' pages together).
-MYNAH_API int mynah_attn_mass(const void* q, void* out, float* mass, int dtype, int T, int B, int max_q_len, int H, int KV, int HD, int ldq,
-                              int ldo, const void* k_cache, const void* v_cache, const int* cu_q, const int* kv_len,
-                              const int* page_indptr, const int* page_ids, const int* page_base, int n_pages, int n_ids, float scale,
-                              float* scratch, long long scratch_floats, int* status, cudaStream_t stream) {
+struct AttnMassCall {
+    const void* q;
+    void* out;
+    float* mass;
+    int dtype, T, B, max_q_len, H, KV, HD, ldq, ldo;
+    const void *k_cache, *v_cache;
+    const int *cu_q, *kv_len, *page_indptr, *page_ids, *page_base;
+    int n_pages, n_ids;
+    float scale;
+    float* scratch;
+    long long scratch_floats;
+    int* status;
+    cudaStream_t stream;
+};
+static_assert(sizeof(AttnMassCall) == 168, "as packed by the caller");
+MYNAH_API int mynah_attn_mass(const AttnMassCall* call) {
+    const auto& [q, out, mass, dtype, T, B, max_q_len, H, KV, HD, ldq, ldo, k_cache, v_cache, cu_q, kv_len, page_indptr, page_ids, page_base,
+                 n_pages, n_ids, scale, scratch, scratch_floats, status, stream] = *call;
     if (T <= 0 || B <= 0) return 0;
     MYNAH_REQUIRE(mass != nullptr && n_ids >= 0, "attn_mass: sums and the number of page entries are required");
     MYNAH_REQUIRE(scale >= 0.f, "attn_mass: the score scale %g is negative", scale);

@@ -358,10 +358,21 @@ bool row_ok(int bytes) { return bytes > 0 && bytes % 16 == 0; }
 
 // k [E, n_pages, KV, 64, k_bytes], v likewise, mass [E, n_pages, KV, 64]; kept [E, B, KV, keep], new_len [B]. `same`: the out
 // page lists are the page lists. n_ids: entries of page_ids.
-MYNAH_API int mynah_cache_evict(void* k, void* v, float* mass, int E, int B, int KV, int n_pages, int k_bytes, int v_bytes,
-                                const int* kv_len, const int* page_indptr, const int* page_ids, const int* page_base, int n_ids,
-                                const int* out_indptr, const int* out_ids, const int* out_base, int same,
-                                int keep, int recent, int first, int* kept, int* new_len, int* status, cudaStream_t stream) {
+struct CacheEvictCall {
+    void *k, *v;
+    float* mass;
+    int E, B, KV, n_pages, k_bytes, v_bytes;
+    const int *kv_len, *page_indptr, *page_ids, *page_base;
+    int n_ids;
+    const int *out_indptr, *out_ids, *out_base;
+    int same, keep, recent, first;
+    int *kept, *new_len, *status;
+    cudaStream_t stream;
+};
+static_assert(sizeof(CacheEvictCall) == 160, "as packed by the caller");
+MYNAH_API int mynah_cache_evict(const CacheEvictCall* call) {
+    const auto& [k, v, mass, E, B, KV, n_pages, k_bytes, v_bytes, kv_len, page_indptr, page_ids, page_base, n_ids, out_indptr, out_ids, out_base,
+                 same, keep, recent, first, kept, new_len, status, stream] = *call;
     if (E <= 0 || B <= 0) return 0;
     MYNAH_REQUIRE(KV > 0 && n_pages >= 0, "cache_evict: %d kv heads, %d pages", KV, n_pages);
     MYNAH_REQUIRE(row_ok(k_bytes) && row_ok(v_bytes), "cache_evict: rows of %d and %d bytes are not whole 16-byte pieces", k_bytes, v_bytes);
@@ -389,10 +400,20 @@ MYNAH_API int mynah_cache_evict(void* k, void* v, float* mass, int E, int B, int
 }
 
 // tokens, parents, chosen [T]; k [E, n_pages, KV, 64, k_bytes], v likewise. path [T] (-1 behind a path's end), count [B], next [B].
-MYNAH_API int mynah_tree_commit(const int* tokens, const int* parents, const int* chosen, int T, int B, int max_q_len, const int* cu_q,
-                                const int* kv_len, const int* page_indptr, const int* page_ids, const int* page_base, int n_pages,
-                                void* k, void* v, int E, int KV, int k_bytes, int v_bytes, int* path, int* count, int* next, int* status,
-                                cudaStream_t stream) {
+struct TreeCommitCall {
+    const int *tokens, *parents, *chosen;
+    int T, B, max_q_len;
+    const int *cu_q, *kv_len, *page_indptr, *page_ids, *page_base;
+    int n_pages;
+    void *k, *v;
+    int E, KV, k_bytes, v_bytes;
+    int *path, *count, *next, *status;
+    cudaStream_t stream;
+};
+static_assert(sizeof(TreeCommitCall) == 160, "as packed by the caller");
+MYNAH_API int mynah_tree_commit(const TreeCommitCall* call) {
+    const auto& [tokens, parents, chosen, T, B, max_q_len, cu_q, kv_len, page_indptr, page_ids, page_base, n_pages, k, v, E, KV, k_bytes, v_bytes,
+                 path, count, next, status, stream] = *call;
     if (B <= 0) return 0;
     MYNAH_REQUIRE(E >= 0 && KV > 0, "tree_commit: %d layers, %d kv heads", E, KV);
     MYNAH_REQUIRE(row_ok(k_bytes) && row_ok(v_bytes), "tree_commit: rows of %d and %d bytes are not whole 16-byte pieces", k_bytes, v_bytes);

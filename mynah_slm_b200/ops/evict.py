@@ -9,6 +9,7 @@ is, while the tokens that follow are rotated for their true positions.)
 from __future__ import annotations
 
 from functools import lru_cache
+from struct import Struct
 from typing import Optional
 
 import torch
@@ -17,7 +18,11 @@ from ..cache.pages import PAGE_TOKENS
 from . import lib
 from .kernels import PageTableView
 from .lib import KernelError, call, code, stream_on
-from .tree import _row_stride, check_layers, check_lists, check_rows, row_scratch
+from .tree import check_layers, check_lists, check_rows, row_scratch
+
+# the arguments of the C entries, which take them as one struct
+_MASS_CALL = Struct("@3P9i7P2ifPq2P")
+_EVICT_CALL = Struct("@3P6i4Pi3P4i4P")
 
 
 @lru_cache(maxsize=256)
@@ -37,9 +42,8 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
     head's query heads give it, added to what it holds for rows that were there before the step, in place of it for the step's own
     (so nothing has to be cleared when a page is taken). Other rows' sums are left as they are. The order of the sums does not
     depend on timing, provided that no page is in two sequences' lists (a shared page's sums would be written by both)."""
-    dt = check_rows("attn_mass", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
-    T = q.shape[0]
-    if mass.dtype != torch.float32 or mass.device != q.device or not mass.is_contiguous() or mass.dim() != 3 \
+    dt, index, T, ldq, ldo = check_rows("attn_mass", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
+    if mass.dtype is not torch.float32 or mass.get_device() != index or not mass.is_contiguous() or mass.dim() != 3 \
             or mass.shape[1:] != (KV, PAGE_TOKENS) or mass.shape[0] < pages.n_pages:
         raise KernelError(f"attn_mass: the sums must be contiguous float32 [{pages.n_pages}, {KV}, {PAGE_TOKENS}] on {q.device}, "
                           f"got {tuple(mass.shape)} {mass.dtype}")
@@ -47,10 +51,10 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
         return
     n_ids = pages.ids.numel()
     scratch = row_scratch("attn_mass", scratch, _mass_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids), ctx.status)
-    call("mynah_attn_mass", q.data_ptr(), out.data_ptr(), mass.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q),
-         _row_stride(out), k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(),
-         pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, n_ids, float(scale), scratch.data_ptr(), scratch.numel(),
-         ctx.status.data_ptr(), stream_on(q.device.index))
+    call("mynah_attn_mass", _MASS_CALL.pack(
+        q.data_ptr(), out.data_ptr(), mass.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, ldq, ldo, k_cache.data_ptr(), v_cache.data_ptr(),
+        ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, n_ids, scale,
+        scratch.data_ptr(), scratch.numel(), ctx.status.data_ptr(), stream_on(index)))
 
 
 def cache_evict(k_caches: torch.Tensor, v_caches: torch.Tensor, masses: torch.Tensor, ctx, pages: PageTableView, keep: int, recent: int,
@@ -63,29 +67,28 @@ def cache_evict(k_caches: torch.Tensor, v_caches: torch.Tensor, masses: torch.Te
 
     k_caches, v_caches [layers, n_pages, kv heads, 64, head], masses [layers, n_pages, kv heads, 64] fp32, ctx.kv_len: the rows
     held. Returns int32 (kept [layers, B, kv heads, keep]: the rows that stayed, ascending, -1 behind them; kv_len [B])."""
-    check_layers("cache_evict", k_caches, v_caches, pages)
+    index = check_layers("cache_evict", k_caches, v_caches, pages)
     E, n_pages, KV, _, HD = k_caches.shape
-    dev = k_caches.device
-    if masses.dtype != torch.float32 or masses.device != dev or not masses.is_contiguous() or masses.shape != (E, n_pages, KV, PAGE_TOKENS):
-        raise KernelError(f"cache_evict: the sums must be contiguous float32 {(E, n_pages, KV, PAGE_TOKENS)} on {dev}, "
+    if masses.dtype is not torch.float32 or masses.get_device() != index or not masses.is_contiguous() or masses.shape != (E, n_pages, KV, PAGE_TOKENS):
+        raise KernelError(f"cache_evict: the sums must be contiguous float32 {(E, n_pages, KV, PAGE_TOKENS)} on cuda:{index}, "
                           f"got {tuple(masses.shape)} {masses.dtype}")
     keep, recent, first = int(keep), int(recent), int(first)
-    if keep < 1 or recent < 0 or first < 0 or recent + first > keep:
+    if not 1 <= keep < 1 << 31 or recent < 0 or first < 0 or recent + first > keep:
         raise KernelError(f"cache_evict: {first} first and {recent} recent rows do not fit the {keep} that are kept")
-    check_lists("cache_evict", dev, ctx.B, None, ctx.kv_len, pages, ctx.status)
+    check_lists("cache_evict", index, ctx.B, None, ctx.kv_len, pages, ctx.status)
     same = out_pages is None
     if same:
         out_pages = pages
     else:
-        check_lists("cache_evict", dev, ctx.B, None, ctx.kv_len, out_pages, ctx.status)
+        check_lists("cache_evict", index, ctx.B, None, ctx.kv_len, out_pages, ctx.status)
         if out_pages.n_pages != n_pages:
             raise KernelError(f"cache_evict: the out pages are of a pool of {out_pages.n_pages}, the pages of one of {n_pages}")
     es = k_caches.element_size()
     kept, new_len = ctx.kv_len.new_empty((E, ctx.B, KV, keep)), ctx.kv_len.new_empty(ctx.B)
     if E == 0 or ctx.B == 0:
         return kept, new_len
-    call("mynah_cache_evict", k_caches.data_ptr(), v_caches.data_ptr(), masses.data_ptr(), E, ctx.B, KV, n_pages, HD * es,
-         v_caches.shape[4] * es, ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(),
-         pages.ids.numel(), out_pages.indptr.data_ptr(), out_pages.ids.data_ptr(), out_pages.base.data_ptr(), 1 if same else 0,
-         keep, recent, first, kept.data_ptr(), new_len.data_ptr(), ctx.status.data_ptr(), stream_on(dev.index))
+    call("mynah_cache_evict", _EVICT_CALL.pack(
+        k_caches.data_ptr(), v_caches.data_ptr(), masses.data_ptr(), E, ctx.B, KV, n_pages, HD * es, v_caches.shape[4] * es, ctx.kv_len.data_ptr(),
+        pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.ids.numel(), out_pages.indptr.data_ptr(), out_pages.ids.data_ptr(),
+        out_pages.base.data_ptr(), same, keep, recent, first, kept.data_ptr(), new_len.data_ptr(), ctx.status.data_ptr(), stream_on(index)))
     return kept, new_len

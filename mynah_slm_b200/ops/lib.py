@@ -26,10 +26,7 @@ _lib: ctypes.CDLL | None = None
 
 P = c_void_p
 _SIGNATURES: dict[str, list] = {
-    "mynah_attn_tree": [P, P] + [c_int] * 9 + [P, P, P, P, P, P, P, c_int, P, c_int, c_float, P, c_longlong, P, P],
-    "mynah_attn_mass": [P, P, P] + [c_int] * 9 + [P, P, P, P, P, P, P, c_int, c_int, c_float, P, c_longlong, P, P],
-    "mynah_cache_evict": [P, P, P] + [c_int] * 6 + [P, P, P, P, c_int, P, P, P] + [c_int] * 4 + [P, P, P, P],
-    "mynah_tree_commit": [P, P, P, c_int, c_int, c_int, P, P, P, P, P, c_int, P, P] + [c_int] * 4 + [P, P, P, P, P],
+    "mynah_attn_tree": [P], "mynah_attn_mass": [P], "mynah_cache_evict": [P], "mynah_tree_commit": [P],      # a packed struct each
     "mynah_embed_gather": [P, c_int, P, P, c_int, c_int, c_int, c_float, P],
     "mynah_rmsnorm": [P, P, P, c_int, P, P, c_int, c_int, c_int, c_float, c_float, P],
     "mynah_residual_add": [P, P, c_int, c_longlong, c_float, P],

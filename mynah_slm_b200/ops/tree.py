@@ -10,6 +10,7 @@ past + 0, 1, 2, ..., where a sequence that had taken the tokens one by one would
 from __future__ import annotations
 
 from functools import lru_cache
+from struct import Struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -22,6 +23,9 @@ from .lib import KernelError, call, code, stream_on
 
 _INF = float("inf")
 _I32 = torch.int32
+# the arguments of the C entries, which take them as one struct
+_TREE_CALL = Struct("@2P9i7PiPifPq2P")
+_COMMIT_CALL = Struct("@3P3i5Pi2P4i5P")
 
 
 def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> tuple[np.ndarray, np.ndarray]:
@@ -46,10 +50,11 @@ def tree_rows(parents: Sequence[int], words: Optional[int] = None) -> tuple[np.n
 
 
 def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor,
-               v_cache: torch.Tensor, pages: PageTableView, scale: float) -> int:
-    """What the attention of a few rows a sequence asks of its arguments. Returns q's type code."""
-    dev, dt = q.device, q.dtype
-    if not q.is_cuda or dev.index != torch.cuda.current_device():
+               v_cache: torch.Tensor, pages: PageTableView, scale: float) -> tuple[int, int, int, int, int]:
+    """What the attention of a few rows a sequence asks of its arguments. Returns q's type code and device, its rows, and the row
+    strides of q and the output. (Every call pays for this in full: few and cheap lookups.)"""
+    index, dt = q.get_device(), q.dtype
+    if index < 0 or index != torch.cuda.current_device():
         raise KernelError(f"{who}: q is not on the current CUDA device")
     if KV < 1 or H < 1 or H % KV:
         raise KernelError(f"{who}: {H} heads over {KV} kv heads")
@@ -58,37 +63,41 @@ def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: in
     if not 0.0 <= scale < _INF:
         raise KernelError(f"{who}: the score scale {scale} is not a positive number, nor 0 for 1 / sqrt(head_dim)")
     dcode = code(dt)
-    width = H * HD
-    for t in (q, out):
-        shape = t.shape
-        if len(shape) != 2 or shape[1] < width or t.stride(1) != 1 or (shape[0] > 1 and not width <= t.stride(0) < 1 << 31):
-            raise KernelError(f"{who}: q and the output must be rows of at least {width} values, one row behind the other, got "
-                              f"{tuple(shape)} with strides {t.stride()}")
-    if out.dtype != dt or out.device != dev or out.shape[0] < q.shape[0]:
-        raise KernelError(f"{who}: the output is {tuple(out.shape)} {out.dtype} on {out.device}, q {tuple(q.shape)} {dt} on {dev}")
-    if q.data_ptr() == out.data_ptr() and q.shape[0]:
+    T, ldq = _rows_of(who, q, H * HD)
+    n_out, ldo = _rows_of(who, out, H * HD)
+    if out.dtype is not dt or out.get_device() != index or n_out < T:
+        raise KernelError(f"{who}: the output is {tuple(out.shape)} {out.dtype} on {out.device}, q {tuple(q.shape)} {dt} on {q.device}")
+    if q.data_ptr() == out.data_ptr() and T:
         raise KernelError(f"{who}: the output lies over q, which is read until the end")
     cache = (KV, PAGE_TOKENS, HD)
     for t in (k_cache, v_cache):
         shape = t.shape
-        if t.dtype != dt or t.device != dev or len(shape) != 4 or shape[1:] != cache or shape[0] < pages.n_pages or not t.is_contiguous():
+        if t.dtype is not dt or t.get_device() != index or len(shape) != 4 or shape[1:] != cache \
+                or shape[0] < pages.n_pages or not t.is_contiguous():
             raise KernelError(f"{who}: the cache must be contiguous [{pages.n_pages}, {KV}, {PAGE_TOKENS}, {HD}] of q's type and device, "
                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
     if ctx.B < 0 or ctx.max_q_len < 0:
         raise KernelError(f"{who}: {ctx.B} sequences of up to {ctx.max_q_len} rows")
-    check_lists(who, dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
-    return dcode
+    check_lists(who, index, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
+    return dcode, index, T, ldq, ldo
 
 
-def check_lists(who: str, dev, B: int, cu_q: Optional[torch.Tensor], kv_len: torch.Tensor, pages: PageTableView, status: torch.Tensor) -> None:
+def _rows_of(who: str, t: torch.Tensor, width: int) -> tuple[int, int]:
+    """(rows, row stride) of q or the output."""
+    if t.dim() == 2:
+        n, w = t.shape
+        ld, one = t.stride()
+        if w >= width and one == 1 and (n < 2 or width <= ld < 1 << 31):
+            return n, ld if n > 1 else w
+    raise KernelError(f"{who}: q and the output must be rows of at least {width} values, one row behind the other, got "
+                      f"{tuple(t.shape)} with strides {t.stride()}")
+
+
+def check_lists(who: str, index: int, B: int, cu_q: Optional[torch.Tensor], kv_len: torch.Tensor, pages: PageTableView, status: torch.Tensor) -> None:
     for t, n in ((cu_q, B + 1), (kv_len, B), (pages.indptr, B + 1), (pages.base, B), (pages.ids, 0), (status, 1)):
-        if t is not None and (t.dtype != _I32 or t.device != dev or t.numel() < n or not t.is_contiguous()):
-            raise KernelError(f"{who}: cu_q, kv_len, the page lists and the status word must be contiguous int32 on {dev} for {B} sequences, "
-                              f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        if t is not None and (t.dtype is not _I32 or t.get_device() != index or t.numel() < n or not t.is_contiguous()):
+            raise KernelError(f"{who}: cu_q, kv_len, the page lists and the status word must be contiguous int32 on cuda:{index} for {B} "
+                              f"sequences, got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 def row_scratch(who: str, scratch: Optional[torch.Tensor], need: int, status: torch.Tensor) -> torch.Tensor:
@@ -119,28 +128,29 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
     1 / sqrt(HD). ctx: the step's description (B, max_q_len, cu_q, kv_len, status). Rows of the cache that a row does not see
     have no influence on it, whatever they hold. float32 and bfloat16, heads of any multiple of 8 up to 256; bfloat16 heads of 64
     and 128 run on the tensor cores. `scratch`: attn_tree_scratch_floats fp32 words, taken from torch's allocator unless given."""
-    dt = check_rows("attn_tree", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
-    T = q.shape[0]
-    if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] < T or masks.shape[1] < 1 or not masks.is_contiguous() \
-            or masks.device != q.device:
+    dt, index, T, ldq, ldo = check_rows("attn_tree", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
+    if masks.dtype is not torch.int64 or masks.dim() != 2 or masks.shape[0] < T or masks.shape[1] < 1 or not masks.is_contiguous() \
+            or masks.get_device() != index:
         raise KernelError(f"attn_tree: the masks must be contiguous int64 [{T}, words] on {q.device}, got {tuple(masks.shape)} {masks.dtype}")
     if T == 0 or ctx.B == 0:
         return
     scratch = row_scratch("attn_tree", scratch, _tree_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), ctx.status)
-    call("mynah_attn_tree", q.data_ptr(), out.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, _row_stride(q), _row_stride(out),
-         k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(),
-         pages.base.data_ptr(), pages.n_pages, masks.data_ptr(), masks.shape[1], float(scale), scratch.data_ptr(), scratch.numel(),
-         ctx.status.data_ptr(), stream_on(q.device.index))
+    call("mynah_attn_tree", _TREE_CALL.pack(
+        q.data_ptr(), out.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, ldq, ldo, k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(),
+        ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, masks.data_ptr(), masks.shape[1],
+        scale, scratch.data_ptr(), scratch.numel(), ctx.status.data_ptr(), stream_on(index)))
 
 
-def check_layers(who: str, k_caches: torch.Tensor, v_caches: torch.Tensor, pages: PageTableView) -> None:
-    ks, vs = k_caches.shape, v_caches.shape
-    if not k_caches.is_cuda or k_caches.device.index != torch.cuda.current_device():
+def check_layers(who: str, k_caches: torch.Tensor, v_caches: torch.Tensor, pages: PageTableView) -> int:
+    """What the operators over all layers' rows ask of a storage group. Returns its device."""
+    ks, vs, index = k_caches.shape, v_caches.shape, k_caches.get_device()
+    if index < 0 or index != torch.cuda.current_device():
         raise KernelError(f"{who}: the cache is not on the current CUDA device")
-    if len(ks) != 5 or len(vs) != 5 or ks[1] != pages.n_pages or ks[3] != PAGE_TOKENS or ks[:4] != vs[:4] or k_caches.dtype != v_caches.dtype \
-            or k_caches.device != v_caches.device or not k_caches.is_contiguous() or not v_caches.is_contiguous():
+    if len(ks) != 5 or len(vs) != 5 or ks[1] != pages.n_pages or ks[3] != PAGE_TOKENS or ks[:4] != vs[:4] or k_caches.dtype is not v_caches.dtype \
+            or v_caches.get_device() != index or not k_caches.is_contiguous() or not v_caches.is_contiguous():
         raise KernelError(f"{who}: the cache must be contiguous [layers, {pages.n_pages}, kv heads, {PAGE_TOKENS}, head], got K {tuple(ks)} "
                           f"{k_caches.dtype}, V {tuple(vs)} {v_caches.dtype}")
+    return index
 
 
 def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tensor, ctx, k_caches: torch.Tensor, v_caches: torch.Tensor,
@@ -154,20 +164,19 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
     kv_len - n_q. Returns int32 (path [T]: the path's rows from every sequence's first place on, -1 behind them; count [B]; next
     [B]: what was chosen behind the path's last row). A sequence without rows has count 0 and next -1. Trees of up to 4,096 rows;
     ctx.max_q_len is the longest one's (a longer one is refused through the status word, with count 0)."""
-    check_layers("tree_commit", k_caches, v_caches, pages)
-    dev = k_caches.device
+    index = check_layers("tree_commit", k_caches, v_caches, pages)
     T = tokens.numel()
     for t in (tokens, parents, chosen):
-        if t.dtype != _I32 or t.device != dev or t.dim() != 1 or t.numel() < T or not t.is_contiguous():
-            raise KernelError(f"tree_commit: tokens, parents and chosen tokens must be {T} contiguous int32 on {dev}")
+        if t.dtype is not _I32 or t.get_device() != index or t.dim() != 1 or t.numel() < T or not t.is_contiguous():
+            raise KernelError(f"tree_commit: tokens, parents and chosen tokens must be {T} contiguous int32 on cuda:{index}")
     if not 0 <= ctx.max_q_len <= 4096:
         raise KernelError(f"tree_commit: trees of {ctx.max_q_len} rows, 4096 are the most")
-    check_lists("tree_commit", dev, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
+    check_lists("tree_commit", index, ctx.B, ctx.cu_q, ctx.kv_len, pages, ctx.status)
     path, count, after = tokens.new_empty(T), tokens.new_empty(ctx.B), tokens.new_empty(ctx.B)       # (torch.empty takes a us more)
     E, _, KV, _, HD = k_caches.shape
     es = k_caches.element_size()
-    call("mynah_tree_commit", tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), T, ctx.B, ctx.max_q_len, ctx.cu_q.data_ptr(),
-         ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, k_caches.data_ptr(),
-         v_caches.data_ptr(), E, KV, HD * es, v_caches.shape[4] * es, path.data_ptr(), count.data_ptr(), after.data_ptr(),
-         ctx.status.data_ptr(), stream_on(dev.index))
+    call("mynah_tree_commit", _COMMIT_CALL.pack(
+        tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), T, ctx.B, ctx.max_q_len, ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(),
+        pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, k_caches.data_ptr(), v_caches.data_ptr(), E, KV, HD * es,
+        v_caches.shape[4] * es, path.data_ptr(), count.data_ptr(), after.data_ptr(), ctx.status.data_ptr(), stream_on(index)))
     return path, count, after
