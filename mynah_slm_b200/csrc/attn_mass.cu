@@ -17,7 +17,7 @@
 
 int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs a, int max_q_len, const void* k_cache, const void* v_cache,
                   const int* cu_q, const int* kv_len, PageTable pt, const long long* masks, float* scratch, long long scratch_floats,
-                  float* lse, float* scores, int score_rows, int n_ids, int* status, cudaStream_t stream);
+                  float* lse, float* scores, int score_rows, int n_ids, float* mass, int* status, cudaStream_t stream);
 
 namespace {
 
@@ -26,6 +26,12 @@ __device__ __forceinline__ float4 four_of(const bf16* p) {
     const uint2 w = *reinterpret_cast<const uint2*>(p);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
+// The same where rows are not aligned (volatile: or the compiler may make one 16-byte access of this and the above).
+__device__ __forceinline__ float4 four_apart(const float* p) {
+    const volatile float* w = p;
+    return make_float4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float4 four_apart(const bf16* p) { return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3])); }
 
 constexpr int GK = 64, GR = 32;      // keys (a page) and packed rows a tile of the general kernel
 
@@ -69,7 +75,7 @@ attn_mass_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const f
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
             if (pr < n_rows) {
                 const T* at = q + (size_t)(u.s.q_begin + tok) * a.r.ldq + (size_t)(g * G + pr - tok * G) * HD + d;
-                x = a.r.q_aligned ? four_of(at) : make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
+                x = a.r.q_aligned ? four_of(at) : four_apart(at);
             }
             *reinterpret_cast<float4*>(q_s + r * p + d) = x;
         }
@@ -159,30 +165,6 @@ int launch_mass_generic(const void* q, const void* k, const float* lse, float* m
     return mynah_check_launch("attn_mass");
 }
 
-// Sums from the scores that the attention has kept (steps of few rows a sequence, on the tensor cores): a thread a key, pages of
-// a sequence in turn. Bound by the scores' and the sums' bytes: a thirtieth of the keys' and values' for two rows a kv head.
-constexpr int SC_THREADS = 256, SC_PAGES = SC_THREADS / PAGE_TOKENS;
-__global__ void __launch_bounds__(SC_THREADS)
-attn_mass_scores_kernel(const float* __restrict__ scores, int score_rows, const float* __restrict__ lse, float* __restrict__ mass,
-                        const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, int entries, int* __restrict__ status) {
-    griddep_wait();
-    const int b = blockIdx.y;
-    const SeqShape s = seq_shape(cu_q, kv_len, pt, b, a, status);
-    const int rows = min(s.n_q * a.G, score_rows), units = s.pages * a.KV, past = s.kvl - s.n_q, e = threadIdx.x % PAGE_TOKENS;
-    for (int u = blockIdx.x * SC_PAGES + threadIdx.x / PAGE_TOKENS; u < units; u += gridDim.x * SC_PAGES) {
-        const int lp = a.by_KV.div(u), g = u - lp * a.KV, key = lp * PAGE_TOKENS + e;
-        const int page = page_at(pt, s, lp);
-        if (page < 0 || key >= s.kvl || s.list0 + lp - s.first >= entries) continue;       // (the attention has reported a missing page)
-        const float* z = scores + (((size_t)(s.list0 + lp - s.first) * a.KV + g) * score_rows) * PAGE_TOKENS + e;
-        const float* l = lse + ((size_t)g * a.T + s.q_begin) * a.G;
-        float* m = mass + ((size_t)page * a.KV + g) * PAGE_TOKENS + e;
-        float sum = key < past ? *m : 0.f;
-#pragma unroll 4
-        for (int r = 0; r < rows; r++) sum += l[r] == -INFINITY ? 0.f : ex2_f(z[(size_t)r * PAGE_TOKENS] - l[r]);
-        *m = sum;
-    }
-}
-
 // Rows of a kv head up to which the attention keeps its scores for the sums rather than having the keys looked at again: they are
 // 256 bytes a row and page written and read, the keys of 128 columns 16 KB.
 constexpr int SCORE_ROWS = 8;
@@ -255,11 +237,11 @@ MYNAH_API int mynah_attn_mass(const AttnMassCall* call) {
     r.T = T, r.B = B, r.H = H, r.KV = KV, r.HD = HD, r.G = H / KV, r.ldq = ldq, r.ldo = ldo, r.causal = 1;
     r.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     const int es = dtype == MYNAH_F32 ? 4 : 2;
-    const bool aligned = ((uintptr_t)q & 15) == 0 && (long long)ldq * es % 16 == 0;
+    // (as the attention has it: which kernel takes that decides whether there are scores to keep)
+    const bool aligned = ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0 && (long long)ldq * es % 16 == 0 && (long long)ldo * es % 16 == 0;
     MassArgs a{};
     a.r = r;
     const bool tc = mass_plan(a, dtype, aligned, max_q_len);
-    MYNAH_REQUIRE(a.score_rows == 0 || B <= 65535, "attn_mass: %d sequences are too many", B);
     const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids);
     MYNAH_REQUIRE(scratch_floats >= need, "attn_mass: scratch holds %lld floats, %lld are needed", scratch_floats, need);
     const long long attn = attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1);
@@ -267,17 +249,9 @@ MYNAH_API int mynah_attn_mass(const AttnMassCall* call) {
     float* part = lse + (((long long)T * H + 3) & ~3ll);
     const PageTable pt{page_indptr, page_ids, page_base, n_pages};
     const int rc = attn_rows_run("attn_mass", q, out, dtype, r, max_q_len, k_cache, v_cache, cu_q, kv_len, pt, nullptr, scratch, attn, lse,
-                                 a.score_rows > 0 ? part : nullptr, a.score_rows, n_ids, status, stream);
+                                 a.score_rows > 0 ? part : nullptr, a.score_rows, n_ids, mass, status, stream);
     if (rc != 0) return rc;
-    if (a.score_rows > 0) {
-        // about two units (four keys' threads each) a thread block and SM eight times over
-        const long long blocks = ceil_div_ll((long long)n_ids * KV, SC_PAGES), each = ceil_div_ll(blocks, B), most = ceil_div_ll(16ll * mynah_sm_count(), B);
-        const dim3 grid((unsigned)(each < 1 ? 1 : each < most ? each : most), B);
-        const cudaError_t e = launch_behind(attn_mass_scores_kernel, grid, dim3(SC_THREADS), 0, stream, (const float*)part, a.score_rows,
-                                            (const float*)lse, mass, cu_q, kv_len, pt, a.r, n_ids, status);
-        if (e != cudaSuccess) return mynah_fail("attn_mass: %s", cudaGetErrorString(e));
-        return mynah_check_launch("attn_mass");
-    }
+    if (a.score_rows > 0) return 0;                                // the joining launch has added them up
     const long long units = mass_units_max(a, n_ids);
     MYNAH_REQUIRE(units * KV < (1ll << 31) && KV <= 65535, "attn_mass: launch too large");
     const dim3 grid((unsigned)units, KV);

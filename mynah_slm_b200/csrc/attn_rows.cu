@@ -31,6 +31,12 @@ __device__ __forceinline__ float4 four_of(const bf16* p) {
     const uint2 w = *reinterpret_cast<const uint2*>(p);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
+// The same where rows are not aligned (volatile: or the compiler may make one 16-byte access of this and the above).
+__device__ __forceinline__ float4 four_apart(const float* p) {
+    const volatile float* w = p;
+    return make_float4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float4 four_apart(const bf16* p) { return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3])); }
 __device__ __forceinline__ void copy16_async(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
@@ -84,7 +90,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < n_rows) {
             const T* at = q + (size_t)(u.s.q_begin + tok) * a.ldq + (size_t)(g * a.G + pr - tok * a.G) * HD + d;
-            x = a.q_aligned ? four_of(at) : make_float4(to_f32(at[0]), to_f32(at[1]), to_f32(at[2]), to_f32(at[3]));
+            x = a.q_aligned ? four_of(at) : four_apart(at);
         }
         *reinterpret_cast<float4*>(q_s + r * qp + d) = x;
     }
@@ -267,12 +273,14 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     griddep_launch_late();
 }
 
-// Four values of a row; rows may begin anywhere.
+// Four values of a row; rows may begin anywhere. (volatile: of the two branches written plainly for fp32 the compiler makes one
+// 16-byte store, which faults where a row is not aligned.)
 __device__ __forceinline__ void store4(float* o, float a, float b, float c, float d) {
     if (((uintptr_t)o & 15) == 0) {
         *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
     } else {
-        o[0] = a, o[1] = b, o[2] = c, o[3] = d;
+        volatile float* w = o;
+        w[0] = a, w[1] = b, w[2] = c, w[3] = d;
     }
 }
 __device__ __forceinline__ void store4(bf16* o, float a, float b, float c, float d) {
@@ -290,11 +298,82 @@ __device__ __forceinline__ void store4(bf16* o, float a, float b, float c, float
 // sequence's numbers, then the segments' maxima and rows together, from L2).
 constexpr int JOIN_WARPS = 8, JOIN_HELPERS = 16;                   // warps of a CTA; CTAs that share an item's rows at most
 constexpr int JOIN_AHEAD = 4;                                      // segments asked for at once
+
+// Sums of the weights from the scores that the attention has kept (steps of up to 8 rows a kv head, so one tile and one item a
+// sequence and kv head): CTA number `cta` of those that add, for one sequence and kv head a run of its pages, a thread a key. The
+// rows' log-sums come from the segments' maxima and sums, as the joining CTAs have them, so neither waits for the other and no
+// launch is needed for it (one of its own behind the join: one token of 16 heads behind 1,535 rows 18.5 us, so 16.4; 64 tokens
+// behind up to 4,000 rows 172 both). Bound by the scores' and the sums' bytes.
+constexpr int SUM_PAGES = JOIN_WARPS * 32 / PAGE_TOKENS;           // at once
+__device__ __forceinline__ void sum_scores(int cta, const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt, const RowsArgs& a,
+                                           const RowsScratch& sc, int* status) {
+    __shared__ RowStart cut_s;                                     // b: the CTA that begins inside the item first, or -1
+    __shared__ float lse_s[JOIN_WARPS];
+    const int chunk = cta % sc.sum_chunks, bg = cta / sc.sum_chunks, g = a.by_KV.mod(bg), b = a.by_KV.div(bg);
+    if (threadIdx.x == 0) cut_s.b = -1;
+    const SeqShape s = seq_shape(cu_q, kv_len, pt, b, a, status);
+    __syncthreads();
+    if (s.n_q == 0) return;
+    if (!a.whole_items) {
+        for (int c = threadIdx.x; c < a.ctas; c += JOIN_WARPS * 32) {
+            const RowStart at = sc.starts[c];
+            if (at.b == b && at.g == g && at.from > 0 && at.from <= at.each) {
+                cut_s.from = at.from;
+                cut_s.each = at.each;
+                cut_s.b = c;
+            }
+        }
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = min(s.n_q * a.G, sc.score_rows), past = s.kvl - s.n_q;
+    if (row < rows) {
+        float lse;
+        if (cut_s.b < 0 || s.pages <= cut_s.from) {                // one CTA had it whole
+            lse = sc.lse[((size_t)g * a.T + s.q_begin) * a.G + row];
+        } else {
+            const int n = 2 + quotient(s.pages - cut_s.from - 1, cut_s.each);
+            float m = -INFINITY, l = 0.f;
+            for (int c = lane; c < n; c += 32) {
+                const float2 ml = sc.ml[((long long)(cut_s.b - 1 + c) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + row];
+                const float m_new = max_or_nan(m, ml.x), m_use = m_new == -INFINITY ? 0.f : m_new;
+                l = fmaf(l, ex2_f(m - m_use), ml.y * ex2_f(ml.x - m_use));
+                m = m_new;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+                const float m_new = max_or_nan(m, m2), m_use = m_new == -INFINITY ? 0.f : m_new;
+                l = fmaf(l, ex2_f(m - m_use), l2 * ex2_f(m2 - m_use));
+                m = m_new;
+            }
+            lse = l == 0.f ? -INFINITY : m + log2f(l);
+        }
+        if (lane == 0) lse_s[row] = lse;
+    }
+    __syncthreads();
+    const int e = threadIdx.x % PAGE_TOKENS;
+    for (int lp = chunk * SUM_PAGES + threadIdx.x / PAGE_TOKENS; lp < s.pages; lp += sc.sum_chunks * SUM_PAGES) {
+        const int key = lp * PAGE_TOKENS + e, page = page_at(pt, s, lp), entry = s.list0 + lp - s.first;
+        if (page < 0 || key >= s.kvl || entry >= sc.entries) continue;         // (the attention has reported a missing page)
+        const float* z = sc.scores + ((size_t)entry * a.KV + g) * sc.score_rows * PAGE_TOKENS + e;
+        float* m = sc.mass + ((size_t)page * a.KV + g) * PAGE_TOKENS + e;
+        float sum = key < past ? *m : 0.f;
+#pragma unroll 4
+        for (int r = 0; r < rows; r++) sum += lse_s[r] == -INFINITY ? 0.f : ex2_f(z[r * PAGE_TOKENS] - lse_s[r]);
+        *m = sum;
+    }
+}
+
+// CTAs from `joining` on: sums of kept scores.
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, RowsScratch sc,
-                      int* __restrict__ status) {
+                      int joining, int* __restrict__ status) {
     griddep_wait();
+    if ((int)blockIdx.x >= joining) {
+        sum_scores(blockIdx.x - joining, cu_q, kv_len, pt, a, sc, status);
+        return;
+    }
     const int cta = a.by_group.div(blockIdx.x) + 1, sub = a.by_group.mod(blockIdx.x);       // (CTA 0 begins inside of nothing)
     const RowStart at = sc.starts[cta];
     if (at.b < 0 || at.from == 0 || at.from > at.each) return;
@@ -387,8 +466,8 @@ RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
     s.starts = reinterpret_cast<RowStart*>(scratch + rows * (a.HD + 2));
     s.lse = lse;
-    s.scores = nullptr;
-    s.score_rows = 0;
+    s.scores = s.mass = nullptr;
+    s.score_rows = s.sum_chunks = 0;
     return s;
 }
 
@@ -438,11 +517,21 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
 
 int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int* status,
                      cudaStream_t stream) {
-    if (a.ctas <= 1 || a.whole_items) return 0;                    // nothing is cut
-    const dim3 grid((a.ctas - 1) * a.group, min(ceil_div(a.most_rows, JOIN_WARPS), JOIN_HELPERS)), block(JOIN_WARPS * 32);
+    const int joining = a.whole_items ? 0 : (a.ctas - 1) * a.group;            // (whole items: nothing is cut)
+    long long ctas = joining;
+    if (s.scores != nullptr) {
+        // a run of at least four pages a CTA, about eight CTAs an SM: with few rows each waits for two reads more than it adds
+        const long long bg = (long long)a.B * a.KV, pages = ceil_div_ll(s.entries, a.B), most = ceil_div_ll(8ll * mynah_sm_count(), bg);
+        const long long chunks = ceil_div_ll(pages, SUM_PAGES) < most ? ceil_div_ll(pages, SUM_PAGES) : most;
+        s.sum_chunks = (int)(chunks < 1 ? 1 : chunks);
+        ctas += bg * s.sum_chunks;
+        MYNAH_REQUIRE(ctas < (1ll << 31), "attn_rows_join: launch too large");
+    }
+    if (ctas == 0) return 0;
+    const dim3 grid((unsigned)ctas, min(ceil_div(a.most_rows, JOIN_WARPS), JOIN_HELPERS)), block(JOIN_WARPS * 32);
     const cudaError_t e = dtype == MYNAH_F32
-        ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, pt, a, s, status)
-        : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, pt, a, s, status);
+        ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, pt, a, s, joining, status)
+        : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, pt, a, s, joining, status);
     if (e != cudaSuccess) return mynah_fail("attn_rows_join: %s", cudaGetErrorString(e));
     return mynah_check_launch("attn_rows_join");
 }
@@ -467,7 +556,7 @@ MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, 
 // What mynah_attn_tree and mynah_attn_mass check and launch alike.
 int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs a, int max_q_len, const void* k_cache, const void* v_cache,
                   const int* cu_q, const int* kv_len, PageTable pt, const long long* masks, float* scratch, long long scratch_floats,
-                  float* lse, float* scores, int score_rows, int n_ids, int* status, cudaStream_t stream) {
+                  float* lse, float* scores, int score_rows, int n_ids, float* mass, int* status, cudaStream_t stream) {
     MYNAH_REQUIRE(dtype == MYNAH_F32 || dtype == MYNAH_BF16, "%s: dtype %d is neither float32 nor bfloat16", who, dtype);
     MYNAH_REQUIRE(a.KV > 0 && a.H > 0 && a.H % a.KV == 0 && a.KV <= 65535, "%s: %d heads over %d kv heads", who, a.H, a.KV);
     MYNAH_REQUIRE(a.HD > 0 && a.HD % 8 == 0 && a.HD <= MAX_HEAD, "%s: head_dim %d is no multiple of 8 up to %d", who, a.HD, MAX_HEAD);
@@ -484,6 +573,7 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
     s.scores = scores;
     s.score_rows = score_rows;
     s.entries = n_ids;
+    s.mass = mass;
     const int rc = tc ? launch_rows_tcgen05(q, out, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream)
                       : launch_rows_generic(q, out, dtype, a, k_cache, v_cache, cu_q, kv_len, pt, masks, s, status, stream);
     if (rc != 0) return rc;
@@ -520,5 +610,5 @@ MYNAH_API int mynah_attn_tree(const AttnTreeCall* call) {
     a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = KV > 0 ? H / KV : 0, a.ldq = ldq, a.ldo = ldo, a.words = words;
     a.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     return attn_rows_run("attn_tree", q, out, dtype, a, max_q_len, k_cache, v_cache, cu_q, kv_len,
-                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, nullptr, 0, 0, status, stream);
+                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, nullptr, 0, 0, nullptr, status, stream);
 }

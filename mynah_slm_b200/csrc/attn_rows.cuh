@@ -12,6 +12,8 @@ struct RowsScratch {
     float* o;                         // [CTAs][2][tile_rows][HD], not normalised
     float* scores;                    // [entries of the page lists][KV][score_rows][64]: scores * scale_log2, -inf for unseen keys; null: not wanted
     int score_rows, entries;          // (entries: of the page lists)
+    float* mass;                      // [n_pages][KV][64]: the sums that the kept scores are added to
+    int sum_chunks;                   // CTAs that add for one sequence and kv head
     float* lse;                       // [KV][T][G]: log2 of the sum of 2^score, -inf for a row that sees nothing; null: not wanted
 };
 

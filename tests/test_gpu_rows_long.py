@@ -140,6 +140,25 @@ def test_sums_however_they_are_cut(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,past", [([1, 1, 1], [300, 64, 5]), ([40, 7], [30, 200])])
+def test_outputs_that_are_not_aligned(rows, past, dtype):
+    """Columns of a wider buffer that begin at an odd one, rows of an odd pitch; q is aligned."""
+    from mynah_slm_b200.ops import evict, tree
+    H, KV, HD = 4, 2, 64
+    step, q, k, v = _case(6, rows, past, H, KV, HD, dtype)
+    mass = torch.rand((step.pages.n_pages, KV, 64), device=DEV) * 3
+    wide = torch.full((sum(rows), H * HD + 3), 7.0, dtype=dtype, device=DEV)
+    out, got = wide[:, 1:1 + H * HD], mass.clone()
+    evict.attn_mass(q, out, got, step, H, KV, HD, k, v, step.pages)
+    assert step.status.item() == 0 and (wide[:, 0] == 7.0).all() and (wide[:, 1 + H * HD:] == 7.0).all()
+    tight = out.contiguous()
+    _agrees(step, q, k, v, H, KV, HD, dtype, tight, plain.causal(step), mass, got)
+    chain = [[-1] + list(range(n - 1)) for n in rows]
+    tree.attn_tree(q, out, step, H, KV, HD, k, v, step.pages, _masks(chain).to(DEV))
+    _agrees(step, q, k, v, H, KV, HD, dtype, out.contiguous(), plain.causal(step))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 def test_a_step_of_nothing_but_padding(dtype):
     """Sequences without rows in the step, and rows of q behind the last one: nothing is written."""
     from mynah_slm_b200.ops import evict, tree
