@@ -172,7 +172,7 @@ struct MoveArgs {
 // next step's already asked for, when the barrier lets the step's writes go; and a row that is written in a step is a source of
 // that step or of an earlier one. Places are worked out 512 rows ahead, so that the copies wait for one read, not for the
 // choice, the page list and the row one behind the other. LANES: 16 (whole rows of 256 bytes: 28 layers of 2 sequences, 2,048 rows
-// of 8 heads of 128, 160 us of both launches' 194, against 329 with 4), or 4 where that would leave too few CTAs (one layer of one
+// of 8 heads of 128, 160 us of both launches' 191, against 329 with 4), or 4 where that would leave too few CTAs (one layer of one
 // sequence, 512 rows of 700: both launches 12.3 against 14.4 us).
 template <int LANES>
 __global__ void __launch_bounds__(MV_THREADS)
