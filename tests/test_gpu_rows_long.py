@@ -260,3 +260,46 @@ def test_calls_at_once_on_two_streams_and_two_graphs():
         torch.cuda.synchronize()
         for (_, outs), (_, want, step) in zip(graphs, jobs):
             assert step.status.item() == 0 and all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+def test_a_captured_eviction_and_acceptance_serve_other_lengths():
+    """One graph of an acceptance and an eviction; its replays go by the lengths, trees and choices of the moment."""
+    from mynah_slm_b200.ops import evict, tree
+    E, KV, HD, rows = 3, 2, 64, [6, 4]
+    g = torch.Generator().manual_seed(3)
+    step = plain.make_step(rows, [700, 400], DEV, g)
+    d = torch.Generator(device=DEV).manual_seed(3)
+    shape = (E, step.pages.n_pages, KV, 64)
+    k, v = (torch.randn((*shape, HD), generator=d, device=DEV).to(BF16) for _ in range(2))
+    mass = torch.rand(shape, generator=d, device=DEV)
+    tokens, parents, chosen = (torch.zeros(10, dtype=torch.int32, device=DEV) for _ in range(3))
+
+    def run(k, v, mass):
+        moved = tree.tree_commit(tokens, parents, chosen, step, k, v, step.pages)
+        return [*moved, *evict.cache_evict(k, v, mass, step, step.pages, 200, 50, 4)]
+    side = torch.cuda.Stream()
+    kg, vg, mg = k.clone(), v.clone(), mass.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = run(kg, vg, mg)
+    rng = random.Random(8)
+    for held in ([706, 404], [650, 150], [200, 201], [6, 4]):
+        step.kv_len.copy_(torch.tensor(held, dtype=torch.int32))
+        trees = [_tree(n, rng) for n in rows]
+        parents.copy_(torch.tensor(trees[0] + trees[1], dtype=torch.int32))
+        tokens.copy_(torch.tensor([rng.randrange(3) for _ in range(10)], dtype=torch.int32))
+        chosen.copy_(torch.tensor([rng.randrange(3) for _ in range(10)], dtype=torch.int32))
+        for a, b in ((kg, k), (vg, v), (mg, mass)):
+            a.copy_(b)
+        ke, ve, me = k.clone(), v.clone(), mass.clone()
+        want = run(ke, ve, me)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert step.status.item() == 0
+        assert all(torch.equal(a, b) for a, b in zip([*outs, kg, vg, mg], [*want, ke, ve, me]))
+        assert outs[4].tolist() == [min(h, 200) for h in held]
+        for b, n in enumerate(rows):
+            at = sum(rows[:b])
+            path, nxt = plain.accepted(tokens[at:at + n].tolist(), trees[b], chosen[at:at + n].tolist())
+            assert outs[1].tolist()[b] == len(path) and outs[2].tolist()[b] == nxt and outs[0].tolist()[at:at + len(path)] == path
