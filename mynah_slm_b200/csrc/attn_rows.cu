@@ -74,6 +74,9 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     RowWalk u = walk_s;
     if (u.b < 0) return;
     const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
+    // the 16-byte pieces of a K or V tile that this thread copies: the first one, and how far on the next is
+    const int per_row = HD * (int)sizeof(T) / 16, copy_r = threadIdx.x / per_row, copy_c = threadIdx.x % per_row;
+    const int rows_on = THREADS / per_row, pieces_on = THREADS % per_row;
     do {
     const int g = u.g, n_rows = u.rows(a), past = u.past(), row0 = u.tile * a.tile_rows;
     const int pg0 = u.pg0, pg1 = u.pg1;
@@ -103,11 +106,12 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     auto bring = [&](int t, int st) {
         const int page = page_at(pt, u.s, t / (PAGE_TOKENS / KT));
         const size_t base = (((size_t)page * a.KV + g) * PAGE_TOKENS + (t * KT) % PAGE_TOKENS) * HD;
-        const int per_row = HD * (int)sizeof(T) / 16;
-        for (int i = threadIdx.x; i < KT * per_row; i += THREADS) {
-            const int r = i / per_row, c = i % per_row;
+#pragma unroll 2
+        for (int r = copy_r, c = copy_c; r < KT;) {
             copy16_async(reinterpret_cast<unsigned char*>(k_s + (st * KT + r) * kp) + c * 16, reinterpret_cast<const unsigned char*>(k_cache + base + (size_t)r * HD) + c * 16);
             copy16_async(reinterpret_cast<unsigned char*>(v_s + (st * KT + r) * kp) + c * 16, reinterpret_cast<const unsigned char*>(v_cache + base + (size_t)r * HD) + c * 16);
+            r += rows_on;
+            if ((c += pieces_on) >= per_row) c -= per_row, r++;
         }
         copies_commit();
     };
