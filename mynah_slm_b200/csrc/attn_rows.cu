@@ -66,7 +66,6 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     float* p_s = q_s + R * qp;                                     // [R][KT + 4]
     T* k_s = reinterpret_cast<T*>(p_s + R * (KT + 4));             // [2][KT][kp]
     T* v_s = k_s + 2 * KT * kp;                                    // [2][KT][kp]
-    __shared__ int bad_s;
     __shared__ RowWalk walk_s;
 
     if (threadIdx.x < 32) find_start(cu_q, kv_len, pt, a, &walk_s, sc.starts, status);
@@ -80,11 +79,10 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     do {
     const int g = u.g, n_rows = u.rows(a), past = u.past(), row0 = u.tile * a.tile_rows;
     const int pg0 = u.pg0, pg1 = u.pg1;
-    if (threadIdx.x == 0) bad_s = 0;
     __syncthreads();                                               // (the segment before is done with shared memory)
     // every page of the segment must be there: one that lacks a page counts as keys that nobody sees
-    for (int p = pg0 + (int)threadIdx.x; p < pg1; p += THREADS)
-        if (page_at(pt, u.s, p) < 0) bad_s = 1;
+    bool lacks = false;
+    for (int p = pg0 + (int)threadIdx.x; p < pg1; p += THREADS) lacks |= page_at(pt, u.s, p) < 0;
     // the tile's queries, four values a thread (one by one where rows are not aligned); rows that are not there are zero
     const int quads = HD >> 2;
 #pragma unroll 4
@@ -97,8 +95,9 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         }
         *reinterpret_cast<float4*>(q_s + r * qp + d) = x;
     }
-    __syncthreads();
-    const bool bad = bad_s != 0;
+    // The answer comes out of the barrier, the same for every thread: a flag in shared memory that the next segment clears could be
+    // read behind that by a late warp, which would go on into the pages alone.
+    const bool bad = __syncthreads_or(lacks);
     if (bad && threadIdx.x == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
 
     const int first_tok = a.by_G.div(row0);

@@ -116,6 +116,37 @@ def test_tree_attention_however_it_is_cut(case, dtype):
     _agrees(step, q, k, v, H, KV, HD, dtype, out, sees)
 
 
+@pytest.mark.parametrize("dtype,HD", [(BF16, 64), (BF16, 128), (BF16, 48), (F32, 64)], ids=["tc64", "tc128", "bf16-48", "f32"])
+def test_missing_pages_where_a_cta_has_several_segments(dtype, HD):
+    """Pages that are not there, in sequences of a long ragged batch (a CTA's share of it reaches over several of them): reported, read by
+    nobody, and every other sequence has the bits that it has without them."""
+    from mynah_slm_b200.ops import tree
+    from mynah_slm_b200.ops.kernels import PageTableView
+    rows, past, H, KV = [1 + b % 9 for b in range(45)], [(b * 397) % 2100 for b in range(45)], 8, 2
+    rng = random.Random(45)
+    step, q, k, v = _case(12, rows, past, H, KV, HD, dtype)
+    masks = _masks([_tree(n, rng) for n in rows]).to(DEV)
+    want = torch.zeros_like(q)
+    tree.attn_tree(q, want, step, H, KV, HD, k, v, step.pages, masks)
+    assert step.status.item() == 0
+    indptr = step.pages.indptr.tolist()
+    lacking = [b for b in range(45) if b % 4 == 1]
+    ids = step.pages.ids.clone()
+    for b in lacking:
+        ids[indptr[b] + rng.randrange(indptr[b + 1] - indptr[b])] = rng.choice([-1, -3, step.pages.n_pages, 1 << 20])
+    bad = PageTableView(step.pages.indptr, ids, step.pages.base, step.pages.n_pages)
+    for _ in range(5):
+        out = torch.full_like(q, 7.0)
+        tree.attn_tree(q, out, step, H, KV, HD, k, v, bad, masks)
+        assert step.status.item() & 1 and step.status.item() & 16 == 0
+        step.status.zero_()
+        at = 0
+        for b, n in enumerate(rows):
+            if b not in lacking:
+                assert torch.equal(out[at:at + n], want[at:at + n]), b
+            at += n
+
+
 STEPS = [
     ([700, 1500, 40], [0, 100, 900], 16, 8, 128),                           # whole items
     ([300, 5, 1], [4000, 50, 9], 4, 2, 128),                                # several tiles of different lengths on a line
