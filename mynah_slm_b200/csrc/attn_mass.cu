@@ -211,7 +211,7 @@ MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, 
 }
 
 // As mynah_attn_tree with causal rows, and mass [n_pages, KV, 64] fp32. n_ids: entries of page_ids (no fewer than the
-// sequences' pages together).
+// sequences' pages together). A sequence of more than max_q_len rows is refused through the status word.
 struct AttnMassCall {
     const void* q;
     void* out;
@@ -237,6 +237,7 @@ MYNAH_API int mynah_attn_mass(const AttnMassCall* call) {
     MYNAH_REQUIRE(scratch != nullptr && ((uintptr_t)scratch & 15) == 0, "attn_mass: 16-byte aligned scratch is required");
     RowsArgs r{};
     r.T = T, r.B = B, r.H = H, r.KV = KV, r.HD = HD, r.G = H / KV, r.ldq = ldq, r.ldo = ldo, r.causal = 1;
+    r.most_q = max_q_len;                                          // (how the sums are cut, and the scores that are kept, go by it)
     r.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     const int es = dtype == MYNAH_F32 ? 4 : 2;
     // (as the attention has it: which kernel takes that decides whether there are scores to keep)

@@ -12,6 +12,7 @@
 // the entry points.
 #include "attn_rows.cuh"
 
+#include <limits.h>
 #include <math.h>
 
 namespace {
@@ -611,6 +612,7 @@ MYNAH_API int mynah_attn_tree(const AttnTreeCall* call) {
     MYNAH_REQUIRE(scale >= 0.f, "attn_tree: the score scale %g is negative", scale);
     RowsArgs a{};
     a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = KV > 0 ? H / KV : 0, a.ldq = ldq, a.ldo = ldo, a.words = words;
+    a.most_q = INT_MAX;                                            // (max_q_len gives the tiles their size, and rows beyond it are more tiles)
     a.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     return attn_rows_run("attn_tree", q, out, dtype, a, max_q_len, k_cache, v_cache, cu_q, kv_len,
                          PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, nullptr, 0, 0, nullptr, status, stream);

@@ -48,6 +48,7 @@ struct FastDiv {
 
 struct RowsArgs {
     int T, B, H, KV, HD, G;
+    int most_q;                       // rows of a sequence at most: a longer one is refused
     int ldq, ldo;
     int tile_rows;                    // packed rows a tile
     int most_rows;                    // of one tile that the step's longest sequence fills
@@ -84,8 +85,8 @@ struct SeqShape {
     int first;
 };
 
-// A sequence's numbers. Bounds that cannot be (rows outside the step, fewer keys than rows) count as a sequence without rows
-// and are reported.
+// A sequence's numbers. Bounds that cannot be (rows outside the step, fewer keys than rows, more rows than the call was made for)
+// count as a sequence without rows and are reported.
 __device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt, int b,
                                               const RowsArgs& a, int* status) {
     SeqShape s;
@@ -96,7 +97,7 @@ __device__ __forceinline__ SeqShape seq_shape(const int* __restrict__ cu_q, cons
     s.first = pt.base[b];
     s.n_q = end - s.q_begin;
     s.kvl = kv_len[b];
-    if (s.n_q <= 0 || s.q_begin < 0 || end > a.T || s.kvl < s.n_q) {
+    if (s.n_q <= 0 || s.q_begin < 0 || end > a.T || s.kvl < s.n_q || s.n_q > a.most_q) {
         if (s.n_q != 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
         s.n_q = 0;
     }

@@ -40,7 +40,9 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
     the rows' own keys and values already, as `attn_tree` with every row seeing the rows up to itself; and the sums of the weights:
     mass [n_pages, KV, 64] fp32 gets, at every cached row of the step's sequences, the weight that the step's rows and the kv
     head's query heads give it, added to what it holds for rows that were there before the step, in place of it for the step's own
-    (so nothing has to be cleared when a page is taken). Other rows' sums are left as they are. The order of the sums does not
+    (so nothing has to be cleared when a page is taken). Other rows' sums are left as they are. No sequence may have more than
+    ctx.max_q_len rows in the step: one that has (a replay with other lengths) is refused through the status word, its outputs and
+    sums left alone. The order of the sums does not
     depend on timing, provided that no page is in two sequences' lists (a shared page's sums would be written by both)."""
     dt, index, T, ldq, ldo = check_rows("attn_mass", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)
     if mass.dtype is not torch.float32 or mass.get_device() != index or not mass.is_contiguous() or mass.dim() != 3 \

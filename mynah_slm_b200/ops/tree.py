@@ -125,7 +125,8 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
     makes the words of a tree; any other mask will do, a row that sees nothing gives zeros). Query head h reads kv head
     h // (H / KV). `q` and `out` are rows with head h in columns [h HD, (h + 1) HD), and may be wider; rows of `out` behind the
     last sequence are left as they are. masks: int64 [T, words]; rows of a tree beyond 64 * words are seen by nobody. scale 0:
-    1 / sqrt(HD). ctx: the step's description (B, max_q_len, cu_q, kv_len, status). Rows of the cache that a row does not see
+    1 / sqrt(HD). ctx: the step's description (B, max_q_len, cu_q, kv_len, status; max_q_len only
+    sizes the tiles, a longer sequence is served too). Rows of the cache that a row does not see
     have no influence on it, whatever they hold. float32 and bfloat16, heads of any multiple of 8 up to 256; bfloat16 heads of 64
     and 128 run on the tensor cores. `scratch`: attn_tree_scratch_floats fp32 words, taken from torch's allocator unless given."""
     dt, index, T, ldq, ldo = check_rows("attn_tree", q, out, ctx, H, KV, HD, k_cache, v_cache, pages, scale)

@@ -171,6 +171,25 @@ def test_sums_however_they_are_cut(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,past,most", [([1, 1, 3], [200, 63, 500], 1), ([20, 3, 150], [100, 700, 90], 20), ([130, 3, 131], [0, 50, 300], 130)])
+def test_a_longer_sequence_than_the_step_says_is_refused(rows, past, most, dtype):
+    """The sums are made for max_q_len rows of a sequence: one with more is reported and left alone, the others are served."""
+    from types import SimpleNamespace
+    from mynah_slm_b200.ops import evict
+    H, KV, HD = 4, 2, 64
+    step, q, k, v = _case(9, rows, past, H, KV, HD, dtype)
+    step.max_q_len = most
+    mass = torch.rand((step.pages.n_pages, KV, 64), device=DEV) * 3
+    got, out = mass.clone(), torch.full_like(q, 7.0)
+    evict.attn_mass(q, out, got, step, H, KV, HD, k, v, step.pages)
+    assert step.status.item() & 1
+    n = sum(rows[:2])
+    assert (out[n:] == 7.0).all()
+    served = SimpleNamespace(q_lens=rows[:2], past=past[:2], lists=step.lists[:2])
+    _agrees(served, q[:n], k, v, H, KV, HD, dtype, out[:n], plain.causal(served), mass, got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("rows,past", [([1, 1, 1], [300, 64, 5]), ([40, 7], [30, 200])])
 def test_outputs_that_are_not_aligned(rows, past, dtype):
     """Columns of a wider buffer that begin at an odd one, rows of an odd pitch; q is aligned."""
