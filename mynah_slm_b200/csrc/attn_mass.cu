@@ -8,7 +8,7 @@
 // the resident operand and the step's packed rows going by: a key's sum stays with its thread, no two CTAs add to the same
 // word, and the order of the sum does not depend on timing. Sums are fp32.
 //
-// Long steps are cut over their rows too (attn_mass.cuh): the cut pieces' sums are left in scratch and added in order by a
+// Long sequences are cut over their rows too (attn_mass.cuh): the cut pieces' sums are left in scratch and added in order by a
 // second launch. Steps of few rows on the tensor cores do not look at the keys again: the attention keeps its scores, and the
 // launch that joins its segments adds them up (sum_scores in attn_rows.cu). This file holds the general kernel (fp32, and bfloat16
 // heads that the tensor-core kernel does not take: 2 pieces of 150 tokens behind 333 rows, 6 heads of 48 on 3, 10 us of 39, bound
@@ -177,11 +177,13 @@ bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
     a.keys = tc ? 128 : GK;
     a.rows = tc ? 128 / a.r.G * a.r.G : GR;
     a.by_keys = (long long)max_q_len * a.r.G <= a.rows;
+    a.own_pieces = tc ? 0 : 16;                                    // (2 pieces of 150, 10 row tiles each: 35.4 us with 16, 38.2 with 8, 39.0 with 4)
+    a.r.most_q = max_q_len;
     a.r.tile_rows = a.rows;
     a.r.group = a.r.ctas = 1;
     a.r.q_aligned = aligned;
     a.r.finish();
-    a.target = (tc ? 4 : (a.by_keys ? 0 : 4)) * mynah_sm_count();
+    a.target = tc ? 4 * mynah_sm_count() : 0;
     a.score_rows = tc && (long long)max_q_len * a.r.G <= SCORE_ROWS ? max_q_len * a.r.G : 0;
     return tc;
 }
@@ -189,25 +191,27 @@ bool mass_plan(MassArgs& a, int dtype, bool aligned, int max_q_len) {
 long long mass_scratch(const MassArgs& a, int n_ids) {
     const long long lse = ((long long)a.r.T * a.r.H + 3) & ~3ll;
     if (a.score_rows > 0) return lse + (long long)n_ids * a.r.KV * a.score_rows * PAGE_TOKENS;
-    return lse + (a.target > 0 && !a.by_keys ? mass_units_max(a, n_ids) * a.r.KV * a.keys : 0);
+    return lse + (a.by_keys ? 0 : mass_units_max(a, n_ids) * a.r.KV * a.keys);
 }
 
 }  // namespace
 
-long long attn_rows_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int causal);
+long long attn_rows_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int causal, int n_ids, int aligned);
 
-// Floats of scratch for mynah_attn_mass, whichever kernels take the call.
-MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int n_ids) {
+// Floats of scratch for mynah_attn_mass. aligned: q's and the output's rows are 16-byte aligned (1) or not (0), which decides what
+// takes the call; -1: enough for either.
+MYNAH_API long long mynah_attn_mass_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int n_ids, int aligned) {
     if (T <= 0 || B <= 0 || KV <= 0 || H % KV != 0 || H <= 0 || HD <= 0) return 0;
     long long need = 0;
-    for (int aligned = 0; aligned < 2; aligned++) {
+    for (int al = 0; al < 2; al++) {
+        if (aligned >= 0 && al != aligned) continue;
         MassArgs a{};
         a.r.T = T, a.r.B = B, a.r.H = H, a.r.KV = KV, a.r.HD = HD, a.r.G = H / KV;
-        mass_plan(a, dtype, aligned != 0, max_q_len);
+        mass_plan(a, dtype, al != 0, max_q_len);
         const long long n = mass_scratch(a, n_ids);
         if (n > need) need = n;
     }
-    return attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1) + need;
+    return attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1, n_ids, aligned) + need;
 }
 
 // As mynah_attn_tree with causal rows, and mass [n_pages, KV, 64] fp32. n_ids: entries of page_ids (no fewer than the
@@ -245,9 +249,9 @@ MYNAH_API int mynah_attn_mass(const AttnMassCall* call) {
     MassArgs a{};
     a.r = r;
     const bool tc = mass_plan(a, dtype, aligned, max_q_len);
-    const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids);
+    const long long need = mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, n_ids, aligned);
     MYNAH_REQUIRE(scratch_floats >= need, "attn_mass: scratch holds %lld floats, %lld are needed", scratch_floats, need);
-    const long long attn = attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1);
+    const long long attn = attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 1, n_ids, aligned);
     float* lse = scratch + attn;
     float* part = lse + (((long long)T * H + 3) & ~3ll);
     const PageTable pt{page_indptr, page_ids, page_base, n_pages};

@@ -1,7 +1,9 @@
 // How the sums of attention weights are cut into units of work (attn_mass.cu, attn_mass_tcgen05.cu): a unit is some key tiles of
 // one sequence against some of its row tiles, for one kv head. A step of many rows (prompts) has one key tile a unit and is cut
 // over its rows too; in one whose sequences have a single row tile each (decode steps, short pieces) a unit takes several key
-// tiles. Both counts are such that all units together are about `target`, worked out on the device from the step's own lengths.
+// tiles. On the tensor cores both counts are such that all units together are about `target`, worked out on the device from the
+// step's own lengths. On the general kernel a unit is one key tile, and a sequence's row tiles are cut into `own_pieces` at most by
+// their own number alone: a sum's bits are then the same whatever else is in the step (row_units.cuh).
 #pragma once
 #include "attn_rows.cuh"
 
@@ -9,7 +11,8 @@ struct MassArgs {
     RowsArgs r;
     int keys, rows;                   // cached rows a key tile, packed rows a row tile
     int by_keys;                      // 1: no sequence of the step has more than one row tile
-    int target;                       // units to aim at over all kv heads; 0: a key tile a unit, rows are never cut
+    int target;                       // units to aim at over all kv heads; 0: a key tile a unit, rows cut by the sequence alone
+    int own_pieces;                   // target 0: pieces of a sequence's row tiles at most
     int score_rows;                   // > 0: the attention keeps its scores, of so many rows a kv head at most
 };
 
@@ -23,14 +26,19 @@ struct MassUnit {
 __device__ __forceinline__ int mass_ktiles(const SeqShape& s, const MassArgs& a) { return s.n_q > 0 ? (s.kvl + a.keys - 1) / a.keys : 0; }
 __device__ __forceinline__ int mass_rtiles(const SeqShape& s, const MassArgs& a) { return a.r.by_tile.div(s.n_q * a.r.G + a.rows - 1); }
 
-// Finds unit `flat`, like find_row_unit: a sequence's units lie together, key tiles ascending (the first keys have the most rows
-// above them), a key tile's pieces one after the other.
+// Row tiles a piece: `each` of the step, or by the sequence alone.
+__device__ __forceinline__ int mass_piece(const SeqShape& s, const MassArgs& a, int each) {
+    return a.target > 0 ? each : max(1, quotient(mass_rtiles(s, a) + a.own_pieces - 1, a.own_pieces));
+}
+
+// Finds unit `flat`: a sequence's units lie together, key tiles ascending (the first keys have the most rows above them), a key
+// tile's pieces one after the other.
 __device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, const int* __restrict__ kv_len, const PageTable& pt, const MassArgs& a, int flat,
                                                MassUnit& u, int* status) {
     __shared__ int found_s[3];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        int each = a.by_keys ? 1 : 1 << 28;                // key tiles a unit, or row tiles
+        int each = 1;                                      // key tiles a unit, or row tiles
         if (a.target > 0) {
             long long work = 0;
             for (int b0 = 0; b0 < a.r.B; b0 += 32) {
@@ -48,7 +56,8 @@ __device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, con
             if (b0 + lane < a.r.B) {
                 const SeqShape s = seq_shape(cu_q, kv_len, pt, b0 + lane, a.r, status);
                 const int kt = mass_ktiles(s, a);
-                n = a.by_keys ? (kt + each - 1) / each : kt * ((mass_rtiles(s, a) + each - 1) / each);
+                const int rt = mass_piece(s, a, each);
+                n = a.by_keys ? (kt + each - 1) / each : kt * quotient(mass_rtiles(s, a) + rt - 1, rt);
             }
             int incl = n;
 #pragma unroll
@@ -84,8 +93,8 @@ __device__ __forceinline__ bool find_mass_unit(const int* __restrict__ cu_q, con
         u.kt0 = at * each;
         u.kt1 = min(u.kt0 + each, mass_ktiles(u.s, a));
     } else {
-        u.rt = each;
-        u.pieces = (mass_rtiles(u.s, a) + each - 1) / each;
+        u.rt = mass_piece(u.s, a, each);
+        u.pieces = quotient(mass_rtiles(u.s, a) + u.rt - 1, u.rt);
         u.kt0 = at / u.pieces;
         u.kt1 = u.kt0 + 1;
         u.piece = at % u.pieces;
@@ -107,9 +116,10 @@ __device__ __forceinline__ long long mass_at(const PageTable& pt, int b, int key
 
 // Most units (of one kv head) for `n_ids` pages of all sequences.
 static inline long long mass_units_max(const MassArgs& a, int n_ids) {
-    const long long cut = a.target > 0 ? ceil_div(a.target, a.r.KV) : 0;
-    if (a.by_keys && a.target > 0) return cut + a.r.B;
-    return ceil_div_ll((long long)n_ids * PAGE_TOKENS, a.keys) + a.r.B + cut;
+    const long long cut = a.target > 0 ? ceil_div(a.target, a.r.KV) : 0, most = ceil_div_ll((long long)n_ids * PAGE_TOKENS, a.keys) + a.r.B;
+    if (a.target > 0) return a.by_keys ? cut + a.r.B : most + cut;
+    const long long tiles = ceil_div_ll((long long)a.r.most_q * a.r.G, a.rows);        // of the longest sequence
+    return most * (a.by_keys ? 1 : tiles < a.own_pieces ? tiles : a.own_pieces);
 }
 
 bool mass_tcgen05_takes(int dtype, int H, int KV, int HD);

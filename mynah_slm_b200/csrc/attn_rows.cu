@@ -5,8 +5,8 @@
 //   s_ihr = scale * q_ih . k_gr,   w = softmax over the visible r,   out_ih = sum_r w_ihr v_gr      (g = h / (H / KV))
 //
 // with past = kv_len - n_q. A token that sees nothing gives zeros. The query heads of a kv head are rows of one problem, so a
-// page is read once for all of them; the keys are shared out among the CTAs in equal ranges, each with its own running maximum
-// and sum, and a second launch joins what was cut (row_units.cuh has the rule).
+// page is read once for all of them; the keys are shared out among the CTAs, each with its own running maximum and sum, and a
+// second launch joins what was cut (row_units.cuh has the rules).
 //
 // This file holds the general kernel (fp32, and bfloat16 heads that the tensor-core kernel does not take), the joining, and
 // the entry points.
@@ -55,7 +55,7 @@ template <typename T> __host__ __device__ constexpr int pitch_of(int HD) { retur
 // masked tiles, and the queries read one by one: 30.5 us against 26.7 for 3 trees of 19 in fp32 behind 1,021 rows). K and V come KT
 // keys at a time by asynchronous copies, two tiles in flight.
 // 16-row tiles (TY = 4, TX = 32) are for the few rows of decode steps and small trees, 64-row tiles (TY = TX = 16) for the rest.
-template <typename T, int TY, int TX, int NC>
+template <typename T, int TY, int TX, int NC, bool CAUSAL>
 __global__ void __launch_bounds__(TY * TX, 2)
 attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
                  const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, const long long* __restrict__ masks,
@@ -67,11 +67,11 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     float* p_s = q_s + R * qp;                                     // [R][KT + 4]
     T* k_s = reinterpret_cast<T*>(p_s + R * (KT + 4));             // [2][KT][kp]
     T* v_s = k_s + 2 * KT * kp;                                    // [2][KT][kp]
-    __shared__ RowWalk walk_s;
+    __shared__ RowWalk<CAUSAL, true> walk_s;
 
     if (threadIdx.x < 32) find_start(cu_q, kv_len, pt, a, &walk_s, sc.starts, status);
     __syncthreads();
-    RowWalk u = walk_s;
+    RowWalk<CAUSAL, true> u = walk_s;
     if (u.b < 0) return;
     const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
     // the 16-byte pieces of a K or V tile that this thread copies: the first one, and how far on the next is
@@ -139,7 +139,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         const T* vs = v_s + st * KT * kp;
         const int key0 = t * KT;
         // is there a key in the tile that some row of the tile must not see?
-        const bool need_mask = key0 + KT > u.s.kvl || (a.causal ? key0 + KT - 1 > past + first_tok : key0 + KT > past);
+        const bool need_mask = key0 + KT > u.s.kvl || (CAUSAL ? key0 + KT - 1 > past + first_tok : key0 + KT > past);
         __syncthreads();
         bool odd = false;                                          // and then a value that is not finite (or a stale row)?
         if (need_mask) {
@@ -177,7 +177,7 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
             const int r = ty + TY * i, pr = row0 + r, tok = a.by_G.div(pr);
             uint32_t seen = 0xffffffffu;
             if (need_mask) {
-                const unsigned long long vis = r < n_rows ? visible64(key0 & ~63, u.s.kvl, past, tok, a.causal, masks + (size_t)(u.s.q_begin + tok) * a.words, a.words) : 0ull;
+                const unsigned long long vis = r < n_rows ? visible64<CAUSAL>(key0 & ~63, u.s.kvl, past, tok, masks + (size_t)(u.s.q_begin + tok) * a.words, a.words) : 0ull;
                 seen = (uint32_t)(vis >> (key0 & 63));
             }
             float mx = -INFINITY;
@@ -245,8 +245,11 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
         __syncthreads();                                           // the stage and the weights are free again
     }
 
-    const long long slot = (long long)blockIdx.x * 2 + u.place();
     const bool whole = u.whole();
+    const long long to = whole ? 0 : u.scratch_row(a);
+    // (lists that hold more pages than the call said would take more scratch than there is)
+    const bool fits = whole || to + n_rows <= a.cut_rows;
+    if (!fits && threadIdx.x == 0) atomicOr(status, MYNAH_ST_PAGE_RANGE);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int r = ty + TY * i;
@@ -262,15 +265,15 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
                     const int col = 4 * tx + 4 * TX * c + e;
                     if (col < HD) o[col] = from_f32<T>(acc[i][c][e] * inv);
                 }
-            if (tx == 0 && sc.lse != nullptr) sc.lse[((size_t)g * a.T + u.s.q_begin) * a.G + pr] = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
-        } else {
-            float* o = sc.o + (slot * a.tile_rows + r) * HD;
+            if (CAUSAL && tx == 0) sc.lse[((size_t)g * a.T + u.s.q_begin) * a.G + pr] = l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]);
+        } else if (fits) {
+            float* o = sc.o + (to + r) * HD;
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 const int col = 4 * tx + 4 * TX * c;
                 if (col < HD) *reinterpret_cast<float4*>(o + col) = make_float4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
             }
-            if (tx == 0) sc.ml[slot * a.tile_rows + r] = make_float2(m[i], l[i]);
+            if (tx == 0) sc.ml[to + r] = make_float2(m[i], l[i]);
         }
     }
     } while (u.next(cu_q, kv_len, pt, a, status));
@@ -297,9 +300,10 @@ __device__ __forceinline__ void store4(bf16* o, float a, float b, float c, float
 }
 
 // Joins the segments of a cut item, running over them with the maximum so far as the softmax does over keys. CTA c's helpers
-// (blockIdx.x = c - 1) take the item that CTA c begins inside of, if the item's first pages are CTA c - 1's (each cut item has
-// one such CTA). A warp a row. Bound by its start behind the attention and three dependent reads (where the CTA begins, the
-// sequence's numbers, then the segments' maxima and rows together, from L2).
+// (blockIdx.x = c - 1) take the item that CTA c begins inside of, if the item's first pages are CTA c - 1's (each cut item has one
+// such CTA). OWN: a CTA for every tile and kv head that the step's rows can make, which leaves where the tile was not cut. A warp
+// a row. Bound by its start behind the attention and three dependent reads (where the CTA begins or which tile it
+// has, the sequence's numbers, then the segments' maxima and rows together, from L2).
 constexpr int JOIN_WARPS = 8, JOIN_HELPERS = 16;                   // warps of a CTA; CTAs that share an item's rows at most
 constexpr int JOIN_AHEAD = 4;                                      // segments asked for at once
 
@@ -369,29 +373,49 @@ __device__ __forceinline__ void sum_scores(int cta, const int* __restrict__ cu_q
 }
 
 // CTAs from `joining` on: sums of kept scores.
-template <typename T>
+template <typename T, bool OWN>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, RowsScratch sc,
                       int joining, int* __restrict__ status) {
     griddep_wait();
-    if ((int)blockIdx.x >= joining) {
-        sum_scores(blockIdx.x - joining, cu_q, kv_len, pt, a, sc, status);
-        return;
+    SeqShape s;
+    int g, tile, n;                                                // n: segments
+    long long first, next, after;                                  // scratch rows of the tile's first row in its first, its second segment, and from one to the next
+    if (OWN) {
+        g = a.by_KV.mod(blockIdx.x);
+        const int b = find_tile(cu_q, kv_len, pt, a, a.by_KV.div(blockIdx.x), tile, first, status);
+        if (b < 0) return;
+        s = seq_shape(cu_q, kv_len, pt, b, a, status);
+        const OwnCut cut = own_cut(s, a);
+        if (cut.n == 1) return;                                    // (it was whole)
+        n = quotient((a.causal ? tile_pages<true>(s, tile, a) : s.pages) + cut.each - 1, cut.each);
+        after = s.n_q * a.G;
+        first += (long long)(g * cut.n) * after + tile * a.tile_rows;
+        next = first + after;
+        if (n == 1 || first + (n - 1) * after + min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows) > a.cut_rows) return;
+    } else {
+        if ((int)blockIdx.x >= joining) {
+            sum_scores(blockIdx.x - joining, cu_q, kv_len, pt, a, sc, status);
+            return;
+        }
+        const int cta = a.by_group.div(blockIdx.x) + 1, sub = a.by_group.mod(blockIdx.x);   // (CTA 0 begins inside of nothing)
+        const RowStart at = sc.starts[cta];
+        if (at.b < 0 || at.from == 0 || at.from > at.each) return;
+        s = seq_shape(cu_q, kv_len, pt, at.b, a, status);
+        g = at.g;
+        tile = at.item * a.group + sub;
+        if (tile >= s.tiles) return;
+        const int pages = a.causal ? tile_pages<true>(s, tile, a) : s.pages;
+        if (pages <= at.from) return;                              // this tile ends before the cut: it was whole
+        n = 2 + quotient(pages - at.from - 1, at.each);
+        after = 2ll * a.group * a.tile_rows;
+        next = 2ll * (cta * a.group + sub) * a.tile_rows;
+        first = next - after + a.tile_rows;                        // (its CTA's second place)
     }
-    const int cta = a.by_group.div(blockIdx.x) + 1, sub = a.by_group.mod(blockIdx.x);       // (CTA 0 begins inside of nothing)
-    const RowStart at = sc.starts[cta];
-    if (at.b < 0 || at.from == 0 || at.from > at.each) return;
-    const SeqShape s = seq_shape(cu_q, kv_len, pt, at.b, a, status);
-    const int tile = at.item * a.group + sub;
-    if (tile >= s.tiles) return;
-    const int pages = tile_pages(s, tile, a);
-    if (pages <= at.from) return;                                  // this tile ends before the cut: it was whole
-    const int n = 2 + quotient(pages - at.from - 1, at.each);      // segments
     const int lane = threadIdx.x & 31, rows = min(a.tile_rows, s.n_q * a.G - tile * a.tile_rows);
 #pragma unroll 1
     for (int row = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5); row < rows; row += gridDim.y * JOIN_WARPS) {
-        const int pr = tile * a.tile_rows + row, tok = a.by_G.div(pr), t = s.q_begin + tok, h = at.g * a.G + pr - tok * a.G;
-        auto slot = [&](int c) { return ((long long)((cta - 1 + c) * a.group + sub) * 2 + (c == 0 ? 1 : 0)) * a.tile_rows + row; };
+        const int pr = tile * a.tile_rows + row, tok = a.by_G.div(pr), t = s.q_begin + tok, h = g * a.G + pr - tok * a.G;
         for (int col = lane * 4; col < a.HD; col += 128) {
             float m = -INFINITY, l = 0.f;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -404,7 +428,7 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
                     ml[c] = make_float2(-INFINITY, 0.f);           // (behind the last: no weight)
                     y[c] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (c0 + c < n) {
-                        const long long i = slot(c0 + c);
+                        const long long i = (c0 + c == 0 ? first : next + (c0 + c - 1) * after) + row;
                         ml[c] = sc.ml[i];
                         y[c] = *reinterpret_cast<const float4*>(sc.o + i * a.HD + col);
                     }
@@ -424,18 +448,18 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a NaN stays one
             T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
             store4(o, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-            if (col == 0 && sc.lse != nullptr) sc.lse[((size_t)at.g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m + log2f(l);
+            if (col == 0 && sc.lse != nullptr) sc.lse[((size_t)g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m + log2f(l);
         }
     }
     griddep_launch_late();
 }
 
-template <typename T, int TY, int TX, int NC>
+template <typename T, int TY, int TX, int NC, bool CAUSAL>
 int go(const void* q, void* out, const RowsArgs& a, const void* k, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
        const long long* masks, RowsScratch s, int* status, cudaStream_t stream) {
     constexpr int R = 4 * TY;
     const size_t smem = (size_t)R * (a.HD + 4) * 4 + (size_t)R * (KT + 4) * 4 + 4 * (size_t)KT * pitch_of<T>(a.HD) * sizeof(T);
-    auto kern = attn_rows_kernel<T, TY, TX, NC>;
+    auto kern = attn_rows_kernel<T, TY, TX, NC, CAUSAL>;
     static std::atomic<unsigned long long> opted{0};
     const cudaError_t e = shared_memory_once(kern, MOST_SHARED, opted);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
@@ -443,10 +467,10 @@ int go(const void* q, void* out, const RowsArgs& a, const void* k, const void* v
     return mynah_check_launch("attn_rows");
 }
 
-template <typename T>
+template <typename T, bool CAUSAL>
 int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
          const long long* masks, RowsScratch s, int* status, cudaStream_t stream) {
-#define ROWS_GO(TY, TX, NC) return go<T, TY, TX, NC>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream)
+#define ROWS_GO(TY, TX, NC) return go<T, TY, TX, NC, CAUSAL>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream)
     if (a.tile_rows == 16) {
         if (a.HD <= 128) ROWS_GO(4, 32, 1);
         ROWS_GO(4, 32, 2);
@@ -457,14 +481,20 @@ int pick(const void* q, void* out, const RowsArgs& a, const void* k, const void*
 #undef ROWS_GO
 }
 
+// Most tiles of a step: what its rows can make (they may lie in any number of its sequences).
+long long most_tiles(const RowsArgs& a) { return (long long)a.T * a.G / a.tile_rows + a.B; }
+
 }  // namespace
 
+// Rows of scratch for cut items.
+static long long scratch_rows(const RowsArgs& a) { return a.own ? a.cut_rows : a.whole_items ? 0 : 2ll * a.ctas * a.group * a.tile_rows; }
+
 long long rows_scratch_floats(const RowsArgs& a) {
-    return (a.whole_items ? 0 : 2ll * a.ctas * a.group * a.tile_rows * (a.HD + 2)) + (long long)(sizeof(RowStart) / 4) * a.ctas;
+    return scratch_rows(a) * (a.HD + 2) + (a.own ? 0 : (long long)(sizeof(RowStart) / 4) * a.ctas);
 }
 
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
-    const long long rows = a.whole_items ? 0 : 2ll * a.ctas * a.group * a.tile_rows;
+    const long long rows = scratch_rows(a);
     RowsScratch s;
     s.o = scratch;                                                 // 16-byte rows first
     s.ml = reinterpret_cast<float2*>(scratch + rows * a.HD);
@@ -475,28 +505,36 @@ RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse) {
     return s;
 }
 
-bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
+bool rows_plan(RowsArgs& a, int dtype, int max_q_len, int n_ids, bool aligned) {
     const bool tc = aligned && rows_tcgen05_takes(dtype, a.H, a.KV, a.HD);
     const long long longest = (long long)max_q_len * a.G;          // packed rows of the longest sequence
     // A page is little for the tensor cores and 20,000 clocks of FFMA for 64 rows: there every further CTA helps (3 trees of 19 in
-    // fp32 behind 1,021 rows: 33.7 us with two pages a CTA at least, 30.5 with one; 8 trees of 24 on the tensor cores: the same).
+    // fp32 behind 1,021 rows: 35 us with two pages a CTA at least, 25 with one; 8 trees of 24 on the tensor cores: the same).
     a.min_range = tc ? 2 : 1;
     a.q_aligned = aligned;
     a.group = 1;
     a.two = 0;
     a.whole_items = 0;
     a.ctas = 2 * mynah_sm_count();                                 // two CTAs an SM
+    a.own = !tc;
+    const long long rows = (long long)a.T * a.G;
     if (!tc) {
-        a.tile_rows = longest <= 16 ? 16 : 64;
+        a.tile_rows = longest <= 16 ? 16 : 64;                     // (both add a row's products, weights and outputs in the same order)
         a.most_rows = (int)(longest < 1 ? 1 : longest < a.tile_rows ? longest : a.tile_rows);      // (a step may be all padding)
+        // Scratch of own_cut for all sequences together: each has up to OWN_PIECES * OWN_ROWS rows of cut items; its pieces of an item
+        // are no more than OWN_PIECES / KV, and no more than its listed pages make.
+        const long long most = OWN_PIECES / a.KV > 1 ? OWN_PIECES / a.KV : 1, seq_rows = (long long)(a.most_q < a.T ? a.most_q : a.T) * a.G;
+        a.cut_rows = (long long)OWN_PIECES * OWN_ROWS * a.B;
+        if (a.cut_rows > rows * a.KV * most) a.cut_rows = rows * a.KV * most;
+        if (n_ids >= 0 && a.cut_rows > seq_rows * a.KV * (n_ids / a.min_range + a.B)) a.cut_rows = seq_rows * a.KV * (n_ids / a.min_range + a.B);
         a.finish();
         return false;
     }
     a.tile_rows = 128 / a.G * a.G;
-    const long long rows = (long long)a.T * a.G, each = (long long)a.B * a.tile_rows;
+    const long long each = (long long)a.B * a.tile_rows;
     if (a.causal && rows / a.tile_rows * a.KV >= mynah_sm_count()) {
         a.whole_items = 1;
-        a.ctas = (int)((rows / a.tile_rows + 1 + a.B) * a.KV);     // as many as the step's rows can make
+        a.ctas = (int)(most_tiles(a) * a.KV);
     } else if (longest > a.tile_rows && 2 * rows >= 3 * each) {
         // From one and a half tiles a sequence on, on average, a CTA takes two; beyond that as many side by side as there are, up to
         // eight tiles (a sequence of fewer leaves CTAs idle).
@@ -515,46 +553,60 @@ bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned) {
 
 int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, const void* k, const void* v, const int* cu_q,
                         const int* kv_len, PageTable pt, const long long* masks, RowsScratch s, int* status, cudaStream_t stream) {
-    if (dtype == MYNAH_F32) return pick<float>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
-    return pick<bf16>(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
+    auto run = dtype == MYNAH_F32 ? (a.causal ? pick<float, true> : pick<float, false>) : (a.causal ? pick<bf16, true> : pick<bf16, false>);
+    return run(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
+}
+
+template <typename T, bool OWN>
+static int join_go(void* out, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int joining, dim3 grid, int* status,
+                   cudaStream_t stream) {
+    const cudaError_t e = launch_behind(attn_rows_join_kernel<T, OWN>, grid, dim3(JOIN_WARPS * 32), 0, stream, (T*)out, cu_q, kv_len, pt, a, s, joining, status);
+    if (e != cudaSuccess) return mynah_fail("attn_rows_join: %s", cudaGetErrorString(e));
+    return mynah_check_launch("attn_rows_join");
 }
 
 int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int* status,
                      cudaStream_t stream) {
-    const int joining = a.whole_items ? 0 : (a.ctas - 1) * a.group;            // (whole items: nothing is cut)
+    const long long joining = a.own ? most_tiles(a) * a.KV : a.whole_items ? 0 : (a.ctas - 1) * a.group;       // (whole items: nothing is cut)
     long long ctas = joining;
+    int helpers = min(ceil_div(a.most_rows, JOIN_WARPS), JOIN_HELPERS);
+    if (a.own) {
+        // (most tiles of many were not cut, and their CTAs only start to leave: no more than about four an SM beyond one a tile)
+        const long long more = ceil_div_ll(4ll * mynah_sm_count(), joining);
+        if (helpers > more) helpers = (int)more;
+    }
     if (s.scores != nullptr) {
         // a run of at least four pages a CTA, about eight CTAs an SM: with few rows each waits for two reads more than it adds
         const long long bg = (long long)a.B * a.KV, pages = ceil_div_ll(s.entries, a.B), most = ceil_div_ll(8ll * mynah_sm_count(), bg);
         const long long chunks = ceil_div_ll(pages, SUM_PAGES) < most ? ceil_div_ll(pages, SUM_PAGES) : most;
         s.sum_chunks = (int)(chunks < 1 ? 1 : chunks);
         ctas += bg * s.sum_chunks;
-        MYNAH_REQUIRE(ctas < (1ll << 31), "attn_rows_join: launch too large");
     }
+    MYNAH_REQUIRE(ctas < (1ll << 31), "attn_rows_join: launch too large");
     if (ctas == 0) return 0;
-    const dim3 grid((unsigned)ctas, min(ceil_div(a.most_rows, JOIN_WARPS), JOIN_HELPERS)), block(JOIN_WARPS * 32);
-    const cudaError_t e = dtype == MYNAH_F32
-        ? launch_behind(attn_rows_join_kernel<float>, grid, block, 0, stream, (float*)out, cu_q, kv_len, pt, a, s, joining, status)
-        : launch_behind(attn_rows_join_kernel<bf16>, grid, block, 0, stream, (bf16*)out, cu_q, kv_len, pt, a, s, joining, status);
-    if (e != cudaSuccess) return mynah_fail("attn_rows_join: %s", cudaGetErrorString(e));
-    return mynah_check_launch("attn_rows_join");
+    const dim3 grid((unsigned)ctas, helpers);
+    auto run = dtype == MYNAH_F32 ? (a.own ? join_go<float, true> : join_go<float, false>) : (a.own ? join_go<bf16, true> : join_go<bf16, false>);
+    return run(out, a, cu_q, kv_len, pt, s, (int)joining, grid, status, stream);
 }
 
-// Floats of scratch for the attention, whichever kernel takes the call.
-long long attn_rows_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int causal) {
+// Floats of scratch for the attention. n_ids: entries of the page lists, -1 for any number; aligned: whether q's and the output's rows
+// are 16-byte aligned, -1 for either.
+long long attn_rows_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int causal, int n_ids, int aligned) {
     if (T <= 0 || B <= 0 || KV <= 0 || H % KV != 0 || H <= 0 || HD <= 0) return 0;
     long long need = 0;
-    for (int aligned = 0; aligned < 2; aligned++) {
+    for (int al = 0; al < 2; al++) {
+        if (aligned >= 0 && al != aligned) continue;
         RowsArgs a{};
         a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = H / KV, a.causal = causal;
-        rows_plan(a, dtype, max_q_len, aligned != 0);
+        a.most_q = causal ? max_q_len : INT_MAX;
+        rows_plan(a, dtype, max_q_len, n_ids, al != 0);
         const long long n = rows_scratch_floats(a);
         if (n > need) need = n;
     }
     return (need + 3) & ~3ll;
 }
-MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype) {
-    return attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 0);
+MYNAH_API long long mynah_attn_tree_scratch_floats(int T, int B, int max_q_len, int H, int KV, int HD, int dtype, int n_ids, int aligned) {
+    return attn_rows_scratch_floats(T, B, max_q_len, H, KV, HD, dtype, 0, n_ids, aligned);
 }
 
 // What mynah_attn_tree and mynah_attn_mass check and launch alike.
@@ -570,7 +622,7 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
     MYNAH_REQUIRE((long long)a.T * a.G < (1ll << 30), "%s: %d rows of %d heads a kv head are too many", who, a.T, a.G);
     MYNAH_REQUIRE(status != nullptr && scratch != nullptr && ((uintptr_t)scratch & 15) == 0, "%s: a status word and 16-byte aligned scratch are required", who);
     const bool aligned = ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0 && (long long)a.ldq * es % 16 == 0 && (long long)a.ldo * es % 16 == 0;
-    const bool tc = rows_plan(a, dtype, max_q_len, aligned);
+    const bool tc = rows_plan(a, dtype, max_q_len, n_ids, aligned);
     const long long need = rows_scratch_floats(a);
     MYNAH_REQUIRE(scratch_floats >= need, "%s: scratch holds %lld floats, %lld are needed", who, scratch_floats, need);
     RowsScratch s = rows_scratch(a, scratch, lse);
@@ -594,7 +646,7 @@ struct AttnTreeCall {
     int dtype, T, B, max_q_len, H, KV, HD, ldq, ldo;
     const void *k_cache, *v_cache;
     const int *cu_q, *kv_len, *page_indptr, *page_ids, *page_base;
-    int n_pages;
+    int n_pages, n_ids;
     const long long* masks;
     int words;
     float scale;
@@ -605,15 +657,15 @@ struct AttnTreeCall {
 };
 static_assert(sizeof(AttnTreeCall) == 168, "as packed by the caller");
 MYNAH_API int mynah_attn_tree(const AttnTreeCall* call) {
-    const auto& [q, out, dtype, T, B, max_q_len, H, KV, HD, ldq, ldo, k_cache, v_cache, cu_q, kv_len, page_indptr, page_ids, page_base, n_pages,
+    const auto& [q, out, dtype, T, B, max_q_len, H, KV, HD, ldq, ldo, k_cache, v_cache, cu_q, kv_len, page_indptr, page_ids, page_base, n_pages, n_ids,
                  masks, words, scale, scratch, scratch_floats, status, stream] = *call;
     if (T <= 0 || B <= 0) return 0;
-    MYNAH_REQUIRE(masks != nullptr && words > 0, "attn_tree: mask words are required");
+    MYNAH_REQUIRE(masks != nullptr && words > 0 && n_ids >= 0, "attn_tree: mask words and the number of page entries are required");
     MYNAH_REQUIRE(scale >= 0.f, "attn_tree: the score scale %g is negative", scale);
     RowsArgs a{};
     a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = KV > 0 ? H / KV : 0, a.ldq = ldq, a.ldo = ldo, a.words = words;
     a.most_q = INT_MAX;                                            // (max_q_len gives the tiles their size, and rows beyond it are more tiles)
     a.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)HD)) * 1.4426950408889634f;
     return attn_rows_run("attn_tree", q, out, dtype, a, max_q_len, k_cache, v_cache, cu_q, kv_len,
-                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, nullptr, 0, 0, nullptr, status, stream);
+                         PageTable{page_indptr, page_ids, page_base, n_pages}, masks, scratch, scratch_floats, nullptr, nullptr, 0, n_ids, nullptr, status, stream);
 }

@@ -7,9 +7,9 @@
 
 // Partial results of cut items, and what every launch of one call reads.
 struct RowsScratch {
-    RowStart* starts;                 // [ctas]: where every CTA begins
-    float2* ml;                       // [CTAs][2][tile_rows]: reference maximum (base 2, scaled) and sum
-    float* o;                         // [CTAs][2][tile_rows][HD], not normalised
+    RowStart* starts;                 // [ctas]: where every CTA begins (not OWN)
+    float2* ml;                       // [rows]: reference maximum (base 2, scaled) and sum (RowWalk::scratch_row says whose)
+    float* o;                         // [rows][HD], not normalised
     float* scores;                    // [entries of the page lists][KV][score_rows][64]: scores * scale_log2, -inf for unseen keys; null: not wanted
     int score_rows, entries;          // (entries: of the page lists)
     float* mass;                      // [n_pages][KV][64]: the sums that the kept scores are added to
@@ -21,8 +21,9 @@ struct RowsScratch {
 long long rows_scratch_floats(const RowsArgs& a);
 RowsScratch rows_scratch(const RowsArgs& a, float* scratch, float* lse);
 
-// Fills tile_rows, min_range and ctas; true where the tcgen05 kernel takes the call.
-bool rows_plan(RowsArgs& a, int dtype, int max_q_len, bool aligned);
+// Fills tile_rows, min_range, ctas and so on; true where the tcgen05 kernel takes the call. n_ids: entries of the page
+// lists (-1: any number).
+bool rows_plan(RowsArgs& a, int dtype, int max_q_len, int n_ids, bool aligned);
 
 int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, const void* k, const void* v, const int* cu_q,
                         const int* kv_len, PageTable pt, const long long* masks, RowsScratch s, int* status, cudaStream_t stream);

@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
     return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool CAUSAL>
 __global__ void __launch_bounds__(96 + 128 * NT, 3 - NT)
 attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const bf16* __restrict__ v_cache, const int* __restrict__ cu_q,
@@ -70,7 +70,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     int* flags = reinterpret_cast<int*>(bars + 48);            // [0], [1]: 1 + the last segment (even, odd) in which a value that is
                                                                // not finite was zeroed; [2 .. 9]: the same for missing pages, by
                                                                // segment % 8 (the producer is up to three segments ahead)
-    __shared__ RowWalk walk_s;
+    __shared__ RowWalk<CAUSAL, false> walk_s;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
@@ -103,7 +103,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    RowWalk u = walk_s;
+    RowWalk<CAUSAL, false> u = walk_s;
     const bool any = u.b >= 0;
     const int tile_rows = NT == 2 ? a.tile_rows >> 1 : a.tile_rows;                    // of one tile; a tile exists if the CTA's rows reach it
 
@@ -252,7 +252,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int first_tok = a.by_G.div(u.tile * a.tile_rows), tok = a.by_G.div(row0 + row);            // of the sequence
             const long long* words = masks + (size_t)(u.s.q_begin + min(tok, u.s.n_q - 1)) * a.words;
             // Is there a key in the page that some row of the CTA must not see?
-            auto masked = [&](int key0) { return key0 + KEYS > kvl || (a.causal ? key0 + KEYS - 1 > past + first_tok : key0 + KEYS > past); };
+            auto masked = [&](int key0) { return key0 + KEYS > kvl || (CAUSAL ? key0 + KEYS - 1 > past + first_tok : key0 + KEYS > past); };
             float m_ref = -INFINITY, l = 0.f;                  // the maximum that the sums are scaled by; the sum
             for (int j = 0; j < n && ok && there; j++, i++, c_own++) {
                 const int st = i % NS, key0 = (u.pg0 + j) * KEYS, buf = c_own & 1;
@@ -267,7 +267,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                     for (int c = 0; c < 2; c++) tc_wait_ld(reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
                     if (mask) {
-                        const unsigned long long vis = row < n_rows ? visible64(key0, kvl, past, tok, a.causal, words, a.words) : 0ull;
+                        const unsigned long long vis = row < n_rows ? visible64<CAUSAL>(key0, kvl, past, tok, words, a.words) : 0ull;
                         const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
@@ -276,7 +276,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         }
                     }
                     const int entry = u.s.list0 + u.pg0 + j - u.s.first;       // of the page lists
-                    if (sc.scores != nullptr && row0 + row < sc.score_rows && row < n_rows && entry >= u.s.list0 && entry < min(u.s.list1, sc.entries)) {
+                    if (CAUSAL && sc.scores != nullptr && row0 + row < sc.score_rows && row < n_rows && entry >= u.s.list0 && entry < min(u.s.list1, sc.entries)) {
                         // for the sums of the weights (one tile, of few rows)
                         float4* to = reinterpret_cast<float4*>(sc.scores + (((size_t)entry * a.KV + u.g) * sc.score_rows + row0 + row) * KEYS);
 #pragma unroll
@@ -360,7 +360,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const bool whole = u.whole();
                 if (lost) m_ref = -INFINITY, l = 0.f;          // a page was missing: nothing counts
                 const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;      // a NaN stays one
-                const long long slot0 = ((long long)blockIdx.x * 2 + u.place()) * a.tile_rows + mine * tile_rows;      // of the tile
+                const long long slot0 = whole ? 0 : u.scratch_row(a) + mine * tile_rows;         // of the tile
                 if (works) {
                     const uint32_t mine_s = smem_u32(stage_s) + (warp - 3) * 32 * STAGE_PITCH * 4;     // this warp's rows, 16 columns at a time
                     const int rows_here = min(32, n_rows - quad * 32);
@@ -383,7 +383,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (poison && !lost && row < n_rows) { // the values that were zeroed, to the rows that see them
 #pragma unroll 1
                             for (int key = u.pg0 * KEYS; key < min(u.pg1 * KEYS, kvl); key++) {
-                                if (!masked(key & ~63) || !((visible64(key & ~63, kvl, past, tok, a.causal, words, a.words) >> (key & 63)) & 1ull)) continue;
+                                if (!masked(key & ~63) || !((visible64<CAUSAL>(key & ~63, kvl, past, tok, words, a.words) >> (key & 63)) & 1ull)) continue;
                                 const bf16* vr = v_cache + (((size_t)page_at(pt, u.s, key / PAGE_TOKENS) * a.KV + u.g) * PAGE_TOKENS + key % PAGE_TOKENS) * HD + c * 64;
 #pragma unroll
                                 for (int e = 0; e < 64; e++) {
@@ -417,7 +417,7 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                     if (row < n_rows) {
                         if (!whole) sc.ml[slot0 + row] = make_float2(m_ref, l);
-                        else if (sc.lse != nullptr) sc.lse[((size_t)u.g * a.T + u.s.q_begin) * a.G + row0 + row] = l == 0.f ? -INFINITY : m_ref + log2f(l);
+                        else if (CAUSAL) sc.lse[((size_t)u.g * a.T + u.s.q_begin) * a.G + row0 + row] = l == 0.f ? -INFINITY : m_ref + log2f(l);
                     }
                 }
                 tc_fence_before();
@@ -437,11 +437,11 @@ attn_rows_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool CAUSAL>
 int go(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const void* v, const int* cu_q, const int* kv_len, PageTable pt,
        const long long* masks, const RowsArgs& a, void* out, RowsScratch s, int* status, cudaStream_t stream) {
     constexpr size_t smem = (size_t)(HD / 64) * (NT * HALF_BYTES + 2 * STAGES<HD, NT> * PAGE_BYTES) + NT * 4 * 32 * STAGE_PITCH * 4 + 448 + 1024;
-    auto kern = attn_rows_tcgen05_kernel<HD, NT>;
+    auto kern = attn_rows_tcgen05_kernel<HD, NT, CAUSAL>;
     static std::atomic<unsigned long long> opted{0};
     const cudaError_t e = shared_memory_once(kern, smem, opted);
     if (e != cudaSuccess) return mynah_fail("attn_rows: %s", cudaGetErrorString(e));
@@ -464,7 +464,7 @@ int launch_rows_tcgen05(const void* q, void* out, const RowsArgs& a, const void*
     if (make_map_rows(&mq, q, a.T, a.H, a.HD, a.G, a.ldq, a.tile_rows / (a.two ? 2 : 1) / a.G)) return -1;
     if (make_map(&mk, k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, a.HD, a.HD, PAGE_TOKENS, 64)) return -1;
     if (make_map(&mv, v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, a.HD, a.HD, PAGE_TOKENS, 64)) return -1;
-#define ROWS_GO(HD, NT) return go<HD, NT>(mq, mk, mv, v, cu_q, kv_len, pt, masks, a, out, s, status, stream)
+#define ROWS_GO(HD, NT) return (a.causal ? go<HD, NT, true> : go<HD, NT, false>)(mq, mk, mv, v, cu_q, kv_len, pt, masks, a, out, s, status, stream)
     if (a.two) {
         if (a.HD == 128) ROWS_GO(128, 2);
         ROWS_GO(64, 2);

@@ -18,7 +18,7 @@ from ..cache.pages import PAGE_TOKENS
 from . import lib
 from .kernels import PageTableView
 from .lib import KernelError, call, code, stream_on
-from .tree import check_layers, check_lists, check_rows, row_scratch
+from .tree import check_layers, check_lists, check_rows, row_scratch, rows_aligned
 
 # the arguments of the C entries, which take them as one struct
 _MASS_CALL = Struct("@3P9i7P2ifPq2P")
@@ -26,12 +26,13 @@ _EVICT_CALL = Struct("@3P6i4Pi3P4i4P")
 
 
 @lru_cache(maxsize=256)
-def _mass_scratch(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dcode: int, n_ids: int) -> int:
-    return int(lib.load().mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dcode, n_ids))
+def _mass_scratch(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dcode: int, n_ids: int, aligned: int) -> int:
+    return int(lib.load().mynah_attn_mass_scratch_floats(T, B, max_q_len, H, KV, HD, dcode, n_ids, aligned))
 
 
 def attn_mass_scratch_floats(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dtype: torch.dtype, n_ids: int) -> int:
-    return _mass_scratch(T, B, max_q_len, H, KV, HD, code(dtype), n_ids)
+    """Words that serve a call of this shape; n_ids: entries of the page lists (a call whose rows are 16-byte aligned may need fewer)."""
+    return _mass_scratch(T, B, max_q_len, H, KV, HD, code(dtype), n_ids, -1)
 
 
 def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor,
@@ -52,7 +53,8 @@ def attn_mass(q: torch.Tensor, out: torch.Tensor, mass: torch.Tensor, ctx, H: in
     if T == 0 or ctx.B == 0:
         return
     n_ids = pages.ids.numel()
-    scratch = row_scratch("attn_mass", scratch, _mass_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids), ctx.status)
+    need = _mass_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids, rows_aligned(q, out, ldq, ldo))
+    scratch = row_scratch("attn_mass", scratch, need, ctx.status)
     call("mynah_attn_mass", _MASS_CALL.pack(
         q.data_ptr(), out.data_ptr(), mass.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, ldq, ldo, k_cache.data_ptr(), v_cache.data_ptr(),
         ctx.cu_q.data_ptr(), ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, n_ids, scale,

@@ -220,9 +220,9 @@ def load() -> ctypes.CDLL:
     lib.mynah_gated_memory_scratch_floats.restype = c_longlong
     lib.mynah_gated_memory_scratch_floats.argtypes = [c_int] * 9
     lib.mynah_attn_tree_scratch_floats.restype = c_longlong
-    lib.mynah_attn_tree_scratch_floats.argtypes = [c_int] * 7
+    lib.mynah_attn_tree_scratch_floats.argtypes = [c_int] * 9
     lib.mynah_attn_mass_scratch_floats.restype = c_longlong
-    lib.mynah_attn_mass_scratch_floats.argtypes = [c_int] * 8
+    lib.mynah_attn_mass_scratch_floats.argtypes = [c_int] * 9
     lib.mynah_moe_grouped_rows.restype = c_int
     lib.mynah_moe_grouped_rows.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
     lib.mynah_moe_max_tiles.restype = c_int

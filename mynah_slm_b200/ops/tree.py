@@ -24,7 +24,7 @@ from .lib import KernelError, call, code, stream_on
 _INF = float("inf")
 _I32 = torch.int32
 # the arguments of the C entries, which take them as one struct
-_TREE_CALL = Struct("@2P9i7PiPifPq2P")
+_TREE_CALL = Struct("@2P9i7P2iPifPq2P")
 _COMMIT_CALL = Struct("@3P3i5Pi2P4i5P")
 
 
@@ -110,12 +110,19 @@ def row_scratch(who: str, scratch: Optional[torch.Tensor], need: int, status: to
 
 
 @lru_cache(maxsize=256)
-def _tree_scratch(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dcode: int) -> int:
-    return int(lib.load().mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dcode))
+def _tree_scratch(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dcode: int, n_ids: int, aligned: int) -> int:
+    return int(lib.load().mynah_attn_tree_scratch_floats(T, B, max_q_len, H, KV, HD, dcode, n_ids, aligned))
+
+
+def rows_aligned(q: torch.Tensor, out: torch.Tensor, ldq: int, ldo: int) -> int:
+    """Whether the rows of q and of the output begin at whole 16 bytes: the tensor cores take such a call."""
+    es = q.element_size()
+    return 0 if (q.data_ptr() | out.data_ptr() | ldq * es | ldo * es) & 15 else 1
 
 
 def attn_tree_scratch_floats(T: int, B: int, max_q_len: int, H: int, KV: int, HD: int, dtype: torch.dtype) -> int:
-    return _tree_scratch(T, B, max_q_len, H, KV, HD, code(dtype))
+    """Words that serve a call of this shape whatever its page lists and alignment are (most calls need fewer)."""
+    return _tree_scratch(T, B, max_q_len, H, KV, HD, code(dtype), -1, -1)
 
 
 def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -135,10 +142,11 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
         raise KernelError(f"attn_tree: the masks must be contiguous int64 [{T}, words] on {q.device}, got {tuple(masks.shape)} {masks.dtype}")
     if T == 0 or ctx.B == 0:
         return
-    scratch = row_scratch("attn_tree", scratch, _tree_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt), ctx.status)
+    n_ids = pages.ids.numel()
+    scratch = row_scratch("attn_tree", scratch, _tree_scratch(T, ctx.B, ctx.max_q_len, H, KV, HD, dt, n_ids, rows_aligned(q, out, ldq, ldo)), ctx.status)
     call("mynah_attn_tree", _TREE_CALL.pack(
         q.data_ptr(), out.data_ptr(), dt, T, ctx.B, ctx.max_q_len, H, KV, HD, ldq, ldo, k_cache.data_ptr(), v_cache.data_ptr(), ctx.cu_q.data_ptr(),
-        ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, masks.data_ptr(), masks.shape[1],
+        ctx.kv_len.data_ptr(), pages.indptr.data_ptr(), pages.ids.data_ptr(), pages.base.data_ptr(), pages.n_pages, n_ids, masks.data_ptr(), masks.shape[1],
         scale, scratch.data_ptr(), scratch.numel(), ctx.status.data_ptr(), stream_on(index)))
 
 

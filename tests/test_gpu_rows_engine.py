@@ -241,6 +241,40 @@ def test_generation_over_a_bounded_cache(folders, name, dtype):
     assert end.finish_reason == "context" and len(end.tokens) == n - 2 + 1
 
 
+@pytest.mark.parametrize("name,dtype", [("A", "float32"), ("B", "float32"), ("D", "float32"), ("A", "bfloat16")])
+def test_a_bounded_sequence_keeps_the_same_rows_alone_and_in_a_batch(folders, name, dtype):
+    """Token by token, with evictions: logits, sums and the keys that stay have the same bits alone and beside longer sequences (in 32
+    bits, and with heads that the tensor cores do not take)."""
+    from mynah_slm_b200.engine.engine import KeepRows, StepEntry
+    rng = random.Random(9)
+    vocab, n = TINY[name]["vocab_size"], 150
+    text = [rng.randrange(vocab) for _ in range(n)]
+    others = [[rng.randrange(vocab) for _ in range(n)] for _ in range(4)]
+
+    def run(beside):
+        eng = _engine(folders[(name, dtype)], dtype, 4096, keep=KeepRows(70, 50, 16))
+        slots = [eng.open_sequence() for _ in range(1 + beside)]
+        for s, o in zip(slots[1:], others):
+            eng.step([StepEntry(s, o[:65], ())])               # further on than the first, so that they are cut at other steps
+        logits = []
+        for i in range(n):
+            out = eng.step([StepEntry(s, (t[i],), (0,)) for s, t in zip(slots, [text] + others)])
+            logits.append(out[0].clone())
+        eng.check_status()
+        held = eng.length(slots[0])
+        views = []
+        for view in eng.cache.views:
+            pages = torch.tensor(eng.cache.pages.held(slots[0], view.group)[0], device=eng.device)
+            for t in (view.mass, view.k, view.v):
+                views.append(t[pages].transpose(0, 1).flatten(1, 2)[:, :held].clone())
+        return torch.stack(logits), views, held
+    want = run(0)
+    for beside in (1, 4):
+        got = run(beside)
+        assert got[2] == want[2] and torch.equal(got[0], want[0])
+        assert all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
+
+
 def test_the_command_line_drafts_and_keeps(folders):
     def run(*extra):
         cmd = [sys.executable, "-m", "mynah_slm_b200.cli", "run", "-m", folders[("A", "float32")], "--dtype", "float32", "--tokens", "1,2,3,1,2,3,1,2",

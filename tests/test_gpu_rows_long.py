@@ -170,6 +170,49 @@ def test_sums_however_they_are_cut(case, dtype):
     _agrees(step, q, k, v, H, KV, HD, dtype, out, plain.causal(step), mass, got)
 
 
+COMPANY = [  # a sequence's rows and past, then the others' in every company
+    (1, 1535, [([1], [40]), ([1] * 5, [6000, 3, 64, 900, 2047]), ([1] * 63, [(b * 631) % 4000 for b in range(63)]),
+               ([1] * 300, [(b * 37) % 300 for b in range(300)])]),
+    (1, 63, [([1] * 9, [9000] * 9)]),
+    (40, 700, [([33], [10]), ([300, 9], [2000, 64]), ([12] * 40, [(b * 211) % 900 for b in range(40)])]),
+    (150, 333, [([150], [333]), ([64, 170], [3000, 5]), ([60] * 10, [500] * 10)]),
+]
+
+
+@pytest.mark.parametrize("dtype,H,KV,HD", [(BF16, 6, 2, 48), (BF16, 16, 8, 80), (F32, 8, 2, 64), (F32, 4, 4, 128), (F32, 32, 8, 128)],
+                         ids=["bf16-48", "bf16-80", "f32-64", "f32-128", "f32-32on8"])
+@pytest.mark.parametrize("case", COMPANY, ids=lambda c: f"{c[0]}x{c[1]}")
+def test_a_sequence_has_the_same_bits_in_any_company(case, dtype, H, KV, HD):
+    """In 32 bits (and for heads that the tensor cores do not take) outputs and sums do not depend on what else the step brings, and
+    with them the path that a tree takes and the rows that an eviction keeps."""
+    from mynah_slm_b200.ops import evict, tree
+    n, p, companies = case
+    d = torch.Generator(device=DEV).manual_seed(77)
+    pages = -(-(n + p) // 64)
+    own = [torch.randn(shape, generator=d, device=DEV).to(dtype) for shape in ((n, H * HD), (pages, KV, 64, HD), (pages, KV, 64, HD))]
+    sums = torch.rand((pages, KV, 64), generator=d, device=DEV) * 3
+    mine_tree = _tree(n, random.Random(n))
+
+    def run(rows, past, at):
+        rng = random.Random(at)
+        step, q, k, v = _case(len(rows), rows, past, H, KV, HD, dtype)
+        masks = _masks([mine_tree if b == at else _tree(r, rng) for b, r in enumerate(rows)])
+        mine, first = torch.tensor(step.lists[at], device=DEV), sum(rows[:at])
+        mass = torch.rand((step.pages.n_pages, KV, 64), device=DEV) * 3
+        q[first:first + n], k[mine], v[mine], mass[mine] = own[0], own[1], own[2], sums
+        out, hung = torch.zeros_like(q), torch.zeros_like(q)
+        evict.attn_mass(q, out, mass, step, H, KV, HD, k, v, step.pages)
+        tree.attn_tree(q, hung, step, H, KV, HD, k, v, step.pages, masks.to(DEV))
+        assert step.status.item() == 0
+        return out[first:first + n].clone(), mass[mine].clone(), hung[first:first + n].clone()
+    alone = run([n], [p], 0)
+    for rows, past in companies:
+        for at in sorted({0, len(rows) // 2, len(rows)}):
+            got = run(rows[:at] + [n] + rows[at:], past[:at] + [p] + past[at:], at)
+            for a, b, what in zip(got, alone, ("outputs", "sums", "tree")):
+                assert torch.equal(a, b), (len(rows), at, what)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("rows,past,most", [([1, 1, 3], [200, 63, 500], 1), ([20, 3, 150], [100, 700, 90], 20), ([130, 3, 131], [0, 50, 300], 130)])
 def test_a_longer_sequence_than_the_step_says_is_refused(rows, past, most, dtype):
