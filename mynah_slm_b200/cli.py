@@ -114,7 +114,7 @@ def cmd_run(argv: list[str]) -> int:
     longest = max(len(p) for p in prompts)
     if o["keep"] < 0 or 0 < o["keep"] < 16:
         return _fail("--keep needs at least 16 rows")
-    per_seq = o["ctx"] if o["ctx"] > 0 else longest + o["max_new"] + 8 + o["draft"]       # cli/main.c:264-265
+    per_seq = o["ctx"] if o["ctx"] > 0 else longest + o["max_new"] + 8       # cli/main.c:264-265
     per_seq = -(-per_seq // 64) * 64
     try:
         max_tokens = per_seq * min(len(prompts), o["batch"])

@@ -47,12 +47,13 @@ class EngineBackend:
         return self.engine.free_tokens()
 
     def rows_held(self, prompt_len: int, max_new: int) -> int:
-        """Cache a request may come to hold: with drafts the rows of a step's tree too, with a bound no more than that (or its prompt)."""
+        """Cache a request may come to hold: with a bound no more than that (or its prompt). A step's drafted tree takes no more rows than
+        the request has tokens to come, so drafts need no room of their own."""
         most, keep = self.max_positions, self.engine.keep
         if keep is not None:
             n = max(prompt_len, min(prompt_len + max(max_new, 0), keep.limit + 1))
             return -(-n // PAGE_TOKENS) * PAGE_TOKENS
-        return tokens_held(prompt_len, max_new, most) if not self.drafts else tokens_held(prompt_len, max_new + self.drafts, most)
+        return tokens_held(prompt_len, max_new, most)
 
     def open(self, request_index: int, prompt: Sequence[int]) -> int:
         slot = self.engine.open_sequence()

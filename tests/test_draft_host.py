@@ -5,7 +5,7 @@ import pytest
 
 from mynah_slm_b200.cache.pages import CacheError, GroupPlan, SequencePages
 from mynah_slm_b200.engine.draft import Lookup
-from mynah_slm_b200.engine.generate import Request, generate, plan_batches
+from mynah_slm_b200.engine.generate import tokens_held, Request, generate, plan_batches
 
 
 def test_a_tree_is_one_and_stays_within_its_room():
@@ -100,3 +100,37 @@ def test_books_that_are_cut_give_their_pages_back():
     windowed.commit(s, 10)
     with pytest.raises(CacheError):
         windowed.shorten(s, 5)
+
+
+def test_drafts_need_no_cache_of_their_own():
+    """A request that fits without drafts fits with them: no step's tree reaches beyond the rows that the request may hold."""
+    from types import SimpleNamespace
+    from mynah_slm_b200.engine.api import EngineBackend
+    from mynah_slm_b200.engine.engine import TreeResult
+    from mynah_slm_b200.sampling.sampler import SamplingParams
+    held, most = {}, {}
+
+    def step_tree(entries):
+        out = []
+        for e in entries:
+            most[e.slot] = max(most.get(e.slot, 0), held[e.slot] + len(e.tokens))
+            path = [0]                                     # the first child of every row, all the way down
+            while path[-1] in e.parents:
+                path.append(list(e.parents).index(path[-1]))
+            held[e.slot] += len(path)
+            out.append(TreeResult([e.tokens[i] for i in path[1:]], 5))
+        return out
+    engine = SimpleNamespace(spec=SimpleNamespace(max_positions=4096), keep=None, use_graphs=False, graph_safe=False, step_tree=step_tree,
+                             sampler=SimpleNamespace(set_params=lambda p: None))
+    for drafts in (1, 8, 200):
+        b = EngineBackend(engine, SamplingParams.greedy(), drafts)
+        for prompt, new in ((40, 24), (1, 63), (100, 28), (5, 1)):
+            assert b.rows_held(prompt, new) == tokens_held(prompt, new, 4096)
+            text = [1, 5, 2, 5, 3] * 20
+            b._lookups[0] = Lookup(text[:prompt])
+            held[0], most[0], produced, last = prompt, 0, 1, 5
+            while produced < new:
+                got = b.decode_drafted([0], [last], [new - produced])[0]
+                assert 1 <= len(got) <= new - produced
+                produced, last = produced + len(got), got[-1]
+            assert most[0] <= prompt + new - 1
