@@ -236,7 +236,7 @@ MYNAH_API int mynah_attn_mass(const AttnMassCall* call) {
                  n_pages, n_ids, scale, scratch, scratch_floats, status, stream] = *call;
     if (T <= 0 || B <= 0) return 0;
     MYNAH_REQUIRE(mass != nullptr && n_ids >= 0, "attn_mass: sums and the number of page entries are required");
-    MYNAH_REQUIRE(scale >= 0.f, "attn_mass: the score scale %g is negative", scale);
+    MYNAH_REQUIRE(scale == 0.f || (scale >= 0x1p-120f && scale <= 0x1p120f), "attn_mass: the score scale %g is not between 2^-120 and 2^120, nor 0", scale);
     MYNAH_REQUIRE(KV > 0 && H > 0 && H % KV == 0, "attn_mass: %d heads over %d kv heads", H, KV);
     MYNAH_REQUIRE(scratch != nullptr && ((uintptr_t)scratch & 15) == 0, "attn_mass: 16-byte aligned scratch is required");
     RowsArgs r{};

@@ -661,7 +661,7 @@ MYNAH_API int mynah_attn_tree(const AttnTreeCall* call) {
                  masks, words, scale, scratch, scratch_floats, status, stream] = *call;
     if (T <= 0 || B <= 0) return 0;
     MYNAH_REQUIRE(masks != nullptr && words > 0 && n_ids >= 0, "attn_tree: mask words and the number of page entries are required");
-    MYNAH_REQUIRE(scale >= 0.f, "attn_tree: the score scale %g is negative", scale);
+    MYNAH_REQUIRE(scale == 0.f || (scale >= 0x1p-120f && scale <= 0x1p120f), "attn_tree: the score scale %g is not between 2^-120 and 2^120, nor 0", scale);
     RowsArgs a{};
     a.T = T, a.B = B, a.H = H, a.KV = KV, a.HD = HD, a.G = KV > 0 ? H / KV : 0, a.ldq = ldq, a.ldo = ldo, a.words = words;
     a.most_q = INT_MAX;                                            // (max_q_len gives the tiles their size, and rows beyond it are more tiles)

@@ -21,7 +21,7 @@ from . import lib
 from .kernels import MAX_HEAD_DIM, PageTableView
 from .lib import KernelError, call, code, stream_on
 
-_INF = float("inf")
+_LEAST, _MOST = 2.0 ** -120, 2.0 ** 120      # a score scale, which the kernels hold in fp32, times log2(e)
 _I32 = torch.int32
 # the arguments of the C entries, which take them as one struct
 _TREE_CALL = Struct("@2P9i7P2iPifPq2P")
@@ -60,8 +60,8 @@ def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: in
         raise KernelError(f"{who}: {H} heads over {KV} kv heads")
     if HD < 1 or HD % 8 or HD > MAX_HEAD_DIM:
         raise KernelError(f"{who}: head_dim {HD} is no multiple of 8 up to {MAX_HEAD_DIM}")
-    if not 0.0 <= scale < _INF:
-        raise KernelError(f"{who}: the score scale {scale} is not a positive number, nor 0 for 1 / sqrt(head_dim)")
+    if scale != 0.0 and not _LEAST <= scale <= _MOST:
+        raise KernelError(f"{who}: the score scale {scale} is not between 2^-120 and 2^120, nor 0 for 1 / sqrt(head_dim)")
     dcode = code(dt)
     T, ldq = _rows_of(who, q, H * HD)
     n_out, ldo = _rows_of(who, out, H * HD)
@@ -132,7 +132,7 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
     makes the words of a tree; any other mask will do, a row that sees nothing gives zeros). Query head h reads kv head
     h // (H / KV). `q` and `out` are rows with head h in columns [h HD, (h + 1) HD), and may be wider; rows of `out` behind the
     last sequence are left as they are. masks: int64 [T, words]; rows of a tree beyond 64 * words are seen by nobody. scale 0:
-    1 / sqrt(HD). ctx: the step's description (B, max_q_len, cu_q, kv_len, status; max_q_len only
+    1 / sqrt(HD), else 2^-120 to 2^120. ctx: the step's description (B, max_q_len, cu_q, kv_len, status; max_q_len only
     sizes the tiles, a longer sequence is served too). Rows of the cache that a row does not see
     have no influence on it, whatever they hold. float32 and bfloat16, heads of any multiple of 8 up to 256; bfloat16 heads of 64
     and 128 run on the tensor cores. `scratch`: attn_tree_scratch_floats fp32 words, taken from torch's allocator unless given."""

@@ -170,6 +170,26 @@ def test_sums_however_they_are_cut(case, dtype):
     _agrees(step, q, k, v, H, KV, HD, dtype, out, plain.causal(step), mass, got)
 
 
+def test_scales_that_fp32_does_not_hold_are_refused():
+    """One that rounds to 0 there would have been taken for "not given"."""
+    from mynah_slm_b200.ops import evict, tree
+    from mynah_slm_b200.ops.lib import KernelError
+    H, KV, HD = 4, 2, 64
+    step, q, k, v = _case(5, [2], [70], H, KV, HD, F32)
+    mass, out, masks = torch.zeros((step.pages.n_pages, KV, 64), device=DEV), torch.zeros_like(q), _masks([[-1, 0]]).to(DEV)
+    for scale in (1e-46, 1e-40, -0.125, 1e38, 1e300, float("inf"), float("nan")):
+        with pytest.raises(KernelError):
+            tree.attn_tree(q, out, step, H, KV, HD, k, v, step.pages, masks, scale)
+        with pytest.raises(KernelError):
+            evict.attn_mass(q, out, mass, step, H, KV, HD, k, v, step.pages, scale)
+    assert (out == 0).all() and (mass == 0).all()
+    small = torch.zeros_like(q)                            # a scale that leaves no difference between the rows: their mean
+    tree.attn_tree(q, small, step, H, KV, HD, k, v, step.pages, masks, 2.0 ** -100)
+    rows = torch.cat([v[p] for p in step.lists[0]], 1)
+    want = torch.stack([rows[:, :n].double().mean(1).repeat_interleave(H // KV, 0) for n in (71, 72)]).view(2, H * HD)
+    assert ((small.double() - want).abs() <= 200 * plain.F32 * rows.abs().max()).all() and step.status.item() == 0
+
+
 COMPANY = [  # a sequence's rows and past, then the others' in every company
     (1, 1535, [([1], [40]), ([1] * 5, [6000, 3, 64, 900, 2047]), ([1] * 63, [(b * 631) % 4000 for b in range(63)]),
                ([1] * 300, [(b * 37) % 300 for b in range(300)])]),
