@@ -67,7 +67,7 @@ def check_rows(who: str, q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: in
     n_out, ldo = _rows_of(who, out, H * HD)
     if out.dtype is not dt or out.get_device() != index or n_out < T:
         raise KernelError(f"{who}: the output is {tuple(out.shape)} {out.dtype} on {out.device}, q {tuple(q.shape)} {dt} on {q.device}")
-    if q.data_ptr() == out.data_ptr() and T:
+    if T and _over(q.data_ptr(), out.data_ptr(), T, ldq, ldo, H * HD, q.element_size()):
         raise KernelError(f"{who}: the output lies over q, which is read until the end")
     cache = (KV, PAGE_TOKENS, HD)
     for t in (k_cache, v_cache):
@@ -91,6 +91,16 @@ def _rows_of(who: str, t: torch.Tensor, width: int) -> tuple[int, int]:
             return n, ld if n > 1 else w
     raise KernelError(f"{who}: q and the output must be rows of at least {width} values, one row behind the other, got "
                       f"{tuple(t.shape)} with strides {t.stride()}")
+
+
+def _over(q: int, out: int, T: int, ldq: int, ldo: int, width: int, es: int) -> bool:
+    """Whether T rows of `width` values at two addresses may share memory. Columns of one buffer may lie side by side."""
+    if q + ((T - 1) * ldq + width) * es <= out or out + ((T - 1) * ldo + width) * es <= q:
+        return False
+    if ldq != ldo:
+        return True
+    apart = (out - q) % (ldq * es)
+    return apart < width * es or apart > (ldq - width) * es
 
 
 def check_lists(who: str, index: int, B: int, cu_q: Optional[torch.Tensor], kv_len: torch.Tensor, pages: PageTableView, status: torch.Tensor) -> None:
@@ -130,7 +140,8 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, ctx, H: int, KV: int, HD: int,
     """Attention of a step's rows over the paged cache, which holds the rows' own keys and values already: with past = kv_len -
     n_q, row i of a sequence sees every cached row below past, and row past + j where bit j of its mask words is set (`tree_rows`
     makes the words of a tree; any other mask will do, a row that sees nothing gives zeros). Query head h reads kv head
-    h // (H / KV). `q` and `out` are rows with head h in columns [h HD, (h + 1) HD), and may be wider; rows of `out` behind the
+    h // (H / KV). `q` and `out` are rows with head h in columns [h HD, (h + 1) HD), and may be wider (columns of one
+    buffer side by side too, but never over one another); rows of `out` behind the
     last sequence are left as they are. masks: int64 [T, words]; rows of a tree beyond 64 * words are seen by nobody. scale 0:
     1 / sqrt(HD), else 2^-120 to 2^120. ctx: the step's description (B, max_q_len, cu_q, kv_len, status; max_q_len only
     sizes the tiles, a longer sequence is served too). Rows of the cache that a row does not see

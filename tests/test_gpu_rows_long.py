@@ -190,6 +190,30 @@ def test_scales_that_fp32_does_not_hold_are_refused():
     assert ((small.double() - want).abs() <= 200 * plain.F32 * rows.abs().max()).all() and step.status.item() == 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_an_output_over_q_is_refused_and_one_beside_it_served(dtype):
+    from mynah_slm_b200.ops import evict, tree
+    from mynah_slm_b200.ops.lib import KernelError
+    rows, past, H, KV, HD = [9, 4], [100, 30], 4, 2, 64
+    step, q, k, v = _case(8, rows, past, H, KV, HD, dtype)
+    W, T = H * HD, sum(rows)
+    masks, mass = _masks([[-1] + list(range(n - 1)) for n in rows]).to(DEV), torch.zeros((step.pages.n_pages, KV, 64), device=DEV)
+    wide = torch.zeros((T + 1, 3 * W), dtype=dtype, device=DEV)
+    wide[:T, :W] = q
+    for out in (wide[1:, :W], wide[:T, 8:W + 8], wide[:T, W - 8:2 * W - 8], wide.view(-1)[W // 2:W // 2 + T * W].view(T, W)):
+        with pytest.raises(KernelError):
+            tree.attn_tree(wide[:T, :W], out, step, H, KV, HD, k, v, step.pages, masks)
+        with pytest.raises(KernelError):
+            evict.attn_mass(wide[:T, :W], out, mass, step, H, KV, HD, k, v, step.pages)
+    assert torch.equal(wide[:T, :W], q) and (wide[:, W:] == 0).all() and (mass == 0).all()
+    want = torch.zeros_like(q)
+    tree.attn_tree(q, want, step, H, KV, HD, k, v, step.pages, masks)
+    for out in (wide[:T, W:2 * W], wide[1:, W:2 * W], wide[:T, 2 * W:]):
+        tree.attn_tree(wide[:T, :W], out, step, H, KV, HD, k, v, step.pages, masks)
+        assert torch.equal(out, want) and torch.equal(wide[:T, :W], q)
+    assert step.status.item() == 0
+
+
 COMPANY = [  # a sequence's rows and past, then the others' in every company
     (1, 1535, [([1], [40]), ([1] * 5, [6000, 3, 64, 900, 2047]), ([1] * 63, [(b * 631) % 4000 for b in range(63)]),
                ([1] * 300, [(b * 37) % 300 for b in range(300)])]),

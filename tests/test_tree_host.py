@@ -1,4 +1,6 @@
 """Trees of drafted tokens on the host: depths, mask words, refusals that need no device."""
+import random
+
 import numpy as np
 import pytest
 import torch
@@ -52,3 +54,24 @@ def test_tensors_that_are_not_on_a_device_are_refused():
         evict.cache_evict(k[None], k[None], t((1, 1, 1, 64)), ctx, pages, 2, 1)
     with pytest.raises(KernelError):
         tree.tree_commit(i32(1), i32(1), i32(1), ctx, k[None], k[None], pages)
+
+
+def test_outputs_over_the_queries_are_told_from_those_beside_them():
+    """Against every byte that the rows take."""
+    from mynah_slm_b200.ops.tree import _over
+    rng = random.Random(3)
+    for _ in range(3000):
+        es, width, T = rng.choice([2, 4]), rng.randrange(1, 9), rng.randrange(1, 5)
+        ldq = width + rng.randrange(0, 20)
+        ldo = ldq if rng.random() < 0.7 else width + rng.randrange(0, 20)
+        q, out = 1000 * es, (1000 + rng.randrange(-40, 41)) * es
+        taken = [{at + (r * ld + c) * es for r in range(T) for c in range(width)} for at, ld in ((q, ldq), (out, ldo))]
+        shared = bool(taken[0] & taken[1])
+        if ldq == ldo:
+            # (equal pitches: exact but for rows that only others of the buffer, not these T, would meet)
+            assert _over(q, out, T, ldq, ldo, width, es) or not shared
+            endless = [{at + (r * ld + c) * es for r in range(-60, 60) for c in range(width)} for at, ld in ((q, ldq), (out, ldo))]
+            if not endless[0] & endless[1]:
+                assert not _over(q, out, T, ldq, ldo, width, es)
+        elif shared:
+            assert _over(q, out, T, ldq, ldo, width, es)
