@@ -28,7 +28,7 @@ __device__ __forceinline__ float4 four_of(const bf16* p) {
     const uint2 w = *reinterpret_cast<const uint2*>(p);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
-// The same where rows are not aligned (volatile: or the compiler may make one 16-byte access of this and the above).
+// The same where rows are not aligned (volatile: read one by one, whatever is made of the other branch).
 __device__ __forceinline__ float4 four_apart(const float* p) {
     const volatile float* w = p;
     return make_float4(w[0], w[1], w[2], w[3]);

@@ -32,7 +32,7 @@ __device__ __forceinline__ float4 four_of(const bf16* p) {
     const uint2 w = *reinterpret_cast<const uint2*>(p);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
-// The same where rows are not aligned (volatile: or the compiler may make one 16-byte access of this and the above).
+// The same where rows are not aligned (volatile: read one by one, whatever is made of the other branch).
 __device__ __forceinline__ float4 four_apart(const float* p) {
     const volatile float* w = p;
     return make_float4(w[0], w[1], w[2], w[3]);
@@ -280,18 +280,14 @@ attn_rows_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restri
     griddep_launch_late();
 }
 
-// Four values of a row; rows may begin anywhere. (volatile: of the two branches written plainly for fp32 the compiler makes one
-// 16-byte store, which faults where a row is not aligned.)
-__device__ __forceinline__ void store4(float* o, float a, float b, float c, float d) {
-    if (((uintptr_t)o & 15) == 0) {
-        *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
-    } else {
-        volatile float* w = o;
-        w[0] = a, w[1] = b, w[2] = c, w[3] = d;
-    }
+// Four values of a row. Whether rows are aligned is the host's to say, and each way is an instance of its own: in one that looked at the
+// address and had both, a row in fp32 that was not aligned met a 16-byte store.
+template <bool ALIGNED> __device__ __forceinline__ void store4(float* o, float a, float b, float c, float d) {
+    if (ALIGNED) *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
+    else o[0] = a, o[1] = b, o[2] = c, o[3] = d;
 }
-__device__ __forceinline__ void store4(bf16* o, float a, float b, float c, float d) {
-    if (((uintptr_t)o & 7) == 0) {
+template <bool ALIGNED> __device__ __forceinline__ void store4(bf16* o, float a, float b, float c, float d) {
+    if (ALIGNED) {
         const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
         *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
     } else {
@@ -373,7 +369,7 @@ __device__ __forceinline__ void sum_scores(int cta, const int* __restrict__ cu_q
 }
 
 // CTAs from `joining` on: sums of kept scores.
-template <typename T, bool OWN>
+template <typename T, bool OWN, bool ALIGNED>
 __global__ void __launch_bounds__(JOIN_WARPS * 32)
 attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const int* __restrict__ kv_len, PageTable pt, RowsArgs a, RowsScratch sc,
                       int joining, int* __restrict__ status) {
@@ -447,7 +443,7 @@ attn_rows_join_kernel(T* __restrict__ out, const int* __restrict__ cu_q, const i
             }
             const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a NaN stays one
             T* o = out + (size_t)t * a.ldo + (size_t)h * a.HD + col;
-            store4(o, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            store4<ALIGNED>(o, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
             if (col == 0 && sc.lse != nullptr) sc.lse[((size_t)g * a.T + s.q_begin) * a.G + pr] = l == 0.f ? -INFINITY : m + log2f(l);
         }
     }
@@ -557,10 +553,10 @@ int launch_rows_generic(const void* q, void* out, int dtype, const RowsArgs& a, 
     return run(q, out, a, k, v, cu_q, kv_len, pt, masks, s, status, stream);
 }
 
-template <typename T, bool OWN>
+template <typename T, bool OWN, bool ALIGNED>
 static int join_go(void* out, const RowsArgs& a, const int* cu_q, const int* kv_len, PageTable pt, RowsScratch s, int joining, dim3 grid, int* status,
                    cudaStream_t stream) {
-    const cudaError_t e = launch_behind(attn_rows_join_kernel<T, OWN>, grid, dim3(JOIN_WARPS * 32), 0, stream, (T*)out, cu_q, kv_len, pt, a, s, joining, status);
+    const cudaError_t e = launch_behind(attn_rows_join_kernel<T, OWN, ALIGNED>, grid, dim3(JOIN_WARPS * 32), 0, stream, (T*)out, cu_q, kv_len, pt, a, s, joining, status);
     if (e != cudaSuccess) return mynah_fail("attn_rows_join: %s", cudaGetErrorString(e));
     return mynah_check_launch("attn_rows_join");
 }
@@ -585,7 +581,10 @@ int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, c
     MYNAH_REQUIRE(ctas < (1ll << 31), "attn_rows_join: launch too large");
     if (ctas == 0) return 0;
     const dim3 grid((unsigned)ctas, helpers);
-    auto run = dtype == MYNAH_F32 ? (a.own ? join_go<float, true> : join_go<float, false>) : (a.own ? join_go<bf16, true> : join_go<bf16, false>);
+    // (what is cut by the step is the tensor-core kernel's, which takes aligned rows of bfloat16)
+    auto run = !a.own ? join_go<bf16, false, true>
+             : dtype == MYNAH_F32 ? (a.q_aligned ? join_go<float, true, true> : join_go<float, true, false>)
+                                  : (a.q_aligned ? join_go<bf16, true, true> : join_go<bf16, true, false>);
     return run(out, a, cu_q, kv_len, pt, s, (int)joining, grid, status, stream);
 }
 

@@ -74,7 +74,7 @@ struct RowsArgs {
     long long cut_rows;               // own: rows of scratch that there are for cut items
     int words;                        // mask words a token
     float scale_log2;                 // score scale * log2(e)
-    int q_aligned;                    // 1: q's rows are whole 16-byte pieces
+    int q_aligned;                    // 1: q's and the output's rows are whole 16-byte pieces
     FastDiv by_G, by_tile, by_group, by_KV, by_ctas, by_quads;
     void finish() {                   // once the numbers above stand
         by_G = FastDiv::of(G), by_tile = FastDiv::of(tile_rows), by_group = FastDiv::of(group), by_KV = FastDiv::of(KV), by_ctas = FastDiv::of(ctas);
