@@ -133,6 +133,34 @@ def test_drafted_steps_gain_tokens(folders):
     assert again.produced == 50 and steps["n"] <= 49
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_text_that_repeats_is_generated_in_fewer_steps(folders, dtype):
+    """A model whose next token goes by the last one alone (its layers add nothing) soon repeats itself: its drafts are accepted."""
+    from mynah_slm_b200 import LLM
+    llm = LLM(folders[("B", dtype)], dtype=dtype, max_tokens=4096)
+    for layer in llm.engine.model.layers:
+        layer.mixer.w_o.zero_()
+        layer.ffn.w_down.zero_()
+    text = [3] + llm.generate([[3]], max_new=400, temp=0.0, ignore_eos=True)[0].tokens
+    start = text.index(text[-1])                           # from here on the text goes round
+    period = text.index(text[-1], start + 1) - start
+    assert start + 3 * period < 300 and all(text[i] == text[i + period] for i in range(start, len(text) - period))
+    at = start + 2 * period + 1
+    results, real = [], llm.engine.step_tree
+
+    def counted(entries, *a, **k):
+        out = real(entries, *a, **k)
+        results.extend(out)
+        return out
+    llm.engine.step_tree = counted
+    got = llm.generate([text[:at]], max_new=60, temp=0.0, ignore_eos=True, draft=8)[0]
+    assert got.tokens == text[at:at + 60]
+    # the round is known when the first tree is drafted: its last place gives min(8, period) tokens, and all of them are right
+    gain = 1 + min(8, period)
+    assert sum(len(r.tokens) + 1 for r in results) == 59 and len(results) <= -(-59 // gain) + 1
+    assert max(len(r.tokens) for r in results) >= min(8, period)
+
+
 def test_what_cannot_draft_refuses(folders):
     from mynah_slm_b200 import LLM
     from mynah_slm_b200.engine.engine import EngineError, KeepRows, TreeEntry
