@@ -23,18 +23,6 @@ int attn_rows_run(const char* who, const void* q, void* out, int dtype, RowsArgs
 
 namespace {
 
-__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 four_of(const bf16* p) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-}
-// The same where rows are not aligned (volatile: read one by one, whatever is made of the other branch).
-__device__ __forceinline__ float4 four_apart(const float* p) {
-    const volatile float* w = p;
-    return make_float4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ float4 four_apart(const bf16* p) { return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3])); }
-
 constexpr int GK = 64, GR = 32;      // keys (a page) and packed rows a tile of the general kernel
 
 // 16 x 16 threads; thread (ty, tx) has the keys ty + 16 i (i < 4) of the page and the rows tx + 16 j of a tile.

@@ -27,17 +27,6 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     return d;
 }
 
-__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 four_of(const bf16* p) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-}
-// The same where rows are not aligned (volatile: read one by one, whatever is made of the other branch).
-__device__ __forceinline__ float4 four_apart(const float* p) {
-    const volatile float* w = p;
-    return make_float4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ float4 four_apart(const bf16* p) { return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3])); }
 __device__ __forceinline__ void copy16_async(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }

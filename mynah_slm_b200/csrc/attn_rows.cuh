@@ -33,6 +33,19 @@ int launch_rows_join(void* out, int dtype, const RowsArgs& a, const int* cu_q, c
                      cudaStream_t stream);
 bool rows_tcgen05_takes(int dtype, int H, int KV, int HD);
 
+// Four values of a row whose pieces of four are aligned.
+__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four_of(const bf16* p) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+}
+// The same where rows are not aligned (volatile: read one by one, whatever is made of the other branch).
+__device__ __forceinline__ float4 four_apart(const float* p) {
+    const volatile float* w = p;
+    return make_float4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float4 four_apart(const bf16* p) { return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3])); }
+
 __device__ __forceinline__ float ex2_f(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -49,7 +62,9 @@ template <typename K> static inline cudaError_t shared_memory_once(K kernel, siz
     return e;
 }
 
-// A launch that may begin while the kernel before it on the stream finishes; every CTA of it waits for that one (griddep_wait), so
+// A launch that may begin while the kernel before it on the stream finishes. (Always, whatever mynah_pdl_enabled() says: that is about
+// launches of one operator behind another's, which cost a decode step more than they gave; this is an operator's own second or
+// third launch, and 2,048 tokens with sums took 75 us instead of 80.) Every CTA of it waits for that one (griddep_wait), so
 // that it cannot end first, and before the wait it reads only what was there before both (the step's description, the page lists).
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {

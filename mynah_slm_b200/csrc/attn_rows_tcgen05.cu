@@ -13,7 +13,7 @@
 //              more than 2^8, weights written back over the scores as bfloat16 (half a step is lost, as much as the output's own
 //              rounding loses; their sum is of the unrounded ones in fp32). Warps whose rows do not exist only keep step.
 //
-// NT = 1: one tile, two CTAs an SM (98 KB and 256 columns of tensor memory each): one's softmax runs under the other's products
+// NT = 1: one tile, two CTAs an SM (107 KB and 256 columns of tensor memory each): one's softmax runs under the other's products
 // and its start and end under the other's pages. NT = 2: two tiles of 128 rows on the same pages, with warps 7-10 for the second,
 // one CTA an SM: a page is brought into shared memory once for 256 rows. Bound by the bytes of K and V while there are few rows;
 // a page takes the tensor cores about 640 clocks a tile whatever its rows (Q.K^T of 64 columns waits for shared memory), the

@@ -26,8 +26,8 @@ struct EvictArgs {
 // word is found in three passes, 11, 11 and 10 bits (a histogram of the words that still agree with it in the bits above, the bin
 // that holds it, and so on); then every warp takes a run of rows, counts those above it and those equal to it, and, once it
 // knows the counts of the runs before, writes its own: those above, and the first of the equal ones. The words are read from
-// memory once where they fit shared memory. Bound by its chain of barriers and passes, so four CTAs an SM (32 registers a thread):
-// 448 choices of 2,048 of 4,100 rows 27.5 us, against 35 with two (64 registers), which are 5% faster for rows beyond shared
+// memory once where they fit shared memory. Bound by its chain of barriers and passes, so up to four CTAs an SM (32 registers a thread;
+// four where the page lists of the step have up to about 190 entries together, three to 265, two beyond: see the launch): 448 choices of 2,048 of 4,100 rows 27.5 us, against 35 with two (64 registers), which are 5% faster for rows beyond shared
 // memory (48 choices of 8,192 of 20,000: 96 and 101 us); with 256 threads 30 and 167.
 __global__ void __launch_bounds__(CH_THREADS, 4)
 evict_choose_kernel(const float* __restrict__ mass, PageTable pt, const int* __restrict__ kv_len, EvictArgs a, int* __restrict__ kept,
@@ -381,7 +381,8 @@ MYNAH_API int mynah_cache_evict(const CacheEvictCall* call) {
     MYNAH_REQUIRE((long long)E * B * KV < (1ll << 31) && (long long)n_pages * KV * PAGE_TOKENS < (1ll << 31), "cache_evict: launch too large");
     MYNAH_REQUIRE(status != nullptr && kept != nullptr && new_len != nullptr && mass != nullptr, "cache_evict: outputs, sums and a status word are required");
     const PageTable from{page_indptr, page_ids, page_base, n_pages}, to{out_indptr, out_ids, out_base, n_pages};
-    // words of up to 96 KB a CTA (two CTAs an SM) are kept in shared memory; longer rows are read again from L2
+    // Words of up to 96 KB a CTA are kept in shared memory; longer rows are read again from L2. The host knows the entries of all page lists
+    // together, not the longest sequence's: many sequences get more than they use, and fewer CTAs an SM for it.
     const long long most = (long long)n_ids * PAGE_TOKENS;
     const int cached = (int)(most < 24576 ? most : 24576);
     const EvictArgs ea{E, B, KV, n_pages, keep, recent, first, cached};

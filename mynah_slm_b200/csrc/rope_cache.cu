@@ -241,7 +241,7 @@ MYNAH_API int mynah_rope_table(float* cos_t, float* sin_t, int n_pos, int rotary
 
 // dtype: type of qkv and of the cache (the 32-bit path keeps both in fp32). tok_row: the cache's rows that the tokens' keys and
 // values are written to, where these are not their positions (null: the positions).
-MYNAH_API int mynah_qk_norm_rope_store_rows(
+MYNAH_API int mynah_qk_norm_rope_store(
     void* qkv, int dtype, int T, int H, int KV, int HD, int ld,
     const void* q_gain, const void* k_gain, int gain_dtype, float eps,
     const float* cos_t, const float* sin_t, int rotary_dim, int n_pos,
@@ -277,15 +277,4 @@ MYNAH_API int mynah_qk_norm_rope_store_rows(
     else
         return mynah_fail("qk_norm_rope_store: unsupported dtype %d", dtype);
     return mynah_check_launch("qk_norm_rope_store");
-}
-
-MYNAH_API int mynah_qk_norm_rope_store(
-    void* qkv, int dtype, int T, int H, int KV, int HD, int ld,
-    const void* q_gain, const void* k_gain, int gain_dtype, float eps,
-    const float* cos_t, const float* sin_t, int rotary_dim, int n_pos,
-    const int* tok_seq, const int* tok_pos,
-    const int* page_indptr, const int* page_ids, const int* page_base, int n_pages,
-    void* k_cache, void* v_cache, int* status, cudaStream_t stream) {
-    return mynah_qk_norm_rope_store_rows(qkv, dtype, T, H, KV, HD, ld, q_gain, k_gain, gain_dtype, eps, cos_t, sin_t, rotary_dim, n_pos,
-                                         tok_seq, tok_pos, nullptr, page_indptr, page_ids, page_base, n_pages, k_cache, v_cache, status, stream);
 }

@@ -1,4 +1,4 @@
-// What the tcgen05 kernels on packed rows share: operand and instruction descriptors, paired fp32 arithmetic, the queries' tensor map.
+// What the tcgen05 kernels on packed rows share beyond tcgen05.cuh: staged rows, the queries' tensor map.
 #pragma once
 #include "tcgen05.cuh"
 
@@ -7,19 +7,6 @@ namespace tc5 {
 constexpr int HALF_BYTES = 128 * 128; // 128 rows of 128 bytes: one 64-column half of a tile
 constexpr int PAGE_BYTES = PAGE_TOKENS * 128;
 
-// K-major operand, 128-byte swizzle, groups of 8 rows 1024 bytes apart.
-static __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-// MN-major operand: a row of 128 bytes holds 64 MN elements of one k; groups of 8 k 1024 bytes apart, the next 64 MN elements
-// `lbo` bytes further on.
-static __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-// fp32 accumulator, bf16 operands, M = 128, N = n; b_mn: B is MN-major.
-static __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
 // One lane of a converged warp, the same every time.
 static __device__ __forceinline__ bool elect_one() {
     uint32_t on;
@@ -34,27 +21,10 @@ static __device__ __forceinline__ float4 ld_shared(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
     return x;
 }
-static __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
-static __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
-    asm("{ .reg .b64 ra, rb, rc, rd;\n\t mov.b64 ra, {%2, %3};\n\t mov.b64 rb, {%4, %4};\n\t mov.b64 rc, {%5, %5};\n\t"
-        " fma.rn.f32x2 rd, ra, rb, rc;\n\t mov.b64 {%0, %1}, rd; }"
-        : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c));
-}
 static __device__ __forceinline__ void fma2v(float& x0, float& x1, float a0, float a1, float b, float c0, float c1) {
     asm("{ .reg .b64 ra, rb, rc, rd;\n\t mov.b64 ra, {%2, %3};\n\t mov.b64 rb, {%4, %4};\n\t mov.b64 rc, {%5, %6};\n\t"
         " fma.rn.f32x2 rd, ra, rb, rc;\n\t mov.b64 {%0, %1}, rd; }"
         : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
-}
-static __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
-    asm("{ .reg .b64 ra, rb;\n\t mov.b64 ra, {%0, %1};\n\t mov.b64 rb, {%2, %3};\n\t add.rn.f32x2 ra, ra, rb;\n\t mov.b64 {%0, %1}, ra; }"
-        : "+f"(x0), "+f"(x1) : "f"(a0), "f"(a1));
-}
-static __device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
 }
 static __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"

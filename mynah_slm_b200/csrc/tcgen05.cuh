@@ -101,6 +101,40 @@ static __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
           "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
         :: "memory");
 }
+// ---- what the attention kernels share: operand and instruction descriptors, paired fp32 arithmetic.
+// K-major operand, 128-byte swizzle, groups of 8 rows 1024 bytes apart.
+static __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major operand, 128-byte swizzle: a row of 128 bytes holds 64 consecutive MN elements of one k; groups of 8 k 1024 bytes apart
+// (stride offset), the next 64 MN elements `lbo` bytes further on (leading offset).
+static __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t lbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulator, bf16 operands, M = 128, N = n; b_mn: B is MN-major.
+static __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? (1u << 16) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// A wait that all lanes of a warp agree on, so that the warp-wide instructions after it keep all their lanes.
+static __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+// Two fp32 operations an instruction (each half is the plain round-to-nearest operation), and the maximum of three: the softmax warps
+// are bound by the number of instructions they issue.
+static __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b, float c) {
+    asm("{ .reg .b64 ra, rb, rc, rd;\n\t mov.b64 ra, {%2, %3};\n\t mov.b64 rb, {%4, %4};\n\t mov.b64 rc, {%5, %5};\n\t"
+        " fma.rn.f32x2 rd, ra, rb, rc;\n\t mov.b64 {%0, %1}, rd; }"
+        : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+static __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
+    asm("{ .reg .b64 ra, rb;\n\t mov.b64 ra, {%0, %1};\n\t mov.b64 rb, {%2, %3};\n\t add.rn.f32x2 ra, ra, rb;\n\t mov.b64 {%0, %1}, ra; }"
+        : "+f"(x0), "+f"(x1) : "f"(a0), "f"(a1));
+}
+static __device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // ---- two CTAs of a cluster working as one (cta_group::2). The even CTA of the pair leads: it issues the products,
 // and its mbarriers collect the transactions of both CTAs' copies. A shared-memory address with bit 24 cleared
 // names the same offset in the leading CTA.

@@ -342,7 +342,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, H: int, KV: int, HD: int,
             raise KernelError("qk_norm_rope_store: the cache and the activations differ in dtype")
         if tuple(k_cache.shape[1:]) != (KV, PAGE_TOKENS, HD):
             raise KernelError(f"qk_norm_rope_store: cache pages are {tuple(k_cache.shape[1:])}, expected {(KV, PAGE_TOKENS, HD)}")
-    call("mynah_qk_norm_rope_store_rows", ptr(qkv), code(qkv.dtype), T, H, KV, HD, ld,
+    call("mynah_qk_norm_rope_store", ptr(qkv), code(qkv.dtype), T, H, KV, HD, ld,
          ptr(q_gain), ptr(k_gain), gd, float(eps),
          ptr(cos), ptr(sin), rotary_dim, n_pos,
          ptr(tok_seq), ptr(tok_pos), ptr(tok_row),

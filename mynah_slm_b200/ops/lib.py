@@ -36,15 +36,9 @@ _SIGNATURES: dict[str, list] = {
     "mynah_qk_norm_rope_store": [P, c_int, c_int, c_int, c_int, c_int, c_int,
                                  P, P, c_int, c_float,
                                  P, P, c_int, c_int,
-                                 P, P,
+                                 P, P, P,
                                  P, P, P, c_int,
                                  P, P, P, P],
-    "mynah_qk_norm_rope_store_rows": [P, c_int, c_int, c_int, c_int, c_int, c_int,
-                                      P, P, c_int, c_float,
-                                      P, P, c_int, c_int,
-                                      P, P, P,
-                                      P, P, P, c_int,
-                                      P, P, P, P],
     "mynah_attn_prefill_generic": [P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                    P, P, P, P,
                                    P, P, P, c_int,
