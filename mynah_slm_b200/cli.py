@@ -19,7 +19,8 @@ go to stdout, one line per prompt; the timing line goes to stderr
 (src/timing.c:56-62), so stdout stays pipeable.
 
 --draft N checks up to N tokens a step that are drafted from the text so far
-(with --temp 0). --keep N bounds the rows that a sequence holds in the cache:
+(with --temp 0; a checked step costs several plain ones, so for text that
+repeats itself at length). --keep N bounds the rows that a sequence holds in the cache:
 beyond N it is cut to three quarters, keeping its first 4 rows, its last N / 4
 and those that gathered the most attention.
 

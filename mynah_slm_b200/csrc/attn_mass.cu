@@ -11,7 +11,7 @@
 // Long sequences are cut over their rows too (attn_mass.cuh): the cut pieces' sums are left in scratch and added in order by a
 // second launch. Steps of few rows on the tensor cores do not look at the keys again: the attention keeps its scores, and the
 // launch that joins its segments adds them up (sum_scores in attn_rows.cu). This file holds the general kernel (fp32, and bfloat16
-// heads that the tensor-core kernel does not take: 2 pieces of 150 tokens behind 333 rows, 6 heads of 48 on 3, 10 us of 39, bound
+// heads that the tensor-core kernel does not take: 2 pieces of 150 tokens behind 333 rows, 6 heads of 48 on 3, 10 us of 37, bound
 // by its launches and its FFMA fed from shared memory), the addition of pieces and the entry points.
 #include "attn_mass.cuh"
 
