@@ -217,7 +217,8 @@ def test_an_output_over_q_is_refused_and_one_beside_it_served(dtype):
 COMPANY = [  # a sequence's rows and past, then the others' in every company
     (1, 1535, [([1], [40]), ([1] * 5, [6000, 3, 64, 900, 2047]), ([1] * 63, [(b * 631) % 4000 for b in range(63)]),
                ([1] * 300, [(b * 37) % 300 for b in range(300)])]),
-    (1, 63, [([1] * 9, [9000] * 9)]),
+    (1, 63, [([1] * 9, [9000] * 9), ([300, 9], [200, 64]), ([17, 1, 0, 2], [5, 70, 90, 400])]),           # (and tiles of another size)
+    (5, 700, [([1, 3], [64, 2000]), ([200], [0])]),
     (40, 700, [([33], [10]), ([300, 9], [2000, 64]), ([12] * 40, [(b * 211) % 900 for b in range(40)])]),
     (150, 333, [([150], [333]), ([64, 170], [3000, 5]), ([60] * 10, [500] * 10)]),
 ]
